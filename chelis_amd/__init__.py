@@ -116,6 +116,12 @@ SIGNATURES = {
     "chelis_hip_causal_attention": (c_int32, [P, P, P, c_double, P]),
     "chelis_hip_softmax_adjoint": (c_int32, [P, P, P]),
     "chelis_hip_layer_norm": (c_int32, [P, P, P, c_double, P]),
+    "chelis_hip_layer_norm_stats": (c_int32, [P, P, P, c_double, P, P, P]),
+    "chelis_hip_layer_norm_adjoint": (c_int32, [P, P, P, P, P, P, P, P]),
+    "chelis_hip_rotary": (c_int32, [POINTER(P), c_int32, P, P, POINTER(c_int64), c_int32, c_int32, POINTER(P)]),
+    "chelis_hip_rotary_adjoint": (c_int32, [POINTER(P), c_int32, P, P, POINTER(c_int64), c_int32, c_int32, POINTER(P)]),
+    "chelis_hip_window_attention": (c_int32, [P, P, P, P, P, c_int64, c_int64, c_double, P, P]),
+    "chelis_hip_window_attention_adjoint": (c_int32, [P, P, P, P, P, P, P, P, c_int64, c_int64, c_double, P, P, P]),
     "chelis_hip_fused_elementwise": (c_int32, [POINTER(FusedChain), POINTER(P), c_int32, P]),
     "chelis_hip_gelu": (c_int32, [P, P]),
     "chelis_hip_relu": (c_int32, [P, P]),
@@ -397,6 +403,88 @@ def layer_norm(x, gamma, beta, eps: float, y=None):
     y = y or empty(x.shape, x.dtype)
     check(lib().chelis_hip_layer_norm(_p(x), _p(gamma), _p(beta), eps, _p(y)), "layer_norm")
     return y
+
+
+def _opt(t):
+    return _p(t) if t is not None else None
+
+
+def layer_norm_stats(x, gamma, beta, eps: float, y=None, mean=None, rstd=None):
+    """layer_norm with its row statistics; returns (y, mean, rstd), the
+    statistics f32 (f64 beside f64 rows) over x's leading axes."""
+    stat = np.float64 if x.dtype == np.float64 else np.float32
+    y, mean, rstd = y or empty(x.shape, x.dtype), mean or empty(x.shape[:-1], stat), rstd or empty(x.shape[:-1], stat)
+    check(lib().chelis_hip_layer_norm_stats(_p(x), _p(gamma), _p(beta), eps, _p(y), _p(mean), _p(rstd)),
+          "layer_norm_stats")
+    return y, mean, rstd
+
+
+def layer_norm_adjoint(x, gamma, mean, rstd, g, dx=None, dgamma=None, dbeta=None, want_dx: bool = True,
+                       want_weights: bool = True):
+    """Gradients of layer_norm for the cotangent g, from layer_norm_stats'
+    mean and rstd; returns (dx, dgamma, dbeta), None for what is not wanted."""
+    if want_dx:
+        dx = dx or empty(x.shape, x.dtype)
+    if want_weights:
+        dgamma, dbeta = dgamma or empty(gamma.shape, gamma.dtype), dbeta or empty(gamma.shape, gamma.dtype)
+    check(lib().chelis_hip_layer_norm_adjoint(_p(x), _p(gamma), _p(mean), _p(rstd), _p(g),
+                                              _p(dx) if want_dx else None, _p(dgamma) if want_weights else None,
+                                              _p(dbeta) if want_weights else None), "layer_norm_adjoint")
+    return dx if want_dx else None, dgamma if want_weights else None, dbeta if want_weights else None
+
+
+ROTARY_PAIRINGS = {"halves": 0, "adjacent": 1}
+
+
+def _rotary(fn, what, xs, positions, freqs, sections, pairing, out):
+    single = not isinstance(xs, (list, tuple))
+    xs = [xs] if single else list(xs)
+    out = [empty(x.shape, x.dtype) for x in xs] if out is None else [out] if single else list(out)
+    if len(out) != len(xs):
+        raise ChelisError(f"{what}: {len(xs)} tensors and {len(out)} results")
+    ins, outs = (P * len(xs))(*[_p(t) for t in xs]), (P * len(xs))(*[_p(t) for t in out])
+    sec = (c_int64 * max(1, len(sections)))(*[int(v) for v in sections])
+    check(fn(ins, len(xs), _p(positions), _p(freqs), sec, len(sections), ROTARY_PAIRINGS[pairing], outs), what)
+    return out[0] if single else out
+
+
+def rotary(xs, positions, freqs, sections, pairing: str = "halves", out=None):
+    """Rotary positions over len(sections) axes, of one [batch, heads, seq,
+    width] tensor or of two (queries and keys) in one launch; positions
+    [axes, batch, seq] i32 / i64, freqs f64 [sum(sections)], pairing "halves"
+    or "adjacent". out may be xs."""
+    return _rotary(lib().chelis_hip_rotary, "rotary", xs, positions, freqs, sections, pairing, out)
+
+
+def rotary_adjoint(gs, positions, freqs, sections, pairing: str = "halves", out=None):
+    """The gradient of rotary: the cotangents turned back."""
+    return _rotary(lib().chelis_hip_rotary_adjoint, "rotary_adjoint", gs, positions, freqs, sections, pairing, out)
+
+
+def window_attention(q, k, v, window: int, sinks: int, scale: float, o=None, lse=None, lengths=None, starts=None):
+    """Attention where a row sees the last `window` keys up to its own
+    position and the first `sinks` keys: q [batch, heads, seq, width] over
+    k, v [batch, kv_heads, keys, width]. lengths [batch]: the keys each
+    sequence holds; starts [batch]: its first row's position (None: the rows
+    are its last). lse: a tensor for the rows' log sums, True to make one.
+    Returns o, or (o, lse) when lse was asked for."""
+    o = o or empty(q.shape, q.dtype)
+    if lse is True:
+        lse = empty(q.shape[:3], np.float32)
+    check(lib().chelis_hip_window_attention(_p(q), _p(k), _p(v), _opt(lengths), _opt(starts), int(window), int(sinks),
+                                            scale, _p(o), _opt(lse)), "window_attention")
+    return o if lse is None else (o, lse)
+
+
+def window_attention_adjoint(q, k, v, o, lse, g, window: int, sinks: int, scale: float, dq=None, dk=None, dv=None,
+                             lengths=None, starts=None):
+    """Gradients (dq, dk, dv) of window_attention for the cotangent g of o,
+    from its o and lse and the same other arguments."""
+    dq, dk, dv = dq or empty(q.shape, q.dtype), dk or empty(k.shape, k.dtype), dv or empty(v.shape, v.dtype)
+    check(lib().chelis_hip_window_attention_adjoint(_p(q), _p(k), _p(v), _p(o), _p(lse), _p(g), _opt(lengths),
+                                                    _opt(starts), int(window), int(sinks), scale, _p(dq), _p(dk),
+                                                    _p(dv)), "window_attention_adjoint")
+    return dq, dk, dv
 
 
 def gelu(x, y=None):

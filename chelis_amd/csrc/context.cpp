@@ -8,6 +8,7 @@
 // hipLaunchKernel on that stream.
 #include <hip/hip_runtime.h>
 
+#include <algorithm>
 #include <atomic>
 #include <cstdarg>
 #include <cstdio>
@@ -75,6 +76,15 @@ hipError_t device_malloc(void **p, size_t bytes) {
     return hipMalloc(p, bytes);
 }
 
+namespace {
+// The library stream is being captured into a graph.
+bool capturing() {
+    hipStream_t s = stream();
+    hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
+    return s && hipStreamIsCapturing(s, &status) == hipSuccess && status == hipStreamCaptureStatusActive;
+}
+}  // namespace
+
 void *scratch_alloc(size_t bytes) {
     if (!bytes) return nullptr;
     g_scratch_requests.fetch_add(1, std::memory_order_relaxed);
@@ -91,13 +101,17 @@ void *scratch_alloc(size_t bytes) {
             return p;
         }
     }
+    // an allocation is no stream operation: allowed while this thread captures
+    hipStreamCaptureMode mode = hipStreamCaptureModeRelaxed;
+    const bool relaxed = capturing() && hipThreadExchangeStreamCaptureMode(&mode) == hipSuccess;
     void *p = nullptr;
-    if (device_malloc(&p, size_t(1) << c) != hipSuccess) return nullptr;
-    return p;
+    const hipError_t e = device_malloc(&p, size_t(1) << c);
+    if (relaxed) (void)hipThreadExchangeStreamCaptureMode(&mode);
+    return e == hipSuccess ? p : nullptr;
 }
 
 void scratch_free(void *p, size_t bytes) {
-    if (!p) return;
+    if (!p || capturing()) return;
     int device = 0;
     if (hipGetDevice(&device) != hipSuccess || device < 0 || device >= kMaxDevices) return;
     std::lock_guard<std::mutex> lock(g_scratch_mutex);
@@ -243,6 +257,39 @@ bool same_shape(const chelis_gpu_tensor *a, const chelis_gpu_tensor *b) {
     for (int32_t i = 0; i < a->rank; ++i)
         if (a->shape[i] != b->shape[i]) return false;
     return true;
+}
+
+bool non_overlapping(const chelis_gpu_tensor *t) {
+    int32_t idx[8];
+    int32_t n = 0;
+    for (int32_t a = 0; a < t->rank; ++a)
+        if (t->shape[a] > 1) idx[n++] = a;
+    std::sort(idx, idx + n, [&](int32_t x, int32_t y) { return t->strides[x] < t->strides[y]; });
+    int64_t span = 1;
+    for (int32_t i = 0; i < n; ++i) {
+        const int64_t s = t->strides[idx[i]];
+        if (s < span) return false;
+        span = s * t->shape[idx[i]];
+    }
+    return true;
+}
+
+int32_t check_device(const chelis_gpu_tensor *t, const char *name) {
+    static const int devices = [] {
+        int n = 0;
+        return hipGetDeviceCount(&n) == hipSuccess ? n : 0;
+    }();
+    if (devices < 2 || !t->count) return CHELIS_HIP_OK;
+    hipPointerAttribute_t at{};
+    int device = 0;
+    if (hipGetDevice(&device) != hipSuccess || hipPointerGetAttributes(&at, t->data) != hipSuccess) {
+        (void)hipGetLastError();
+        return set_error(CHELIS_HIP_EDOMAIN, "%s: data is no device memory", name);
+    }
+    if (at.type == hipMemoryTypeDevice && at.device != device)
+        return set_error(CHELIS_HIP_EDOMAIN, "%s: data lies on device %d, the current device is %d", name, at.device,
+                         device);
+    return CHELIS_HIP_OK;
 }
 
 bool row_view(const chelis_gpu_tensor *t, RowView *v) {

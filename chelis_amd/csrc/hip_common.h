@@ -49,7 +49,10 @@ int32_t *status_words(int32_t **host);
 // stream: blocks are recycled in stream order (a freed block's earlier users
 // are already enqueued ahead of any later user) and cached for reuse, so
 // the hot path makes no allocation calls. scratch_free takes the size given
-// to scratch_alloc. Returns null when the device cannot allocate.
+// to scratch_alloc. Returns null when the device cannot allocate. While the
+// library stream is being captured into a graph, the block leaves the cache
+// for good: each replay uses it again, so no other call and no other graph
+// may get it.
 void *scratch_alloc(size_t bytes);
 // hipMalloc, counted (chelis_hip_allocation_counts): every device allocation
 // the library makes goes through it.
@@ -94,6 +97,12 @@ inline int64_t dtype_width(chelis_dtype d) {
 int32_t check_tensor(const chelis_gpu_tensor *t, const char *name);
 bool is_contiguous(const chelis_gpu_tensor *t);
 bool same_shape(const chelis_gpu_tensor *a, const chelis_gpu_tensor *b);
+// Distinct indices of a view address distinct elements (no write races):
+// sorted by stride, each axis steps past everything the smaller axes span.
+bool non_overlapping(const chelis_gpu_tensor *t);
+// On a machine with several devices: the tensor's storage lies on the
+// current one (whose library stream the launch goes to).
+int32_t check_device(const chelis_gpu_tensor *t, const char *name);
 
 // A [rows, n] view of a tensor whose last axis is contiguous (stride 1) and
 // whose leading axes collapse to one row index with a uniform row stride.
@@ -101,6 +110,11 @@ struct RowView {
     int64_t rows = 0, n = 0, ld = 0;
 };
 bool row_view(const chelis_gpu_tensor *t, RowView *v);
+// The layer norm rows of checked f32 / f64 operands; mean and rstd (both or
+// neither, contiguous over the rows) receive the row statistics.
+int32_t layer_norm_rows(const chelis_gpu_tensor *x, const chelis_gpu_tensor *gamma, const chelis_gpu_tensor *beta,
+                        double epsilon, const chelis_gpu_tensor *y, const RowView &vx, const RowView &vy,
+                        const chelis_gpu_tensor *mean, const chelis_gpu_tensor *rstd);
 
 // Keyed dropout (and, applied to a cotangent, its replay) with the key read
 // on the device from key_dev, the storage of a KEY tensor: no host round trip.

@@ -726,11 +726,14 @@ __global__ __launch_bounds__(64 * W * R) void softmax_adjoint_kernel(const T *__
 
 // layer_norm: mean = tree(x)/n; c = x - mean; var = tree(c*c)/n;
 // y = (c / sqrt(var + eps)) * gamma + beta, every primitive finalized.
+// mean_out and rstd_out (both or neither) receive the row's mean and
+// 1 / sqrt(var + eps).
 template <typename T, int V, int S, int W, int R, int L, bool RAGGED>
 __global__ __launch_bounds__(64 * W * R) void layer_norm_kernel(const T *__restrict__ x, const T *__restrict__ gamma,
                                                                  const T *__restrict__ beta, T *__restrict__ y,
                                                                  int64_t rows, int n, int64_t ldx, int64_t ldy,
-                                                                 T eps) {
+                                                                 T eps, T *__restrict__ mean_out,
+                                                                 T *__restrict__ rstd_out) {
     __shared__ T lds[R * W * S];
     RowCoord<W, R, L> c(rows);
     if (L == 64 && !c.live) return;
@@ -767,6 +770,10 @@ __global__ __launch_bounds__(64 * W * R) void layer_norm_kernel(const T *__restr
                             lds, c)) /
                         extent);
     const T denom = canon_bits(sqrt(canon(var + eps)));
+    if (mean_out && c.live && c.tid_in_row == 0) {
+        mean_out[c.row] = mean;
+        rstd_out[c.row] = canon(T(1) / denom);
+    }
 #pragma unroll
     for (int s = 0; s < S; ++s) {
         if constexpr (EARLY) {
@@ -802,6 +809,7 @@ struct RowArgs {
     double scale;
     int64_t q_len;
     double eps;
+    void *mean, *rstd;
 };
 
 template <typename T, int V, int S, int W, int R, int L, bool DENSE, bool RAGGED>
@@ -827,7 +835,8 @@ void launch_pair(RowOp op, const RowArgs &a, unsigned grid, hipStream_t st) {
             (const T *)a.a, (const T *)a.b, (T *)a.out, a.rows, (int)a.n, a.lda, a.ldb, a.ldo);
     else
         layer_norm_kernel<T, V, S, W, R, L, RAGGED><<<grid, block, 0, st>>>(
-            (const T *)a.a, (const T *)a.b, (const T *)a.c, (T *)a.out, a.rows, (int)a.n, a.lda, a.ldo, (T)a.eps);
+            (const T *)a.a, (const T *)a.b, (const T *)a.c, (T *)a.out, a.rows, (int)a.n, a.lda, a.ldo, (T)a.eps,
+            (T *)a.mean, (T *)a.rstd);
 }
 
 template <typename T, int V, int S, int W, int R, int L>
@@ -965,7 +974,9 @@ struct RowScratch {
     void *p = nullptr;
     size_t bytes = 0;
     explicit RowScratch(size_t b) : p(scratch_alloc(b)), bytes(b) {}
-    ~RowScratch() { scratch_free(p, bytes); }
+    ~RowScratch() {
+        if (bytes) scratch_free(p, bytes);
+    }
 };
 
 int32_t long_softmax(const chelis_gpu_tensor *x, const chelis_gpu_tensor *y, const RowView &vx, const RowView &vy) {
@@ -1008,10 +1019,12 @@ int32_t long_softmax_adjoint(const chelis_gpu_tensor *y, const chelis_gpu_tensor
 }
 
 int32_t long_layer_norm(const chelis_gpu_tensor *x, const chelis_gpu_tensor *gamma, const chelis_gpu_tensor *beta,
-                        double eps, const chelis_gpu_tensor *y, const RowView &vx, const RowView &vy) {
+                        double eps, const chelis_gpu_tensor *y, const RowView &vx, const RowView &vy,
+                        const chelis_gpu_tensor *mean_out, const chelis_gpu_tensor *rstd_out) {
     const chelis_dtype dt = x->dtype;
     const int64_t w = dtype_width(dt), R = vx.rows, n = vx.n;
-    RowScratch tmp(R * w), mean(R * w), den(R * w);
+    RowScratch tmp(R * w), mean(mean_out ? 0 : R * w), den(R * w);
+    if (mean_out) mean.p = mean_out->data;
     if (!tmp.p || !mean.p || !den.p)
         return set_error(CHELIS_HIP_EHIP, "layer_norm: row scratch of %lld bytes", (long long)(3 * R * w));
     const Rows2 X(x->data, dt, R, n, vx.ld, 1, x->byte_capacity), Y(y->data, dt, R, n, vy.ld, 1, y->byte_capacity);
@@ -1033,6 +1046,12 @@ int32_t long_layer_norm(const chelis_gpu_tensor *x, const chelis_gpu_tensor *gam
                                           fstep(CHELIS_FUSED_CONST, 0, 0, eps), fstep(CHELIS_FUSED_ADD, prv(1), prv(2)),
                                           fstep(CHELIS_FUSED_SQRT, prv(3))});
     if (int32_t st = chelis_hip_fused_elementwise(&dn, t1, 1, &Dv.t)) return st;
+    if (rstd_out) {
+        const chelis_fused_chain inv = fchain({fstep(CHELIS_FUSED_RECIP, 0)});
+        const Vec1 Rv(rstd_out->data, dt, R);
+        const chelis_gpu_tensor *d1[1] = {&Dv.t};
+        if (int32_t st = chelis_hip_fused_elementwise(&inv, d1, 1, &Rv.t)) return st;
+    }
     // y = ((x - mean) / denom) * gamma + beta
     const chelis_fused_chain out = fchain({fstep(CHELIS_FUSED_SUB, 0, 1), fstep(CHELIS_FUSED_DIV, prv(0), 2),
                                            fstep(CHELIS_FUSED_MUL, prv(1), 3), fstep(CHELIS_FUSED_ADD, prv(2), 4)});
@@ -1043,6 +1062,15 @@ int32_t long_layer_norm(const chelis_gpu_tensor *x, const chelis_gpu_tensor *gam
 bool long_rows(chelis_dtype dt, int64_t n) { return n > kRowCapacityBytes / dtype_width(dt); }
 
 }  // namespace
+
+int32_t layer_norm_rows(const chelis_gpu_tensor *x, const chelis_gpu_tensor *gamma, const chelis_gpu_tensor *beta,
+                        double epsilon, const chelis_gpu_tensor *y, const RowView &vx, const RowView &vy,
+                        const chelis_gpu_tensor *mean, const chelis_gpu_tensor *rstd) {
+    if (vx.rows && long_rows(x->dtype, vx.n)) return long_layer_norm(x, gamma, beta, epsilon, y, vx, vy, mean, rstd);
+    RowArgs a{x->data, gamma->data, beta->data, y->data, vx.rows, vx.n, vx.ld, 0, vy.ld, 0, 1.0, 1, epsilon,
+              mean ? mean->data : nullptr, rstd ? rstd->data : nullptr};
+    return dispatch(x->dtype, RowOp::LayerNorm, a);
+}
 }  // namespace chelis
 
 using namespace chelis;
@@ -1090,7 +1118,5 @@ extern "C" int32_t chelis_hip_layer_norm(const chelis_gpu_tensor *x, const cheli
         if (p->dtype != x->dtype || p->rank != 1 || p->shape[0] != vx.n || (vx.n > 1 && p->strides[0] != 1))
             return set_error(CHELIS_HIP_EDOMAIN, "layer_norm: gamma/beta must be contiguous [hidden]");
     if (vx.n == 0) return set_error(CHELIS_HIP_EDOMAIN, "layer_norm: hidden extent must be positive");
-    if (vx.rows && long_rows(x->dtype, vx.n)) return long_layer_norm(x, gamma, beta, epsilon, y, vx, vy);
-    RowArgs a{x->data, gamma->data, beta->data, y->data, vx.rows, vx.n, vx.ld, 0, vy.ld, 0, 1.0, 1, epsilon};
-    return dispatch(x->dtype, RowOp::LayerNorm, a);
+    return layer_norm_rows(x, gamma, beta, epsilon, y, vx, vy, nullptr, nullptr);
 }

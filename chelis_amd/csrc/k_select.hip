@@ -1067,21 +1067,6 @@ int32_t check_out(const chelis_gpu_tensor *out, const char *what) {
     return CHELIS_HIP_OK;
 }
 
-// A strided output no two of whose elements share an address: sorted by
-// stride, each axis steps past everything the smaller axes span.
-bool non_overlapping(const chelis_gpu_tensor *t) {
-    std::vector<std::pair<int64_t, int64_t>> ax;
-    for (int32_t a = 0; a < t->rank; ++a)
-        if (t->shape[a] > 1) ax.push_back({t->strides[a], t->shape[a]});
-    std::sort(ax.begin(), ax.end());
-    int64_t span = 1;
-    for (const auto &p : ax) {
-        if (p.first < span) return false;
-        span = p.first * p.second;
-    }
-    return true;
-}
-
 int64_t map_blocks(int64_t count) { return std::max<int64_t>(1, std::min<int64_t>((count + 255) / 256, 65536)); }
 
 template <class F>

@@ -1,0 +1,828 @@
+// Attention with a sliding window and always-visible first tokens (sinks):
+// query row i of a sequence of n keys stands at position p = start + i and
+// sees key j when 0 <= j <= p < n and (p - j < window or j < sinks), so
+//   o_i = sum_j P_ij v_j,  P_ij = exp(scale q_i.k_j - lse_i)
+// over the visible j, o_i = 0 and lse_i = -inf where there is none, and with
+// D_i = g_i . o_i and dS_ij = P_ij (g_i . v_j - D_i)
+//   dq_i = scale sum_j dS_ij k_j, dk_j = scale sum_i dS_ij q_i,
+//   dv_j = sum_i P_ij g_i
+// summed over the query heads that share a key head.
+//
+// All products run on the matrix cores as 32 x 32 blocks (16 elements of the
+// summed axis a step; binary32 operands as eight steps of 2). Layouts, for
+// lane l with i = l % 32 and h = l / 32:
+//   A and B hold eight elements of row (column) i: elements 8h .. 8h + 7 of
+//   the step's 16, or any other order that both share;
+//   C[8 (r / 4) + 4 h + r % 4][i] is item r of 16.
+// Scores are formed so that the rows of C are what the next product sums
+// over: eight consecutive items of C, rounded to the operand type, are then
+// the B operand of the next product as they stand, in the order
+// 4h .. 4h + 3, 8 + 4h .. 8 + 4h + 3 (and 16 more for items 8 .. 15), and
+// nothing crosses lanes. The other operand reads the tile across its rows in
+// the same order (16-bit types with the transposing LDS read).
+//
+// Scores, softmax statistics and sums are binary32. P and dS are rounded to
+// the operand type for the products that sum over them, as the operands
+// themselves are; the sum of P that divides the result is of the unrounded
+// values.
+#include "elem.h"
+
+#include <algorithm>
+#include <type_traits>
+
+namespace chelis {
+namespace {
+
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+template <typename T>
+using V8 = T __attribute__((ext_vector_type(8)));
+
+constexpr int kWaves = 4;
+constexpr int kThreads = 64 * kWaves;
+constexpr int kKeys = 64;   // keys of a staged tile (forward, dq)
+constexpr int kRows = 32;   // query rows of a staged tile (dk, dv)
+constexpr float kLog2e = 1.44269504088896340736f, kLn2 = 0.69314718055994530942f;
+// rows and keys: sums of three of them stay inside 32 bits
+constexpr int64_t kMaxExtent = (int64_t(1) << 29) - 1024;
+
+__device__ inline f32x16 mma(V8<__bf16> a, V8<__bf16> b, f32x16 c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
+}
+__device__ inline f32x16 mma(V8<_Float16> a, V8<_Float16> b, f32x16 c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
+}
+__device__ inline f32x16 mma(V8<float> a, V8<float> b, f32x16 c) {
+#pragma unroll
+    for (int t = 0; t < 8; ++t) c = __builtin_amdgcn_mfma_f32_32x32x2f32(a[t], b[t], c, 0, 0, 0);
+    return c;
+}
+
+// LDS rows of D elements, 32 bytes apart from a multiple of the 256-byte
+// bank span: 16-byte reads down a column of rows and the transposing reads
+// of four rows both touch every bank once.
+template <typename T, int D>
+constexpr int kPitch = D + 32 / (int)sizeof(T);
+
+// Eight elements of tile row `row` from element `at`.
+template <typename T, int D>
+__device__ inline V8<T> along(const T *tile, int row, int at) {
+    return *reinterpret_cast<const V8<T> *>(tile + row * kPitch<T, D> + at);
+}
+// Column d0 + l % 32 of tile rows row0 + 4h .. + 3 and row0 + 8 + 4h .. + 3.
+template <typename T, int D>
+__device__ inline V8<T> across(const T *tile, int row0, int d0, int lane) {
+    const int h = lane >> 5;
+    if constexpr (sizeof(T) == 2) {
+        // each 16 lanes read four rows of 16 elements, lane i the four
+        // elements 4 (i % 4) .. of row i / 4, and lane i gets column i
+        const T *p = tile + (row0 + 4 * h + ((lane & 15) >> 2)) * kPitch<T, D> + d0 + (lane & 16) + 4 * (lane & 3);
+        typedef __attribute__((address_space(3))) s16x4 *Lds;
+        union {
+            s16x4 q[2];
+            V8<T> v;
+        } u;
+        u.q[0] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((Lds)p);
+        u.q[1] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((Lds)(p + 8 * kPitch<T, D>));
+        return u.v;
+    } else {
+        const T *p = tile + (row0 + 4 * h) * kPitch<T, D> + d0 + (lane & 31);
+        V8<T> v;
+#pragma unroll
+        for (int t = 0; t < 8; ++t) v[t] = p[(t < 4 ? t : 4 + t) * kPitch<T, D>];
+        return v;
+    }
+}
+
+template <typename T>
+__device__ inline bool not_finite(T v) {
+    if constexpr (sizeof(T) == 2) {
+        constexpr uint16_t e = std::is_same<T, _Float16>::value ? 0x7c00 : 0x7f80;
+        return (__builtin_bit_cast(uint16_t, v) & e) == e;
+    } else {
+        return (f32_bits(v) & 0x7f800000u) == 0x7f800000u;
+    }
+}
+
+// c += a . b where b (weights of pairs, eight of them with their visible
+// ones in `seen`) is zero at hidden pairs. A hidden pair adds nothing, also
+// where a holds an infinity or a NaN: those elements are taken out of the
+// product, and what they add at visible pairs is found by counting. With
+// SIGNED weights the count stands for NaN, else (weights >= 0) infinities
+// keep their sign.
+template <bool SIGNED, typename T>
+__device__ inline f32x16 mma_hidden(V8<T> a, V8<T> b, uint32_t seen, f32x16 c) {
+    bool bad = false;
+#pragma unroll
+    for (int t = 0; t < 8; ++t) bad |= not_finite(a[t]);
+    if (!__any(bad)) return mma(a, b, c);
+    V8<T> part, vis;
+#pragma unroll
+    for (int t = 0; t < 8; ++t) {
+        part[t] = not_finite(a[t]) ? (T)0.f : a[t];
+        vis[t] = (T)((seen >> t) & 1 ? 1.f : 0.f);
+    }
+    c = mma(part, b, c);
+#pragma unroll 1
+    for (int k = 0; k < 3; ++k) {  // NaN, +inf, -inf
+#pragma unroll
+        for (int t = 0; t < 8; ++t) {
+            const int kind = SIGNED || a[t] != a[t] ? 0 : a[t] > (T)0.f ? 1 : 2;
+            part[t] = (T)(not_finite(a[t]) && kind == k ? 1.f : 0.f);
+        }
+        const f32x16 found = mma(part, vis, f32x16{});
+        const float adds = k == 0 ? __builtin_nanf("") : k == 1 ? INFINITY : -INFINITY;
+#pragma unroll
+        for (int r = 0; r < 16; ++r)
+            if (found[r] > 0.f) c[r] += adds;
+    }
+    return c;
+}
+
+template <typename T>
+__device__ inline V8<T> rounded(const f32x16 &s, int from) {
+    V8<T> v;
+#pragma unroll
+    for (int t = 0; t < 8; ++t) v[t] = (T)s[from + t];
+    return v;
+}
+
+struct View {
+    const void *p;
+    int64_t b, h, s;  // strides of batch, head, sequence
+};
+
+struct WinArgs {
+    View q, k, v, o, g, dq, dk, dv;
+    const float *lse_in;
+    float *lse, *delta, *range;
+    const void *lengths, *starts;
+    int64_t length_step, start_step;
+    int lengths_wide, starts_wide;
+    int sq, sk, window, sinks, heads, kv, group, width, flip;
+    float c, scale;  // |scale| log2(e), scale
+};
+
+// The keys and the first row's position of sequence b. Stored lengths and
+// starts are taken into the extents the launch was checked for.
+struct Seq {
+    int n, start;
+    __device__ Seq(const WinArgs &a, int64_t b) {
+        n = a.sk;
+        if (a.lengths) n = (int)pick(a.lengths, a.lengths_wide, b * a.length_step, 0, a.sk);
+        start = a.starts ? (int)pick(a.starts, a.starts_wide, b * a.start_step, -kMaxExtent, a.sk) : n - a.sq;
+    }
+    __device__ static int64_t pick(const void *p, int wide, int64_t at, int64_t lo, int64_t hi) {
+        const int64_t v = wide ? static_cast<const int64_t *>(p)[at] : static_cast<const int32_t *>(p)[at];
+        return v < lo ? lo : v > hi ? hi : v;
+    }
+};
+
+template <typename T>
+__device__ inline const T *head_of(const View &v, int64_t b, int64_t h) {
+    return static_cast<const T *>(v.p) + b * v.b + h * v.h;
+}
+
+// Eight elements `at` .. of a row in memory, zero past the head's width or
+// where the row is not `live` (row 0 is read in its place).
+template <typename T>
+__device__ inline V8<T> row_part(const T *row, int at, int width, bool live) {
+    Pack<T, 8> p;
+    p.load(row + (at < width ? at : 0));
+    V8<T> z = {};
+    return live && at < width ? p.q : z;
+}
+
+// A tile of N rows of D elements on its way from memory to LDS. Rows past
+// `last` and elements past the width repeat others of the operand: the rows
+// are hidden from every pair, and the other factor's elements are zero.
+template <typename T, int D, int N>
+struct Staged {
+    static constexpr int ALL = N * (D / 8), PARTS = (ALL + kThreads - 1) / kThreads;
+    Pack<T, 8> part[PARTS];
+    __device__ void load(const T *base, int64_t step, int row0, int last, int width, int tid) {
+#pragma unroll
+        for (int i = 0; i < PARTS; ++i) {
+            const int id = tid + i * kThreads, r = min(row0 + id / (D / 8), last), at = id % (D / 8) * 8;
+            part[i].load(base + r * step + (at < width ? at : 0));
+        }
+    }
+    __device__ void store(T *tile, int tid) const {
+#pragma unroll
+        for (int i = 0; i < PARTS; ++i) {
+            const int id = tid + i * kThreads;
+            if (ALL % kThreads && id >= ALL) break;
+            *reinterpret_cast<V8<T> *>(tile + id / (D / 8) * kPitch<T, D> + id % (D / 8) * 8) = part[i].q;
+        }
+    }
+};
+
+// The key tiles that rows of positions first .. last see: those of the
+// sinks, then those of the window.
+struct KeyWalk {
+    int count, sink_tiles, window_from;
+    __device__ KeyWalk(int first, int last, int n, int window, int sinks) {
+        last = min(last, n - 1);
+        count = sink_tiles = window_from = 0;
+        if (last < 0 || first >= n) return;
+        const int hi = last / kKeys, lo = max(0, first - window + 1) / kKeys;
+        sink_tiles = min((sinks + kKeys - 1) / kKeys, hi + 1);
+        window_from = max(sink_tiles, lo);
+        count = sink_tiles + max(0, hi - window_from + 1);
+    }
+    __device__ int tile(int t) const { return t < sink_tiles ? t : window_from + t - sink_tiles; }
+};
+
+// What 32 rows from position `first` (live rows of them exist) see of keys
+// k0 .. k0 + count - 1.
+enum Sight { kNone, kSome, kAll };
+__device__ inline Sight sight(int first, int live, int n, int window, int sinks, int k0, int count) {
+    const int last = min(first + live - 1, n - 1), k1 = k0 + count - 1;
+    if (live <= 0 || first >= n || k0 > last || (k0 >= sinks && k1 <= first - window)) return kNone;
+    const bool all = live >= 32 && first + 31 < n && k1 <= first && (k0 > first + 31 - window || k1 < sinks);
+    return all ? kAll : kSome;
+}
+
+// Which of the keys k0 + 8 (r / 4) + 4 h + r % 4, items r of a column of
+// scores, a row sees whose last visible key is `top` (-1: none) and whose
+// window starts behind key `low`. Selections only, no branches.
+struct SeenKeys {
+    int top, low, sinks;
+    __device__ SeenKeys(int top_, int low_, int sinks_, int k0, int h)
+        : top(top_ - k0 - 4 * h), low(low_ - k0 - 4 * h), sinks(sinks_ - k0 - 4 * h) {}
+    __device__ bool operator()(int r) const {
+        const int k = 8 * (r >> 2) + (r & 3);
+        return (k <= top) & ((k > low) | (k < sinks));
+    }
+};
+// Which of the rows r0 + 8 (r / 4) + 4 h + r % 4, of positions from start,
+// see a key: those from the key's own position up to the window's end, or up
+// to the last row inside the sequence for a sink.
+struct SeenRows {
+    int from, end;
+    __device__ SeenRows(int key, int start, int r0, int h, int rows, int n, int window, int sinks) {
+        const int base = r0 + 4 * h, last = min(rows, n - start);
+        from = key - start - base;
+        end = (key < sinks ? last : min(last, key - start + window)) - base;
+    }
+    __device__ bool operator()(int r) const {
+        const int k = 8 * (r >> 2) + (r & 3);
+        return (k >= from) & (k < end);
+    }
+};
+
+__device__ inline float exp2_(float x) { return __builtin_amdgcn_exp2f(x); }
+__device__ inline float other_half(float x) { return __shfl_xor(x, 32, 64); }
+
+// Four consecutive elements of an accumulated column to memory.
+template <typename T>
+__device__ inline void store4(T *p, const f32x16 &c, int from, float f) {
+    Pack<T, 4> out;
+#pragma unroll
+    for (int t = 0; t < 4; ++t) out.set(t, c[from + t] * f);
+    out.store(p);
+}
+// Column block d0 .. of an accumulated result row.
+template <typename T>
+__device__ inline void store_column(T *row, const f32x16 &c, int d0, int width, int h, float f) {
+#pragma unroll
+    for (int r = 0; r < 16; r += 4) {
+        const int d = d0 + 2 * r + 4 * h;
+        if (d < width) store4(row + d, c, r, f);
+    }
+}
+
+// ---------------------------------------------------------------- forward
+// f16 weights are held 2^10 times larger: the smallest keep their bits.
+template <typename T>
+constexpr float kShift = std::is_same<T, _Float16>::value ? 10.f : 0.f;
+
+// A workgroup takes 128 rows of one head, each wave 32 of them.
+template <typename T, int D>
+__global__ __launch_bounds__(kThreads, 2) void window_forward_kernel(WinArgs a) {
+    __shared__ __attribute__((aligned(16))) T Ks[kKeys * kPitch<T, D>], Vs[kKeys * kPitch<T, D>];
+    const int tid = threadIdx.x, lane = tid & 63, i = lane & 31, h = lane >> 5;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int64_t b = blockIdx.z, head = blockIdx.y;
+    const Seq seq(a, b);
+    const int row0 = blockIdx.x * (32 * kWaves), mine = row0 + 32 * wave, row = mine + i;
+    const int live = min(32, a.sq - mine);
+    const T *Q = head_of<T>(a.q, b, head), *K = head_of<T>(a.k, b, head / a.group), *V = head_of<T>(a.v, b, head / a.group);
+    V8<T> qf[D / 16];
+#pragma unroll
+    for (int s = 0; s < D / 16; ++s) {
+        qf[s] = row_part(Q + (row < a.sq ? row : 0) * a.q.s, 16 * s + 8 * h, a.width, row < a.sq);
+        if (a.flip) qf[s] = -qf[s];
+    }
+    f32x16 acc[D / 32] = {};
+    float m = -INFINITY, l = 0.f;
+    const int first = seq.start + mine, p = first + i, top = row < a.sq && p < seq.n ? p : -1, low = p - a.window;
+    const KeyWalk walk(seq.start + row0, seq.start + min(row0 + 32 * kWaves, a.sq) - 1, seq.n, a.window, a.sinks);
+    Staged<T, D, kKeys> ks, vs;
+    if (walk.count) {
+        ks.load(K, a.k.s, walk.tile(0) * kKeys, seq.n - 1, a.width, tid);
+        vs.load(V, a.v.s, walk.tile(0) * kKeys, seq.n - 1, a.width, tid);
+    }
+    for (int t = 0; t < walk.count; ++t) {
+        const int k0 = walk.tile(t) * kKeys;
+        __syncthreads();
+        ks.store(Ks, tid);
+        vs.store(Vs, tid);
+        __syncthreads();
+        if (t + 1 < walk.count) {
+            ks.load(K, a.k.s, walk.tile(t + 1) * kKeys, seq.n - 1, a.width, tid);
+            vs.load(V, a.v.s, walk.tile(t + 1) * kKeys, seq.n - 1, a.width, tid);
+        }
+        const Sight see = sight(first, live, seq.n, a.window, a.sinks, k0, kKeys);
+        if (see == kNone) continue;
+        f32x16 s[2] = {};
+#pragma unroll
+        for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+            for (int u = 0; u < D / 16; ++u) s[kb] = mma(along<T, D>(Ks, 32 * kb + i, 16 * u + 8 * h), qf[u], s[kb]);
+        uint32_t seen = 0xffffffffu;
+        if (see == kSome) {
+            seen = 0;
+#pragma unroll
+            for (int kb = 0; kb < 2; ++kb) {
+                const SeenKeys keys(top, low, a.sinks, k0 + 32 * kb, h);
+#pragma unroll
+                for (int r = 0; r < 16; ++r) {
+                    const bool vis = keys(r);
+                    seen |= (uint32_t)vis << (16 * kb + r);
+                    s[kb][r] = vis ? s[kb][r] : -INFINITY;
+                }
+            }
+        }
+        float mx = -INFINITY;
+#pragma unroll
+        for (int r = 0; r < 32; ++r) mx = fmaxf(mx, s[r >> 4][r & 15]);
+        mx = fmaxf(mx, other_half(mx)) * a.c;
+        const float m_new = fmaxf(m, mx);
+        // while every score is -inf, 0 in place of the maximum keeps the
+        // weights 0 (-inf - -inf would be NaN, and stay)
+        const float ref = m_new == -INFINITY ? 0.f : m_new;
+        const float alpha = exp2_(m - ref), off = kShift<T> - ref;
+        m = m_new;
+        float sum = 0.f;
+#pragma unroll
+        for (int r = 0; r < 32; ++r) {
+            const float e = exp2_(fmaf(s[r >> 4][r & 15], a.c, off));
+            s[r >> 4][r & 15] = e;
+            sum += e;
+        }
+        if (see == kSome) {
+            // hidden scores of a zero scale are -inf * 0
+            sum = 0.f;
+#pragma unroll
+            for (int r = 0; r < 32; ++r) {
+                const float e = (seen >> r) & 1 ? s[r >> 4][r & 15] : 0.f;
+                s[r >> 4][r & 15] = e;
+                sum += e;
+            }
+        }
+        l = l * alpha + sum;
+#pragma unroll
+        for (int d = 0; d < D / 32; ++d) acc[d] *= alpha;
+#pragma unroll
+        for (int kc = 0; kc < 4; ++kc) {
+            const V8<T> pf = rounded<T>(s[kc >> 1], 8 * (kc & 1));
+#pragma unroll
+            for (int d = 0; d < D / 32; ++d) {
+                const V8<T> vf = across<T, D>(Vs, 16 * kc, 32 * d, lane);
+                acc[d] = see == kAll ? mma(vf, pf, acc[d]) : mma_hidden<false, T>(vf, pf, (seen >> (8 * kc)) & 0xff, acc[d]);
+            }
+        }
+    }
+    l += other_half(l);
+    if (row >= a.sq) return;
+    const bool empty = top < 0;
+    const float inv = empty ? 0.f : 1.f / l;
+    T *O = const_cast<T *>(head_of<T>(a.o, b, head)) + row * a.o.s;
+#pragma unroll
+    for (int d = 0; d < D / 32; ++d) store_column(O, acc[d], 32 * d, a.width, h, inv);
+    if (a.lse && h == 0)
+        a.lse[(b * a.heads + head) * a.sq + row] = empty ? -INFINITY : canon_bits((m - kShift<T> + log2f(l)) * kLn2);
+}
+
+// ---------------------------------------------------------------- backward
+// f16 holds dS times a power of two that brings its largest possible value,
+// 2 max|g| max|v| width, just under f16's: gradients of any size keep their
+// bits. A first launch takes both maxima (over kRanges workgroups each); the
+// other types need no scale.
+constexpr int kRanges = 256;
+
+// The largest finite |g| of rows inside their sequence (KEYS: |v| of keys).
+template <typename T, bool KEYS>
+__global__ __launch_bounds__(256) void window_range_kernel(WinArgs a, int64_t total, float *out) {
+    __shared__ float waves[4];
+    const View &x = KEYS ? a.v : a.g;
+    const int heads = KEYS ? a.kv : a.heads, rows = KEYS ? a.sk : a.sq, parts = a.width / 8;
+    float m = 0.f;
+    for (int64_t id = (int64_t)blockIdx.x * 256 + threadIdx.x; id < total; id += (int64_t)kRanges * 256) {
+        const int64_t at = id / parts, bh = at / rows, b = bh / heads;
+        const int row = (int)(at % rows);
+        const Seq seq(a, b);
+        const int p = KEYS ? row : seq.start + row;
+        if (p < 0 || p >= seq.n) continue;
+        Pack<T, 8> q;
+        q.load(head_of<T>(x, b, bh % heads) + row * x.s + id % parts * 8);
+#pragma unroll
+        for (int t = 0; t < 8; ++t)
+            if (!not_finite(q.q[t])) m = fmaxf(m, fabsf(q.get(t)));
+    }
+    m = wave_vmax(m);
+    if ((threadIdx.x & 63) == 0) waves[threadIdx.x >> 6] = m;
+    __syncthreads();
+    if (threadIdx.x == 0) out[blockIdx.x] = fmaxf(fmaxf(waves[0], waves[1]), fmaxf(waves[2], waves[3]));
+}
+
+// The power of two; every thread of the workgroup calls it once.
+template <typename T>
+__device__ inline float gradient_scale(const WinArgs &a) {
+    if constexpr (!std::is_same<T, _Float16>::value) return 1.f;
+    __shared__ float waves[2][kWaves];
+    static_assert(kRanges == kThreads, "one partial maximum a thread");
+    const float g = wave_vmax(a.range[threadIdx.x]), v = wave_vmax(a.range[kRanges + threadIdx.x]);
+    if ((threadIdx.x & 63) == 0) {
+        waves[0][threadIdx.x >> 6] = g;
+        waves[1][threadIdx.x >> 6] = v;
+    }
+    __syncthreads();
+    float mg = 0.f, mv = 0.f;
+#pragma unroll
+    for (int w = 0; w < kWaves; ++w) {
+        mg = fmaxf(mg, waves[0][w]);
+        mv = fmaxf(mv, waves[1][w]);
+    }
+    const float most = 2.f * mg * mv * (float)a.width;
+    // most < 2^(ilogb + 1), taken to less than 2^15
+    return most > 0.f ? ldexpf(1.f, min(14 - ilogbf(most), 100)) : 1.f;
+}
+
+// dq, and D for the second kernel: rows as in the forward kernel.
+template <typename T, int D>
+__global__ __launch_bounds__(kThreads, 2) void window_dq_kernel(WinArgs a) {
+    __shared__ __attribute__((aligned(16))) T Ks[kKeys * kPitch<T, D>], Vs[kKeys * kPitch<T, D>];
+    const int tid = threadIdx.x, lane = tid & 63, i = lane & 31, h = lane >> 5;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int64_t b = blockIdx.z, head = blockIdx.y;
+    const Seq seq(a, b);
+    const int row0 = blockIdx.x * (32 * kWaves), mine = row0 + 32 * wave, row = mine + i;
+    const int live = min(32, a.sq - mine), safe = row < a.sq ? row : 0;
+    const T *Q = head_of<T>(a.q, b, head), *K = head_of<T>(a.k, b, head / a.group), *V = head_of<T>(a.v, b, head / a.group);
+    const T *G = head_of<T>(a.g, b, head), *O = head_of<T>(a.o, b, head);
+    V8<T> qf[D / 16], gf[D / 16];
+    float delta = 0.f;
+#pragma unroll
+    for (int s = 0; s < D / 16; ++s) {
+        const int at = 16 * s + 8 * h;
+        qf[s] = row_part(Q + safe * a.q.s, at, a.width, row < a.sq);
+        if (a.flip) qf[s] = -qf[s];
+        gf[s] = row_part(G + safe * a.g.s, at, a.width, row < a.sq);
+        const V8<T> of = row_part(O + safe * a.o.s, at, a.width, row < a.sq);
+#pragma unroll
+        for (int t = 0; t < 8; ++t) delta = fmaf(widen<T>(gf[s][t]), widen<T>(of[t]), delta);
+    }
+    delta += other_half(delta);
+    const int64_t stat = (b * a.heads + head) * a.sq + safe;
+    if (row < a.sq && h == 0) a.delta[stat] = delta;
+    const float lse = a.lse_in[stat] * kLog2e, up = gradient_scale<T>(a);
+    f32x16 acc[D / 32] = {};
+    const int first = seq.start + mine, p = first + i, top = row < a.sq && p < seq.n ? p : -1, low = p - a.window;
+    const KeyWalk walk(seq.start + row0, seq.start + min(row0 + 32 * kWaves, a.sq) - 1, seq.n, a.window, a.sinks);
+    Staged<T, D, kKeys> ks, vs;
+    if (walk.count) {
+        ks.load(K, a.k.s, walk.tile(0) * kKeys, seq.n - 1, a.width, tid);
+        vs.load(V, a.v.s, walk.tile(0) * kKeys, seq.n - 1, a.width, tid);
+    }
+    for (int t = 0; t < walk.count; ++t) {
+        const int k0 = walk.tile(t) * kKeys;
+        __syncthreads();
+        ks.store(Ks, tid);
+        vs.store(Vs, tid);
+        __syncthreads();
+        if (t + 1 < walk.count) {
+            ks.load(K, a.k.s, walk.tile(t + 1) * kKeys, seq.n - 1, a.width, tid);
+            vs.load(V, a.v.s, walk.tile(t + 1) * kKeys, seq.n - 1, a.width, tid);
+        }
+#pragma unroll
+        for (int kb = 0; kb < 2; ++kb) {
+            const int kk = k0 + 32 * kb;
+            const Sight see = sight(first, live, seq.n, a.window, a.sinks, kk, 32);
+            if (see == kNone) continue;
+            f32x16 s = {}, dp = {};
+#pragma unroll
+            for (int u = 0; u < D / 16; ++u) {
+                s = mma(along<T, D>(Ks, 32 * kb + i, 16 * u + 8 * h), qf[u], s);
+                dp = mma(along<T, D>(Vs, 32 * kb + i, 16 * u + 8 * h), gf[u], dp);
+            }
+            uint32_t seen = 0xffffu;
+#pragma unroll
+            for (int r = 0; r < 16; ++r) s[r] = exp2_(fmaf(s[r], a.c, -lse)) * ((dp[r] - delta) * up);
+            if (see == kSome) {
+                seen = 0;
+                const SeenKeys keys(top, low, a.sinks, kk, h);
+#pragma unroll
+                for (int r = 0; r < 16; ++r) {
+                    const bool vis = keys(r);
+                    seen |= (uint32_t)vis << r;
+                    s[r] = vis ? s[r] : 0.f;
+                }
+            }
+#pragma unroll
+            for (int kc = 0; kc < 2; ++kc) {
+                const V8<T> df = rounded<T>(s, 8 * kc);
+#pragma unroll
+                for (int d = 0; d < D / 32; ++d) {
+                    const V8<T> kf = across<T, D>(Ks, 32 * kb + 16 * kc, 32 * d, lane);
+                    acc[d] = see == kAll ? mma(kf, df, acc[d])
+                                         : mma_hidden<true, T>(kf, df, (seen >> (8 * kc)) & 0xff, acc[d]);
+                }
+            }
+        }
+    }
+    if (row >= a.sq) return;
+    T *DQ = const_cast<T *>(head_of<T>(a.dq, b, head)) + row * a.dq.s;
+#pragma unroll
+    for (int d = 0; d < D / 32; ++d) store_column(DQ, acc[d], 32 * d, a.width, h, a.scale / up);
+}
+
+// dk and dv: a workgroup takes 128 keys of one key head, each wave 32 of
+// them, and walks the rows that see any of them, of every query head of the
+// group.
+template <typename T, int D>
+__global__ __launch_bounds__(kThreads, 1) void window_dkv_kernel(WinArgs a) {
+    __shared__ __attribute__((aligned(16))) T Qs[kRows * kPitch<T, D>], Gs[kRows * kPitch<T, D>];
+    __shared__ __attribute__((aligned(16))) float Ls[kRows], Ds[kRows];
+    const int tid = threadIdx.x, lane = tid & 63, i = lane & 31, h = lane >> 5;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int64_t b = blockIdx.z, kvh = blockIdx.y;
+    const Seq seq(a, b);
+    const int tile0 = blockIdx.x * (32 * kWaves), mine = tile0 + 32 * wave, key = mine + i;
+    const bool have = key < seq.n;
+    const T *K = head_of<T>(a.k, b, kvh), *V = head_of<T>(a.v, b, kvh);
+    V8<T> kf[D / 16], vf[D / 16];
+#pragma unroll
+    for (int s = 0; s < D / 16; ++s) {
+        kf[s] = have ? row_part(K + key * a.k.s, 16 * s + 8 * h, a.width, true) : V8<T>{};
+        if (a.flip) kf[s] = -kf[s];
+        vf[s] = have ? row_part(V + key * a.v.s, 16 * s + 8 * h, a.width, true) : V8<T>{};
+    }
+    const float up = gradient_scale<T>(a), half = up * exp2_(-kShift<T>);
+    f32x16 dk[D / 32] = {}, dv[D / 32] = {};
+    // rows first .. last see some key of the tile
+    const int64_t end = tile0 < a.sinks ? kMaxExtent * 2 : (int64_t)tile0 + 32 * kWaves - 1 + a.window - 1;
+    const int lo = max(0, tile0 - seq.start);
+    const int hi = (int)min(min((int64_t)a.sq - 1, (int64_t)seq.n - 1 - seq.start), end - seq.start);
+    const int from = lo / kRows, tiles = hi < lo || tile0 >= seq.n ? 0 : hi / kRows - from + 1, items = tiles * a.group;
+    Staged<T, D, kRows> qs, gs;
+    float ls = 0.f, ds = 0.f;
+    auto load = [&](int t) {
+        const int64_t head = kvh * a.group + t / tiles;
+        const int r0 = (from + t % tiles) * kRows;
+        qs.load(head_of<T>(a.q, b, head), a.q.s, r0, a.sq - 1, a.width, tid);
+        gs.load(head_of<T>(a.g, b, head), a.g.s, r0, a.sq - 1, a.width, tid);
+        if (tid < kRows) {
+            const int64_t stat = (b * a.heads + head) * a.sq + min(r0 + tid, a.sq - 1);
+            ls = a.lse_in[stat];
+            ds = a.delta[stat];
+        }
+    };
+    if (items) load(0);
+    for (int t = 0; t < items; ++t) {
+        const int r0 = (from + t % tiles) * kRows;
+        __syncthreads();
+        qs.store(Qs, tid);
+        gs.store(Gs, tid);
+        if (tid < kRows) {
+            Ls[tid] = kShift<T> - ls * kLog2e;
+            Ds[tid] = ds;
+        }
+        __syncthreads();
+        if (t + 1 < items) load(t + 1);
+        const Sight see = sight(seq.start + r0, min(kRows, a.sq - r0), seq.n, a.window, a.sinks, mine, 32);
+        if (see == kNone) continue;
+        f32x16 s = {}, dp = {};
+#pragma unroll
+        for (int u = 0; u < D / 16; ++u) {
+            s = mma(along<T, D>(Qs, i, 16 * u + 8 * h), kf[u], s);
+            dp = mma(along<T, D>(Gs, i, 16 * u + 8 * h), vf[u], dp);
+        }
+        uint32_t seen = 0xffffu;
+#pragma unroll
+        for (int r4 = 0; r4 < 4; ++r4) {
+            const f32x4 lr = *reinterpret_cast<const f32x4 *>(Ls + 8 * r4 + 4 * h);
+            const f32x4 dr = *reinterpret_cast<const f32x4 *>(Ds + 8 * r4 + 4 * h);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const int r = 4 * r4 + j;
+                const float p = exp2_(fmaf(s[r], a.c, lr[j]));
+                s[r] = p;
+                dp[r] = p * ((dp[r] - dr[j]) * half);
+            }
+        }
+        if (see == kSome) {
+            seen = 0;
+            const SeenRows rows(key, seq.start, r0, h, a.sq, seq.n, a.window, a.sinks);
+#pragma unroll
+            for (int r = 0; r < 16; ++r) {
+                const bool vis = rows(r);
+                seen |= (uint32_t)vis << r;
+                s[r] = vis ? s[r] : 0.f;
+                dp[r] = vis ? dp[r] : 0.f;
+            }
+        }
+#pragma unroll
+        for (int kc = 0; kc < 2; ++kc) {
+            const V8<T> pf = rounded<T>(s, 8 * kc), df = rounded<T>(dp, 8 * kc);
+            const uint32_t bits = (seen >> (8 * kc)) & 0xff;
+#pragma unroll
+            for (int d = 0; d < D / 32; ++d) {
+                const V8<T> gf = across<T, D>(Gs, 16 * kc, 32 * d, lane), qf = across<T, D>(Qs, 16 * kc, 32 * d, lane);
+                dv[d] = see == kAll ? mma(gf, pf, dv[d]) : mma_hidden<false, T>(gf, pf, bits, dv[d]);
+                dk[d] = see == kAll ? mma(qf, df, dk[d]) : mma_hidden<true, T>(qf, df, bits, dk[d]);
+            }
+        }
+    }
+    if (key >= a.sk) return;
+    T *DK = const_cast<T *>(head_of<T>(a.dk, b, kvh)) + key * a.dk.s, *DV = const_cast<T *>(head_of<T>(a.dv, b, kvh)) + key * a.dv.s;
+#pragma unroll
+    for (int d = 0; d < D / 32; ++d) {
+        store_column(DK, dk[d], 32 * d, a.width, h, a.scale / up);
+        store_column(DV, dv[d], 32 * d, a.width, h, exp2_(-kShift<T>));
+    }
+}
+
+// ---------------------------------------------------------------- dispatch
+// f(T(), D): the operand type and the head width the registers hold.
+template <class F>
+int32_t with_head(chelis_dtype dt, int width, F &&f) {
+    auto by_width = [&](auto t) -> int32_t {
+        if (width <= 64) return f(t, std::integral_constant<int, 64>());
+        if (width <= 96) return f(t, std::integral_constant<int, 96>());
+        return f(t, std::integral_constant<int, 128>());
+    };
+    if (dt == CHELIS_DTYPE_F32) return by_width(float());
+    if (dt == CHELIS_DTYPE_BF16) return by_width(__bf16());
+    return by_width(_Float16());
+}
+
+View view_of(const chelis_gpu_tensor *t) { return {t->data, t->strides[0], t->strides[1], t->strides[2]}; }
+
+int32_t check_part(const chelis_gpu_tensor *t, const char *name, const chelis_gpu_tensor *like, const char *what) {
+    if (int32_t s = check_tensor(t, name)) return s;
+    if (t->rank != 4 || !(t->dtype == CHELIS_DTYPE_F32 || is_narrow16(t->dtype)))
+        return set_error(CHELIS_HIP_EDOMAIN, "%s: %s must be f32, bf16 or f16 [batch, heads, seq, width]", what, name);
+    if (t->dtype != like->dtype) return set_error(CHELIS_HIP_EDOMAIN, "%s: %s must have q's dtype", what, name);
+    if (t->shape[3] > 1 && t->strides[3] != 1)
+        return set_error(CHELIS_HIP_EUNSUPPORTED, "%s: %s: the last axis must be contiguous", what, name);
+    return check_device(t, name);
+}
+
+int32_t check_same(const chelis_gpu_tensor *t, const char *name, const chelis_gpu_tensor *like, const char *other,
+                   const char *what) {
+    if (!same_shape(t, like)) return set_error(CHELIS_HIP_EDOMAIN, "%s: %s must have %s's shape", what, name, other);
+    return CHELIS_HIP_OK;
+}
+
+int32_t check_stat(const chelis_gpu_tensor *t, const char *name, const chelis_gpu_tensor *q, const char *what) {
+    if (int32_t s = check_tensor(t, name)) return s;
+    bool fits = t->dtype == CHELIS_DTYPE_F32 && t->rank == 3 && is_contiguous(t);
+    for (int32_t i = 0; fits && i < 3; ++i) fits = t->shape[i] == q->shape[i];
+    if (!fits) return set_error(CHELIS_HIP_EDOMAIN, "%s: %s must be contiguous f32 [batch, heads, seq]", what, name);
+    return check_device(t, name);
+}
+
+int32_t check_index(const chelis_gpu_tensor *t, const char *name, int64_t batch, const char *what) {
+    if (int32_t s = check_tensor(t, name)) return s;
+    if ((t->dtype != CHELIS_DTYPE_I32 && t->dtype != CHELIS_DTYPE_I64) || t->rank != 1 || t->shape[0] != batch)
+        return set_error(CHELIS_HIP_EDOMAIN, "%s: %s must be i32 or i64 [batch]", what, name);
+    return check_device(t, name);
+}
+
+// Checks what both directions share and fills the arguments.
+int32_t window_args(const chelis_gpu_tensor *q, const chelis_gpu_tensor *k, const chelis_gpu_tensor *v,
+                    const chelis_gpu_tensor *lengths, const chelis_gpu_tensor *starts, int64_t window, int64_t sinks,
+                    double scale, WinArgs *a, const char *what) {
+    int32_t s;
+    if ((s = check_tensor(q, "q")) || (s = check_part(q, "q", q, what)) || (s = check_part(k, "k", q, what)) ||
+        (s = check_part(v, "v", q, what)) || (s = check_same(v, "v", k, "k", what)))
+        return s;
+    const int64_t B = q->shape[0], H = q->shape[1], KV = k->shape[1], W = q->shape[3];
+    if (k->shape[0] != B || k->shape[3] != W)
+        return set_error(CHELIS_HIP_EDOMAIN, "%s: q and k must share batch and width", what);
+    if (KV ? H % KV != 0 : H != 0)
+        return set_error(CHELIS_HIP_EDOMAIN, "%s: %lld query heads over %lld key heads", what, (long long)H, (long long)KV);
+    if (W < 8 || W > 128 || W % 8)
+        return set_error(CHELIS_HIP_EUNSUPPORTED, "%s: heads of %lld: a multiple of 8 up to 128", what, (long long)W);
+    if (window < 1 || sinks < 0)
+        return set_error(CHELIS_HIP_EDOMAIN, "%s: window must be at least 1 and sinks not negative", what);
+    if (!std::isfinite(scale) || !std::isfinite((float)(std::fabs(scale) * kLog2e)))
+        return set_error(CHELIS_HIP_EDOMAIN, "%s: scale must be finite", what);
+    if (q->shape[2] > kMaxExtent || k->shape[2] > kMaxExtent || B > 65535 || H > 65535)
+        return set_error(CHELIS_HIP_EUNSUPPORTED, "%s: more than 2^29 - 1024 rows or keys, or 65535 sequences or heads", what);
+    if ((lengths && (s = check_index(lengths, "lengths", B, what))) ||
+        (starts && (s = check_index(starts, "starts", B, what))))
+        return s;
+    a->q = view_of(q), a->k = view_of(k), a->v = view_of(v);
+    if (lengths) {
+        a->lengths = lengths->data, a->length_step = lengths->strides[0];
+        a->lengths_wide = lengths->dtype == CHELIS_DTYPE_I64;
+    }
+    if (starts) {
+        a->starts = starts->data, a->start_step = starts->strides[0];
+        a->starts_wide = starts->dtype == CHELIS_DTYPE_I64;
+    }
+    a->sq = (int)q->shape[2], a->sk = (int)k->shape[2];
+    a->window = (int)std::min<int64_t>(window, std::max(a->sk, 1)), a->sinks = (int)std::min<int64_t>(sinks, a->sk);
+    a->heads = (int)H, a->kv = (int)KV, a->group = KV ? (int)(H / KV) : 1, a->width = (int)W;
+    a->flip = scale < 0, a->scale = (float)scale, a->c = (float)(std::fabs(scale) * 1.4426950408889634074);
+    return CHELIS_HIP_OK;
+}
+
+int32_t check_result(const chelis_gpu_tensor *t, const char *name, std::initializer_list<const chelis_gpu_tensor *> ins,
+                     const char *what) {
+    if (!non_overlapping(t)) return set_error(CHELIS_HIP_EDOMAIN, "%s: %s overlaps itself", what, name);
+    for (const chelis_gpu_tensor *in : ins)
+        if (t->count && in->count && t->data == in->data)
+            return set_error(CHELIS_HIP_EDOMAIN, "%s: %s overlaps another operand", what, name);
+    return CHELIS_HIP_OK;
+}
+
+}  // namespace
+}  // namespace chelis
+
+using namespace chelis;
+
+extern "C" int32_t chelis_hip_window_attention(const chelis_gpu_tensor *q, const chelis_gpu_tensor *k,
+                                               const chelis_gpu_tensor *v, const chelis_gpu_tensor *lengths,
+                                               const chelis_gpu_tensor *starts, int64_t window, int64_t sinks,
+                                               double scale, const chelis_gpu_tensor *o,
+                                               const chelis_gpu_tensor *lse) {
+    const char *what = "window_attention";
+    WinArgs a{};
+    int32_t s;
+    if ((s = window_args(q, k, v, lengths, starts, window, sinks, scale, &a, what)) ||
+        (s = check_part(o, "o", q, what)) || (s = check_same(o, "o", q, "q", what)) ||
+        (lse && (s = check_stat(lse, "lse", q, what))) || (s = check_result(o, "o", {q, k, v}, what)))
+        return s;
+    a.o = view_of(o);
+    a.lse = lse ? static_cast<float *>(lse->data) : nullptr;
+    if (!q->count) return CHELIS_HIP_OK;
+    hipStream_t st = stream();
+    if (!st) return set_error(CHELIS_HIP_EHIP, "no HIP device");
+    const dim3 grid((a.sq + 127) / 128, a.heads, (unsigned)q->shape[0]);
+    if (!grid_fits(grid.x, kThreads)) return set_error(CHELIS_HIP_EUNSUPPORTED, "%s: grid too large", what);
+    return with_head(q->dtype, a.width, [&](auto t, auto d) -> int32_t {
+        window_forward_kernel<decltype(t), d><<<grid, kThreads, 0, st>>>(a);
+        CHELIS_LAUNCH_CHECK();
+        return CHELIS_HIP_OK;
+    });
+}
+
+extern "C" int32_t chelis_hip_window_attention_adjoint(
+    const chelis_gpu_tensor *q, const chelis_gpu_tensor *k, const chelis_gpu_tensor *v, const chelis_gpu_tensor *o,
+    const chelis_gpu_tensor *lse, const chelis_gpu_tensor *g, const chelis_gpu_tensor *lengths,
+    const chelis_gpu_tensor *starts, int64_t window, int64_t sinks, double scale, const chelis_gpu_tensor *dq,
+    const chelis_gpu_tensor *dk, const chelis_gpu_tensor *dv) {
+    const char *what = "window_attention_adjoint";
+    WinArgs a{};
+    int32_t s;
+    if ((s = window_args(q, k, v, lengths, starts, window, sinks, scale, &a, what))) return s;
+    for (auto [t, name] : {std::pair(o, "o"), std::pair(g, "g"), std::pair(dq, "dq")})
+        if ((s = check_part(t, name, q, what)) || (s = check_same(t, name, q, "q", what))) return s;
+    for (auto [t, name] : {std::pair(dk, "dk"), std::pair(dv, "dv")})
+        if ((s = check_part(t, name, q, what)) || (s = check_same(t, name, k, "k", what))) return s;
+    if ((s = check_stat(lse, "lse", q, what)) || (s = check_result(dq, "dq", {q, k, v, o, g, dk, dv}, what)) ||
+        (s = check_result(dk, "dk", {q, k, v, o, g, dv}, what)) || (s = check_result(dv, "dv", {q, k, v, o, g}, what)))
+        return s;
+    a.o = view_of(o), a.g = view_of(g), a.dq = view_of(dq), a.dk = view_of(dk), a.dv = view_of(dv);
+    a.lse_in = static_cast<const float *>(lse->data);
+    if (!q->count && !k->count) return CHELIS_HIP_OK;
+    hipStream_t st = stream();
+    if (!st) return set_error(CHELIS_HIP_EHIP, "no HIP device");
+    const dim3 rows((a.sq + 127) / 128, a.heads, (unsigned)q->shape[0]);
+    const dim3 keys((a.sk + 127) / 128, a.kv, (unsigned)q->shape[0]);
+    if (!grid_fits(rows.x, kThreads) || !grid_fits(keys.x, kThreads))
+        return set_error(CHELIS_HIP_EUNSUPPORTED, "%s: grid too large", what);
+    const size_t bytes = (2 * kRanges + (size_t)lse->count) * sizeof(float);
+    a.range = static_cast<float *>(scratch_alloc(bytes));
+    a.delta = a.range + 2 * kRanges;
+    if (!a.range) return set_error(CHELIS_HIP_EHIP, "%s: scratch of %zu bytes", what, bytes);
+    s = with_head(q->dtype, a.width, [&](auto t, auto d) -> int32_t {
+        using T = decltype(t);
+        if constexpr (std::is_same<T, _Float16>::value) {
+            window_range_kernel<T, false><<<kRanges, 256, 0, st>>>(a, q->count / 8, a.range);
+            window_range_kernel<T, true><<<kRanges, 256, 0, st>>>(a, k->count / 8, a.range + kRanges);
+        }
+        if (q->count) window_dq_kernel<decltype(t), d><<<rows, kThreads, 0, st>>>(a);
+        if (k->count) window_dkv_kernel<decltype(t), d><<<keys, kThreads, 0, st>>>(a);
+        return CHELIS_HIP_OK;
+    });
+    const hipError_t e = hipGetLastError();
+    scratch_free(a.range, bytes);
+    if (e != hipSuccess) return set_error(CHELIS_HIP_EHIP, "kernel launch: %s", hipGetErrorString(e));
+    return s;
+}

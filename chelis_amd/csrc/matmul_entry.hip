@@ -53,22 +53,6 @@ bool as_mat(const chelis_gpu_tensor *t, bool as_row, Mat *m) {
     return true;
 }
 
-// Distinct indices of a view must address distinct elements (no write races).
-bool non_overlapping(const chelis_gpu_tensor *t) {
-    int32_t idx[8];
-    int32_t n = 0;
-    for (int32_t a = 0; a < t->rank; ++a)
-        if (t->shape[a] > 1) idx[n++] = a;
-    std::sort(idx, idx + n, [&](int32_t x, int32_t y) { return t->strides[x] < t->strides[y]; });
-    int64_t span = 1;
-    for (int32_t i = 0; i < n; ++i) {
-        const int64_t s = t->strides[idx[i]];
-        if (s < span) return false;
-        span = s * t->shape[idx[i]];
-    }
-    return true;
-}
-
 int32_t build_problem(const chelis_gpu_tensor *a, const chelis_gpu_tensor *b, const chelis_gpu_tensor *c,
                       GemmProblem *p, const char *what) {
     int32_t s;

@@ -85,6 +85,83 @@ int32_t chelis_hip_softmax_adjoint(const chelis_gpu_tensor *y, const chelis_gpu_
 int32_t chelis_hip_layer_norm(const chelis_gpu_tensor *x, const chelis_gpu_tensor *gamma,
                               const chelis_gpu_tensor *beta, double epsilon, const chelis_gpu_tensor *y);
 
+/* ---- training and serving a block: norm, positions, windowed attention ----
+ * No counterparts in the reference. Inputs and results are f32, f64 (not
+ * window_attention), bf16 or f16; sums, statistics, scores and softmax
+ * weights are held in binary32 (binary64 for f64) and a 16-bit result is
+ * rounded once. Sums run in the kernels' own fixed order: the same bits on
+ * every run, not the canonical tree's. Results may not share storage with
+ * inputs unless said so. */
+
+/* layer_norm with the row statistics its gradient needs: y as
+ * chelis_hip_layer_norm (bit for bit at f32 and f64), mean and
+ * rstd = 1 / sqrt(variance + epsilon) contiguous over x's leading axes, f32
+ * (f64 beside f64 rows). gamma and beta have x's dtype, or are f32 beside
+ * 16-bit rows. y may be x. */
+int32_t chelis_hip_layer_norm_stats(const chelis_gpu_tensor *x, const chelis_gpu_tensor *gamma,
+                                    const chelis_gpu_tensor *beta, double epsilon, const chelis_gpu_tensor *y,
+                                    const chelis_gpu_tensor *mean, const chelis_gpu_tensor *rstd);
+/* Its gradients for the cotangent g, h = (x - mean) * rstd:
+ *   dx = rstd * (g gamma - avg(g gamma) - h * avg(g gamma h)) per row,
+ *   dgamma = sum over rows of g h, dbeta = sum over rows of g (of gamma's
+ * dtype; zero without rows). dx, or dgamma and dbeta together, may be NULL.
+ * dx may be g or x. */
+int32_t chelis_hip_layer_norm_adjoint(const chelis_gpu_tensor *x, const chelis_gpu_tensor *gamma,
+                                      const chelis_gpu_tensor *mean, const chelis_gpu_tensor *rstd,
+                                      const chelis_gpu_tensor *g, const chelis_gpu_tensor *dx,
+                                      const chelis_gpu_tensor *dgamma, const chelis_gpu_tensor *dbeta);
+
+/* Rotary positions over n_axes axes (1 to 8). xs: one or two [batch, heads,
+ * seq, width] views that differ at most in their heads (queries and keys),
+ * the last axis contiguous. The first 2 P elements of the width, P the sum of
+ * sections, are P pairs (p, P + p) for HALVES or (2p, 2p + 1) for ADJACENT;
+ * the first sections[0] pairs turn with axis 0's position, the next
+ * sections[1] with axis 1's, and so on: by the angle
+ * t = position * freqs[p] in binary64,
+ *   (u, v) -> (u cos t - v sin t, u sin t + v cos t).
+ * Elements past the pairs are copied. positions: i32 or i64 [n_axes, batch,
+ * seq], any strides; freqs: contiguous f64 [P]. ys may be xs. The adjoint
+ * turns the cotangents by -t. */
+enum { CHELIS_ROTARY_HALVES = 0, CHELIS_ROTARY_ADJACENT = 1 };
+int32_t chelis_hip_rotary(const chelis_gpu_tensor *const *xs, int32_t n, const chelis_gpu_tensor *positions,
+                          const chelis_gpu_tensor *freqs, const int64_t *sections, int32_t n_axes, int32_t pairing,
+                          const chelis_gpu_tensor *const *ys);
+int32_t chelis_hip_rotary_adjoint(const chelis_gpu_tensor *const *gs, int32_t n, const chelis_gpu_tensor *positions,
+                                  const chelis_gpu_tensor *freqs, const int64_t *sections, int32_t n_axes,
+                                  int32_t pairing, const chelis_gpu_tensor *const *dxs);
+
+/* Attention with a sliding window and always-visible first keys (sinks).
+ * q, o: [batch, heads, seq, width]; k, v: [batch, kv_heads, keys, width],
+ * heads a multiple of kv_heads (query head h reads key head
+ * h / (heads / kv_heads)); width a multiple of 8 up to 128; any strides with
+ * the last axis contiguous (k and v also with stride 0).
+ * Sequence b holds lengths[b] keys (NULL: all; taken into 0 .. keys), and its
+ * query row i stands at position starts[b] + i (NULL: the rows are its last
+ * ones, starts[b] = lengths[b] - seq: a prompt, a chunk of new tokens or one
+ * token at the end of a cache; zeros beside lengths: a training batch padded
+ * at its end). Row i sees key j when 0 <= j <= p < lengths[b] for its
+ * position p and (p - j < window or j < sinks);
+ *   o = softmax over the visible keys of (scale * q . k), times v,
+ *   lse = log of the sum of exp(scale * q . k) over them.
+ * A row that sees nothing gets o = 0 and lse = -inf. Keys past a length are
+ * not read, and a key that a row does not see adds nothing to it, whatever it
+ * holds. lse: contiguous f32 [batch, heads, seq], or NULL. lengths, starts:
+ * i32 or i64 [batch]. */
+int32_t chelis_hip_window_attention(const chelis_gpu_tensor *q, const chelis_gpu_tensor *k,
+                                    const chelis_gpu_tensor *v, const chelis_gpu_tensor *lengths,
+                                    const chelis_gpu_tensor *starts, int64_t window, int64_t sinks, double scale,
+                                    const chelis_gpu_tensor *o, const chelis_gpu_tensor *lse);
+/* Its gradients for the cotangent g of o, from the forward call's o and lse
+ * and the same lengths, starts, window, sinks and scale. dk and dv sum over
+ * the query heads of a key head and are zero at keys nothing sees; dq is zero
+ * at rows that see nothing. No atomics: the same bits on every run. */
+int32_t chelis_hip_window_attention_adjoint(const chelis_gpu_tensor *q, const chelis_gpu_tensor *k,
+                                            const chelis_gpu_tensor *v, const chelis_gpu_tensor *o,
+                                            const chelis_gpu_tensor *lse, const chelis_gpu_tensor *g,
+                                            const chelis_gpu_tensor *lengths, const chelis_gpu_tensor *starts,
+                                            int64_t window, int64_t sinks, double scale, const chelis_gpu_tensor *dq,
+                                            const chelis_gpu_tensor *dk, const chelis_gpu_tensor *dv);
+
 /* ---- fused elementwise chains (RiscOp::FusedElem, dag.rs:485-524,673-678) ----
  * A step's args index the chain inputs when >= 0, and a previous step k as
  * -(k + 1) (FusedInput::External / FusedInput::PreviousStep). The chain's
