@@ -220,14 +220,15 @@ struct Staged {
 
 // The key tiles that rows of positions first .. last see: those of the
 // sinks, then those of the window.
+template <int KEYS>
 struct KeyWalk {
     int count, sink_tiles, window_from;
     __device__ KeyWalk(int first, int last, int n, int window, int sinks) {
         last = min(last, n - 1);
         count = sink_tiles = window_from = 0;
         if (last < 0 || first >= n) return;
-        const int hi = last / kKeys, lo = max(0, first - window + 1) / kKeys;
-        sink_tiles = min((sinks + kKeys - 1) / kKeys, hi + 1);
+        const int hi = last / KEYS, lo = max(0, first - window + 1) / KEYS;
+        sink_tiles = min((sinks + KEYS - 1) / KEYS, hi + 1);
         window_from = max(sink_tiles, lo);
         count = sink_tiles + max(0, hi - window_from + 1);
     }
@@ -318,7 +319,7 @@ __global__ __launch_bounds__(kThreads, 2) void window_forward_kernel(WinArgs a) 
     f32x16 acc[D / 32] = {};
     float m = -INFINITY, l = 0.f;
     const int first = seq.start + mine, p = first + i, top = row < a.sq && p < seq.n ? p : -1, low = p - a.window;
-    const KeyWalk walk(seq.start + row0, seq.start + min(row0 + 32 * kWaves, a.sq) - 1, seq.n, a.window, a.sinks);
+    const KeyWalk<kKeys> walk(seq.start + row0, seq.start + min(row0 + 32 * kWaves, a.sq) - 1, seq.n, a.window, a.sinks);
     Staged<T, D, kKeys> ks, vs;
     if (walk.count) {
         ks.load(K, a.k.s, walk.tile(0) * kKeys, seq.n - 1, a.width, tid);
@@ -406,6 +407,211 @@ __global__ __launch_bounds__(kThreads, 2) void window_forward_kernel(WinArgs a) 
         a.lse[(b * a.heads + head) * a.sq + row] = empty ? -INFINITY : canon_bits((m - kShift<T> + log2f(l)) * kLn2);
 }
 
+// ---------------------------------------------------------------- few rows
+// A few rows over many keys (single tokens over a cache): the rows of every
+// query head that shares a key head are taken together, 32 to a task, and the
+// key blocks of a task are dealt to `splits` waves, each on its own: it keeps
+// its next 32 keys in flight in registers (a row of k per lane pair as the
+// products want it, v on its way to the wave's own LDS tile) and no wave
+// waits for another. Bound by the reads of k and v. With one split the wave
+// stores its rows; else it leaves their sums, maxima and unscaled results in
+// scratch and a second launch joins them in split order.
+struct SplitArgs {
+    float *part;  // per task, split and row: [width] results, then maxima and sums
+    float *stat;
+    int splits, rows, tiles, pack;  // rows of all heads of a group, row tiles, rows a part holds
+    int64_t tasks;
+};
+
+template <typename T, int D>
+__global__ __launch_bounds__(kThreads, 2) void window_split_kernel(WinArgs a, SplitArgs p) {
+    constexpr int N = 32;
+    __shared__ __attribute__((aligned(16))) T tiles[kWaves][N * kPitch<T, D>];
+    const int tid = threadIdx.x, lane = tid & 63, i = lane & 31, h = lane >> 5;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int64_t id = (int64_t)blockIdx.x * kWaves + wave, task = id / p.splits;
+    if (task >= p.tasks) return;
+    const int split = (int)(id % p.splits), rt = (int)(task % p.tiles);
+    const int64_t kvh = task / p.tiles % a.kv, b = task / p.tiles / a.kv;
+    const Seq seq(a, b);
+    const int r = rt * N + i, live = r < p.rows, rs = live ? r : 0;
+    const int64_t head = kvh * a.group + rs / a.sq;
+    const int row = rs % a.sq, pos = seq.start + row;
+    const T *Q = head_of<T>(a.q, b, head) + row * a.q.s, *K = head_of<T>(a.k, b, kvh), *V = head_of<T>(a.v, b, kvh);
+    V8<T> qf[D / 16];
+#pragma unroll
+    for (int s = 0; s < D / 16; ++s) {
+        qf[s] = row_part(Q, 16 * s + 8 * h, a.width, live);
+        if (a.flip) qf[s] = -qf[s];
+    }
+    // the tile's rows: one head's run of them, or all where it spans heads
+    const int last_row = min(rt * N + N, p.rows) - 1;
+    const bool one = rt * N / a.sq == last_row / a.sq;
+    const int first = seq.start + (one ? rt * N % a.sq : 0), last = seq.start + (one ? last_row % a.sq : a.sq - 1);
+    const int top = live && pos < seq.n ? pos : -1, low = pos - a.window;
+    const KeyWalk<N> walk(first, last, seq.n, a.window, a.sinks);
+    f32x16 acc[D / 32] = {};
+    float m = -INFINITY, l = 0.f;
+    T *tile = tiles[wave];
+    constexpr int PARTS = D / 16;  // 16-byte (f32: 32-byte) parts of a lane
+    V8<T> kf[PARTS], vf[PARTS];
+    auto load = [&](int t) {
+        const int k0 = walk.tile(t) * N;
+        const T *kr = K + min(k0 + i, seq.n - 1) * a.k.s;
+#pragma unroll
+        for (int s = 0; s < PARTS; ++s) {
+            const int at = 16 * s + 8 * h;
+            Pack<T, 8> q;
+            q.load_streamed(kr + (at < a.width ? at : 0));
+            kf[s] = q.q;
+        }
+#pragma unroll
+        for (int s = 0; s < PARTS; ++s) {
+            const int part = lane + 64 * s, at = part % (D / 8) * 8;
+            Pack<T, 8> q;
+            q.load_streamed(V + min(k0 + part / (D / 8), seq.n - 1) * a.v.s + (at < a.width ? at : 0));
+            vf[s] = q.q;
+        }
+    };
+    if (split < walk.count) load(split);
+    for (int t = split; t < walk.count; t += p.splits) {
+        const int k0 = walk.tile(t) * N;
+        f32x16 s = {};
+#pragma unroll
+        for (int u = 0; u < D / 16; ++u) s = mma(kf[u], qf[u], s);
+#pragma unroll
+        for (int u = 0; u < PARTS; ++u) {
+            const int part = lane + 64 * u;
+            *reinterpret_cast<V8<T> *>(tile + part / (D / 8) * kPitch<T, D> + part % (D / 8) * 8) = vf[u];
+        }
+        if (t + p.splits < walk.count) load(t + p.splits);
+        const bool all = k0 + N - 1 <= first && last < seq.n && (k0 > last - a.window || k0 + N - 1 < a.sinks);
+        uint32_t seen = 0xffffu;
+        if (!all) {
+            seen = 0;
+            const SeenKeys keys(top, low, a.sinks, k0, h);
+#pragma unroll
+            for (int c = 0; c < 16; ++c) {
+                const bool vis = keys(c);
+                seen |= (uint32_t)vis << c;
+                s[c] = vis ? s[c] : -INFINITY;
+            }
+        }
+        float mx = -INFINITY;
+#pragma unroll
+        for (int c = 0; c < 16; ++c) mx = fmaxf(mx, s[c]);
+        mx = fmaxf(mx, other_half(mx)) * a.c;
+        const float m_new = fmaxf(m, mx), ref = m_new == -INFINITY ? 0.f : m_new;
+        const float alpha = exp2_(m - ref), off = kShift<T> - ref;
+        m = m_new;
+        float sum = 0.f;
+#pragma unroll
+        for (int c = 0; c < 16; ++c) {
+            const float e = exp2_(fmaf(s[c], a.c, off));
+            s[c] = (seen >> c) & 1 ? e : 0.f;
+            sum += s[c];
+        }
+        l = l * alpha + sum;
+#pragma unroll
+        for (int d = 0; d < D / 32; ++d) acc[d] *= alpha;
+#pragma unroll
+        for (int kc = 0; kc < 2; ++kc) {
+            const V8<T> pf = rounded<T>(s, 8 * kc);
+#pragma unroll
+            for (int d = 0; d < D / 32; ++d) {
+                const V8<T> vt = across<T, D>(tile, 16 * kc, 32 * d, lane);
+                acc[d] = all ? mma(vt, pf, acc[d]) : mma_hidden<false, T>(vt, pf, (seen >> (8 * kc)) & 0xff, acc[d]);
+            }
+        }
+    }
+    l += other_half(l);
+    if (!live) return;
+    if (p.splits > 1) {
+        const int64_t at = (task * p.splits + split) * p.pack + i;
+        float *out = p.part + at * a.width;
+#pragma unroll
+        for (int d = 0; d < D / 32; ++d)
+#pragma unroll
+            for (int c = 0; c < 16; c += 4) {
+                const int e = 32 * d + 2 * c + 4 * h;
+                if (e < a.width) *reinterpret_cast<f32x4 *>(out + e) = f32x4{acc[d][c], acc[d][c + 1], acc[d][c + 2], acc[d][c + 3]};
+            }
+        if (h == 0) {
+            p.stat[2 * at] = m;
+            p.stat[2 * at + 1] = l;
+        }
+        return;
+    }
+    const bool empty = top < 0;
+    const float inv = empty ? 0.f : 1.f / l;
+    T *O = const_cast<T *>(head_of<T>(a.o, b, head)) + row * a.o.s;
+#pragma unroll
+    for (int d = 0; d < D / 32; ++d) store_column(O, acc[d], 32 * d, a.width, h, inv);
+    if (a.lse && h == 0)
+        a.lse[(b * a.heads + head) * a.sq + row] = empty ? -INFINITY : canon_bits((m - kShift<T> + log2f(l)) * kLn2);
+}
+
+// One row a workgroup: the splits' results under their common maximum, every
+// eighth (or sixteenth) split to a group of threads, the groups joined in
+// order. (One wave walking the splits one after another took 24 us for the 35
+// splits of a single token over 1024 keys, the loads' latency each time.)
+constexpr int kMaxSplits = 2048;
+
+template <typename T, int D>
+__global__ __launch_bounds__(kThreads) void window_join_kernel(WinArgs a, SplitArgs p) {
+    constexpr int LANES = D / 4, GROUPS = kThreads / LANES;
+    __shared__ float weight[kMaxSplits], waves[2][kWaves];
+    __shared__ f32x4 join[GROUPS][LANES];
+    const int64_t id = blockIdx.x, row = id % a.sq, bh = id / a.sq, b = bh / a.heads, head = bh % a.heads;
+    const int tid = threadIdx.x, r = (int)(head % a.group * a.sq + row);
+    const int64_t task = (b * a.kv + head / a.group) * p.tiles + r / 32, at = task * p.splits * p.pack + r % 32;
+    const int lane = tid % LANES, group = tid / LANES;
+    const bool own = group < GROUPS && 4 * lane < a.width;
+    float m = -INFINITY;
+    for (int s = tid; s < p.splits; s += kThreads) {
+        weight[s] = p.stat[2 * (at + (int64_t)s * p.pack)];
+        m = fmaxf(m, weight[s]);
+    }
+    m = wave_vmax(m);
+    if ((tid & 63) == 0) waves[0][tid >> 6] = m;
+    __syncthreads();
+    m = fmaxf(fmaxf(waves[0][0], waves[0][1]), fmaxf(waves[0][2], waves[0][3]));
+    const float ref = m == -INFINITY ? 0.f : m;
+    float l = 0.f;
+    for (int s = tid; s < p.splits; s += kThreads) {
+        const float f = exp2_(weight[s] - ref);
+        weight[s] = f;
+        l = fmaf(f, p.stat[2 * (at + (int64_t)s * p.pack) + 1], l);
+    }
+    l = wave_tree_sum(l);
+    if ((tid & 63) == 0) waves[1][tid >> 6] = l;
+    __syncthreads();
+    l = (waves[1][0] + waves[1][1]) + (waves[1][2] + waves[1][3]);
+    f32x4 x = {};
+    if (own) {
+        const float *part = p.part + at * a.width + 4 * lane;
+#pragma unroll 4
+        for (int s = group; s < p.splits; s += GROUPS)
+            x += weight[s] * *reinterpret_cast<const f32x4 *>(part + (int64_t)s * p.pack * a.width);
+        join[group][lane] = x;
+    }
+    __syncthreads();
+    const Seq seq(a, b);
+    const int pos = seq.start + (int)row;
+    const bool empty = pos < 0 || pos >= seq.n;
+    if (own && group == 0) {
+#pragma unroll
+        for (int k = 1; k < GROUPS; ++k) x += join[k][lane];
+        const float inv = empty ? 0.f : 1.f / l;
+        Pack<T, 4> out;
+#pragma unroll
+        for (int t = 0; t < 4; ++t) out.set(t, x[t] * inv);
+        out.store(const_cast<T *>(head_of<T>(a.o, b, head)) + row * a.o.s + 4 * lane);
+    }
+    if (a.lse && tid == 0)
+        a.lse[id] = empty ? -INFINITY : canon_bits((m - kShift<T> + log2f(l)) * kLn2);
+}
+
 // ---------------------------------------------------------------- backward
 // f16 holds dS times a power of two that brings its largest possible value,
 // 2 max|g| max|v| width, just under f16's: gradients of any size keep their
@@ -491,7 +697,7 @@ __global__ __launch_bounds__(kThreads, 2) void window_dq_kernel(WinArgs a) {
     const float lse = a.lse_in[stat] * kLog2e, up = gradient_scale<T>(a);
     f32x16 acc[D / 32] = {};
     const int first = seq.start + mine, p = first + i, top = row < a.sq && p < seq.n ? p : -1, low = p - a.window;
-    const KeyWalk walk(seq.start + row0, seq.start + min(row0 + 32 * kWaves, a.sq) - 1, seq.n, a.window, a.sinks);
+    const KeyWalk<kKeys> walk(seq.start + row0, seq.start + min(row0 + 32 * kWaves, a.sq) - 1, seq.n, a.window, a.sinks);
     Staged<T, D, kKeys> ks, vs;
     if (walk.count) {
         ks.load(K, a.k.s, walk.tile(0) * kKeys, seq.n - 1, a.width, tid);
@@ -549,11 +755,105 @@ __global__ __launch_bounds__(kThreads, 2) void window_dq_kernel(WinArgs a) {
     for (int d = 0; d < D / 32; ++d) store_column(DQ, acc[d], 32 * d, a.width, h, a.scale / up);
 }
 
-// dk and dv: a workgroup takes 128 keys of one key head, each wave 32 of
-// them, and walks the rows that see any of them, of every query head of the
-// group.
+// dk and dv. A wave holds 32 keys of one key head and takes tiles of 32 query
+// rows, staged in LDS with their lse and D.
 template <typename T, int D>
-__global__ __launch_bounds__(kThreads, 1) void window_dkv_kernel(WinArgs a) {
+struct KeyGradients {
+    V8<T> kf[D / 16], vf[D / 16];
+    f32x16 dk[D / 32] = {}, dv[D / 32] = {};
+    // columns of keys past the sequence are zero
+    __device__ void load(const WinArgs &a, int64_t b, int64_t kvh, int key, int n, int h) {
+        const T *K = head_of<T>(a.k, b, kvh), *V = head_of<T>(a.v, b, kvh);
+        const int64_t at = key < n ? key : 0;
+#pragma unroll
+        for (int s = 0; s < D / 16; ++s) {
+            kf[s] = n > 0 ? row_part(K + at * a.k.s, 16 * s + 8 * h, a.width, key < n) : V8<T>{};
+            if (a.flip) kf[s] = -kf[s];
+            vf[s] = n > 0 ? row_part(V + at * a.v.s, 16 * s + 8 * h, a.width, key < n) : V8<T>{};
+        }
+    }
+    // Ls holds shift - lse log2(e), Ds the rows' D; half scales dS.
+    __device__ void tile(const T *Qs, const T *Gs, const float *Ls, const float *Ds, float c, float half, bool all,
+                         const SeenRows &rows, int lane) {
+        const int i = lane & 31, h = lane >> 5;
+        f32x16 s = {}, dp = {};
+#pragma unroll
+        for (int u = 0; u < D / 16; ++u) {
+            s = mma(along<T, D>(Qs, i, 16 * u + 8 * h), kf[u], s);
+            dp = mma(along<T, D>(Gs, i, 16 * u + 8 * h), vf[u], dp);
+        }
+#pragma unroll
+        for (int r4 = 0; r4 < 4; ++r4) {
+            const f32x4 lr = *reinterpret_cast<const f32x4 *>(Ls + 8 * r4 + 4 * h);
+            const f32x4 dr = *reinterpret_cast<const f32x4 *>(Ds + 8 * r4 + 4 * h);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const int r = 4 * r4 + j;
+                const float p = exp2_(fmaf(s[r], c, lr[j]));
+                s[r] = p;
+                dp[r] = p * ((dp[r] - dr[j]) * half);
+            }
+        }
+        uint32_t seen = 0xffffu;
+        if (!all) {
+            seen = 0;
+#pragma unroll
+            for (int r = 0; r < 16; ++r) {
+                const bool vis = rows(r);
+                seen |= (uint32_t)vis << r;
+                s[r] = vis ? s[r] : 0.f;
+                dp[r] = vis ? dp[r] : 0.f;
+            }
+        }
+#pragma unroll
+        for (int kc = 0; kc < 2; ++kc) {
+            const V8<T> pf = rounded<T>(s, 8 * kc), df = rounded<T>(dp, 8 * kc);
+            const uint32_t bits = (seen >> (8 * kc)) & 0xff;
+#pragma unroll
+            for (int d = 0; d < D / 32; ++d) {
+                const V8<T> gf = across<T, D>(Gs, 16 * kc, 32 * d, lane), qf = across<T, D>(Qs, 16 * kc, 32 * d, lane);
+                dv[d] = all ? mma(gf, pf, dv[d]) : mma_hidden<false, T>(gf, pf, bits, dv[d]);
+                dk[d] = all ? mma(qf, df, dk[d]) : mma_hidden<true, T>(qf, df, bits, dk[d]);
+            }
+        }
+    }
+};
+
+// Rows far behind the window see the sinks alone. A workgroup of keys would
+// walk all of them (one workgroup of 128 keys walking 8192 rows of four heads
+// took 3.8 ms beside 0.2 ms for the others), so they are dealt to waves of
+// their own, `splits` of them to each block of 32 sink keys. Such a block's
+// sums are then unscaled parts in scratch: part 0 from the near rows, the
+// others from the far waves, joined in order by a last launch.
+struct FarArgs {
+    float *part;  // [block][1 + splits][dk, dv][32 keys][width]; null: no far rows
+    int splits, blocks;
+    __device__ float *at(int64_t pair, int block, int part_index, int width) const {
+        return part + ((pair * blocks + block) * (1 + splits) + part_index) * 64 * width;
+    }
+};
+
+// First position whose rows are far for the workgroup of keys from tile0.
+__device__ inline int far_from(int tile0, int window) { return tile0 + 32 * kWaves - 1 + window; }
+
+template <typename T, int D>
+__device__ inline void store_part(float *part, const KeyGradients<T, D> &w, int i, int h, int width, bool keep) {
+#pragma unroll
+    for (int d = 0; d < D / 32; ++d)
+#pragma unroll
+        for (int r = 0; r < 16; r += 4) {
+            const int e = 32 * d + 2 * r + 4 * h;
+            if (e >= width) continue;
+            const f32x16 &k = w.dk[d], &v = w.dv[d];
+            f32x4 x = {k[r], k[r + 1], k[r + 2], k[r + 3]}, y = {v[r], v[r + 1], v[r + 2], v[r + 3]};
+            *reinterpret_cast<f32x4 *>(part + i * width + e) = keep ? x : f32x4{};
+            *reinterpret_cast<f32x4 *>(part + (32 + i) * width + e) = keep ? y : f32x4{};
+        }
+}
+
+// The near rows: a workgroup takes 128 keys, its waves share the row tiles.
+template <typename T, int D>
+__global__ __launch_bounds__(kThreads, 1) void window_dkv_kernel(WinArgs a, FarArgs f) {
     __shared__ __attribute__((aligned(16))) T Qs[kRows * kPitch<T, D>], Gs[kRows * kPitch<T, D>];
     __shared__ __attribute__((aligned(16))) float Ls[kRows], Ds[kRows];
     const int tid = threadIdx.x, lane = tid & 63, i = lane & 31, h = lane >> 5;
@@ -561,22 +861,15 @@ __global__ __launch_bounds__(kThreads, 1) void window_dkv_kernel(WinArgs a) {
     const int64_t b = blockIdx.z, kvh = blockIdx.y;
     const Seq seq(a, b);
     const int tile0 = blockIdx.x * (32 * kWaves), mine = tile0 + 32 * wave, key = mine + i;
-    const bool have = key < seq.n;
-    const T *K = head_of<T>(a.k, b, kvh), *V = head_of<T>(a.v, b, kvh);
-    V8<T> kf[D / 16], vf[D / 16];
-#pragma unroll
-    for (int s = 0; s < D / 16; ++s) {
-        kf[s] = have ? row_part(K + key * a.k.s, 16 * s + 8 * h, a.width, true) : V8<T>{};
-        if (a.flip) kf[s] = -kf[s];
-        vf[s] = have ? row_part(V + key * a.v.s, 16 * s + 8 * h, a.width, true) : V8<T>{};
-    }
+    KeyGradients<T, D> w;
+    w.load(a, b, kvh, key, seq.n, h);
     const float up = gradient_scale<T>(a), half = up * exp2_(-kShift<T>);
-    f32x16 dk[D / 32] = {}, dv[D / 32] = {};
-    // rows first .. last see some key of the tile
-    const int64_t end = tile0 < a.sinks ? kMaxExtent * 2 : (int64_t)tile0 + 32 * kWaves - 1 + a.window - 1;
+    // rows lo .. rows - 1 see some key of the tile
+    const int64_t end = tile0 < a.sinks && !f.part ? 2 * kMaxExtent : far_from(tile0, a.window);
     const int lo = max(0, tile0 - seq.start);
-    const int hi = (int)min(min((int64_t)a.sq - 1, (int64_t)seq.n - 1 - seq.start), end - seq.start);
-    const int from = lo / kRows, tiles = hi < lo || tile0 >= seq.n ? 0 : hi / kRows - from + 1, items = tiles * a.group;
+    const int rows = (int)min(min((int64_t)a.sq, (int64_t)seq.n - seq.start), end - seq.start);
+    const int from = lo / kRows, tiles = rows <= lo || tile0 >= seq.n ? 0 : (rows - 1) / kRows - from + 1;
+    const int items = tiles * a.group;
     Staged<T, D, kRows> qs, gs;
     float ls = 0.f, ds = 0.f;
     auto load = [&](int t) {
@@ -602,57 +895,101 @@ __global__ __launch_bounds__(kThreads, 1) void window_dkv_kernel(WinArgs a) {
         }
         __syncthreads();
         if (t + 1 < items) load(t + 1);
-        const Sight see = sight(seq.start + r0, min(kRows, a.sq - r0), seq.n, a.window, a.sinks, mine, 32);
+        const Sight see = sight(seq.start + r0, rows - r0, seq.n, a.window, a.sinks, mine, 32);
         if (see == kNone) continue;
-        f32x16 s = {}, dp = {};
-#pragma unroll
-        for (int u = 0; u < D / 16; ++u) {
-            s = mma(along<T, D>(Qs, i, 16 * u + 8 * h), kf[u], s);
-            dp = mma(along<T, D>(Gs, i, 16 * u + 8 * h), vf[u], dp);
-        }
-        uint32_t seen = 0xffffu;
-#pragma unroll
-        for (int r4 = 0; r4 < 4; ++r4) {
-            const f32x4 lr = *reinterpret_cast<const f32x4 *>(Ls + 8 * r4 + 4 * h);
-            const f32x4 dr = *reinterpret_cast<const f32x4 *>(Ds + 8 * r4 + 4 * h);
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                const int r = 4 * r4 + j;
-                const float p = exp2_(fmaf(s[r], a.c, lr[j]));
-                s[r] = p;
-                dp[r] = p * ((dp[r] - dr[j]) * half);
-            }
-        }
-        if (see == kSome) {
-            seen = 0;
-            const SeenRows rows(key, seq.start, r0, h, a.sq, seq.n, a.window, a.sinks);
-#pragma unroll
-            for (int r = 0; r < 16; ++r) {
-                const bool vis = rows(r);
-                seen |= (uint32_t)vis << r;
-                s[r] = vis ? s[r] : 0.f;
-                dp[r] = vis ? dp[r] : 0.f;
-            }
-        }
-#pragma unroll
-        for (int kc = 0; kc < 2; ++kc) {
-            const V8<T> pf = rounded<T>(s, 8 * kc), df = rounded<T>(dp, 8 * kc);
-            const uint32_t bits = (seen >> (8 * kc)) & 0xff;
-#pragma unroll
-            for (int d = 0; d < D / 32; ++d) {
-                const V8<T> gf = across<T, D>(Gs, 16 * kc, 32 * d, lane), qf = across<T, D>(Qs, 16 * kc, 32 * d, lane);
-                dv[d] = see == kAll ? mma(gf, pf, dv[d]) : mma_hidden<false, T>(gf, pf, bits, dv[d]);
-                dk[d] = see == kAll ? mma(qf, df, dk[d]) : mma_hidden<true, T>(qf, df, bits, dk[d]);
-            }
-        }
+        w.tile(Qs, Gs, Ls, Ds, a.c, half, see == kAll, SeenRows(key, seq.start, r0, h, rows, seq.n, a.window, a.sinks), lane);
+    }
+    if (f.part && mine < a.sinks) {
+        store_part(f.at(b * a.kv + kvh, mine / 32, 0, a.width), w, i, h, a.width, true);
+        return;
     }
     if (key >= a.sk) return;
     T *DK = const_cast<T *>(head_of<T>(a.dk, b, kvh)) + key * a.dk.s, *DV = const_cast<T *>(head_of<T>(a.dv, b, kvh)) + key * a.dv.s;
 #pragma unroll
     for (int d = 0; d < D / 32; ++d) {
-        store_column(DK, dk[d], 32 * d, a.width, h, a.scale / up);
-        store_column(DV, dv[d], 32 * d, a.width, h, exp2_(-kShift<T>));
+        store_column(DK, w.dk[d], 32 * d, a.width, h, a.scale / up);
+        store_column(DV, w.dv[d], 32 * d, a.width, h, exp2_(-kShift<T>));
     }
+}
+
+// The far rows of one block of sink keys: every `splits`-th tile to a wave,
+// which stages it for itself.
+template <typename T, int D>
+__global__ __launch_bounds__(kThreads, 1) void window_far_kernel(WinArgs a, FarArgs f) {
+    __shared__ __attribute__((aligned(16))) T tiles[kWaves][2][kRows * kPitch<T, D>];
+    __shared__ __attribute__((aligned(16))) float stats[kWaves][2][kRows];
+    const int tid = threadIdx.x, lane = tid & 63, i = lane & 31, h = lane >> 5;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const float up = gradient_scale<T>(a), half = up * exp2_(-kShift<T>);
+    const int64_t b = blockIdx.z / f.blocks, kvh = blockIdx.y;
+    const int block = blockIdx.z % f.blocks, split = blockIdx.x * kWaves + wave;
+    if (split >= f.splits) return;
+    const Seq seq(a, b);
+    const int key = block * 32 + i;
+    KeyGradients<T, D> w;
+    w.load(a, b, kvh, key, seq.n, h);
+    const int from = max(0, far_from(block / kWaves * 32 * kWaves, a.window) - seq.start);
+    const int rows = min(a.sq, seq.n - seq.start), count = rows > from ? (rows - from + kRows - 1) / kRows : 0;
+    T *Qs = tiles[wave][0], *Gs = tiles[wave][1];
+    float *Ls = stats[wave][0], *Ds = stats[wave][1];
+    constexpr int PARTS = D / 16;
+    V8<T> qr[PARTS], gr[PARTS];
+    float ls = 0.f;
+    auto load = [&](int t) {
+        const int64_t head = kvh * a.group + t / count;
+        const int r0 = from + t % count * kRows;
+        const T *Q = head_of<T>(a.q, b, head), *G = head_of<T>(a.g, b, head);
+#pragma unroll
+        for (int s = 0; s < PARTS; ++s) {
+            const int part = lane + 64 * s, at = part % (D / 8) * 8, r = min(r0 + part / (D / 8), a.sq - 1);
+            Pack<T, 8> x, y;
+            x.load(Q + r * a.q.s + (at < a.width ? at : 0));
+            y.load(G + r * a.g.s + (at < a.width ? at : 0));
+            qr[s] = x.q;
+            gr[s] = y.q;
+        }
+        const int64_t stat = (b * a.heads + head) * a.sq + min(r0 + i, a.sq - 1);
+        ls = h ? a.delta[stat] : kShift<T> - a.lse_in[stat] * kLog2e;
+    };
+    const int items = count * a.group;
+    if (split < items) load(split);
+    for (int t = split; t < items; t += f.splits) {
+        const int r0 = from + t % count * kRows;
+#pragma unroll
+        for (int s = 0; s < PARTS; ++s) {
+            const int part = lane + 64 * s, at = part / (D / 8) * kPitch<T, D> + part % (D / 8) * 8;
+            *reinterpret_cast<V8<T> *>(Qs + at) = qr[s];
+            *reinterpret_cast<V8<T> *>(Gs + at) = gr[s];
+        }
+        (h ? Ds : Ls)[i] = ls;
+        if (t + f.splits < items) load(t + f.splits);
+        // the wave alone writes and reads its tile
+        __builtin_amdgcn_wave_barrier();
+        w.tile(Qs, Gs, Ls, Ds, a.c, half, r0 + kRows <= rows,
+               SeenRows(key, seq.start, r0, h, rows, seq.n, a.window, key + 1), lane);
+        __builtin_amdgcn_wave_barrier();
+    }
+    store_part(f.at(b * a.kv + kvh, block, 1 + split, a.width), w, i, h, a.width, key < a.sinks);
+}
+
+// Four keys of a sink block, dk and dv.
+template <typename T>
+__global__ __launch_bounds__(kThreads) void window_sinks_kernel(WinArgs a, FarArgs f) {
+    const float up = gradient_scale<T>(a);
+    const int64_t b = blockIdx.z / f.blocks, kvh = blockIdx.y;
+    const int block = blockIdx.z % f.blocks, lane = threadIdx.x & 31, which = threadIdx.x >> 5 & 1;
+    const int i = blockIdx.x * 4 + (threadIdx.x >> 6), key = block * 32 + i;
+    if (4 * lane >= a.width || key >= a.sk) return;
+    const float *part = f.at(b * a.kv + kvh, block, 0, a.width) + (32 * which + i) * a.width + 4 * lane;
+    f32x4 x = {};
+#pragma unroll 8
+    for (int s = 0; s <= f.splits; ++s) x += *reinterpret_cast<const f32x4 *>(part + (int64_t)s * 64 * a.width);
+    const View &out = which ? a.dv : a.dk;
+    const float scale = which ? exp2_(-kShift<T>) : a.scale / up;
+    Pack<T, 4> y;
+#pragma unroll
+    for (int t = 0; t < 4; ++t) y.set(t, x[t] * scale);
+    y.store(const_cast<T *>(head_of<T>(out, b, kvh)) + key * out.s + 4 * lane);
 }
 
 // ---------------------------------------------------------------- dispatch
@@ -751,6 +1088,42 @@ int32_t check_result(const chelis_gpu_tensor *t, const char *name, std::initiali
     return CHELIS_HIP_OK;
 }
 
+// Rows that fill a wave's 32 columns badly in tiles of one head: taken
+// together over the heads of a group.
+bool few_rows(const WinArgs &a) { return a.sq <= 32; }
+
+int32_t window_split(const WinArgs &a, chelis_dtype dt, int64_t batch, hipStream_t st, const char *what) {
+    SplitArgs p{};
+    p.rows = a.group * a.sq;
+    p.tiles = (p.rows + 31) / 32;
+    p.pack = std::min(p.rows, 32);
+    p.tasks = batch * a.kv * p.tiles;
+    // key blocks a task can see; eight waves a compute unit, a block each at least
+    const int64_t span = std::min<int64_t>(a.sk, (int64_t)a.window + a.sq - 1) / 32 + 2 + (a.sinks + 31) / 32;
+    const int64_t blocks = std::max<int64_t>(1, std::min<int64_t>((a.sk + 31) / 32, span));
+    p.splits = (int)std::min<int64_t>(std::min<int64_t>(blocks, kMaxSplits), std::max<int64_t>(1, 8 * (int64_t)device_cus() / p.tasks));
+    const int64_t grid = (p.tasks * p.splits + kWaves - 1) / kWaves, parts = p.tasks * p.splits * p.pack;
+    const int64_t rows = batch * a.heads * a.sq;
+    if (!grid_fits(grid, kThreads) || !grid_fits(rows, kThreads))
+        return set_error(CHELIS_HIP_EUNSUPPORTED, "%s: grid too large", what);
+    const size_t bytes = p.splits > 1 ? (size_t)parts * (a.width + 2) * sizeof(float) : 0;
+    if (bytes) {
+        p.part = static_cast<float *>(scratch_alloc(bytes));
+        if (!p.part) return set_error(CHELIS_HIP_EHIP, "%s: scratch of %zu bytes", what, bytes);
+        p.stat = p.part + parts * a.width;
+    }
+    const int32_t s = with_head(dt, a.width, [&](auto t, auto d) -> int32_t {
+        using T = decltype(t);
+        window_split_kernel<T, d><<<(unsigned)grid, kThreads, 0, st>>>(a, p);
+        if (bytes) window_join_kernel<T, d><<<(unsigned)rows, kThreads, 0, st>>>(a, p);
+        return CHELIS_HIP_OK;
+    });
+    const hipError_t e = hipGetLastError();
+    scratch_free(p.part, bytes);
+    if (e != hipSuccess) return set_error(CHELIS_HIP_EHIP, "kernel launch: %s", hipGetErrorString(e));
+    return s;
+}
+
 }  // namespace
 }  // namespace chelis
 
@@ -773,6 +1146,7 @@ extern "C" int32_t chelis_hip_window_attention(const chelis_gpu_tensor *q, const
     if (!q->count) return CHELIS_HIP_OK;
     hipStream_t st = stream();
     if (!st) return set_error(CHELIS_HIP_EHIP, "no HIP device");
+    if (few_rows(a)) return window_split(a, q->dtype, q->shape[0], st, what);
     const dim3 grid((a.sq + 127) / 128, a.heads, (unsigned)q->shape[0]);
     if (!grid_fits(grid.x, kThreads)) return set_error(CHELIS_HIP_EUNSUPPORTED, "%s: grid too large", what);
     return with_head(q->dtype, a.width, [&](auto t, auto d) -> int32_t {
@@ -807,18 +1181,36 @@ extern "C" int32_t chelis_hip_window_attention_adjoint(
     const dim3 keys((a.sk + 127) / 128, a.kv, (unsigned)q->shape[0]);
     if (!grid_fits(rows.x, kThreads) || !grid_fits(keys.x, kThreads))
         return set_error(CHELIS_HIP_EUNSUPPORTED, "%s: grid too large", what);
-    const size_t bytes = (2 * kRanges + (size_t)lse->count) * sizeof(float);
+    // rows far behind the window of the first keys: dealt out 16 tiles to a
+    // wave, over no more waves than fill the device twice
+    FarArgs f{};
+    const int64_t pairs = q->shape[0] * a.kv, far = (int64_t)a.sk - (32 * kWaves - 1) - a.window;
+    if (a.sinks > 0 && q->count && far > 0) {
+        f.blocks = (a.sinks + 31) / 32;
+        const int64_t tiles = (std::min<int64_t>(far, a.sq) + kRows - 1) / kRows * a.group;
+        f.splits = (int)std::max<int64_t>(1, std::min<int64_t>((tiles + 15) / 16, 8 * (int64_t)device_cus() / (pairs * f.blocks)));
+        if (q->shape[0] * f.blocks > 65535)
+            return set_error(CHELIS_HIP_EUNSUPPORTED, "%s: sequences times sink blocks past 65535", what);
+    }
+    const size_t parts = f.blocks ? (size_t)pairs * f.blocks * (1 + f.splits) * 64 * a.width : 0;
+    const size_t bytes = (2 * kRanges + parts + (size_t)lse->count) * sizeof(float);
     a.range = static_cast<float *>(scratch_alloc(bytes));
-    a.delta = a.range + 2 * kRanges;
     if (!a.range) return set_error(CHELIS_HIP_EHIP, "%s: scratch of %zu bytes", what, bytes);
+    f.part = parts ? a.range + 2 * kRanges : nullptr;
+    a.delta = a.range + 2 * kRanges + parts;
     s = with_head(q->dtype, a.width, [&](auto t, auto d) -> int32_t {
         using T = decltype(t);
         if constexpr (std::is_same<T, _Float16>::value) {
             window_range_kernel<T, false><<<kRanges, 256, 0, st>>>(a, q->count / 8, a.range);
             window_range_kernel<T, true><<<kRanges, 256, 0, st>>>(a, k->count / 8, a.range + kRanges);
         }
-        if (q->count) window_dq_kernel<decltype(t), d><<<rows, kThreads, 0, st>>>(a);
-        if (k->count) window_dkv_kernel<decltype(t), d><<<keys, kThreads, 0, st>>>(a);
+        if (q->count) window_dq_kernel<T, d><<<rows, kThreads, 0, st>>>(a);
+        if (k->count) window_dkv_kernel<T, d><<<keys, kThreads, 0, st>>>(a, f);
+        if (parts) {
+            const unsigned z = (unsigned)(q->shape[0] * f.blocks);
+            window_far_kernel<T, d><<<dim3((f.splits + kWaves - 1) / kWaves, a.kv, z), kThreads, 0, st>>>(a, f);
+            window_sinks_kernel<T><<<dim3(8, a.kv, z), kThreads, 0, st>>>(a, f);
+        }
         return CHELIS_HIP_OK;
     });
     const hipError_t e = hipGetLastError();
