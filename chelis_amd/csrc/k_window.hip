@@ -105,39 +105,89 @@ __device__ inline bool not_finite(T v) {
     }
 }
 
-// c += a . b where b (weights of pairs, eight of them with their visible
-// ones in `seen`) is zero at hidden pairs. A hidden pair adds nothing, also
-// where a holds an infinity or a NaN: those elements are taken out of the
-// product, and what they add at visible pairs is found by counting. With
-// SIGNED weights the count stands for NaN, else (weights >= 0) infinities
-// keep their sign.
-template <bool SIGNED, typename T>
-__device__ inline f32x16 mma_hidden(V8<T> a, V8<T> b, uint32_t seen, f32x16 c) {
-    bool bad = false;
-#pragma unroll
-    for (int t = 0; t < 8; ++t) bad |= not_finite(a[t]);
-    if (!__any(bad)) return mma(a, b, c);
-    V8<T> part, vis;
-#pragma unroll
-    for (int t = 0; t < 8; ++t) {
-        part[t] = not_finite(a[t]) ? (T)0.f : a[t];
-        vis[t] = (T)((seen >> t) & 1 ? 1.f : 0.f);
+// A hidden pair adds nothing, whatever it holds: its weight is 0, but 0 times
+// an infinity or a NaN would be NaN. Tiles that some row or key does not see
+// whole are looked over while they are staged; where one holds such an
+// element, the pairs that see it get it added by themselves (add_special) and
+// the tile is cleaned before its product. Rarely run.
+template <typename T>
+struct Largest {
+    using U = std::conditional_t<sizeof(T) == 2, uint16_t, uint32_t>;
+    static constexpr U kInf = sizeof(T) == 4 ? (U)0x7f800000u : std::is_same<T, _Float16>::value ? (U)0x7c00 : (U)0x7f80;
+    V8<U> m = {};
+    __device__ void add(V8<T> v) {
+        m = __builtin_elementwise_max(m, __builtin_bit_cast(V8<U>, v) & (U)~((U)1 << (8 * sizeof(U) - 1)));
     }
-    c = mma(part, b, c);
+    __device__ bool special() const {
+        bool any = false;
+#pragma unroll
+        for (int t = 0; t < 8; ++t) any |= m[t] >= kInf;
+        return any;
+    }
+};
+
+// Adds the infinities and NaN of tile rows that `sees` holds for to the
+// accumulated columns of weights >= 0.
+template <typename T, int D, int N, class Sees>
+__device__ inline void add_special(f32x16 (&acc)[D / 32], const T *tile, int h, Sees sees) {
 #pragma unroll 1
-    for (int k = 0; k < 3; ++k) {  // NaN, +inf, -inf
+    for (int row = 0; row < N; ++row) {
+        const bool seen = sees(row);
 #pragma unroll
-        for (int t = 0; t < 8; ++t) {
-            const int kind = SIGNED || a[t] != a[t] ? 0 : a[t] > (T)0.f ? 1 : 2;
-            part[t] = (T)(not_finite(a[t]) && kind == k ? 1.f : 0.f);
-        }
-        const f32x16 found = mma(part, vis, f32x16{});
-        const float adds = k == 0 ? __builtin_nanf("") : k == 1 ? INFINITY : -INFINITY;
+        for (int d = 0; d < D / 32; ++d)
 #pragma unroll
-        for (int r = 0; r < 16; ++r)
-            if (found[r] > 0.f) c[r] += adds;
+            for (int r = 0; r < 16; ++r) {
+                const T x = tile[row * kPitch<T, D> + 32 * d + 8 * (r >> 2) + 4 * h + (r & 3)];
+                acc[d][r] += (seen & not_finite(x)) ? widen<T>(x) : 0.f;
+            }
     }
-    return c;
+}
+// The same as marks, one bit an accumulated element, for kernels whose
+// accumulators only the matrix cores touch while they run (touching them here
+// made the compiler move all of them between register files on every tile).
+// With SIGNED weights the sum becomes NaN.
+template <int D>
+struct Marks {
+    static constexpr int W = (D / 2 + 31) / 32;
+    uint32_t nan[W] = {}, up[W] = {}, down[W] = {};
+    template <bool SIGNED, typename T, int N, class Sees>
+    __device__ void note(const T *tile, int h, Sees sees) {
+#pragma unroll 1
+        for (int row = 0; row < N; ++row) {
+            const bool seen = sees(row);
+#pragma unroll
+            for (int e = 0; e < D / 2; ++e) {
+                const T x = tile[row * kPitch<T, D> + 32 * (e >> 4) + 8 * ((e & 15) >> 2) + 4 * h + (e & 3)];
+                const bool hit = seen & not_finite(x), is_nan = SIGNED | (x != x);
+                nan[e / 32] |= (uint32_t)(hit & is_nan) << (e % 32);
+                up[e / 32] |= (uint32_t)(hit & !is_nan & (x > (T)0.f)) << (e % 32);
+                down[e / 32] |= (uint32_t)(hit & !is_nan & (x < (T)0.f)) << (e % 32);
+            }
+        }
+    }
+    __device__ void apply(f32x16 (&acc)[D / 32]) const {
+        uint32_t any = 0;
+#pragma unroll
+        for (int w = 0; w < W; ++w) any |= nan[w] | up[w] | down[w];
+        if (!__any(any != 0)) return;
+#pragma unroll
+        for (int e = 0; e < D / 2; ++e) {
+            float x = (up[e / 32] >> (e % 32)) & 1 ? INFINITY : 0.f;
+            x += (down[e / 32] >> (e % 32)) & 1 ? -INFINITY : 0.f;
+            x = (nan[e / 32] >> (e % 32)) & 1 ? __builtin_nanf("") : x;
+            acc[e >> 4][e & 15] += x;
+        }
+    }
+};
+template <typename T, int D, int N, int THREADS>
+__device__ inline void clean(T *tile, int tid) {
+    for (int id = tid; id < N * (D / 8); id += THREADS) {
+        V8<T> *p = reinterpret_cast<V8<T> *>(tile + id / (D / 8) * kPitch<T, D> + id % (D / 8) * 8);
+        V8<T> v = *p;
+#pragma unroll
+        for (int t = 0; t < 8; ++t) v[t] = not_finite(v[t]) ? (T)0.f : v[t];
+        *p = v;
+    }
 }
 
 template <typename T>
@@ -208,6 +258,12 @@ struct Staged {
             part[i].load(base + r * step + (at < width ? at : 0));
         }
     }
+    __device__ bool special() const {
+        Largest<T> m;
+#pragma unroll
+        for (int i = 0; i < PARTS; ++i) m.add(part[i].q);
+        return m.special();
+    }
     __device__ void store(T *tile, int tid) const {
 #pragma unroll
         for (int i = 0; i < PARTS; ++i) {
@@ -238,11 +294,18 @@ struct KeyWalk {
 // What 32 rows from position `first` (live rows of them exist) see of keys
 // k0 .. k0 + count - 1.
 enum Sight { kNone, kSome, kAll };
+__device__ inline bool sees_all(int first, int last, int n, int window, int sinks, int k0, int k1) {
+    return (k1 <= first) & (last < n) & ((k0 > last - window) | (k1 < sinks));
+}
 __device__ inline Sight sight(int first, int live, int n, int window, int sinks, int k0, int count) {
     const int last = min(first + live - 1, n - 1), k1 = k0 + count - 1;
-    if (live <= 0 || first >= n || k0 > last || (k0 >= sinks && k1 <= first - window)) return kNone;
-    const bool all = live >= 32 && first + 31 < n && k1 <= first && (k0 > first + 31 - window || k1 < sinks);
-    return all ? kAll : kSome;
+    if ((live <= 0) | (first >= n) | (k0 > last) | ((k0 >= sinks) & (k1 <= first - window))) return kNone;
+    return (sees_all(first, first + 31, n, window, sinks, k0, k1) & (live >= 32)) ? kAll : kSome;
+}
+// The workgroup's answer to whether a wave staged an infinity or a NaN.
+__device__ inline bool any_wave(const int *flags) {
+    const int f = flags[0] | flags[1] | flags[2] | flags[3];
+    return __builtin_amdgcn_readfirstlane(f) != 0;
 }
 
 // Which of the keys k0 + 8 (r / 4) + 4 h + r % 4, items r of a column of
@@ -252,10 +315,8 @@ struct SeenKeys {
     int top, low, sinks;
     __device__ SeenKeys(int top_, int low_, int sinks_, int k0, int h)
         : top(top_ - k0 - 4 * h), low(low_ - k0 - 4 * h), sinks(sinks_ - k0 - 4 * h) {}
-    __device__ bool operator()(int r) const {
-        const int k = 8 * (r >> 2) + (r & 3);
-        return (k <= top) & ((k > low) | (k < sinks));
-    }
+    __device__ bool operator()(int r) const { return at(8 * (r >> 2) + (r & 3)); }
+    __device__ bool at(int k) const { return (k <= top) & ((k > low) | (k < sinks)); }
 };
 // Which of the rows r0 + 8 (r / 4) + 4 h + r % 4, of positions from start,
 // see a key: those from the key's own position up to the window's end, or up
@@ -267,10 +328,8 @@ struct SeenRows {
         from = key - start - base;
         end = (key < sinks ? last : min(last, key - start + window)) - base;
     }
-    __device__ bool operator()(int r) const {
-        const int k = 8 * (r >> 2) + (r & 3);
-        return (k >= from) & (k < end);
-    }
+    __device__ bool operator()(int r) const { return at(8 * (r >> 2) + (r & 3)); }
+    __device__ bool at(int k) const { return (k >= from) & (k < end); }
 };
 
 __device__ inline float exp2_(float x) { return __builtin_amdgcn_exp2f(x); }
@@ -303,6 +362,7 @@ constexpr float kShift = std::is_same<T, _Float16>::value ? 10.f : 0.f;
 template <typename T, int D>
 __global__ __launch_bounds__(kThreads, 2) void window_forward_kernel(WinArgs a) {
     __shared__ __attribute__((aligned(16))) T Ks[kKeys * kPitch<T, D>], Vs[kKeys * kPitch<T, D>];
+    __shared__ int flags[kWaves];
     const int tid = threadIdx.x, lane = tid & 63, i = lane & 31, h = lane >> 5;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int64_t b = blockIdx.z, head = blockIdx.y;
@@ -320,6 +380,7 @@ __global__ __launch_bounds__(kThreads, 2) void window_forward_kernel(WinArgs a) 
     float m = -INFINITY, l = 0.f;
     const int first = seq.start + mine, p = first + i, top = row < a.sq && p < seq.n ? p : -1, low = p - a.window;
     const KeyWalk<kKeys> walk(seq.start + row0, seq.start + min(row0 + 32 * kWaves, a.sq) - 1, seq.n, a.window, a.sinks);
+    const int group_first = seq.start + row0, group_last = seq.start + min(row0 + 32 * kWaves, a.sq) - 1;
     Staged<T, D, kKeys> ks, vs;
     if (walk.count) {
         ks.load(K, a.k.s, walk.tile(0) * kKeys, seq.n - 1, a.width, tid);
@@ -327,73 +388,65 @@ __global__ __launch_bounds__(kThreads, 2) void window_forward_kernel(WinArgs a) 
     }
     for (int t = 0; t < walk.count; ++t) {
         const int k0 = walk.tile(t) * kKeys;
+        const bool whole = sees_all(group_first, group_last, seq.n, a.window, a.sinks, k0, k0 + kKeys - 1);
         __syncthreads();
         ks.store(Ks, tid);
         vs.store(Vs, tid);
+        if (!whole) flags[wave] = __any(vs.special());
         __syncthreads();
         if (t + 1 < walk.count) {
             ks.load(K, a.k.s, walk.tile(t + 1) * kKeys, seq.n - 1, a.width, tid);
             vs.load(V, a.v.s, walk.tile(t + 1) * kKeys, seq.n - 1, a.width, tid);
         }
         const Sight see = sight(first, live, seq.n, a.window, a.sinks, k0, kKeys);
-        if (see == kNone) continue;
         f32x16 s[2] = {};
+        if (see != kNone) {
 #pragma unroll
-        for (int kb = 0; kb < 2; ++kb)
+            for (int kb = 0; kb < 2; ++kb)
 #pragma unroll
-            for (int u = 0; u < D / 16; ++u) s[kb] = mma(along<T, D>(Ks, 32 * kb + i, 16 * u + 8 * h), qf[u], s[kb]);
-        uint32_t seen = 0xffffffffu;
-        if (see == kSome) {
-            seen = 0;
+                for (int u = 0; u < D / 16; ++u) s[kb] = mma(along<T, D>(Ks, 32 * kb + i, 16 * u + 8 * h), qf[u], s[kb]);
+            if (see == kSome) {
 #pragma unroll
-            for (int kb = 0; kb < 2; ++kb) {
-                const SeenKeys keys(top, low, a.sinks, k0 + 32 * kb, h);
+                for (int kb = 0; kb < 2; ++kb) {
+                    const SeenKeys keys(top, low, a.sinks, k0 + 32 * kb, h);
 #pragma unroll
-                for (int r = 0; r < 16; ++r) {
-                    const bool vis = keys(r);
-                    seen |= (uint32_t)vis << (16 * kb + r);
-                    s[kb][r] = vis ? s[kb][r] : -INFINITY;
+                    for (int r = 0; r < 16; ++r) s[kb][r] = keys(r) ? s[kb][r] : -INFINITY;
                 }
             }
-        }
-        float mx = -INFINITY;
+            float mx = -INFINITY;
 #pragma unroll
-        for (int r = 0; r < 32; ++r) mx = fmaxf(mx, s[r >> 4][r & 15]);
-        mx = fmaxf(mx, other_half(mx)) * a.c;
-        const float m_new = fmaxf(m, mx);
-        // while every score is -inf, 0 in place of the maximum keeps the
-        // weights 0 (-inf - -inf would be NaN, and stay)
-        const float ref = m_new == -INFINITY ? 0.f : m_new;
-        const float alpha = exp2_(m - ref), off = kShift<T> - ref;
-        m = m_new;
-        float sum = 0.f;
-#pragma unroll
-        for (int r = 0; r < 32; ++r) {
-            const float e = exp2_(fmaf(s[r >> 4][r & 15], a.c, off));
-            s[r >> 4][r & 15] = e;
-            sum += e;
-        }
-        if (see == kSome) {
-            // hidden scores of a zero scale are -inf * 0
-            sum = 0.f;
+            for (int r = 0; r < 32; ++r) mx = fmaxf(mx, s[r >> 4][r & 15]);
+            mx = fmaxf(mx, other_half(mx)) * a.c;
+            const float m_new = fmaxf(m, mx);
+            // while every score is -inf, 0 in place of the maximum keeps the
+            // weights 0 (-inf - -inf would be NaN, and stay)
+            const float ref = m_new == -INFINITY ? 0.f : m_new;
+            const float alpha = exp2_(m - ref), off = kShift<T> - ref;
+            m = m_new;
+            float sum = 0.f;
 #pragma unroll
             for (int r = 0; r < 32; ++r) {
-                const float e = (seen >> r) & 1 ? s[r >> 4][r & 15] : 0.f;
+                const float e = exp2_(fmaf(s[r >> 4][r & 15], a.c, off));
                 s[r >> 4][r & 15] = e;
                 sum += e;
             }
-        }
-        l = l * alpha + sum;
+            l = l * alpha + sum;
 #pragma unroll
-        for (int d = 0; d < D / 32; ++d) acc[d] *= alpha;
+            for (int d = 0; d < D / 32; ++d) acc[d] *= alpha;
+        }
+        if (!whole && any_wave(flags)) {
+            if (see != kNone)
+                add_special<T, D, kKeys>(acc, Vs, h, [&](int k) { return SeenKeys(top, low, a.sinks, k0, 0).at(k); });
+            __syncthreads();
+            clean<T, D, kKeys, kThreads>(Vs, tid);
+            __syncthreads();
+        }
+        if (see == kNone) continue;
 #pragma unroll
         for (int kc = 0; kc < 4; ++kc) {
             const V8<T> pf = rounded<T>(s[kc >> 1], 8 * (kc & 1));
 #pragma unroll
-            for (int d = 0; d < D / 32; ++d) {
-                const V8<T> vf = across<T, D>(Vs, 16 * kc, 32 * d, lane);
-                acc[d] = see == kAll ? mma(vf, pf, acc[d]) : mma_hidden<false, T>(vf, pf, (seen >> (8 * kc)) & 0xff, acc[d]);
-            }
+            for (int d = 0; d < D / 32; ++d) acc[d] = mma(across<T, D>(Vs, 16 * kc, 32 * d, lane), pf, acc[d]);
         }
     }
     l += other_half(l);
@@ -484,18 +537,19 @@ __global__ __launch_bounds__(kThreads, 2) void window_split_kernel(WinArgs a, Sp
             const int part = lane + 64 * u;
             *reinterpret_cast<V8<T> *>(tile + part / (D / 8) * kPitch<T, D> + part % (D / 8) * 8) = vf[u];
         }
-        if (t + p.splits < walk.count) load(t + p.splits);
-        const bool all = k0 + N - 1 <= first && last < seq.n && (k0 > last - a.window || k0 + N - 1 < a.sinks);
-        uint32_t seen = 0xffffu;
+        const bool all = sees_all(first, last, seq.n, a.window, a.sinks, k0, k0 + N - 1);
+        bool special = false;
         if (!all) {
-            seen = 0;
+            Largest<T> most;
+#pragma unroll
+            for (int u = 0; u < PARTS; ++u) most.add(vf[u]);
+            special = __any(most.special());
+        }
+        if (t + p.splits < walk.count) load(t + p.splits);
+        if (!all) {
             const SeenKeys keys(top, low, a.sinks, k0, h);
 #pragma unroll
-            for (int c = 0; c < 16; ++c) {
-                const bool vis = keys(c);
-                seen |= (uint32_t)vis << c;
-                s[c] = vis ? s[c] : -INFINITY;
-            }
+            for (int c = 0; c < 16; ++c) s[c] = keys(c) ? s[c] : -INFINITY;
         }
         float mx = -INFINITY;
 #pragma unroll
@@ -507,21 +561,22 @@ __global__ __launch_bounds__(kThreads, 2) void window_split_kernel(WinArgs a, Sp
         float sum = 0.f;
 #pragma unroll
         for (int c = 0; c < 16; ++c) {
-            const float e = exp2_(fmaf(s[c], a.c, off));
-            s[c] = (seen >> c) & 1 ? e : 0.f;
+            s[c] = exp2_(fmaf(s[c], a.c, off));
             sum += s[c];
         }
         l = l * alpha + sum;
 #pragma unroll
         for (int d = 0; d < D / 32; ++d) acc[d] *= alpha;
+        if (special) {
+            // the wave alone reads and writes its tile
+            add_special<T, D, N>(acc, tile, h, [&](int k) { return SeenKeys(top, low, a.sinks, k0, 0).at(k); });
+            clean<T, D, N, 64>(tile, lane);
+        }
 #pragma unroll
         for (int kc = 0; kc < 2; ++kc) {
             const V8<T> pf = rounded<T>(s, 8 * kc);
 #pragma unroll
-            for (int d = 0; d < D / 32; ++d) {
-                const V8<T> vt = across<T, D>(tile, 16 * kc, 32 * d, lane);
-                acc[d] = all ? mma(vt, pf, acc[d]) : mma_hidden<false, T>(vt, pf, (seen >> (8 * kc)) & 0xff, acc[d]);
-            }
+            for (int d = 0; d < D / 32; ++d) acc[d] = mma(across<T, D>(tile, 16 * kc, 32 * d, lane), pf, acc[d]);
         }
     }
     l += other_half(l);
@@ -671,6 +726,7 @@ __device__ inline float gradient_scale(const WinArgs &a) {
 template <typename T, int D>
 __global__ __launch_bounds__(kThreads, 2) void window_dq_kernel(WinArgs a) {
     __shared__ __attribute__((aligned(16))) T Ks[kKeys * kPitch<T, D>], Vs[kKeys * kPitch<T, D>];
+    __shared__ int flags[kWaves];
     const int tid = threadIdx.x, lane = tid & 63, i = lane & 31, h = lane >> 5;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int64_t b = blockIdx.z, head = blockIdx.y;
@@ -696,8 +752,10 @@ __global__ __launch_bounds__(kThreads, 2) void window_dq_kernel(WinArgs a) {
     if (row < a.sq && h == 0) a.delta[stat] = delta;
     const float lse = a.lse_in[stat] * kLog2e, up = gradient_scale<T>(a);
     f32x16 acc[D / 32] = {};
+    Marks<D> marks;
     const int first = seq.start + mine, p = first + i, top = row < a.sq && p < seq.n ? p : -1, low = p - a.window;
     const KeyWalk<kKeys> walk(seq.start + row0, seq.start + min(row0 + 32 * kWaves, a.sq) - 1, seq.n, a.window, a.sinks);
+    const int group_first = seq.start + row0, group_last = seq.start + min(row0 + 32 * kWaves, a.sq) - 1;
     Staged<T, D, kKeys> ks, vs;
     if (walk.count) {
         ks.load(K, a.k.s, walk.tile(0) * kKeys, seq.n - 1, a.width, tid);
@@ -705,50 +763,53 @@ __global__ __launch_bounds__(kThreads, 2) void window_dq_kernel(WinArgs a) {
     }
     for (int t = 0; t < walk.count; ++t) {
         const int k0 = walk.tile(t) * kKeys;
+        const bool whole = sees_all(group_first, group_last, seq.n, a.window, a.sinks, k0, k0 + kKeys - 1);
         __syncthreads();
         ks.store(Ks, tid);
         vs.store(Vs, tid);
+        if (!whole) flags[wave] = __any(ks.special());
         __syncthreads();
         if (t + 1 < walk.count) {
             ks.load(K, a.k.s, walk.tile(t + 1) * kKeys, seq.n - 1, a.width, tid);
             vs.load(V, a.v.s, walk.tile(t + 1) * kKeys, seq.n - 1, a.width, tid);
         }
+        const bool special = !whole && any_wave(flags);
 #pragma unroll
         for (int kb = 0; kb < 2; ++kb) {
             const int kk = k0 + 32 * kb;
             const Sight see = sight(first, live, seq.n, a.window, a.sinks, kk, 32);
-            if (see == kNone) continue;
             f32x16 s = {}, dp = {};
+            if (see != kNone) {
 #pragma unroll
-            for (int u = 0; u < D / 16; ++u) {
-                s = mma(along<T, D>(Ks, 32 * kb + i, 16 * u + 8 * h), qf[u], s);
-                dp = mma(along<T, D>(Vs, 32 * kb + i, 16 * u + 8 * h), gf[u], dp);
-            }
-            uint32_t seen = 0xffffu;
+                for (int u = 0; u < D / 16; ++u) {
+                    s = mma(along<T, D>(Ks, 32 * kb + i, 16 * u + 8 * h), qf[u], s);
+                    dp = mma(along<T, D>(Vs, 32 * kb + i, 16 * u + 8 * h), gf[u], dp);
+                }
 #pragma unroll
-            for (int r = 0; r < 16; ++r) s[r] = exp2_(fmaf(s[r], a.c, -lse)) * ((dp[r] - delta) * up);
-            if (see == kSome) {
-                seen = 0;
-                const SeenKeys keys(top, low, a.sinks, kk, h);
+                for (int r = 0; r < 16; ++r) s[r] = exp2_(fmaf(s[r], a.c, -lse)) * ((dp[r] - delta) * up);
+                if (see == kSome) {
+                    const SeenKeys keys(top, low, a.sinks, kk, h);
 #pragma unroll
-                for (int r = 0; r < 16; ++r) {
-                    const bool vis = keys(r);
-                    seen |= (uint32_t)vis << r;
-                    s[r] = vis ? s[r] : 0.f;
+                    for (int r = 0; r < 16; ++r) s[r] = keys(r) ? s[r] : 0.f;
                 }
             }
+            if (special) {
+                T *half = Ks + 32 * kb * kPitch<T, D>;
+                marks.template note<true, T, 32>(half, h, [&](int k) { return SeenKeys(top, low, a.sinks, kk, 0).at(k); });
+                __syncthreads();
+                clean<T, D, 32, kThreads>(half, tid);
+                __syncthreads();
+            }
+            if (see == kNone) continue;
 #pragma unroll
             for (int kc = 0; kc < 2; ++kc) {
                 const V8<T> df = rounded<T>(s, 8 * kc);
 #pragma unroll
-                for (int d = 0; d < D / 32; ++d) {
-                    const V8<T> kf = across<T, D>(Ks, 32 * kb + 16 * kc, 32 * d, lane);
-                    acc[d] = see == kAll ? mma(kf, df, acc[d])
-                                         : mma_hidden<true, T>(kf, df, (seen >> (8 * kc)) & 0xff, acc[d]);
-                }
+                for (int d = 0; d < D / 32; ++d) acc[d] = mma(across<T, D>(Ks, 32 * kb + 16 * kc, 32 * d, lane), df, acc[d]);
             }
         }
     }
+    marks.apply(acc);
     if (row >= a.sq) return;
     T *DQ = const_cast<T *>(head_of<T>(a.dq, b, head)) + row * a.dq.s;
 #pragma unroll
@@ -761,6 +822,7 @@ template <typename T, int D>
 struct KeyGradients {
     V8<T> kf[D / 16], vf[D / 16];
     f32x16 dk[D / 32] = {}, dv[D / 32] = {};
+    Marks<D> mk, mv;
     // columns of keys past the sequence are zero
     __device__ void load(const WinArgs &a, int64_t b, int64_t kvh, int key, int n, int h) {
         const T *K = head_of<T>(a.k, b, kvh), *V = head_of<T>(a.v, b, kvh);
@@ -772,11 +834,12 @@ struct KeyGradients {
             vf[s] = n > 0 ? row_part(V + at * a.v.s, 16 * s + 8 * h, a.width, key < n) : V8<T>{};
         }
     }
-    // Ls holds shift - lse log2(e), Ds the rows' D; half scales dS.
-    __device__ void tile(const T *Qs, const T *Gs, const float *Ls, const float *Ds, float c, float half, bool all,
-                         const SeenRows &rows, int lane) {
+    // Weights and dS of a tile, one key a column. Ls holds
+    // shift - lse log2(e), Ds the rows' D; half scales dS.
+    __device__ void scores(f32x16 &s, f32x16 &dp, const T *Qs, const T *Gs, const float *Ls, const float *Ds, float c,
+                           float half, bool all, const SeenRows &rows, int lane) const {
         const int i = lane & 31, h = lane >> 5;
-        f32x16 s = {}, dp = {};
+        s = dp = f32x16{};
 #pragma unroll
         for (int u = 0; u < D / 16; ++u) {
             s = mma(along<T, D>(Qs, i, 16 * u + 8 * h), kf[u], s);
@@ -794,28 +857,32 @@ struct KeyGradients {
                 dp[r] = p * ((dp[r] - dr[j]) * half);
             }
         }
-        uint32_t seen = 0xffffu;
         if (!all) {
-            seen = 0;
 #pragma unroll
             for (int r = 0; r < 16; ++r) {
-                const bool vis = rows(r);
-                seen |= (uint32_t)vis << r;
-                s[r] = vis ? s[r] : 0.f;
-                dp[r] = vis ? dp[r] : 0.f;
+                s[r] = rows(r) ? s[r] : 0.f;
+                dp[r] = rows(r) ? dp[r] : 0.f;
             }
         }
+    }
+    __device__ void add(const f32x16 &s, const f32x16 &dp, const T *Qs, const T *Gs, int lane) {
 #pragma unroll
         for (int kc = 0; kc < 2; ++kc) {
             const V8<T> pf = rounded<T>(s, 8 * kc), df = rounded<T>(dp, 8 * kc);
-            const uint32_t bits = (seen >> (8 * kc)) & 0xff;
 #pragma unroll
             for (int d = 0; d < D / 32; ++d) {
-                const V8<T> gf = across<T, D>(Gs, 16 * kc, 32 * d, lane), qf = across<T, D>(Qs, 16 * kc, 32 * d, lane);
-                dv[d] = all ? mma(gf, pf, dv[d]) : mma_hidden<false, T>(gf, pf, bits, dv[d]);
-                dk[d] = all ? mma(qf, df, dk[d]) : mma_hidden<true, T>(qf, df, bits, dk[d]);
+                dv[d] = mma(across<T, D>(Gs, 16 * kc, 32 * d, lane), pf, dv[d]);
+                dk[d] = mma(across<T, D>(Qs, 16 * kc, 32 * d, lane), df, dk[d]);
             }
         }
+    }
+    __device__ void special(const T *Qs, const T *Gs, const SeenRows &rows, int h) {
+        mv.template note<false, T, kRows>(Gs, h, [&](int r) { return rows.at(r); });
+        mk.template note<true, T, kRows>(Qs, h, [&](int r) { return rows.at(r); });
+    }
+    __device__ void finish() {
+        mv.apply(dv);
+        mk.apply(dk);
     }
 };
 
@@ -856,6 +923,7 @@ template <typename T, int D>
 __global__ __launch_bounds__(kThreads, 1) void window_dkv_kernel(WinArgs a, FarArgs f) {
     __shared__ __attribute__((aligned(16))) T Qs[kRows * kPitch<T, D>], Gs[kRows * kPitch<T, D>];
     __shared__ __attribute__((aligned(16))) float Ls[kRows], Ds[kRows];
+    __shared__ int flags[kWaves];
     const int tid = threadIdx.x, lane = tid & 63, i = lane & 31, h = lane >> 5;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int64_t b = blockIdx.z, kvh = blockIdx.y;
@@ -885,20 +953,32 @@ __global__ __launch_bounds__(kThreads, 1) void window_dkv_kernel(WinArgs a, FarA
     };
     if (items) load(0);
     for (int t = 0; t < items; ++t) {
-        const int r0 = (from + t % tiles) * kRows;
+        const int r0 = (from + t % tiles) * kRows, p0 = seq.start + r0;
+        const bool whole = (r0 + kRows <= rows) & sees_all(p0, p0 + kRows - 1, seq.n, a.window, a.sinks, tile0, tile0 + 32 * kWaves - 1);
         __syncthreads();
         qs.store(Qs, tid);
         gs.store(Gs, tid);
+        if (!whole) flags[wave] = __any(qs.special() | gs.special());
         if (tid < kRows) {
             Ls[tid] = kShift<T> - ls * kLog2e;
             Ds[tid] = ds;
         }
         __syncthreads();
         if (t + 1 < items) load(t + 1);
-        const Sight see = sight(seq.start + r0, rows - r0, seq.n, a.window, a.sinks, mine, 32);
-        if (see == kNone) continue;
-        w.tile(Qs, Gs, Ls, Ds, a.c, half, see == kAll, SeenRows(key, seq.start, r0, h, rows, seq.n, a.window, a.sinks), lane);
+        const Sight see = sight(p0, rows - r0, seq.n, a.window, a.sinks, mine, 32);
+        f32x16 s, dp;
+        if (see != kNone)
+            w.scores(s, dp, Qs, Gs, Ls, Ds, a.c, half, see == kAll, SeenRows(key, seq.start, r0, h, rows, seq.n, a.window, a.sinks), lane);
+        if (!whole && any_wave(flags)) {
+            if (see != kNone) w.special(Qs, Gs, SeenRows(key, seq.start, r0, 0, rows, seq.n, a.window, a.sinks), h);
+            __syncthreads();
+            clean<T, D, kRows, kThreads>(Qs, tid);
+            clean<T, D, kRows, kThreads>(Gs, tid);
+            __syncthreads();
+        }
+        if (see != kNone) w.add(s, dp, Qs, Gs, lane);
     }
+    w.finish();
     if (f.part && mine < a.sinks) {
         store_part(f.at(b * a.kv + kvh, mine / 32, 0, a.width), w, i, h, a.width, true);
         return;
@@ -962,13 +1042,31 @@ __global__ __launch_bounds__(kThreads, 1) void window_far_kernel(WinArgs a, FarA
             *reinterpret_cast<V8<T> *>(Gs + at) = gr[s];
         }
         (h ? Ds : Ls)[i] = ls;
+        const bool whole = r0 + kRows <= rows;
+        bool special = false;
+        if (!whole) {
+            Largest<T> most;
+#pragma unroll
+            for (int s = 0; s < PARTS; ++s) {
+                most.add(qr[s]);
+                most.add(gr[s]);
+            }
+            special = __any(most.special());
+        }
         if (t + f.splits < items) load(t + f.splits);
         // the wave alone writes and reads its tile
         __builtin_amdgcn_wave_barrier();
-        w.tile(Qs, Gs, Ls, Ds, a.c, half, r0 + kRows <= rows,
-               SeenRows(key, seq.start, r0, h, rows, seq.n, a.window, key + 1), lane);
+        f32x16 s, dp;
+        w.scores(s, dp, Qs, Gs, Ls, Ds, a.c, half, whole, SeenRows(key, seq.start, r0, h, rows, seq.n, a.window, key + 1), lane);
+        if (special) {
+            w.special(Qs, Gs, SeenRows(key, seq.start, r0, 0, rows, seq.n, a.window, key + 1), h);
+            clean<T, D, kRows, 64>(Qs, lane);
+            clean<T, D, kRows, 64>(Gs, lane);
+        }
+        w.add(s, dp, Qs, Gs, lane);
         __builtin_amdgcn_wave_barrier();
     }
+    w.finish();
     store_part(f.at(b * a.kv + kvh, block, 1 + split, a.width), w, i, h, a.width, key < a.sinks);
 }
 
@@ -1076,6 +1174,8 @@ int32_t window_args(const chelis_gpu_tensor *q, const chelis_gpu_tensor *k, cons
     a->window = (int)std::min<int64_t>(window, std::max(a->sk, 1)), a->sinks = (int)std::min<int64_t>(sinks, a->sk);
     a->heads = (int)H, a->kv = (int)KV, a->group = KV ? (int)(H / KV) : 1, a->width = (int)W;
     a->flip = scale < 0, a->scale = (float)scale, a->c = (float)(std::fabs(scale) * 1.4426950408889634074);
+    // hidden scores are -inf, and 0 times that is NaN
+    if (a->c == 0.f) a->c = 0x1p-126f;
     return CHELIS_HIP_OK;
 }
 
