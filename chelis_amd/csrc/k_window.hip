@@ -211,7 +211,7 @@ struct WinArgs {
     int64_t length_step, start_step;
     int lengths_wide, starts_wide;
     int sq, sk, window, sinks, heads, kv, group, width, flip;
-    float c, scale;  // |scale| log2(e), scale
+    float c, signed_c, scale;  // |scale| log2(e), scale log2(e), scale
 };
 
 // The keys and the first row's position of sequence b. Stored lengths and
@@ -248,7 +248,7 @@ __device__ inline V8<T> row_part(const T *row, int at, int width, bool live) {
 // `last` and elements past the width repeat others of the operand: the rows
 // are hidden from every pair, and the other factor's elements are zero.
 template <typename T, int D, int N>
-struct Staged {
+struct Staged {  // by kThreads threads
     static constexpr int ALL = N * (D / 8), PARTS = (ALL + kThreads - 1) / kThreads;
     Pack<T, 8> part[PARTS];
     __device__ void load(const T *base, int64_t step, int row0, int last, int width, int tid) {
@@ -705,10 +705,11 @@ __device__ inline float gradient_scale(const WinArgs &a) {
     if constexpr (!std::is_same<T, _Float16>::value) return 1.f;
     __shared__ float waves[2][kWaves];
     static_assert(kRanges == kThreads, "one partial maximum a thread");
-    const float g = wave_vmax(a.range[threadIdx.x]), v = wave_vmax(a.range[kRanges + threadIdx.x]);
-    if ((threadIdx.x & 63) == 0) {
-        waves[0][threadIdx.x >> 6] = g;
-        waves[1][threadIdx.x >> 6] = v;
+    const int t = threadIdx.x & (kThreads - 1);  // groups of threads do the same
+    const float g = wave_vmax(a.range[t]), v = wave_vmax(a.range[kRanges + t]);
+    if ((t & 63) == 0) {
+        waves[0][t >> 6] = g;
+        waves[1][t >> 6] = v;
     }
     __syncthreads();
     float mg = 0.f, mv = 0.f;
@@ -741,7 +742,6 @@ __global__ __launch_bounds__(kThreads, 2) void window_dq_kernel(WinArgs a) {
     for (int s = 0; s < D / 16; ++s) {
         const int at = 16 * s + 8 * h;
         qf[s] = row_part(Q + safe * a.q.s, at, a.width, row < a.sq);
-        if (a.flip) qf[s] = -qf[s];
         gf[s] = row_part(G + safe * a.g.s, at, a.width, row < a.sq);
         const V8<T> of = row_part(O + safe * a.o.s, at, a.width, row < a.sq);
 #pragma unroll
@@ -786,7 +786,7 @@ __global__ __launch_bounds__(kThreads, 2) void window_dq_kernel(WinArgs a) {
                     dp = mma(along<T, D>(Vs, 32 * kb + i, 16 * u + 8 * h), gf[u], dp);
                 }
 #pragma unroll
-                for (int r = 0; r < 16; ++r) s[r] = exp2_(fmaf(s[r], a.c, -lse)) * ((dp[r] - delta) * up);
+                for (int r = 0; r < 16; ++r) s[r] = exp2_(fmaf(s[r], a.signed_c, -lse)) * ((dp[r] - delta) * up);
                 if (see == kSome) {
                     const SeenKeys keys(top, low, a.sinks, kk, h);
 #pragma unroll
@@ -820,30 +820,24 @@ __global__ __launch_bounds__(kThreads, 2) void window_dq_kernel(WinArgs a) {
 // rows, staged in LDS with their lse and D.
 template <typename T, int D>
 struct KeyGradients {
-    V8<T> kf[D / 16], vf[D / 16];
     f32x16 dk[D / 32] = {}, dv[D / 32] = {};
     Marks<D> mk, mv;
     // columns of keys past the sequence are zero
-    __device__ void load(const WinArgs &a, int64_t b, int64_t kvh, int key, int n, int h) {
-        const T *K = head_of<T>(a.k, b, kvh), *V = head_of<T>(a.v, b, kvh);
-        const int64_t at = key < n ? key : 0;
-#pragma unroll
-        for (int s = 0; s < D / 16; ++s) {
-            kf[s] = n > 0 ? row_part(K + at * a.k.s, 16 * s + 8 * h, a.width, key < n) : V8<T>{};
-            if (a.flip) kf[s] = -kf[s];
-            vf[s] = n > 0 ? row_part(V + at * a.v.s, 16 * s + 8 * h, a.width, key < n) : V8<T>{};
-        }
+    static __device__ V8<T> part(const T *base, int64_t step, int key, int n, int at, int width) {
+        if (n <= 0) return V8<T>{};
+        return row_part(base + (key < n ? key : 0) * step, at, width, key < n);
     }
     // Weights and dS of a tile, one key a column. Ls holds
     // shift - lse log2(e), Ds the rows' D; half scales dS.
-    __device__ void scores(f32x16 &s, f32x16 &dp, const T *Qs, const T *Gs, const float *Ls, const float *Ds, float c,
+    template <class Keys, class Values>
+    __device__ void scores(f32x16 &s, f32x16 &dp, Keys keys, Values values, const T *Qs, const T *Gs, const float *Ls, const float *Ds, float c,
                            float half, bool all, const SeenRows &rows, int lane) const {
         const int i = lane & 31, h = lane >> 5;
         s = dp = f32x16{};
 #pragma unroll
         for (int u = 0; u < D / 16; ++u) {
-            s = mma(along<T, D>(Qs, i, 16 * u + 8 * h), kf[u], s);
-            dp = mma(along<T, D>(Gs, i, 16 * u + 8 * h), vf[u], dp);
+            s = mma(along<T, D>(Qs, i, 16 * u + 8 * h), keys(u), s);
+            dp = mma(along<T, D>(Gs, i, 16 * u + 8 * h), values(u), dp);
         }
 #pragma unroll
         for (int r4 = 0; r4 < 4; ++r4) {
@@ -918,59 +912,117 @@ __device__ inline void store_part(float *part, const KeyGradients<T, D> &w, int 
         }
 }
 
-// The near rows: a workgroup takes 128 keys, its waves share the row tiles.
+// The near rows: a workgroup takes 128 keys, 32 to a wave, in `GROUPS` groups
+// of four waves that take the row tiles in turn and add their sums up at the
+// end. k and v stay in LDS. Row tiles are double buffered, one barrier a tile.
 template <typename T, int D>
-__global__ __launch_bounds__(kThreads, 1) void window_dkv_kernel(WinArgs a, FarArgs f) {
-    __shared__ __attribute__((aligned(16))) T Qs[kRows * kPitch<T, D>], Gs[kRows * kPitch<T, D>];
-    __shared__ __attribute__((aligned(16))) float Ls[kRows], Ds[kRows];
-    __shared__ int flags[kWaves];
-    const int tid = threadIdx.x, lane = tid & 63, i = lane & 31, h = lane >> 5;
-    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+constexpr int kGroups = sizeof(T) == 4 && D > 64 ? 1 : 2;
+
+template <typename T, int D>
+__global__ __launch_bounds__((kThreads * kGroups<T, D>), 1) void window_dkv_kernel(WinArgs a, FarArgs f) {
+    constexpr int GROUPS = kGroups<T, D>, TILE = kRows * kPitch<T, D>, KEYS = 32 * kWaves;
+    struct Buffers {
+        T q[2][GROUPS][TILE], g[2][GROUPS][TILE], v[KEYS * kPitch<T, D>], k[GROUPS > 1 ? KEYS * kPitch<T, D> : 1];
+    };
+    union Shared {
+        Buffers in;
+        float sums[GROUPS > 1 ? kWaves * D / 2 * 64 : 1];
+    };
+    __shared__ __attribute__((aligned(16))) Shared sh;
+    __shared__ __attribute__((aligned(16))) float Ls[2][GROUPS][kRows], Ds[2][GROUPS][kRows];
+    __shared__ int flags[2][kWaves * GROUPS];
+    const int tid = threadIdx.x & (kThreads - 1), lane = tid & 63, i = lane & 31, h = lane >> 5;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), group = __builtin_amdgcn_readfirstlane(threadIdx.x / kThreads);
     const int64_t b = blockIdx.z, kvh = blockIdx.y;
     const Seq seq(a, b);
-    const int tile0 = blockIdx.x * (32 * kWaves), mine = tile0 + 32 * wave, key = mine + i;
+    const int tile0 = blockIdx.x * KEYS, mine = tile0 + 32 * wave, key = mine + i;
     KeyGradients<T, D> w;
-    w.load(a, b, kvh, key, seq.n, h);
+    for (int id = threadIdx.x; id < KEYS * (D / 8); id += kThreads * GROUPS) {
+        const int r = id / (D / 8), at = id % (D / 8) * 8, to = r * kPitch<T, D> + at;
+        *reinterpret_cast<V8<T> *>(sh.in.v + to) = KeyGradients<T, D>::part(head_of<T>(a.v, b, kvh), a.v.s, tile0 + r, seq.n, at, a.width);
+        if constexpr (GROUPS > 1)
+            *reinterpret_cast<V8<T> *>(sh.in.k + to) = KeyGradients<T, D>::part(head_of<T>(a.k, b, kvh), a.k.s, tile0 + r, seq.n, at, a.width);
+    }
+    const T *Vs = sh.in.v + (32 * wave + i) * kPitch<T, D> + 8 * h, *Ks = sh.in.k + (32 * wave + i) * kPitch<T, D> + 8 * h;
+    V8<T> kf[GROUPS > 1 ? 1 : D / 16];
+    if constexpr (GROUPS == 1) {
+#pragma unroll
+        for (int u = 0; u < D / 16; ++u)
+            kf[u] = KeyGradients<T, D>::part(head_of<T>(a.k, b, kvh), a.k.s, key, seq.n, 16 * u + 8 * h, a.width);
+    }
+    auto keys = [&](int u) -> V8<T> {
+        if constexpr (GROUPS > 1) return *reinterpret_cast<const V8<T> *>(Ks + 16 * u);
+        else return kf[u];
+    };
+    auto values = [&](int u) { return *reinterpret_cast<const V8<T> *>(Vs + 16 * u); };
     const float up = gradient_scale<T>(a), half = up * exp2_(-kShift<T>);
     // rows lo .. rows - 1 see some key of the tile
     const int64_t end = tile0 < a.sinks && !f.part ? 2 * kMaxExtent : far_from(tile0, a.window);
     const int lo = max(0, tile0 - seq.start);
     const int rows = (int)min(min((int64_t)a.sq, (int64_t)seq.n - seq.start), end - seq.start);
     const int from = lo / kRows, tiles = rows <= lo || tile0 >= seq.n ? 0 : (rows - 1) / kRows - from + 1;
-    const int items = tiles * a.group;
+    const int items = tiles * a.group, turns = (items + GROUPS - 1) / GROUPS;
     Staged<T, D, kRows> qs, gs;
     float ls = 0.f, ds = 0.f;
-    auto load = [&](int t) {
-        const int64_t head = kvh * a.group + t / tiles;
-        const int r0 = (from + t % tiles) * kRows;
-        qs.load(head_of<T>(a.q, b, head), a.q.s, r0, a.sq - 1, a.width, tid);
-        gs.load(head_of<T>(a.g, b, head), a.g.s, r0, a.sq - 1, a.width, tid);
+    // the group's tile of a turn: its head and first row
+    struct Item {
+        int head, r0;
+        bool live;
+    };
+    auto item = [&](int turn) {
+        const int t = turn * GROUPS + group;
+        return Item{t / max(tiles, 1), (from + t % max(tiles, 1)) * kRows, t < items};
+    };
+    auto load = [&](int turn) {
+        const Item x = item(turn);
+        if (!x.live) return;
+        const int64_t head = kvh * a.group + x.head;
+        qs.load(head_of<T>(a.q, b, head), a.q.s, x.r0, a.sq - 1, a.width, tid);
+        gs.load(head_of<T>(a.g, b, head), a.g.s, x.r0, a.sq - 1, a.width, tid);
         if (tid < kRows) {
-            const int64_t stat = (b * a.heads + head) * a.sq + min(r0 + tid, a.sq - 1);
+            const int64_t stat = (b * a.heads + head) * a.sq + min(x.r0 + tid, a.sq - 1);
             ls = a.lse_in[stat];
             ds = a.delta[stat];
         }
     };
-    if (items) load(0);
-    for (int t = 0; t < items; ++t) {
-        const int r0 = (from + t % tiles) * kRows, p0 = seq.start + r0;
-        const bool whole = (r0 + kRows <= rows) & sees_all(p0, p0 + kRows - 1, seq.n, a.window, a.sinks, tile0, tile0 + 32 * kWaves - 1);
-        __syncthreads();
-        qs.store(Qs, tid);
-        gs.store(Gs, tid);
-        if (!whole) flags[wave] = __any(qs.special() | gs.special());
-        if (tid < kRows) {
-            Ls[tid] = kShift<T> - ls * kLog2e;
-            Ds[tid] = ds;
+    auto whole = [&](const Item &x) {
+        const int p0 = seq.start + x.r0;
+        return (int)(x.r0 + kRows <= rows) & (int)sees_all(p0, p0 + kRows - 1, seq.n, a.window, a.sinks, tile0, tile0 + KEYS - 1);
+    };
+    auto store = [&](int turn) {
+        const Item x = item(turn);
+        const int to = turn & 1;
+        bool special = false;
+        if (x.live) {
+            qs.store(sh.in.q[to][group], tid);
+            gs.store(sh.in.g[to][group], tid);
+            if (tid < kRows) {
+                Ls[to][group][tid] = kShift<T> - ls * kLog2e;
+                Ds[to][group][tid] = ds;
+            }
+            if (!whole(x)) special = __any((int)qs.special() | (int)gs.special());
         }
+        flags[to][group * kWaves + wave] = special;
+    };
+    if (turns) {
+        load(0);
+        store(0);
+        if (turns > 1) load(1);
+    }
+    for (int turn = 0; turn < turns; ++turn) {
         __syncthreads();
-        if (t + 1 < items) load(t + 1);
-        const Sight see = sight(p0, rows - r0, seq.n, a.window, a.sinks, mine, 32);
+        if (turn + 1 < turns) store(turn + 1);
+        if (turn + 2 < turns) load(turn + 2);
+        const Item x = item(turn);
+        const int at = turn & 1;
+        T *Qs = sh.in.q[at][group], *Gs = sh.in.g[at][group];
+        const Sight see = x.live ? sight(seq.start + x.r0, rows - x.r0, seq.n, a.window, a.sinks, mine, 32) : kNone;
         f32x16 s, dp;
         if (see != kNone)
-            w.scores(s, dp, Qs, Gs, Ls, Ds, a.c, half, see == kAll, SeenRows(key, seq.start, r0, h, rows, seq.n, a.window, a.sinks), lane);
-        if (!whole && any_wave(flags)) {
-            if (see != kNone) w.special(Qs, Gs, SeenRows(key, seq.start, r0, 0, rows, seq.n, a.window, a.sinks), h);
+            w.scores(s, dp, keys, values, Qs, Gs, Ls[at][group], Ds[at][group], a.signed_c, half, see == kAll,
+                     SeenRows(key, seq.start, x.r0, h, rows, seq.n, a.window, a.sinks), lane);
+        if (any_wave(flags[at]) || (GROUPS > 1 && any_wave(flags[at] + kWaves * (GROUPS - 1)))) {
+            if (see != kNone) w.special(Qs, Gs, SeenRows(key, seq.start, x.r0, 0, rows, seq.n, a.window, a.sinks), h);
             __syncthreads();
             clean<T, D, kRows, kThreads>(Qs, tid);
             clean<T, D, kRows, kThreads>(Gs, tid);
@@ -979,6 +1031,25 @@ __global__ __launch_bounds__(kThreads, 1) void window_dkv_kernel(WinArgs a, FarA
         if (see != kNone) w.add(s, dp, Qs, Gs, lane);
     }
     w.finish();
+    if constexpr (GROUPS > 1) {
+        // the second group's sums through LDS, dk and then dv
+#pragma unroll
+        for (int which = 0; which < 2; ++which) {
+            f32x16(&acc)[D / 32] = which ? w.dv : w.dk;
+            float *mineat = sh.sums + wave * (D / 2) * 64 + lane;
+            __syncthreads();
+            if (group == 1) {
+#pragma unroll
+                for (int e = 0; e < D / 2; ++e) mineat[e * 64] = acc[e >> 4][e & 15];
+            }
+            __syncthreads();
+            if (group == 0) {
+#pragma unroll
+                for (int e = 0; e < D / 2; ++e) acc[e >> 4][e & 15] += mineat[e * 64];
+            }
+        }
+        if (group) return;
+    }
     if (f.part && mine < a.sinks) {
         store_part(f.at(b * a.kv + kvh, mine / 32, 0, a.width), w, i, h, a.width, true);
         return;
@@ -1007,7 +1078,11 @@ __global__ __launch_bounds__(kThreads, 1) void window_far_kernel(WinArgs a, FarA
     const Seq seq(a, b);
     const int key = block * 32 + i;
     KeyGradients<T, D> w;
-    w.load(a, b, kvh, key, seq.n, h);
+    V8<T> kf[D / 16], vf[D / 16];
+#pragma unroll
+    for (int s = 0; s < D / 16; ++s)
+        kf[s] = KeyGradients<T, D>::part(head_of<T>(a.k, b, kvh), a.k.s, key, seq.n, 16 * s + 8 * h, a.width),
+        vf[s] = KeyGradients<T, D>::part(head_of<T>(a.v, b, kvh), a.v.s, key, seq.n, 16 * s + 8 * h, a.width);
     const int from = max(0, far_from(block / kWaves * 32 * kWaves, a.window) - seq.start);
     const int rows = min(a.sq, seq.n - seq.start), count = rows > from ? (rows - from + kRows - 1) / kRows : 0;
     T *Qs = tiles[wave][0], *Gs = tiles[wave][1];
@@ -1057,7 +1132,7 @@ __global__ __launch_bounds__(kThreads, 1) void window_far_kernel(WinArgs a, FarA
         // the wave alone writes and reads its tile
         __builtin_amdgcn_wave_barrier();
         f32x16 s, dp;
-        w.scores(s, dp, Qs, Gs, Ls, Ds, a.c, half, whole, SeenRows(key, seq.start, r0, h, rows, seq.n, a.window, key + 1), lane);
+        w.scores(s, dp, [&](int u) { return kf[u]; }, [&](int u) { return vf[u]; }, Qs, Gs, Ls, Ds, a.signed_c, half, whole, SeenRows(key, seq.start, r0, h, rows, seq.n, a.window, key + 1), lane);
         if (special) {
             w.special(Qs, Gs, SeenRows(key, seq.start, r0, 0, rows, seq.n, a.window, key + 1), h);
             clean<T, D, kRows, 64>(Qs, lane);
@@ -1070,24 +1145,32 @@ __global__ __launch_bounds__(kThreads, 1) void window_far_kernel(WinArgs a, FarA
     store_part(f.at(b * a.kv + kvh, block, 1 + split, a.width), w, i, h, a.width, key < a.sinks);
 }
 
-// Four keys of a sink block, dk and dv.
+// One key of a sink block, dk and dv: every fourth part to a wave.
 template <typename T>
 __global__ __launch_bounds__(kThreads) void window_sinks_kernel(WinArgs a, FarArgs f) {
+    __shared__ f32x4 join[kWaves][64];
     const float up = gradient_scale<T>(a);
     const int64_t b = blockIdx.z / f.blocks, kvh = blockIdx.y;
-    const int block = blockIdx.z % f.blocks, lane = threadIdx.x & 31, which = threadIdx.x >> 5 & 1;
-    const int i = blockIdx.x * 4 + (threadIdx.x >> 6), key = block * 32 + i;
-    if (4 * lane >= a.width || key >= a.sk) return;
-    const float *part = f.at(b * a.kv + kvh, block, 0, a.width) + (32 * which + i) * a.width + 4 * lane;
+    const int block = blockIdx.z % f.blocks, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int which = lane >> 5, at = 4 * (lane & 31), i = blockIdx.x, key = block * 32 + i;
+    if (key >= a.sk) return;
     f32x4 x = {};
+    if (at < a.width) {
+        const float *part = f.at(b * a.kv + kvh, block, 0, a.width) + (32 * which + i) * a.width + at;
 #pragma unroll 8
-    for (int s = 0; s <= f.splits; ++s) x += *reinterpret_cast<const f32x4 *>(part + (int64_t)s * 64 * a.width);
+        for (int s = wave; s <= f.splits; s += kWaves) x += *reinterpret_cast<const f32x4 *>(part + (int64_t)s * 64 * a.width);
+    }
+    join[wave][lane] = x;
+    __syncthreads();
+    if (wave || at >= a.width) return;
+#pragma unroll
+    for (int w = 1; w < kWaves; ++w) x += join[w][lane];
     const View &out = which ? a.dv : a.dk;
     const float scale = which ? exp2_(-kShift<T>) : a.scale / up;
     Pack<T, 4> y;
 #pragma unroll
     for (int t = 0; t < 4; ++t) y.set(t, x[t] * scale);
-    y.store(const_cast<T *>(head_of<T>(out, b, kvh)) + key * out.s + 4 * lane);
+    y.store(const_cast<T *>(head_of<T>(out, b, kvh)) + key * out.s + at);
 }
 
 // ---------------------------------------------------------------- dispatch
@@ -1176,6 +1259,7 @@ int32_t window_args(const chelis_gpu_tensor *q, const chelis_gpu_tensor *k, cons
     a->flip = scale < 0, a->scale = (float)scale, a->c = (float)(std::fabs(scale) * 1.4426950408889634074);
     // hidden scores are -inf, and 0 times that is NaN
     if (a->c == 0.f) a->c = 0x1p-126f;
+    a->signed_c = a->flip ? -a->c : a->c;
     return CHELIS_HIP_OK;
 }
 
@@ -1281,14 +1365,14 @@ extern "C" int32_t chelis_hip_window_attention_adjoint(
     const dim3 keys((a.sk + 127) / 128, a.kv, (unsigned)q->shape[0]);
     if (!grid_fits(rows.x, kThreads) || !grid_fits(keys.x, kThreads))
         return set_error(CHELIS_HIP_EUNSUPPORTED, "%s: grid too large", what);
-    // rows far behind the window of the first keys: dealt out 16 tiles to a
+    // rows far behind the window of the first keys: dealt out four tiles to a
     // wave, over no more waves than fill the device twice
     FarArgs f{};
     const int64_t pairs = q->shape[0] * a.kv, far = (int64_t)a.sk - (32 * kWaves - 1) - a.window;
     if (a.sinks > 0 && q->count && far > 0) {
         f.blocks = (a.sinks + 31) / 32;
         const int64_t tiles = (std::min<int64_t>(far, a.sq) + kRows - 1) / kRows * a.group;
-        f.splits = (int)std::max<int64_t>(1, std::min<int64_t>((tiles + 15) / 16, 8 * (int64_t)device_cus() / (pairs * f.blocks)));
+        f.splits = (int)std::max<int64_t>(1, std::min<int64_t>((tiles + 3) / 4, 8 * (int64_t)device_cus() / (pairs * f.blocks)));
         if (q->shape[0] * f.blocks > 65535)
             return set_error(CHELIS_HIP_EUNSUPPORTED, "%s: sequences times sink blocks past 65535", what);
     }
@@ -1305,11 +1389,11 @@ extern "C" int32_t chelis_hip_window_attention_adjoint(
             window_range_kernel<T, true><<<kRanges, 256, 0, st>>>(a, k->count / 8, a.range + kRanges);
         }
         if (q->count) window_dq_kernel<T, d><<<rows, kThreads, 0, st>>>(a);
-        if (k->count) window_dkv_kernel<T, d><<<keys, kThreads, 0, st>>>(a, f);
+        if (k->count) window_dkv_kernel<T, d><<<keys, kThreads * kGroups<T, d>, 0, st>>>(a, f);
         if (parts) {
             const unsigned z = (unsigned)(q->shape[0] * f.blocks);
             window_far_kernel<T, d><<<dim3((f.splits + kWaves - 1) / kWaves, a.kv, z), kThreads, 0, st>>>(a, f);
-            window_sinks_kernel<T><<<dim3(8, a.kv, z), kThreads, 0, st>>>(a, f);
+            window_sinks_kernel<T><<<dim3(32, a.kv, z), kThreads, 0, st>>>(a, f);
         }
         return CHELIS_HIP_OK;
     });
