@@ -198,6 +198,21 @@ __device__ inline V8<T> rounded(const f32x16 &s, int from) {
     return v;
 }
 
+// The order of a product loop's instructions: LDS reads for AHEAD products
+// first, then one product and the reads for a later one in turn, so that no
+// product waits for its own reads. (The compiler kept two reads in flight and
+// waited for them before every second product.)
+template <int PRODUCTS, int READS, int AHEAD>
+__device__ inline void interleave() {
+    __builtin_amdgcn_sched_group_barrier(0x100, READS * AHEAD, 0);
+#pragma unroll
+    for (int k = 0; k < PRODUCTS - AHEAD; ++k) {
+        __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+        __builtin_amdgcn_sched_group_barrier(0x100, READS, 0);
+    }
+    __builtin_amdgcn_sched_group_barrier(0x008, AHEAD, 0);
+}
+
 struct View {
     const void *p;
     int64_t b, h, s;  // strides of batch, head, sequence
@@ -244,18 +259,29 @@ __device__ inline V8<T> row_part(const T *row, int at, int width, bool live) {
     return live && at < width ? p.q : z;
 }
 
-// A tile of N rows of D elements on its way from memory to LDS. Rows past
-// `last` and elements past the width repeat others of the operand: the rows
-// are hidden from every pair, and the other factor's elements are zero.
+// A tile of N rows of D elements on its way from memory to LDS, staged by
+// kThreads threads. Rows past `last` and elements past the width repeat others
+// of the operand: the rows are hidden from every pair, and the other factor's
+// elements are zero. Whole tiles take one address a thread and a uniform step
+// between its parts (52 of the 380 vector instructions a tile went into
+// addresses otherwise).
 template <typename T, int D, int N>
-struct Staged {  // by kThreads threads
-    static constexpr int ALL = N * (D / 8), PARTS = (ALL + kThreads - 1) / kThreads;
+struct Staged {
+    static constexpr int C = D / 8, ALL = N * C, PARTS = (ALL + kThreads - 1) / kThreads;
+    static constexpr bool EVEN = kThreads % C == 0;
     Pack<T, 8> part[PARTS];
     __device__ void load(const T *base, int64_t step, int row0, int last, int width, int tid) {
+        const int own = tid % C * 8, at = own < width ? own : 0;
+        if (EVEN && row0 + N - 1 <= last) {
+            const T *p = base + row0 * step + (tid / C * step + at);
+#pragma unroll
+            for (int i = 0; i < PARTS; ++i) part[i].load(p + i * (kThreads / C) * step);
+            return;
+        }
 #pragma unroll
         for (int i = 0; i < PARTS; ++i) {
-            const int id = tid + i * kThreads, r = min(row0 + id / (D / 8), last), at = id % (D / 8) * 8;
-            part[i].load(base + r * step + (at < width ? at : 0));
+            const int id = tid + i * kThreads, r = min(row0 + id / C, last), e = id % C * 8;
+            part[i].load(base + r * step + (e < width ? e : 0));
         }
     }
     __device__ bool special() const {
@@ -357,19 +383,77 @@ __device__ inline void store_column(T *row, const f32x16 &c, int d0, int width, 
 // f16 weights are held 2^10 times larger: the smallest keep their bits.
 template <typename T>
 constexpr float kShift = std::is_same<T, _Float16>::value ? 10.f : 0.f;
+// The reference of the exponentials follows the running maximum only when
+// some row's passes it by more than this (in powers of two; 2^15 is the
+// largest f16 weight then): nearly every tile leaves the results unscaled.
+constexpr float kSlack = 5.f;
+
+// LDS tiles of keys: two of each operand (one barrier a tile) where two
+// workgroups then still fit a compute unit's 160 KB.
+template <typename T>
+constexpr int kBuffers = sizeof(T) == 2 ? 2 : 1;
+
+// What the waves of a workgroup share of a walk over key tiles: staging ahead,
+// and whether a tile holds infinities or NaN that some row does not see
+// (LOOK: 0 looks over k, 1 over v).
+template <typename T, int D, int LOOK>
+struct KeyTiles {
+    static constexpr int B = kBuffers<T>, SIZE = kKeys * kPitch<T, D>;
+    struct Shared {
+        T k[B][SIZE], v[B][SIZE];
+        int flags[2][kWaves];
+    };
+    const WinArgs &a;
+    Shared &sh;
+    const T *K, *V;
+    const KeyWalk<kKeys> &walk;
+    int n, first, last, tid, wave;  // keys; positions of the workgroup's rows
+    Staged<T, D, kKeys> ks, vs;
+    __device__ bool whole(int k0) const { return sees_all(first, last, n, a.window, a.sinks, k0, k0 + kKeys - 1); }
+    __device__ void load(int t) {
+        if (t >= walk.count) return;
+        ks.load(K, a.k.s, walk.tile(t) * kKeys, n - 1, a.width, tid);
+        vs.load(V, a.v.s, walk.tile(t) * kKeys, n - 1, a.width, tid);
+    }
+    __device__ void store(int t) {
+        if (t >= walk.count) return;
+        ks.store(sh.k[t % B], tid);
+        vs.store(sh.v[t % B], tid);
+        if (!whole(walk.tile(t) * kKeys)) sh.flags[t & 1][wave] = __any(LOOK ? vs.special() : ks.special());
+    }
+    __device__ void begin() {
+        load(0);
+        if (B == 2) {
+            store(0);
+            load(1);
+        }
+    }
+    // tile t is in LDS for every wave after this
+    __device__ void next(int t) {
+        __syncthreads();
+        if (B == 2) {
+            store(t + 1);
+            load(t + 2);
+        } else {
+            store(t);
+            __syncthreads();
+            load(t + 1);
+        }
+    }
+    __device__ bool special(int t) const { return !whole(walk.tile(t) * kKeys) && any_wave(sh.flags[t & 1]); }
+};
 
 // A workgroup takes 128 rows of one head, each wave 32 of them.
 template <typename T, int D>
 __global__ __launch_bounds__(kThreads, 2) void window_forward_kernel(WinArgs a) {
-    __shared__ __attribute__((aligned(16))) T Ks[kKeys * kPitch<T, D>], Vs[kKeys * kPitch<T, D>];
-    __shared__ int flags[kWaves];
+    __shared__ __attribute__((aligned(16))) typename KeyTiles<T, D, 1>::Shared sh;
     const int tid = threadIdx.x, lane = tid & 63, i = lane & 31, h = lane >> 5;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int64_t b = blockIdx.z, head = blockIdx.y;
     const Seq seq(a, b);
     const int row0 = blockIdx.x * (32 * kWaves), mine = row0 + 32 * wave, row = mine + i;
     const int live = min(32, a.sq - mine);
-    const T *Q = head_of<T>(a.q, b, head), *K = head_of<T>(a.k, b, head / a.group), *V = head_of<T>(a.v, b, head / a.group);
+    const T *Q = head_of<T>(a.q, b, head);
     V8<T> qf[D / 16];
 #pragma unroll
     for (int s = 0; s < D / 16; ++s) {
@@ -379,32 +463,44 @@ __global__ __launch_bounds__(kThreads, 2) void window_forward_kernel(WinArgs a) 
     f32x16 acc[D / 32] = {};
     float m = -INFINITY, l = 0.f;
     const int first = seq.start + mine, p = first + i, top = row < a.sq && p < seq.n ? p : -1, low = p - a.window;
-    const KeyWalk<kKeys> walk(seq.start + row0, seq.start + min(row0 + 32 * kWaves, a.sq) - 1, seq.n, a.window, a.sinks);
     const int group_first = seq.start + row0, group_last = seq.start + min(row0 + 32 * kWaves, a.sq) - 1;
-    Staged<T, D, kKeys> ks, vs;
-    if (walk.count) {
-        ks.load(K, a.k.s, walk.tile(0) * kKeys, seq.n - 1, a.width, tid);
-        vs.load(V, a.v.s, walk.tile(0) * kKeys, seq.n - 1, a.width, tid);
-    }
+    const KeyWalk<kKeys> walk(group_first, group_last, seq.n, a.window, a.sinks);
+    KeyTiles<T, D, 1> tiles{a, sh, head_of<T>(a.k, b, head / a.group), head_of<T>(a.v, b, head / a.group), walk, seq.n,
+                            group_first, group_last, tid, wave};
+    tiles.begin();
     for (int t = 0; t < walk.count; ++t) {
+        tiles.next(t);
         const int k0 = walk.tile(t) * kKeys;
-        const bool whole = sees_all(group_first, group_last, seq.n, a.window, a.sinks, k0, k0 + kKeys - 1);
-        __syncthreads();
-        ks.store(Ks, tid);
-        vs.store(Vs, tid);
-        if (!whole) flags[wave] = __any(vs.special());
-        __syncthreads();
-        if (t + 1 < walk.count) {
-            ks.load(K, a.k.s, walk.tile(t + 1) * kKeys, seq.n - 1, a.width, tid);
-            vs.load(V, a.v.s, walk.tile(t + 1) * kKeys, seq.n - 1, a.width, tid);
-        }
+        const T *Ks = sh.k[t % kBuffers<T>];
+        T *Vs = sh.v[t % kBuffers<T>];
         const Sight see = sight(first, live, seq.n, a.window, a.sinks, k0, kKeys);
-        f32x16 s[2] = {};
-        if (see != kNone) {
+        // binary32 products cost sixteen times the 16-bit ones: there the
+        // halves of a tile that a wave sees nothing of are left out ([8, 16,
+        // 512, 64] with a window of 128: 54.7 -> 51.4 us); the branches cost
+        // the 16-bit kernel more than they save (199 -> 216 us)
+        constexpr bool HALVES = sizeof(T) == 4;
+        bool half[2] = {true, true};
+        if constexpr (HALVES) {
 #pragma unroll
             for (int kb = 0; kb < 2; ++kb)
+                half[kb] = sight(first, live, seq.n, a.window, a.sinks, k0 + 32 * kb, 32) != kNone;
+        }
+        f32x16 s[2] = {};
+        if (see != kNone) {
+            if constexpr (HALVES) {
 #pragma unroll
-                for (int u = 0; u < D / 16; ++u) s[kb] = mma(along<T, D>(Ks, 32 * kb + i, 16 * u + 8 * h), qf[u], s[kb]);
+                for (int kb = 0; kb < 2; ++kb)
+                    if (half[kb]) {
+#pragma unroll
+                        for (int u = 0; u < D / 16; ++u) s[kb] = mma(along<T, D>(Ks, 32 * kb + i, 16 * u + 8 * h), qf[u], s[kb]);
+                    }
+            } else {
+#pragma unroll
+                for (int u = 0; u < D / 16; ++u)
+#pragma unroll
+                    for (int kb = 0; kb < 2; ++kb) s[kb] = mma(along<T, D>(Ks, 32 * kb + i, 16 * u + 8 * h), qf[u], s[kb]);
+                interleave<D / 8, 1, 4>();
+            }
             if (see == kSome) {
 #pragma unroll
                 for (int kb = 0; kb < 2; ++kb) {
@@ -417,12 +513,16 @@ __global__ __launch_bounds__(kThreads, 2) void window_forward_kernel(WinArgs a) 
 #pragma unroll
             for (int r = 0; r < 32; ++r) mx = fmaxf(mx, s[r >> 4][r & 15]);
             mx = fmaxf(mx, other_half(mx)) * a.c;
-            const float m_new = fmaxf(m, mx);
+            if (__any(mx > m + kSlack)) {
+                const float m_new = fmaxf(m, mx), alpha = exp2_(m - (m_new == -INFINITY ? 0.f : m_new));
+                m = m_new;
+                l *= alpha;
+#pragma unroll
+                for (int d = 0; d < D / 32; ++d) acc[d] *= alpha;
+            }
             // while every score is -inf, 0 in place of the maximum keeps the
             // weights 0 (-inf - -inf would be NaN, and stay)
-            const float ref = m_new == -INFINITY ? 0.f : m_new;
-            const float alpha = exp2_(m - ref), off = kShift<T> - ref;
-            m = m_new;
+            const float off = kShift<T> - (m == -INFINITY ? 0.f : m);
             float sum = 0.f;
 #pragma unroll
             for (int r = 0; r < 32; ++r) {
@@ -430,11 +530,9 @@ __global__ __launch_bounds__(kThreads, 2) void window_forward_kernel(WinArgs a) 
                 s[r >> 4][r & 15] = e;
                 sum += e;
             }
-            l = l * alpha + sum;
-#pragma unroll
-            for (int d = 0; d < D / 32; ++d) acc[d] *= alpha;
+            l += sum;
         }
-        if (!whole && any_wave(flags)) {
+        if (tiles.special(t)) {
             if (see != kNone)
                 add_special<T, D, kKeys>(acc, Vs, h, [&](int k) { return SeenKeys(top, low, a.sinks, k0, 0).at(k); });
             __syncthreads();
@@ -444,10 +542,12 @@ __global__ __launch_bounds__(kThreads, 2) void window_forward_kernel(WinArgs a) 
         if (see == kNone) continue;
 #pragma unroll
         for (int kc = 0; kc < 4; ++kc) {
+            if (HALVES && !half[kc >> 1]) continue;
             const V8<T> pf = rounded<T>(s[kc >> 1], 8 * (kc & 1));
 #pragma unroll
             for (int d = 0; d < D / 32; ++d) acc[d] = mma(across<T, D>(Vs, 16 * kc, 32 * d, lane), pf, acc[d]);
         }
+        if (!HALVES) interleave<4 * D / 32, 2, 3>();
     }
     l += other_half(l);
     if (row >= a.sq) return;
@@ -674,29 +774,40 @@ __global__ __launch_bounds__(kThreads) void window_join_kernel(WinArgs a, SplitA
 // other types need no scale.
 constexpr int kRanges = 256;
 
-// The largest finite |g| of rows inside their sequence (KEYS: |v| of keys).
-template <typename T, bool KEYS>
-__global__ __launch_bounds__(256) void window_range_kernel(WinArgs a, int64_t total, float *out) {
+// Partial maxima of |g| over the rows inside their sequence (workgroups
+// 0 .. kRanges - 1) and of |v| over its keys (the others); one row of one head
+// to 16 lanes.
+template <typename T>
+__global__ __launch_bounds__(256) void window_range_kernel(WinArgs a, int batch) {
     __shared__ float waves[4];
-    const View &x = KEYS ? a.v : a.g;
-    const int heads = KEYS ? a.kv : a.heads, rows = KEYS ? a.sk : a.sq, parts = a.width / 8;
-    float m = 0.f;
-    for (int64_t id = (int64_t)blockIdx.x * 256 + threadIdx.x; id < total; id += (int64_t)kRanges * 256) {
-        const int64_t at = id / parts, bh = at / rows, b = bh / heads;
-        const int row = (int)(at % rows);
+    const bool keys = blockIdx.x >= kRanges;
+    const View &x = keys ? a.v : a.g;
+    const int heads = keys ? a.kv : a.heads, rows = keys ? a.sk : a.sq, at = threadIdx.x % 16 * 8;
+    Largest<T> most;
+    for (int b = 0; b < batch; ++b) {
         const Seq seq(a, b);
-        const int p = KEYS ? row : seq.start + row;
-        if (p < 0 || p >= seq.n) continue;
-        Pack<T, 8> q;
-        q.load(head_of<T>(x, b, bh % heads) + row * x.s + id % parts * 8);
+        const int from = keys ? 0 : max(0, -seq.start), to = keys ? seq.n : min(rows, seq.n - seq.start);
+        if (to <= from) continue;
+        const uint32_t count = to - from, all = min((int64_t)count * heads, (int64_t)UINT32_MAX);
+        for (uint64_t id = blockIdx.x % kRanges * 16 + threadIdx.x / 16; id < (uint64_t)count * heads; id += kRanges * 16) {
+            const int64_t h = all == UINT32_MAX ? id / count : (uint32_t)id / count;
+            if (at < a.width) {
+                Pack<T, 8> q;
+                q.load(head_of<T>(x, b, h) + (int64_t)(from + (id - h * count)) * x.s + at);
 #pragma unroll
-        for (int t = 0; t < 8; ++t)
-            if (!not_finite(q.q[t])) m = fmaxf(m, fabsf(q.get(t)));
+                for (int t = 0; t < 8; ++t) q.q[t] = not_finite(q.q[t]) ? (T)0.f : q.q[t];
+                most.add(q.q);
+            }
+        }
     }
+    const V8<T> top = __builtin_bit_cast(V8<T>, most.m);
+    float m = 0.f;
+#pragma unroll
+    for (int t = 0; t < 8; ++t) m = fmaxf(m, widen<T>(top[t]));
     m = wave_vmax(m);
     if ((threadIdx.x & 63) == 0) waves[threadIdx.x >> 6] = m;
     __syncthreads();
-    if (threadIdx.x == 0) out[blockIdx.x] = fmaxf(fmaxf(waves[0], waves[1]), fmaxf(waves[2], waves[3]));
+    if (threadIdx.x == 0) a.range[blockIdx.x] = fmaxf(fmaxf(waves[0], waves[1]), fmaxf(waves[2], waves[3]));
 }
 
 // The power of two; every thread of the workgroup calls it once.
@@ -726,15 +837,14 @@ __device__ inline float gradient_scale(const WinArgs &a) {
 // dq, and D for the second kernel: rows as in the forward kernel.
 template <typename T, int D>
 __global__ __launch_bounds__(kThreads, 2) void window_dq_kernel(WinArgs a) {
-    __shared__ __attribute__((aligned(16))) T Ks[kKeys * kPitch<T, D>], Vs[kKeys * kPitch<T, D>];
-    __shared__ int flags[kWaves];
+    __shared__ __attribute__((aligned(16))) typename KeyTiles<T, D, 0>::Shared sh;
     const int tid = threadIdx.x, lane = tid & 63, i = lane & 31, h = lane >> 5;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int64_t b = blockIdx.z, head = blockIdx.y;
     const Seq seq(a, b);
     const int row0 = blockIdx.x * (32 * kWaves), mine = row0 + 32 * wave, row = mine + i;
     const int live = min(32, a.sq - mine), safe = row < a.sq ? row : 0;
-    const T *Q = head_of<T>(a.q, b, head), *K = head_of<T>(a.k, b, head / a.group), *V = head_of<T>(a.v, b, head / a.group);
+    const T *Q = head_of<T>(a.q, b, head);
     const T *G = head_of<T>(a.g, b, head), *O = head_of<T>(a.o, b, head);
     V8<T> qf[D / 16], gf[D / 16];
     float delta = 0.f;
@@ -754,26 +864,17 @@ __global__ __launch_bounds__(kThreads, 2) void window_dq_kernel(WinArgs a) {
     f32x16 acc[D / 32] = {};
     Marks<D> marks;
     const int first = seq.start + mine, p = first + i, top = row < a.sq && p < seq.n ? p : -1, low = p - a.window;
-    const KeyWalk<kKeys> walk(seq.start + row0, seq.start + min(row0 + 32 * kWaves, a.sq) - 1, seq.n, a.window, a.sinks);
     const int group_first = seq.start + row0, group_last = seq.start + min(row0 + 32 * kWaves, a.sq) - 1;
-    Staged<T, D, kKeys> ks, vs;
-    if (walk.count) {
-        ks.load(K, a.k.s, walk.tile(0) * kKeys, seq.n - 1, a.width, tid);
-        vs.load(V, a.v.s, walk.tile(0) * kKeys, seq.n - 1, a.width, tid);
-    }
+    const KeyWalk<kKeys> walk(group_first, group_last, seq.n, a.window, a.sinks);
+    KeyTiles<T, D, 0> tiles{a, sh, head_of<T>(a.k, b, head / a.group), head_of<T>(a.v, b, head / a.group), walk, seq.n,
+                            group_first, group_last, tid, wave};
+    tiles.begin();
     for (int t = 0; t < walk.count; ++t) {
+        tiles.next(t);
         const int k0 = walk.tile(t) * kKeys;
-        const bool whole = sees_all(group_first, group_last, seq.n, a.window, a.sinks, k0, k0 + kKeys - 1);
-        __syncthreads();
-        ks.store(Ks, tid);
-        vs.store(Vs, tid);
-        if (!whole) flags[wave] = __any(ks.special());
-        __syncthreads();
-        if (t + 1 < walk.count) {
-            ks.load(K, a.k.s, walk.tile(t + 1) * kKeys, seq.n - 1, a.width, tid);
-            vs.load(V, a.v.s, walk.tile(t + 1) * kKeys, seq.n - 1, a.width, tid);
-        }
-        const bool special = !whole && any_wave(flags);
+        T *Ks = sh.k[t % kBuffers<T>];
+        const T *Vs = sh.v[t % kBuffers<T>];
+        const bool special = tiles.special(t);
 #pragma unroll
         for (int kb = 0; kb < 2; ++kb) {
             const int kk = k0 + 32 * kb;
@@ -785,6 +886,7 @@ __global__ __launch_bounds__(kThreads, 2) void window_dq_kernel(WinArgs a) {
                     s = mma(along<T, D>(Ks, 32 * kb + i, 16 * u + 8 * h), qf[u], s);
                     dp = mma(along<T, D>(Vs, 32 * kb + i, 16 * u + 8 * h), gf[u], dp);
                 }
+                if (sizeof(T) == 2) interleave<D / 8, 1, 4>();
 #pragma unroll
                 for (int r = 0; r < 16; ++r) s[r] = exp2_(fmaf(s[r], a.signed_c, -lse)) * ((dp[r] - delta) * up);
                 if (see == kSome) {
@@ -807,6 +909,7 @@ __global__ __launch_bounds__(kThreads, 2) void window_dq_kernel(WinArgs a) {
 #pragma unroll
                 for (int d = 0; d < D / 32; ++d) acc[d] = mma(across<T, D>(Ks, 32 * kb + 16 * kc, 32 * d, lane), df, acc[d]);
             }
+            if (sizeof(T) == 2) interleave<2 * D / 32, 2, 3>();
         }
     }
     marks.apply(acc);
@@ -829,7 +932,7 @@ struct KeyGradients {
     }
     // Weights and dS of a tile, one key a column. Ls holds
     // shift - lse log2(e), Ds the rows' D; half scales dS.
-    template <class Keys, class Values>
+    template <int READS, class Keys, class Values>  // LDS reads a product
     __device__ void scores(f32x16 &s, f32x16 &dp, Keys keys, Values values, const T *Qs, const T *Gs, const float *Ls, const float *Ds, float c,
                            float half, bool all, const SeenRows &rows, int lane) const {
         const int i = lane & 31, h = lane >> 5;
@@ -839,6 +942,7 @@ struct KeyGradients {
             s = mma(along<T, D>(Qs, i, 16 * u + 8 * h), keys(u), s);
             dp = mma(along<T, D>(Gs, i, 16 * u + 8 * h), values(u), dp);
         }
+        if (sizeof(T) == 2) interleave<D / 8, READS, 2>();
 #pragma unroll
         for (int r4 = 0; r4 < 4; ++r4) {
             const f32x4 lr = *reinterpret_cast<const f32x4 *>(Ls + 8 * r4 + 4 * h);
@@ -869,6 +973,7 @@ struct KeyGradients {
                 dk[d] = mma(across<T, D>(Qs, 16 * kc, 32 * d, lane), df, dk[d]);
             }
         }
+        if (sizeof(T) == 2) interleave<4 * D / 32, 2, 3>();
     }
     __device__ void special(const T *Qs, const T *Gs, const SeenRows &rows, int h) {
         mv.template note<false, T, kRows>(Gs, h, [&](int r) { return rows.at(r); });
@@ -1019,7 +1124,7 @@ __global__ __launch_bounds__((kThreads * kGroups<T, D>), 1) void window_dkv_kern
         const Sight see = x.live ? sight(seq.start + x.r0, rows - x.r0, seq.n, a.window, a.sinks, mine, 32) : kNone;
         f32x16 s, dp;
         if (see != kNone)
-            w.scores(s, dp, keys, values, Qs, Gs, Ls[at][group], Ds[at][group], a.signed_c, half, see == kAll,
+            w.template scores<GROUPS>(s, dp, keys, values, Qs, Gs, Ls[at][group], Ds[at][group], a.signed_c, half, see == kAll,
                      SeenRows(key, seq.start, x.r0, h, rows, seq.n, a.window, a.sinks), lane);
         if (any_wave(flags[at]) || (GROUPS > 1 && any_wave(flags[at] + kWaves * (GROUPS - 1)))) {
             if (see != kNone) w.special(Qs, Gs, SeenRows(key, seq.start, x.r0, 0, rows, seq.n, a.window, a.sinks), h);
@@ -1132,7 +1237,7 @@ __global__ __launch_bounds__(kThreads, 1) void window_far_kernel(WinArgs a, FarA
         // the wave alone writes and reads its tile
         __builtin_amdgcn_wave_barrier();
         f32x16 s, dp;
-        w.scores(s, dp, [&](int u) { return kf[u]; }, [&](int u) { return vf[u]; }, Qs, Gs, Ls, Ds, a.signed_c, half, whole, SeenRows(key, seq.start, r0, h, rows, seq.n, a.window, key + 1), lane);
+        w.template scores<1>(s, dp, [&](int u) { return kf[u]; }, [&](int u) { return vf[u]; }, Qs, Gs, Ls, Ds, a.signed_c, half, whole, SeenRows(key, seq.start, r0, h, rows, seq.n, a.window, key + 1), lane);
         if (special) {
             w.special(Qs, Gs, SeenRows(key, seq.start, r0, 0, rows, seq.n, a.window, key + 1), h);
             clean<T, D, kRows, 64>(Qs, lane);
@@ -1385,8 +1490,7 @@ extern "C" int32_t chelis_hip_window_attention_adjoint(
     s = with_head(q->dtype, a.width, [&](auto t, auto d) -> int32_t {
         using T = decltype(t);
         if constexpr (std::is_same<T, _Float16>::value) {
-            window_range_kernel<T, false><<<kRanges, 256, 0, st>>>(a, q->count / 8, a.range);
-            window_range_kernel<T, true><<<kRanges, 256, 0, st>>>(a, k->count / 8, a.range + kRanges);
+            window_range_kernel<T><<<2 * kRanges, 256, 0, st>>>(a, (int)q->shape[0]);
         }
         if (q->count) window_dq_kernel<T, d><<<rows, kThreads, 0, st>>>(a);
         if (k->count) window_dkv_kernel<T, d><<<keys, kThreads * kGroups<T, d>, 0, st>>>(a, f);
