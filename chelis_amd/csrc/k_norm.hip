@@ -328,8 +328,10 @@ __global__ __launch_bounds__(1024) void norm_weights_kernel(const A *part, int c
     const int col = threadIdx.x & 31, k = threadIdx.x >> 5;
     const int64_t j = (int64_t)blockIdx.x * 32 + col;
     A sum = A(0);
-    if (j < 2 * n)
+    if (j < 2 * n) {
+#pragma unroll 8
         for (int b = k; b < count; b += 32) sum += part[(int64_t)b * 2 * n + j];
+    }
     lds[k][col] = sum;
     __syncthreads();
     if (k == 0 && j < 2 * n) {

@@ -32,8 +32,8 @@ struct RotaryArgs {
     int64_t pa, pb, ps;  // strides of axis, batch, sequence
     int64_t seq, tokens;
     int wide;            // positions are i64
-    int tensors, heads;  // of all tensors together
-    int pairs, width, lanes, per_thread, end[kAxes], axes;
+    int chunks;  // of the first tensor's heads; the second's follow
+    int pairs, width, lanes, per_thread, end[kAxes - 1];  // pairs before axis 1, 2, ..
     double sign;
 };
 
@@ -64,59 +64,71 @@ __global__ __launch_bounds__(256) void rotary_kernel(RotaryArgs a) {
     const int64_t token = id / a.lanes;
     if (token >= a.tokens) return;
     const int64_t b = token / a.seq, i = token % a.seq;
-    const int first = blockIdx.y * a.per_thread, last = min(first + a.per_thread, a.heads);
+    const bool second = (int)blockIdx.y >= a.chunks;
+    const RotaryTensor &t = a.t[second];
+    const int first = ((int)blockIdx.y - (second ? a.chunks : 0)) * a.per_thread, last = min(first + a.per_thread, t.heads);
+    const T *x = static_cast<const T *>(t.x) + b * t.xb + i * t.xs;
+    T *y = static_cast<T *>(t.y) + b * t.yb + i * t.ys;
     const int turned = HALVES ? a.pairs / V : 2 * a.pairs / V;
-    if (lane < turned) {
-        constexpr int N = HALVES ? V : (V > 1 ? V / 2 : 1);  // pairs of this thread
-        A sn[N], cs[N];
+    if (lane >= turned) {  // past the pairs
+        const int from = 2 * a.pairs + (lane - turned) * V;
+        for (int h = first; h < last; ++h)
+            for (int k = from; k < min(from + V, a.width); ++k) y[h * t.yh + k] = x[h * t.xh + k];
+        return;
+    }
+    constexpr int N = HALVES ? V : V / 2;  // pairs of this thread
+    A sn[N], cs[N];
 #pragma unroll
-        for (int k = 0; k < N; ++k) {
-            const int p = lane * N + k;
-            int axis = 0;
-            while (axis + 1 < a.axes && p >= a.end[axis]) ++axis;
-            const int64_t at = axis * a.pa + b * a.pb + i * a.ps;
-            const double pos = a.wide ? (double)static_cast<const int64_t *>(a.positions)[at]
-                                      : (double)static_cast<const int32_t *>(a.positions)[at];
-            sin_cos(pos * a.freqs[p], sn[k], cs[k]);
-            sn[k] = (A)a.sign * sn[k];
-        }
-        for (int head = first; head < last; ++head) {
-            const RotaryTensor &t = a.t[head >= a.t[0].heads];
-            const int h = head >= a.t[0].heads ? head - a.t[0].heads : head;
-            const T *x = static_cast<const T *>(t.x) + b * t.xb + h * t.xh + i * t.xs + lane * V;
-            T *y = static_cast<T *>(t.y) + b * t.yb + h * t.yh + i * t.ys + lane * V;
-            Pack<T, V> u, w;
-            u.load(x);
-            if constexpr (HALVES) {
-                w.load(x + a.pairs);
-                Pack<T, V> ru, rw;
+    for (int k = 0; k < N; ++k) {
+        const int p = lane * N + k;
+        int axis = 0;
 #pragma unroll
-                for (int k = 0; k < V; ++k) {
-                    ru.set(k, u.get(k) * cs[k] - w.get(k) * sn[k]);
-                    rw.set(k, u.get(k) * sn[k] + w.get(k) * cs[k]);
-                }
-                ru.store(y);
-                rw.store(y + a.pairs);
-            } else {
-                Pack<T, V> r;
+        for (int e = 0; e < kAxes - 1; ++e) axis += p >= a.end[e];
+        const int64_t at = axis * a.pa + b * a.pb + i * a.ps;
+        const double pos = a.wide ? (double)static_cast<const int64_t *>(a.positions)[at]
+                                  : (double)static_cast<const int32_t *>(a.positions)[at];
+        sin_cos(pos * a.freqs[p], sn[k], cs[k]);
+        sn[k] = (A)a.sign * sn[k];
+    }
+    x += lane * V;
+    y += lane * V;
+    auto turn = [&](const Pack<T, V> &u, const Pack<T, V> &w, T *out) {
+        Pack<T, V> ru, rw;
+        if constexpr (HALVES) {
 #pragma unroll
-                for (int k = 0; k < N; ++k) {
-                    const A p = u.get(2 * k), q = u.get(2 * k + 1);
-                    r.set(2 * k, p * cs[k] - q * sn[k]);
-                    r.set(2 * k + 1, p * sn[k] + q * cs[k]);
-                }
-                r.store(y);
+            for (int k = 0; k < V; ++k) {
+                ru.set(k, u.get(k) * cs[k] - w.get(k) * sn[k]);
+                rw.set(k, u.get(k) * sn[k] + w.get(k) * cs[k]);
+            }
+            rw.store_streamed(out + a.pairs);
+        } else {
+#pragma unroll
+            for (int k = 0; k < N; ++k) {
+                const A p = u.get(2 * k), q = u.get(2 * k + 1);
+                ru.set(2 * k, p * cs[k] - q * sn[k]);
+                ru.set(2 * k + 1, p * sn[k] + q * cs[k]);
             }
         }
-    } else {
-        const int from = 2 * a.pairs + (lane - turned) * V;
-        for (int head = first; head < last; ++head) {
-            const RotaryTensor &t = a.t[head >= a.t[0].heads];
-            const int h = head >= a.t[0].heads ? head - a.t[0].heads : head;
-            const T *x = static_cast<const T *>(t.x) + b * t.xb + h * t.xh + i * t.xs;
-            T *y = static_cast<T *>(t.y) + b * t.yb + h * t.yh + i * t.ys;
-            for (int k = from; k < min(from + V, a.width); ++k) y[k] = x[k];
+        ru.store_streamed(out);
+    };
+    // the loads of four heads go out together
+    constexpr int G = 4;
+    int h = first;
+    for (; h + G <= last; h += G) {
+        Pack<T, V> u[G], w[G];
+#pragma unroll
+        for (int g = 0; g < G; ++g) {
+            u[g].load_streamed(x + (h + g) * t.xh);
+            if constexpr (HALVES) w[g].load_streamed(x + (h + g) * t.xh + a.pairs);
         }
+#pragma unroll
+        for (int g = 0; g < G; ++g) turn(u[g], w[g], y + (h + g) * t.yh);
+    }
+    for (; h < last; ++h) {
+        Pack<T, V> u, w;
+        u.load_streamed(x + h * t.xh);
+        if constexpr (HALVES) w.load_streamed(x + h * t.xh + a.pairs);
+        turn(u, w, y + h * t.yh);
     }
 }
 
@@ -128,8 +140,11 @@ int32_t launch(RotaryArgs a, hipStream_t st) {
     // heads a thread turns with one set of sines: as many as leave two
     // workgroups a compute unit, at most eight
     const int64_t blocks = (threads + 255) / 256, want = 2 * (int64_t)device_cus();
-    a.per_thread = (int)std::max<int64_t>(1, std::min<int64_t>(8, blocks * a.heads / want));
-    const dim3 grid((unsigned)std::min<int64_t>(blocks, 0xffffffffLL), (unsigned)((a.heads + a.per_thread - 1) / a.per_thread));
+    const int heads = a.t[0].heads + a.t[1].heads;
+    a.per_thread = (int)std::max<int64_t>(1, std::min<int64_t>(8, blocks * heads / want));
+    a.chunks = (a.t[0].heads + a.per_thread - 1) / a.per_thread;
+    const dim3 grid((unsigned)std::min<int64_t>(blocks, 0xffffffffLL),
+                    (unsigned)(a.chunks + (a.t[1].heads + a.per_thread - 1) / a.per_thread));
     if (!grid_fits(blocks, 256) || grid.y > 65535)
         return set_error(CHELIS_HIP_EUNSUPPORTED, "rotary: grid too large");
     rotary_kernel<T, V, HALVES><<<grid, 256, 0, st>>>(a);
@@ -167,8 +182,10 @@ int32_t rotary(const chelis_gpu_tensor *const *xs, int32_t n, const chelis_gpu_t
     for (int32_t k = 0; k < axes; ++k) {
         if (sections[k] < 1 || sections[k] > INT32_MAX / 4 - pairs)
             return set_error(CHELIS_HIP_EDOMAIN, "%s: sections must be positive", what);
-        a.end[k] = (int)(pairs += sections[k]);
+        pairs += sections[k];
+        if (k < kAxes - 1) a.end[k] = (int)pairs;
     }
+    for (int32_t k = axes - 1; k < kAxes - 1; ++k) a.end[k] = INT32_MAX;
     for (int32_t k = 0; k < n; ++k) {
         const chelis_gpu_tensor *x = xs[k], *y = ys[k];
         if ((s = check_tensor(x, "x")) || (s = check_tensor(y, "y")) || (s = check_device(x, "x")) ||
@@ -200,7 +217,6 @@ int32_t rotary(const chelis_gpu_tensor *const *xs, int32_t n, const chelis_gpu_t
         t.x = x->data, t.y = y->data, t.heads = (int)x->shape[1];
         t.xb = x->strides[0], t.xh = x->strides[1], t.xs = x->strides[2];
         t.yb = y->strides[0], t.yh = y->strides[1], t.ys = y->strides[2];
-        a.heads += t.heads;
     }
     if (n == 2 && ys[0]->count && ys[1]->count && ys[0]->data == ys[1]->data)
         return set_error(CHELIS_HIP_EDOMAIN, "%s: the results overlap", what);
@@ -212,13 +228,12 @@ int32_t rotary(const chelis_gpu_tensor *const *xs, int32_t n, const chelis_gpu_t
         (pairs > 1 && freqs->strides[0] != 1))
         return set_error(CHELIS_HIP_EDOMAIN, "%s: freqs must be contiguous f64 [pairs]", what);
     if ((s = check_device(positions, "positions")) || (s = check_device(freqs, "freqs"))) return s;
-    a.tensors = n;
     a.positions = positions->data, a.wide = positions->dtype == CHELIS_DTYPE_I64;
     a.freqs = static_cast<const double *>(freqs->data);
     a.pa = positions->strides[0], a.pb = positions->strides[1], a.ps = positions->strides[2];
-    a.seq = seq, a.tokens = batch * seq, a.pairs = (int)pairs, a.width = (int)xs[0]->shape[3], a.axes = axes;
+    a.seq = seq, a.tokens = batch * seq, a.pairs = (int)pairs, a.width = (int)xs[0]->shape[3];
     a.sign = sign;
-    if (!a.tokens || !a.heads) return CHELIS_HIP_OK;
+    if (!a.tokens || !(a.t[0].heads + a.t[1].heads)) return CHELIS_HIP_OK;
     hipStream_t st = stream();
     if (!st) return set_error(CHELIS_HIP_EHIP, "no HIP device");
     return with_elem(xs[0]->dtype,

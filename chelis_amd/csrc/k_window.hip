@@ -987,10 +987,10 @@ struct KeyGradients {
 
 // Rows far behind the window see the sinks alone. A workgroup of keys would
 // walk all of them (one workgroup of 128 keys walking 8192 rows of four heads
-// took 3.8 ms beside 0.2 ms for the others), so they are dealt to waves of
-// their own, `splits` of them to each block of 32 sink keys. Such a block's
-// sums are then unscaled parts in scratch: part 0 from the near rows, the
-// others from the far waves, joined in order by a last launch.
+// took 3.8 ms beside 0.2 ms for the others), so they are dealt to `splits`
+// workgroups of their own for each block of 32 sink keys. Such a block's sums
+// are then unscaled parts in scratch: part 0 from the near rows, the others
+// from the far workgroups, joined in order by a last launch.
 struct FarArgs {
     float *part;  // [block][1 + splits][dk, dv][32 keys][width]; null: no far rows
     int splits, blocks;
@@ -1168,8 +1168,8 @@ __global__ __launch_bounds__((kThreads * kGroups<T, D>), 1) void window_dkv_kern
     }
 }
 
-// The far rows of one block of sink keys: every `splits`-th tile to a wave,
-// which stages it for itself.
+// The far rows of one block of sink keys: the tiles dealt to the waves, each of
+// which stages its own.
 template <typename T, int D>
 __global__ __launch_bounds__(kThreads, 1) void window_far_kernel(WinArgs a, FarArgs f) {
     __shared__ __attribute__((aligned(16))) T tiles[kWaves][2][kRows * kPitch<T, D>];
@@ -1178,8 +1178,7 @@ __global__ __launch_bounds__(kThreads, 1) void window_far_kernel(WinArgs a, FarA
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const float up = gradient_scale<T>(a), half = up * exp2_(-kShift<T>);
     const int64_t b = blockIdx.z / f.blocks, kvh = blockIdx.y;
-    const int block = blockIdx.z % f.blocks, split = blockIdx.x * kWaves + wave;
-    if (split >= f.splits) return;
+    const int block = blockIdx.z % f.blocks, split = blockIdx.x * kWaves + wave, splits = f.splits * kWaves;
     const Seq seq(a, b);
     const int key = block * 32 + i;
     KeyGradients<T, D> w;
@@ -1213,7 +1212,7 @@ __global__ __launch_bounds__(kThreads, 1) void window_far_kernel(WinArgs a, FarA
     };
     const int items = count * a.group;
     if (split < items) load(split);
-    for (int t = split; t < items; t += f.splits) {
+    for (int t = split; t < items; t += splits) {
         const int r0 = from + t % count * kRows;
 #pragma unroll
         for (int s = 0; s < PARTS; ++s) {
@@ -1233,7 +1232,7 @@ __global__ __launch_bounds__(kThreads, 1) void window_far_kernel(WinArgs a, FarA
             }
             special = __any(most.special());
         }
-        if (t + f.splits < items) load(t + f.splits);
+        if (t + splits < items) load(t + splits);
         // the wave alone writes and reads its tile
         __builtin_amdgcn_wave_barrier();
         f32x16 s, dp;
@@ -1247,7 +1246,26 @@ __global__ __launch_bounds__(kThreads, 1) void window_far_kernel(WinArgs a, FarA
         __builtin_amdgcn_wave_barrier();
     }
     w.finish();
-    store_part(f.at(b * a.kv + kvh, block, 1 + split, a.width), w, i, h, a.width, key < a.sinks);
+    // the waves' sums through LDS, dk and then dv
+    float *sums = reinterpret_cast<float *>(&tiles[0][0][0]) + lane;
+    static_assert(sizeof tiles >= sizeof(float) * (kWaves - 1) * D / 2 * 64, "sums of three waves");
+#pragma unroll
+    for (int which = 0; which < 2; ++which) {
+        f32x16(&acc)[D / 32] = which ? w.dv : w.dk;
+        __syncthreads();
+        if (wave) {
+#pragma unroll
+            for (int e = 0; e < D / 2; ++e) sums[((wave - 1) * (D / 2) + e) * 64] = acc[e >> 4][e & 15];
+        }
+        __syncthreads();
+        if (!wave) {
+#pragma unroll
+            for (int e = 0; e < D / 2; ++e)
+                acc[e >> 4][e & 15] += (sums[e * 64] + sums[(D / 2 + e) * 64]) + sums[(D + e) * 64];
+        }
+    }
+    if (wave) return;
+    store_part(f.at(b * a.kv + kvh, block, 1 + blockIdx.x, a.width), w, i, h, a.width, key < a.sinks);
 }
 
 // One key of a sink block, dk and dv: every fourth part to a wave.
@@ -1470,14 +1488,14 @@ extern "C" int32_t chelis_hip_window_attention_adjoint(
     const dim3 keys((a.sk + 127) / 128, a.kv, (unsigned)q->shape[0]);
     if (!grid_fits(rows.x, kThreads) || !grid_fits(keys.x, kThreads))
         return set_error(CHELIS_HIP_EUNSUPPORTED, "%s: grid too large", what);
-    // rows far behind the window of the first keys: dealt out four tiles to a
-    // wave, over no more waves than fill the device twice
+    // rows far behind the window of the first keys: dealt out a tile to a wave,
+    // over no more workgroups than fill the device
     FarArgs f{};
     const int64_t pairs = q->shape[0] * a.kv, far = (int64_t)a.sk - (32 * kWaves - 1) - a.window;
     if (a.sinks > 0 && q->count && far > 0) {
         f.blocks = (a.sinks + 31) / 32;
         const int64_t tiles = (std::min<int64_t>(far, a.sq) + kRows - 1) / kRows * a.group;
-        f.splits = (int)std::max<int64_t>(1, std::min<int64_t>((tiles + 3) / 4, 8 * (int64_t)device_cus() / (pairs * f.blocks)));
+        f.splits = (int)std::max<int64_t>(1, std::min<int64_t>((tiles + kWaves - 1) / kWaves, (int64_t)device_cus() / (pairs * f.blocks)));
         if (q->shape[0] * f.blocks > 65535)
             return set_error(CHELIS_HIP_EUNSUPPORTED, "%s: sequences times sink blocks past 65535", what);
     }
@@ -1496,7 +1514,7 @@ extern "C" int32_t chelis_hip_window_attention_adjoint(
         if (k->count) window_dkv_kernel<T, d><<<keys, kThreads * kGroups<T, d>, 0, st>>>(a, f);
         if (parts) {
             const unsigned z = (unsigned)(q->shape[0] * f.blocks);
-            window_far_kernel<T, d><<<dim3((f.splits + kWaves - 1) / kWaves, a.kv, z), kThreads, 0, st>>>(a, f);
+            window_far_kernel<T, d><<<dim3(f.splits, a.kv, z), kThreads, 0, st>>>(a, f);
             window_sinks_kernel<T><<<dim3(32, a.kv, z), kThreads, 0, st>>>(a, f);
         }
         return CHELIS_HIP_OK;
