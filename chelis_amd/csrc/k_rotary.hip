@@ -33,6 +33,7 @@ struct RotaryArgs {
     int64_t seq, tokens;
     int wide;            // positions are i64
     int chunks;  // of the first tensor's heads; the second's follow
+    int groups;  // neighbouring threads that take neighbouring heads
     int pairs, width, lanes, per_thread, end[kAxes - 1];  // pairs before axis 1, 2, ..
     double sign;
 };
@@ -60,22 +61,39 @@ template <typename T, int V, bool HALVES>
 __global__ __launch_bounds__(256) void rotary_kernel(RotaryArgs a) {
     using A = typename Wide<T>::type;
     const int64_t id = (int64_t)blockIdx.x * 256 + threadIdx.x;
-    const int lane = (int)(id % a.lanes);
-    const int64_t token = id / a.lanes;
+    const int lane = (int)(id % a.lanes), group = (int)(id / a.lanes % a.groups);
+    const int64_t token = id / a.lanes / a.groups;
     if (token >= a.tokens) return;
     const int64_t b = token / a.seq, i = token % a.seq;
     const bool second = (int)blockIdx.y >= a.chunks;
     const RotaryTensor &t = a.t[second];
-    const int first = ((int)blockIdx.y - (second ? a.chunks : 0)) * a.per_thread, last = min(first + a.per_thread, t.heads);
+    const int step = a.groups;
+    const int first = ((int)blockIdx.y - (second ? a.chunks : 0)) * a.per_thread * step + group;
+    const int last = min(first + a.per_thread * step, t.heads);
+    if (first >= last) return;
     const T *x = static_cast<const T *>(t.x) + b * t.xb + i * t.xs;
     T *y = static_cast<T *>(t.y) + b * t.yb + i * t.ys;
     const int turned = HALVES ? a.pairs / V : 2 * a.pairs / V;
     if (lane >= turned) {  // past the pairs
         const int from = 2 * a.pairs + (lane - turned) * V;
-        for (int h = first; h < last; ++h)
+        for (int h = first; h < last; h += step)
             for (int k = from; k < min(from + V, a.width); ++k) y[h * t.yh + k] = x[h * t.xh + k];
         return;
     }
+    x += lane * V;
+    y += lane * V;
+    // the loads of four heads go out together, the first before the angles
+    constexpr int G = 4;
+    Pack<T, V> u[G], w[G];
+    auto fetch = [&](int h) {
+#pragma unroll
+        for (int g = 0; g < G; ++g) {
+            const T *p = x + (h + g * step < last ? h + g * step : h) * t.xh;
+            u[g].load_streamed(p);
+            if constexpr (HALVES) w[g].load_streamed(p + a.pairs);
+        }
+    };
+    fetch(first);
     constexpr int N = HALVES ? V : V / 2;  // pairs of this thread
     A sn[N], cs[N];
 #pragma unroll
@@ -90,45 +108,30 @@ __global__ __launch_bounds__(256) void rotary_kernel(RotaryArgs a) {
         sin_cos(pos * a.freqs[p], sn[k], cs[k]);
         sn[k] = (A)a.sign * sn[k];
     }
-    x += lane * V;
-    y += lane * V;
-    auto turn = [&](const Pack<T, V> &u, const Pack<T, V> &w, T *out) {
-        Pack<T, V> ru, rw;
+    auto turn = [&](const Pack<T, V> &p, const Pack<T, V> &q, T *out) {
+        Pack<T, V> rp, rq;
         if constexpr (HALVES) {
 #pragma unroll
             for (int k = 0; k < V; ++k) {
-                ru.set(k, u.get(k) * cs[k] - w.get(k) * sn[k]);
-                rw.set(k, u.get(k) * sn[k] + w.get(k) * cs[k]);
+                rp.set(k, p.get(k) * cs[k] - q.get(k) * sn[k]);
+                rq.set(k, p.get(k) * sn[k] + q.get(k) * cs[k]);
             }
-            rw.store_streamed(out + a.pairs);
+            rq.store_streamed(out + a.pairs);
         } else {
 #pragma unroll
             for (int k = 0; k < N; ++k) {
-                const A p = u.get(2 * k), q = u.get(2 * k + 1);
-                ru.set(2 * k, p * cs[k] - q * sn[k]);
-                ru.set(2 * k + 1, p * sn[k] + q * cs[k]);
+                const A c = p.get(2 * k), d = p.get(2 * k + 1);
+                rp.set(2 * k, c * cs[k] - d * sn[k]);
+                rp.set(2 * k + 1, c * sn[k] + d * cs[k]);
             }
         }
-        ru.store_streamed(out);
+        rp.store_streamed(out);
     };
-    // the loads of four heads go out together
-    constexpr int G = 4;
-    int h = first;
-    for (; h + G <= last; h += G) {
-        Pack<T, V> u[G], w[G];
+    for (int h = first; h < last; h += G * step) {
 #pragma unroll
-        for (int g = 0; g < G; ++g) {
-            u[g].load_streamed(x + (h + g) * t.xh);
-            if constexpr (HALVES) w[g].load_streamed(x + (h + g) * t.xh + a.pairs);
-        }
-#pragma unroll
-        for (int g = 0; g < G; ++g) turn(u[g], w[g], y + (h + g) * t.yh);
-    }
-    for (; h < last; ++h) {
-        Pack<T, V> u, w;
-        u.load_streamed(x + h * t.xh);
-        if constexpr (HALVES) w.load_streamed(x + h * t.xh + a.pairs);
-        turn(u, w, y + h * t.yh);
+        for (int g = 0; g < G; ++g)
+            if (h + g * step < last) turn(u[g], w[g], y + (h + g * step) * t.yh);
+        if (h + G * step < last) fetch(h + G * step);
     }
 }
 
@@ -136,15 +139,18 @@ template <typename T, int V, bool HALVES>
 int32_t launch(RotaryArgs a, hipStream_t st) {
     const int turned = HALVES ? a.pairs / V : 2 * a.pairs / V;
     a.lanes = turned + (a.width - 2 * a.pairs + V - 1) / V;
-    const int64_t threads = a.tokens * a.lanes;
+    // where a token's heads lie side by side, neighbouring threads take
+    // neighbouring heads: a wave then reads whole kilobytes
+    const int heads = a.t[0].heads + a.t[1].heads;
+    a.groups = a.t[0].xh < a.t[0].xs && a.t[0].heads >= 4 ? 4 : 1;
+    const int64_t threads = a.tokens * a.lanes * a.groups;
     // heads a thread turns with one set of sines: as many as leave two
     // workgroups a compute unit, at most eight
     const int64_t blocks = (threads + 255) / 256, want = 2 * (int64_t)device_cus();
-    const int heads = a.t[0].heads + a.t[1].heads;
-    a.per_thread = (int)std::max<int64_t>(1, std::min<int64_t>(8, blocks * heads / want));
-    a.chunks = (a.t[0].heads + a.per_thread - 1) / a.per_thread;
-    const dim3 grid((unsigned)std::min<int64_t>(blocks, 0xffffffffLL),
-                    (unsigned)(a.chunks + (a.t[1].heads + a.per_thread - 1) / a.per_thread));
+    a.per_thread = (int)std::max<int64_t>(1, std::min<int64_t>(8, blocks * ((heads + a.groups - 1) / a.groups) / want));
+    const int each = a.per_thread * a.groups;
+    a.chunks = (a.t[0].heads + each - 1) / each;
+    const dim3 grid((unsigned)std::min<int64_t>(blocks, 0xffffffffLL), (unsigned)(a.chunks + (a.t[1].heads + each - 1) / each));
     if (!grid_fits(blocks, 256) || grid.y > 65535)
         return set_error(CHELIS_HIP_EUNSUPPORTED, "rotary: grid too large");
     rotary_kernel<T, V, HALVES><<<grid, 256, 0, st>>>(a);
