@@ -317,16 +317,16 @@ struct KeyWalk {
     __device__ int tile(int t) const { return t < sink_tiles ? t : window_from + t - sink_tiles; }
 };
 
-// What 32 rows from position `first` (live rows of them exist) see of keys
-// k0 .. k0 + count - 1.
+// What the rows from position `first` (at most 32; `live` of them, or more,
+// are real) see of keys k0 .. k0 + count - 1.
 enum Sight { kNone, kSome, kAll };
 __device__ inline bool sees_all(int first, int last, int n, int window, int sinks, int k0, int k1) {
     return (k1 <= first) & (last < n) & ((k0 > last - window) | (k1 < sinks));
 }
 __device__ inline Sight sight(int first, int live, int n, int window, int sinks, int k0, int count) {
-    const int last = min(first + live - 1, n - 1), k1 = k0 + count - 1;
+    const int end = first + min(live, 32) - 1, last = min(end, n - 1), k1 = k0 + count - 1;
     if ((live <= 0) | (first >= n) | (k0 > last) | ((k0 >= sinks) & (k1 <= first - window))) return kNone;
-    return (sees_all(first, first + 31, n, window, sinks, k0, k1) & (live >= 32)) ? kAll : kSome;
+    return sees_all(first, end, n, window, sinks, k0, k1) ? kAll : kSome;
 }
 // The workgroup's answer to whether a wave staged an infinity or a NaN.
 __device__ inline bool any_wave(const int *flags) {
@@ -452,7 +452,7 @@ __global__ __launch_bounds__(kThreads, 2) void window_forward_kernel(WinArgs a) 
     const int64_t b = blockIdx.z, head = blockIdx.y;
     const Seq seq(a, b);
     const int row0 = blockIdx.x * (32 * kWaves), mine = row0 + 32 * wave, row = mine + i;
-    const int live = min(32, a.sq - mine);
+    const int live = a.sq - mine;  // rows past the last hold zeros and are not stored
     const T *Q = head_of<T>(a.q, b, head);
     V8<T> qf[D / 16];
 #pragma unroll
@@ -1122,9 +1122,10 @@ __global__ __launch_bounds__((kThreads * kGroups<T, D>), 1) void window_dkv_kern
         const int at = turn & 1;
         T *Qs = sh.in.q[at][group], *Gs = sh.in.g[at][group];
         const Sight see = x.live ? sight(seq.start + x.r0, rows - x.r0, seq.n, a.window, a.sinks, mine, 32) : kNone;
+        const bool all = see == kAll && x.r0 + kRows <= rows;  // a row past the last is hidden from every key
         f32x16 s, dp;
         if (see != kNone)
-            w.template scores<GROUPS>(s, dp, keys, values, Qs, Gs, Ls[at][group], Ds[at][group], a.signed_c, half, see == kAll,
+            w.template scores<GROUPS>(s, dp, keys, values, Qs, Gs, Ls[at][group], Ds[at][group], a.signed_c, half, all,
                      SeenRows(key, seq.start, x.r0, h, rows, seq.n, a.window, a.sinks), lane);
         if (any_wave(flags[at]) || (GROUPS > 1 && any_wave(flags[at] + kWaves * (GROUPS - 1)))) {
             if (see != kNone) w.special(Qs, Gs, SeenRows(key, seq.start, x.r0, 0, rows, seq.n, a.window, a.sinks), h);
@@ -1395,9 +1396,28 @@ int32_t check_result(const chelis_gpu_tensor *t, const char *name, std::initiali
     return CHELIS_HIP_OK;
 }
 
-// Rows that fill a wave's 32 columns badly in tiles of one head: taken
-// together over the heads of a group.
-bool few_rows(const WinArgs &a) { return a.sq <= 32; }
+// Key blocks of 32 that a run of `rows` query rows can see.
+int64_t seen_blocks(const WinArgs &a, int64_t rows) {
+    const int64_t span = std::min<int64_t>(a.sk, a.window + rows - 1) / 32 + 2 + (a.sinks + 31) / 32;
+    return std::max<int64_t>(1, std::min<int64_t>((a.sk + 31) / 32, span));
+}
+
+// The rows are taken together over the heads of a group and the keys split
+// over waves when that is estimated to be faster. Measured with bf16 heads of
+// 128 (us, split against whole rows): 16 heads on 4, 16384 keys: one row 19
+// against 490, 256 rows 137 against 366; window 1024 of 8 sequences: 16 rows
+// 35 against 40, 32 rows 41 against 32; 2048 keys of 32 sequences, 32 heads on
+// 8: 8 rows 77 against 143, 32 rows 233 against 109. Both kernels' times
+// follow these lines (binary32: the products cost whole rows more than the
+// split, whose waves hold no idle rows).
+bool few_rows(const WinArgs &a, chelis_dtype dt, int64_t batch) {
+    const double f32 = dt == CHELIS_DTYPE_F32 ? 1 : 0;
+    const int64_t tasks = batch * a.kv * (((int64_t)a.group * a.sq + 31) / 32);
+    const int64_t groups = batch * a.heads * ((a.sq + 127) / 128), rounds = (groups + 511) / 512;
+    const double split = 8 + (double)tasks * seen_blocks(a, a.sq) * a.width / 32000 * (1 + 0.5 * f32);
+    const double whole = 5 + rounds * (seen_blocks(a, std::min(a.sq, 128)) / 2.0) * (0.75 + 0.005 * a.width) * (1 + 3 * f32);
+    return split < whole;
+}
 
 int32_t window_split(const WinArgs &a, chelis_dtype dt, int64_t batch, hipStream_t st, const char *what) {
     SplitArgs p{};
@@ -1405,10 +1425,11 @@ int32_t window_split(const WinArgs &a, chelis_dtype dt, int64_t batch, hipStream
     p.tiles = (p.rows + 31) / 32;
     p.pack = std::min(p.rows, 32);
     p.tasks = batch * a.kv * p.tiles;
-    // key blocks a task can see; eight waves a compute unit, a block each at least
-    const int64_t span = std::min<int64_t>(a.sk, (int64_t)a.window + a.sq - 1) / 32 + 2 + (a.sinks + 31) / 32;
-    const int64_t blocks = std::max<int64_t>(1, std::min<int64_t>((a.sk + 31) / 32, span));
-    p.splits = (int)std::min<int64_t>(std::min<int64_t>(blocks, kMaxSplits), std::max<int64_t>(1, 8 * (int64_t)device_cus() / p.tasks));
+    // eight waves a compute unit, a key block each at least; past 8 MB of
+    // parts, no more of them than a quarter of the keys and values read
+    const int64_t blocks = seen_blocks(a, a.sq), fill = 8 * (int64_t)device_cus() / p.tasks;
+    const int64_t cheap = std::max<int64_t>(blocks * 8 / p.pack, (int64_t(8) << 20) / (p.tasks * p.pack * a.width * 4));
+    p.splits = (int)std::max<int64_t>(1, std::min<int64_t>({blocks, fill, cheap, kMaxSplits}));
     const int64_t grid = (p.tasks * p.splits + kWaves - 1) / kWaves, parts = p.tasks * p.splits * p.pack;
     const int64_t rows = batch * a.heads * a.sq;
     if (!grid_fits(grid, kThreads) || !grid_fits(rows, kThreads))
@@ -1453,7 +1474,7 @@ extern "C" int32_t chelis_hip_window_attention(const chelis_gpu_tensor *q, const
     if (!q->count) return CHELIS_HIP_OK;
     hipStream_t st = stream();
     if (!st) return set_error(CHELIS_HIP_EHIP, "no HIP device");
-    if (few_rows(a)) return window_split(a, q->dtype, q->shape[0], st, what);
+    if (few_rows(a, q->dtype, q->shape[0])) return window_split(a, q->dtype, q->shape[0], st, what);
     const dim3 grid((a.sq + 127) / 128, a.heads, (unsigned)q->shape[0]);
     if (!grid_fits(grid.x, kThreads)) return set_error(CHELIS_HIP_EUNSUPPORTED, "%s: grid too large", what);
     return with_head(q->dtype, a.width, [&](auto t, auto d) -> int32_t {
