@@ -203,3 +203,24 @@ def test_captured_gradients_replay(kind, weights, rows, n):
             C.synchronize()
             for o, e, w in zip(out, eager, want):
                 assert np.array_equal(bits(o.numpy()), w) and np.array_equal(bits(e.numpy()), w)
+
+
+def test_a_call_captured_before_any_other():
+    """The scratch of a size no call asked for before is allocated while the
+    stream is being captured, and stays with the graph: eager calls of that
+    size between the replays take other storage."""
+    rows, n = 1111, 11111
+    (x, _), (gm, _), (_, _), (g, _) = operands("f32", "f32", rows, n, 3)
+    t = [C.to_device(a) for a in (x, gm, g)]
+    mean, rstd = C.to_device(x.mean(1)), C.to_device(1 / x.std(1))
+    out = [C.empty((rows, n), np.float32), C.empty((n,), np.float32), C.empty((n,), np.float32)]
+    C.synchronize()
+    graph = Captured(lambda: C.layer_norm_adjoint(t[0], t[1], mean, rstd, t[2], *out))
+    want = [bits(o.numpy()) for o in C.layer_norm_adjoint(t[0], t[1], mean, rstd, t[2])]
+    other = C.to_device(2 * g)
+    for _ in range(3):
+        graph.launch()
+        C.layer_norm_adjoint(t[0], t[1], mean, rstd, other)
+        C.synchronize()
+        for o, w in zip(out, want):
+            assert np.array_equal(bits(o.numpy()), w)

@@ -371,3 +371,51 @@ def test_captured_calls_replay(kind, S, N):
             C.synchronize()
             for a, b, w in zip(out, eager, want):
                 assert np.array_equal(bits(a.numpy()), w) and np.array_equal(bits(b.numpy()), w)
+
+
+@pytest.mark.parametrize("kind", KINDS)
+def test_numbers_at_their_limits(kind):
+    """A window and sinks past every key, and first positions past both ends
+    of any sequence."""
+    q, k, v, g = operands(kind, 2, 2, 1, 20, 20, 64, 26)
+    t = [C.to_device(x) for x in (q, k, v, g)]
+    plain = C.window_attention(*t[:3], 20, 0, 0.125).numpy()
+    for window, sinks in ((2**62, 0), (1, 2**40), (2**62, 2**62)):
+        assert np.array_equal(bits(C.window_attention(*t[:3], window, sinks, 0.125).numpy()), bits(plain))
+    far = index([-2**62, 2**62], np.int64)
+    o, lse = C.window_attention(*t[:3], 5, 1, 0.125, lse=True, starts=far)
+    assert not decode(kind, o.numpy()).any() and (lse.numpy() == -np.inf).all()
+    for d in C.window_attention_adjoint(*t[:3], o, lse, t[3], 5, 1, 0.125, starts=far):
+        assert not decode(kind, d.numpy()).any()
+
+
+@pytest.mark.parametrize("S,N", [(1, 3), (3, 3)])
+def test_rows_four_gigabytes_apart(S, N):
+    """Keys, values and gradients whose rows lie 2^31 elements apart (offsets
+    past 32 bits), in one storage: results are those of dense operands. Rotary
+    positions of 0 (a turn by nothing) write the rows where they lie."""
+    kind, W, far = "bf16", 64, 2**31
+    q, k, v, g = operands(kind, 1, 1, 1, S, N, W, 27)
+    base = C.empty((2 * far + 4 * W,), np.uint16)
+    ks, vs, dk, dv = (base.view((1, 1, N, W), (3 * far, 3 * far, far, 1), at * W) for at in range(4))
+    none, freqs = C.to_device(np.zeros((1, 1, N), np.int32)), C.to_device(np.ones(W // 2))
+    for x, to in ((k, ks), (v, vs)):
+        C.rotary(C.to_device(x), none, freqs, [W // 2], out=to)
+        assert np.array_equal(to.numpy(), x)
+    t = [C.to_device(x) for x in (q, k, v, g)]
+    o, lse = C.window_attention(*t[:3], 2, 1, 0.125, lse=True)
+    of, lf = C.window_attention(t[0], ks, vs, 2, 1, 0.125, lse=True)
+    assert np.array_equal(of.numpy(), o.numpy()) and np.array_equal(lf.numpy(), lse.numpy())
+    want = C.window_attention_adjoint(*t[:3], o, lse, t[3], 2, 1, 0.125)
+    got = C.window_attention_adjoint(t[0], ks, vs, o, lse, t[3], 2, 1, 0.125, None, dk, dv)
+    for a, b in zip(got, want):
+        assert np.array_equal(a.numpy(), b.numpy())
+    # the same rows through the norm, in place
+    one, zero = C.to_device(encode(kind, np.ones(W))), C.to_device(encode(kind, np.zeros(W)))
+    rows, dense = base.view((N, W), (far, 1)), C.to_device(k.reshape(N, W))
+    y, mean, rstd = C.layer_norm_stats(dense, one, zero, 1e-5)
+    grad = C.layer_norm_adjoint(dense, one, mean, rstd, dense)[0].numpy()
+    C.layer_norm_adjoint(rows, one, mean, rstd, rows, dx=base.view((N, W), (far, 1), 2 * W), want_weights=False)
+    assert np.array_equal(base.view((N, W), (far, 1), 2 * W).numpy(), grad)
+    C.layer_norm_stats(rows, one, zero, 1e-5, y=rows)
+    assert np.array_equal(rows.numpy(), y.numpy())
