@@ -119,10 +119,11 @@ struct Largest {
         m = __builtin_elementwise_max(m, __builtin_bit_cast(V8<U>, v) & (U)~((U)1 << (8 * sizeof(U) - 1)));
     }
     __device__ bool special() const {
-        bool any = false;
-#pragma unroll
-        for (int t = 0; t < 8; ++t) any |= m[t] >= kInf;
-        return any;
+        using U4 = U __attribute__((ext_vector_type(4)));
+        using U2 = U __attribute__((ext_vector_type(2)));
+        const U4 a = __builtin_elementwise_max(U4(m.lo), U4(m.hi));
+        const U2 b = __builtin_elementwise_max(U2(a.lo), U2(a.hi));
+        return (b[0] >= kInf) | (b[1] >= kInf);
     }
 };
 
@@ -229,6 +230,34 @@ struct WinArgs {
     float c, signed_c, scale;  // |scale| log2(e), scale log2(e), scale
 };
 
+// Which tile of which head a workgroup takes. Workgroups go round robin over
+// the eight XCDs, each with its own L2: `chunk` neighbouring tiles of a key
+// head (of all its query heads) stay on one XCD, so the keys or rows that
+// their windows share are read into one L2 instead of all eight. Later tiles
+// go first: without a window they are the longest.
+constexpr int kXcds = 8;
+struct Deal {
+    int tiles, heads, chunk;  // tiles of a pair (sequence, key head); query heads dealt with each tile
+    int64_t pairs;
+    __host__ __device__ int64_t chunks() const { return (int64_t)((tiles + chunk - 1) / chunk) * pairs; }
+    __host__ __device__ int64_t blocks() const { return (chunks() + kXcds - 1) / kXcds * kXcds * chunk * heads; }
+    // false: the workgroup has no tile
+    __device__ bool take(int64_t id, int &tile, int &head, int64_t &pair) const {
+        const int64_t xcd = id % kXcds, j = id / kXcds, unit = chunk * heads, which = j / unit * kXcds + xcd;
+        const int in = (int)(j % unit), each = (tiles + chunk - 1) / chunk;
+        pair = which / each;
+        tile = tiles - 1 - ((int)(which % each) * chunk + in / heads);
+        head = in % heads;
+        return pair < pairs && tile >= 0;
+    }
+};
+// At most 8 tiles to a chunk, and four chunks to an XCD while there are enough.
+Deal deal(int64_t extent, int per_tile, int heads, int64_t pairs) {
+    Deal d{(int)((extent + per_tile - 1) / per_tile), heads, 1, pairs};
+    d.chunk = (int)std::max<int64_t>(1, std::min<int64_t>({8, d.tiles, d.tiles * pairs / (4 * kXcds)}));
+    return d;
+}
+
 // The keys and the first row's position of sequence b. Stored lengths and
 // starts are taken into the extents the launch was checked for.
 struct Seq {
@@ -276,6 +305,15 @@ struct Staged {
             const T *p = base + row0 * step + (tid / C * step + at);
 #pragma unroll
             for (int i = 0; i < PARTS; ++i) part[i].load(p + i * (kThreads / C) * step);
+            return;
+        }
+        if (!EVEN && row0 + N - 1 <= last) {
+            const T *p = base + row0 * step;
+#pragma unroll
+            for (int i = 0; i < PARTS; ++i) {
+                const int id = min(tid + i * kThreads, ALL - 1), e = id % C * 8;
+                part[i].load(p + (id / C * step + (e < width ? e : 0)));
+            }
             return;
         }
 #pragma unroll
@@ -445,13 +483,16 @@ struct KeyTiles {
 
 // A workgroup takes 128 rows of one head, each wave 32 of them.
 template <typename T, int D>
-__global__ __launch_bounds__(kThreads, 2) void window_forward_kernel(WinArgs a) {
+__global__ __launch_bounds__(kThreads, 2) void window_forward_kernel(WinArgs a, Deal deal) {
     __shared__ __attribute__((aligned(16))) typename KeyTiles<T, D, 1>::Shared sh;
     const int tid = threadIdx.x, lane = tid & 63, i = lane & 31, h = lane >> 5;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const int64_t b = blockIdx.z, head = blockIdx.y;
+    int tile, member;
+    int64_t pair;
+    if (!deal.take(blockIdx.x, tile, member, pair)) return;
+    const int64_t b = pair / a.kv, head = pair % a.kv * a.group + member;
     const Seq seq(a, b);
-    const int row0 = blockIdx.x * (32 * kWaves), mine = row0 + 32 * wave, row = mine + i;
+    const int row0 = tile * (32 * kWaves), mine = row0 + 32 * wave, row = mine + i;
     const int live = a.sq - mine;  // rows past the last hold zeros and are not stored
     const T *Q = head_of<T>(a.q, b, head);
     V8<T> qf[D / 16];
@@ -836,13 +877,16 @@ __device__ inline float gradient_scale(const WinArgs &a) {
 
 // dq, and D for the second kernel: rows as in the forward kernel.
 template <typename T, int D>
-__global__ __launch_bounds__(kThreads, 2) void window_dq_kernel(WinArgs a) {
+__global__ __launch_bounds__(kThreads, 2) void window_dq_kernel(WinArgs a, Deal deal) {
     __shared__ __attribute__((aligned(16))) typename KeyTiles<T, D, 0>::Shared sh;
     const int tid = threadIdx.x, lane = tid & 63, i = lane & 31, h = lane >> 5;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const int64_t b = blockIdx.z, head = blockIdx.y;
+    int tile, member;
+    int64_t pair;
+    if (!deal.take(blockIdx.x, tile, member, pair)) return;
+    const int64_t b = pair / a.kv, head = pair % a.kv * a.group + member;
     const Seq seq(a, b);
-    const int row0 = blockIdx.x * (32 * kWaves), mine = row0 + 32 * wave, row = mine + i;
+    const int row0 = tile * (32 * kWaves), mine = row0 + 32 * wave, row = mine + i;
     const int live = min(32, a.sq - mine), safe = row < a.sq ? row : 0;
     const T *Q = head_of<T>(a.q, b, head);
     const T *G = head_of<T>(a.g, b, head), *O = head_of<T>(a.o, b, head);
@@ -1024,7 +1068,7 @@ template <typename T, int D>
 constexpr int kGroups = sizeof(T) == 4 && D > 64 ? 1 : 2;
 
 template <typename T, int D>
-__global__ __launch_bounds__((kThreads * kGroups<T, D>), 1) void window_dkv_kernel(WinArgs a, FarArgs f) {
+__global__ __launch_bounds__((kThreads * kGroups<T, D>), 1) void window_dkv_kernel(WinArgs a, FarArgs f, Deal deal) {
     constexpr int GROUPS = kGroups<T, D>, TILE = kRows * kPitch<T, D>, KEYS = 32 * kWaves;
     struct Buffers {
         T q[2][GROUPS][TILE], g[2][GROUPS][TILE], v[KEYS * kPitch<T, D>], k[GROUPS > 1 ? KEYS * kPitch<T, D> : 1];
@@ -1038,9 +1082,12 @@ __global__ __launch_bounds__((kThreads * kGroups<T, D>), 1) void window_dkv_kern
     __shared__ int flags[2][kWaves * GROUPS];
     const int tid = threadIdx.x & (kThreads - 1), lane = tid & 63, i = lane & 31, h = lane >> 5;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), group = __builtin_amdgcn_readfirstlane(threadIdx.x / kThreads);
-    const int64_t b = blockIdx.z, kvh = blockIdx.y;
+    int tile, member;
+    int64_t pair;
+    if (!deal.take(blockIdx.x, tile, member, pair)) return;
+    const int64_t b = pair / a.kv, kvh = pair % a.kv;
     const Seq seq(a, b);
-    const int tile0 = blockIdx.x * KEYS, mine = tile0 + 32 * wave, key = mine + i;
+    const int tile0 = tile * KEYS, mine = tile0 + 32 * wave, key = mine + i;
     KeyGradients<T, D> w;
     for (int id = threadIdx.x; id < KEYS * (D / 8); id += kThreads * GROUPS) {
         const int r = id / (D / 8), at = id % (D / 8) * 8, to = r * kPitch<T, D> + at;
@@ -1475,10 +1522,10 @@ extern "C" int32_t chelis_hip_window_attention(const chelis_gpu_tensor *q, const
     hipStream_t st = stream();
     if (!st) return set_error(CHELIS_HIP_EHIP, "no HIP device");
     if (few_rows(a, q->dtype, q->shape[0])) return window_split(a, q->dtype, q->shape[0], st, what);
-    const dim3 grid((a.sq + 127) / 128, a.heads, (unsigned)q->shape[0]);
-    if (!grid_fits(grid.x, kThreads)) return set_error(CHELIS_HIP_EUNSUPPORTED, "%s: grid too large", what);
+    const Deal rows = deal(a.sq, 32 * kWaves, a.group, q->shape[0] * a.kv);
+    if (!grid_fits(rows.blocks(), kThreads)) return set_error(CHELIS_HIP_EUNSUPPORTED, "%s: grid too large", what);
     return with_head(q->dtype, a.width, [&](auto t, auto d) -> int32_t {
-        window_forward_kernel<decltype(t), d><<<grid, kThreads, 0, st>>>(a);
+        window_forward_kernel<decltype(t), d><<<(unsigned)rows.blocks(), kThreads, 0, st>>>(a, rows);
         CHELIS_LAUNCH_CHECK();
         return CHELIS_HIP_OK;
     });
@@ -1505,9 +1552,9 @@ extern "C" int32_t chelis_hip_window_attention_adjoint(
     if (!q->count && !k->count) return CHELIS_HIP_OK;
     hipStream_t st = stream();
     if (!st) return set_error(CHELIS_HIP_EHIP, "no HIP device");
-    const dim3 rows((a.sq + 127) / 128, a.heads, (unsigned)q->shape[0]);
-    const dim3 keys((a.sk + 127) / 128, a.kv, (unsigned)q->shape[0]);
-    if (!grid_fits(rows.x, kThreads) || !grid_fits(keys.x, kThreads))
+    const Deal rows = deal(a.sq, 32 * kWaves, a.group, q->shape[0] * a.kv);
+    const Deal keys = deal(a.sk, 32 * kWaves, 1, q->shape[0] * a.kv);
+    if (!grid_fits(rows.blocks(), kThreads) || !grid_fits(keys.blocks(), 2 * kThreads))
         return set_error(CHELIS_HIP_EUNSUPPORTED, "%s: grid too large", what);
     // rows far behind the window of the first keys: dealt out a tile to a wave,
     // over no more workgroups than fill the device
@@ -1531,8 +1578,8 @@ extern "C" int32_t chelis_hip_window_attention_adjoint(
         if constexpr (std::is_same<T, _Float16>::value) {
             window_range_kernel<T><<<2 * kRanges, 256, 0, st>>>(a, (int)q->shape[0]);
         }
-        if (q->count) window_dq_kernel<T, d><<<rows, kThreads, 0, st>>>(a);
-        if (k->count) window_dkv_kernel<T, d><<<keys, kThreads * kGroups<T, d>, 0, st>>>(a, f);
+        if (q->count) window_dq_kernel<T, d><<<(unsigned)rows.blocks(), kThreads, 0, st>>>(a, rows);
+        if (k->count) window_dkv_kernel<T, d><<<(unsigned)keys.blocks(), kThreads * kGroups<T, d>, 0, st>>>(a, f, keys);
         if (parts) {
             const unsigned z = (unsigned)(q->shape[0] * f.blocks);
             window_far_kernel<T, d><<<dim3(f.splits, a.kv, z), kThreads, 0, st>>>(a, f);
