@@ -12,6 +12,10 @@
 // a second launch adds them in workgroup order: no atomics, the same bits on
 // every run. Sums and statistics are binary32 (binary64 for f64), 16-bit
 // results are rounded once.
+//
+// Bound by HBM: x, g and dx once each. [65536, 1024] bf16 with f32 weights:
+// 70-73 us (5.5 TB/s) and 3-4 us for the second launch; [4096, 1024] f32: 12-13
+// and 3 us, the partial sums' 2 MB and the second launch's latency showing.
 #include "elem.h"
 
 #include <algorithm>
@@ -59,24 +63,23 @@ __device__ inline A lane_sum(A x) {
     else return (read_lane(x, 0) + read_lane(x, 16)) + (read_lane(x, 32) + read_lane(x, 48));
 }
 
-// Two sums over a row of W waves. `slot` alternates between calls, so one
+// N sums over a row of W waves. `slot` alternates between calls, so one
 // barrier a call keeps a call's reads apart from the next one's writes.
-template <int W, int L, typename A>
-__device__ inline void row_sums(A &a, A &b, A (*lds)[2][W], int slot, int wave) {
-    a = lane_sum<L>(a);
-    b = lane_sum<L>(b);
+template <int W, int L, int N, typename A>
+__device__ inline void row_sums(A (&v)[N], A (*lds)[2][W], int slot, int wave) {
+#pragma unroll
+    for (int k = 0; k < N; ++k) v[k] = lane_sum<L>(v[k]);
     if constexpr (W > 1) {
         if ((threadIdx.x & 63) == 0) {
-            lds[slot][0][wave] = a;
-            lds[slot][1][wave] = b;
+#pragma unroll
+            for (int k = 0; k < N; ++k) lds[slot][k][wave] = v[k];
         }
         __syncthreads();
-        a = lds[slot][0][0];
-        b = lds[slot][1][0];
 #pragma unroll
-        for (int w = 1; w < W; ++w) {
-            a += lds[slot][0][w];
-            b += lds[slot][1][w];
+        for (int k = 0; k < N; ++k) {
+            v[k] = lds[slot][k][0];
+#pragma unroll
+            for (int w = 1; w < W; ++w) v[k] += lds[slot][k][w];
         }
     }
 }
@@ -110,23 +113,23 @@ __global__ __launch_bounds__(64 * W * R) void norm16_kernel(NormArgs a) {
         gm[s].load(static_cast<const WT *>(a.gamma) + c.at[s]);
         bt[s].load(static_cast<const WT *>(a.beta) + c.at[s]);
     }
-    float sum = 0.f, none = 0.f;
+    float sum[1] = {};
 #pragma unroll
     for (int s = 0; s < S; ++s)
 #pragma unroll
-        for (int i = 0; i < V; ++i) sum += i >= c.dup[s] ? q[s].get(i) : 0.f;
-    row_sums<W, L>(sum, none, lds, 0, wave % W);
-    const float mean = sum / (float)a.n;
-    float sq = 0.f;
+        for (int i = 0; i < V; ++i) sum[0] += i >= c.dup[s] ? q[s].get(i) : 0.f;
+    row_sums<W, L>(sum, lds, 0, wave % W);
+    const float mean = sum[0] / (float)a.n;
+    float sq[1] = {};
 #pragma unroll
     for (int s = 0; s < S; ++s)
 #pragma unroll
         for (int i = 0; i < V; ++i) {
             const float d = q[s].get(i) - mean;
-            sq += i >= c.dup[s] ? d * d : 0.f;
+            sq[0] += i >= c.dup[s] ? d * d : 0.f;
         }
-    row_sums<W, L>(sq, none, lds, 1, wave % W);
-    const float rstd = 1.f / sqrtf(sq / (float)a.n + (float)a.eps);
+    row_sums<W, L>(sq, lds, 1, wave % W);
+    const float rstd = 1.f / sqrtf(sq[0] / (float)a.n + (float)a.eps);
     if (!live) return;
     T *y = static_cast<T *>(a.y) + row * a.ldy;
 #pragma unroll
@@ -145,12 +148,11 @@ __global__ __launch_bounds__(64 * W * R) void norm16_kernel(NormArgs a) {
 // Rows past the register capacity: one workgroup a row, three passes.
 constexpr int kLongThreads = 1024;
 
-template <typename A>
-__device__ inline void block_sums(A &a, A &b) {
+template <int N, typename A>
+__device__ inline void block_sums(A (&v)[N]) {
     __shared__ A lds[2][2][kLongThreads / 64];
-    static_assert(kLongThreads == 1024, "sixteen waves");
     __syncthreads();
-    row_sums<kLongThreads / 64, 64>(a, b, lds, 0, threadIdx.x >> 6);
+    row_sums<kLongThreads / 64, 64>(v, lds, 0, threadIdx.x >> 6);
 }
 
 template <typename T, typename WT>
@@ -158,16 +160,16 @@ __global__ __launch_bounds__(kLongThreads) void norm16_long_kernel(NormArgs a) {
     for (int64_t row = blockIdx.x; row < a.rows; row += gridDim.x) {
         const T *x = static_cast<const T *>(a.x) + row * a.ldx;
         T *y = static_cast<T *>(a.y) + row * a.ldy;
-        float sum = 0.f, sq = 0.f, none = 0.f;
-        for (int j = threadIdx.x; j < a.n; j += kLongThreads) sum += widen(x[j]);
-        block_sums(sum, none);
-        const float mean = sum / (float)a.n;
+        float sum[1] = {}, sq[1] = {};
+        for (int j = threadIdx.x; j < a.n; j += kLongThreads) sum[0] += widen(x[j]);
+        block_sums(sum);
+        const float mean = sum[0] / (float)a.n;
         for (int j = threadIdx.x; j < a.n; j += kLongThreads) {
             const float d = widen(x[j]) - mean;
-            sq += d * d;
+            sq[0] += d * d;
         }
-        block_sums(sq, none);
-        const float rstd = 1.f / sqrtf(sq / (float)a.n + (float)a.eps);
+        block_sums(sq);
+        const float rstd = 1.f / sqrtf(sq[0] / (float)a.n + (float)a.eps);
         for (int j = threadIdx.x; j < a.n; j += kLongThreads)
             y[j] = finalize<T>((widen(x[j]) - mean) * rstd * widen(static_cast<const WT *>(a.gamma)[j]) +
                                widen(static_cast<const WT *>(a.beta)[j]));
@@ -191,10 +193,10 @@ __global__ __launch_bounds__(64 * W * R) void norm_adjoint_kernel(NormArgs a) {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const int tid = L == 64 ? (wave % W) * 64 + lane : lane % L;
     const int group = L == 64 ? wave / W : wave * (64 / L) + lane / L;
-    const Columns<V, S, W, L> c(a.n, tid);
+    const Columns<V, S, W, L> col(a.n, tid);
     Pack<WT, V> gm[S];
 #pragma unroll
-    for (int s = 0; s < S; ++s) gm[s].load(static_cast<const WT *>(a.gamma) + c.at[s]);
+    for (int s = 0; s < S; ++s) gm[s].load(static_cast<const WT *>(a.gamma) + col.at[s]);
     A dg[S][V], db[S][V];
 #pragma unroll
     for (int s = 0; s < S; ++s)
@@ -209,29 +211,28 @@ __global__ __launch_bounds__(64 * W * R) void norm_adjoint_kernel(NormArgs a) {
         const T *x = static_cast<const T *>(a.x) + row * a.ldx, *g = static_cast<const T *>(a.g) + row * a.ldg;
         Pack<T, V> xq[S], gq[S];
 #pragma unroll
-        for (int s = 0; s < S; ++s) xq[s].load_streamed(x + c.at[s]);
+        for (int s = 0; s < S; ++s) xq[s].load_streamed(x + col.at[s]);
 #pragma unroll
-        for (int s = 0; s < S; ++s) gq[s].load_streamed(g + c.at[s]);
+        for (int s = 0; s < S; ++s) gq[s].load_streamed(g + col.at[s]);
         const A mean = static_cast<const A *>(a.mean)[row], rstd = static_cast<const A *>(a.rstd)[row];
-        A c1 = A(0), c2 = A(0);
+        A c[2] = {};
 #pragma unroll
         for (int s = 0; s < S; ++s)
 #pragma unroll
             for (int i = 0; i < V; ++i) {
                 const A h = (xq[s].get(i) - mean) * rstd, gv = gq[s].get(i), w = gv * gm[s].get(i);
-                const bool own = i >= c.dup[s];
-                c1 += own ? w : A(0);
-                c2 += own ? w * h : A(0);
+                const bool own = i >= col.dup[s];
+                c[0] += own ? w : A(0);
+                c[1] += own ? w * h : A(0);
                 if (live) {
                     dg[s][i] += gv * h;
                     db[s][i] += gv;
                 }
             }
         if (a.dx) {
-            row_sums<W, L>(c1, c2, lds, slot, wave % W);
+            row_sums<W, L>(c, lds, slot, wave % W);
             slot ^= 1;
-            c1 *= inv_n;
-            c2 *= inv_n;
+            const A c1 = c[0] * inv_n, c2 = c[1] * inv_n;
             T *dx = static_cast<T *>(a.dx) + row * a.ldy;
             if (live) {
 #pragma unroll
@@ -242,7 +243,7 @@ __global__ __launch_bounds__(64 * W * R) void norm_adjoint_kernel(NormArgs a) {
                         const A h = (xq[s].get(i) - mean) * rstd;
                         out.set(i, rstd * (gq[s].get(i) * gm[s].get(i) - c1 - h * c2));
                     }
-                    store_own<V>(out, dx, c.at[s], c.dup[s]);
+                    store_own<V>(out, dx, col.at[s], col.dup[s]);
                 }
             }
         }
@@ -254,9 +255,9 @@ __global__ __launch_bounds__(64 * W * R) void norm_adjoint_kernel(NormArgs a) {
         for (int s = 0; s < S; ++s)
 #pragma unroll
             for (int i = 0; i < V; ++i)
-                if (i >= c.dup[s]) {
-                    part[c.at[s] + i] = dg[s][i];
-                    part[a.n + c.at[s] + i] = db[s][i];
+                if (i >= col.dup[s]) {
+                    part[col.at[s] + i] = dg[s][i];
+                    part[a.n + col.at[s] + i] = db[s][i];
                 }
     } else {
 #pragma unroll
@@ -266,7 +267,7 @@ __global__ __launch_bounds__(64 * W * R) void norm_adjoint_kernel(NormArgs a) {
             for (int s = 0; s < S; ++s)
 #pragma unroll
                 for (int i = 0; i < V; ++i)
-                    if (i >= c.dup[s]) join[group * CAP + c.at[s] + i] = which ? db[s][i] : dg[s][i];
+                    if (i >= col.dup[s]) join[group * CAP + col.at[s] + i] = which ? db[s][i] : dg[s][i];
             __syncthreads();
             for (int j = threadIdx.x; j < a.n; j += 64 * W * R) {
                 A sum = join[j];
@@ -285,15 +286,14 @@ __global__ __launch_bounds__(kLongThreads) void norm_adjoint_long_kernel(NormArg
         const T *x = static_cast<const T *>(a.x) + row * a.ldx, *g = static_cast<const T *>(a.g) + row * a.ldg;
         const WT *gamma = static_cast<const WT *>(a.gamma);
         const A mean = static_cast<const A *>(a.mean)[row], rstd = static_cast<const A *>(a.rstd)[row];
-        A c1 = A(0), c2 = A(0);
+        A c[2] = {};
         for (int j = threadIdx.x; j < a.n; j += kLongThreads) {
             const A w = widen(g[j]) * (A)widen(gamma[j]);
-            c1 += w;
-            c2 += w * ((widen(x[j]) - mean) * rstd);
+            c[0] += w;
+            c[1] += w * ((widen(x[j]) - mean) * rstd);
         }
-        block_sums(c1, c2);
-        c1 /= (A)a.n;
-        c2 /= (A)a.n;
+        block_sums(c);
+        const A c1 = c[0] / (A)a.n, c2 = c[1] / (A)a.n;
         T *dx = static_cast<T *>(a.dx) + row * a.ldy;
         for (int j = threadIdx.x; j < a.n; j += kLongThreads)
             dx[j] = finalize<T>(rstd * (widen(g[j]) * (A)widen(gamma[j]) - c1 - (widen(x[j]) - mean) * rstd * c2));
@@ -411,7 +411,8 @@ int32_t adjoint(NormArgs a, void *dgamma, void *dbeta, hipStream_t st) {
             norm_adjoint_long_kernel<T, WT><<<(unsigned)std::min<int64_t>(a.rows, 65536), kLongThreads, 0, st>>>(a);
     } else {
         status = with_shape<T>(a.n, [&](auto V, auto S, auto W, auto R, auto L) -> int32_t {
-            // two waves a SIMD over the whole device
+            // two waves a SIMD over the whole device: more would only
+            // write more partial sums
             const int64_t most = (int64_t)device_cus() * 8 / (W * R);
             const int64_t grid = std::max<int64_t>(1, std::min<int64_t>(most, (a.rows + R * (64 / L) - 1) / (R * (64 / L))));
             if (int32_t s = partials(grid)) return s;

@@ -4,7 +4,9 @@
 //   (u, v) -> (u cos t - v sin t, u sin t + v cos t),
 // the gradient by -t, and the width past the pairs is copied.
 //
-// Bound by the reads and writes of x. Angles are binary64 (a position of 10^5
+// Bound by the reads and writes of x ([2, 8192, 16 + 16 heads of 64] f32, the
+// heads inside the sequence axis: 47 us, 5.7 TB/s; 59 us while neighbouring
+// threads took neighbouring tokens). Angles are binary64 (a position of 10^5
 // leaves no correct digit of the fraction of a turn at binary32), brought to
 // [-pi/4, pi/4] by quarter turns and then taken to the arithmetic width; one
 // thread computes the sines of V pairs of a token once and turns them in

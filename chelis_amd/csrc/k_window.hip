@@ -143,10 +143,10 @@ __device__ inline void add_special(f32x16 (&acc)[D / 32], const T *tile, int h, 
             }
     }
 }
-// The same as marks, one bit an accumulated element, for kernels whose
-// accumulators only the matrix cores touch while they run (touching them here
-// made the compiler move all of them between register files on every tile).
-// With SIGNED weights the sum becomes NaN.
+// The same as marks, one bit an accumulated element, put in once the sums are
+// whole: for kernels whose accumulators only the matrix cores touch while they
+// run (any other use made the compiler move all of them between register files
+// on every tile). With weights of either sign any special value makes the sum NaN.
 template <int D>
 struct Marks {
     static constexpr int W = (D / 2 + 31) / 32;
@@ -305,15 +305,6 @@ struct Staged {
             const T *p = base + row0 * step + (tid / C * step + at);
 #pragma unroll
             for (int i = 0; i < PARTS; ++i) part[i].load(p + i * (kThreads / C) * step);
-            return;
-        }
-        if (!EVEN && row0 + N - 1 <= last) {
-            const T *p = base + row0 * step;
-#pragma unroll
-            for (int i = 0; i < PARTS; ++i) {
-                const int id = min(tid + i * kThreads, ALL - 1), e = id % C * 8;
-                part[i].load(p + (id / C * step + (e < width ? e : 0)));
-            }
             return;
         }
 #pragma unroll
@@ -481,7 +472,11 @@ struct KeyTiles {
     __device__ bool special(int t) const { return !whole(walk.tile(t) * kKeys) && any_wave(sh.flags[t & 1]); }
 };
 
-// A workgroup takes 128 rows of one head, each wave 32 of them.
+// A workgroup takes 128 rows of one head, each wave 32 of them, which share
+// the staged keys; the rows' q stays in registers. Bound by the softmax
+// between the two products at two waves a SIMD: [2, 16 on 4, 8192, 128] bf16,
+// window 1024, 198 us (matrix cores 29 %, LDS 37 % busy; 650 TFLOP/s over the visible
+// pairs, 1.1 PFLOP/s without a window); [8, 16, 512, 64] f32, window 128, 51 us.
 template <typename T, int D>
 __global__ __launch_bounds__(kThreads, 2) void window_forward_kernel(WinArgs a, Deal deal) {
     __shared__ __attribute__((aligned(16))) typename KeyTiles<T, D, 1>::Shared sh;
@@ -607,9 +602,11 @@ __global__ __launch_bounds__(kThreads, 2) void window_forward_kernel(WinArgs a, 
 // key blocks of a task are dealt to `splits` waves, each on its own: it keeps
 // its next 32 keys in flight in registers (a row of k per lane pair as the
 // products want it, v on its way to the wave's own LDS tile) and no wave
-// waits for another. Bound by the reads of k and v. With one split the wave
-// stores its rows; else it leaves their sums, maxima and unscaled results in
-// scratch and a second launch joins them in split order.
+// waits for another. With one split the wave stores its rows; else it leaves
+// their sums, maxima and unscaled results in scratch and a second launch joins
+// them in split order. Bound by the reads of k and v: one token of each of 64
+// sequences of up to 16384 keys, window 4096, 32 heads of 128 on 8, bf16: 219
+// us (4.9 TB/s); of one sequence 10.5 us, both launches' latency.
 struct SplitArgs {
     float *part;  // per task, split and row: [width] results, then maxima and sums
     float *stat;
@@ -875,7 +872,9 @@ __device__ inline float gradient_scale(const WinArgs &a) {
     return most > 0.f ? ldexpf(1.f, min(14 - ilogbf(most), 100)) : 1.f;
 }
 
-// dq, and D for the second kernel: rows as in the forward kernel.
+// dq, and D for the second kernel: rows as in the forward kernel, q and g in
+// registers, three products a block. [1, 16 on 4, 8192, 128] bf16, window
+// 1024: 140 us (matrix cores 28 %, LDS 34 % busy).
 template <typename T, int D>
 __global__ __launch_bounds__(kThreads, 2) void window_dq_kernel(WinArgs a, Deal deal) {
     __shared__ __attribute__((aligned(16))) typename KeyTiles<T, D, 0>::Shared sh;
@@ -1064,6 +1063,10 @@ __device__ inline void store_part(float *part, const KeyGradients<T, D> &w, int 
 // The near rows: a workgroup takes 128 keys, 32 to a wave, in `GROUPS` groups
 // of four waves that take the row tiles in turn and add their sums up at the
 // end. k and v stay in LDS. Row tiles are double buffered, one barrier a tile.
+// [1, 16 on 4, 8192, 128] bf16, window 1024: 212 us, bound by LDS (48 % busy)
+// with one workgroup a CU. k and v in registers at one wave a SIMD took 240-245;
+// two groups with k alone there spill (325); four waves for dv and four for
+// dk, which form the scores twice, 262-278.
 template <typename T, int D>
 constexpr int kGroups = sizeof(T) == 4 && D > 64 ? 1 : 2;
 
@@ -1453,12 +1456,14 @@ int64_t seen_blocks(const WinArgs &a, int64_t rows) {
 // over waves when that is estimated to be faster. Measured with bf16 heads of
 // 128 (us, split against whole rows): 16 heads on 4, 16384 keys: one row 19
 // against 490, 256 rows 137 against 366; window 1024 of 8 sequences: 16 rows
-// 35 against 40, 32 rows 41 against 32; 2048 keys of 32 sequences, 32 heads on
-// 8: 8 rows 77 against 143, 32 rows 233 against 109. Both kernels' times
+// 23 against 40, 32 rows 34-41 against 32; 2048 keys of 32 sequences, 32 heads on
+// 8: 8 rows 77 against 143, 16 rows 136 against 110, 32 rows 233 against 110. Both kernels' times
 // follow these lines (binary32: the products cost whole rows more than the
 // split, whose waves hold no idle rows).
 bool few_rows(const WinArgs &a, chelis_dtype dt, int64_t batch) {
     const double f32 = dt == CHELIS_DTYPE_F32 ? 1 : 0;
+    // the split's rows are counted in 32 bits
+    if ((int64_t)a.group * a.sq > kMaxExtent) return false;
     const int64_t tasks = batch * a.kv * (((int64_t)a.group * a.sq + 31) / 32);
     const int64_t groups = batch * a.heads * ((a.sq + 127) / 128), rounds = (groups + 511) / 512;
     const double split = 8 + (double)tasks * seen_blocks(a, a.sq) * a.width / 32000 * (1 + 0.5 * f32);

@@ -15,8 +15,9 @@
  * Numerics: every float result is finalized at its dtype with NaN stored as
  * the canonical quiet NaN ([04-NUM-2]); every float sum follows the
  * canonical adjacent-pair tree ([05-OP-30]) bit for bit; RNG, relu, count
- * and max/min selection are bit-exact. Matmuls on the MFMA path are the
- * only results that differ from the canonical tree (by rounding only).
+ * and max/min selection are bit-exact. Matmuls on the MFMA path, the fused
+ * attentions and the training operators below are the only results that
+ * differ from the canonical tree (by rounding only).
  */
 #ifndef CHELIS_HIP_H
 #define CHELIS_HIP_H
@@ -91,7 +92,9 @@ int32_t chelis_hip_layer_norm(const chelis_gpu_tensor *x, const chelis_gpu_tenso
  * weights are held in binary32 (binary64 for f64) and a 16-bit result is
  * rounded once. Sums run in the kernels' own fixed order: the same bits on
  * every run, not the canonical tree's. Results may not share storage with
- * inputs unless said so. */
+ * inputs unless said so. Calls captured into a graph keep the scratch they
+ * took for that graph. On a machine with several devices, operands must lie
+ * on the current one. */
 
 /* layer_norm with the row statistics its gradient needs: y as
  * chelis_hip_layer_norm (bit for bit at f32 and f64), mean and
