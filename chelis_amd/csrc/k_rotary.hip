@@ -62,11 +62,12 @@ __device__ inline void sin_cos(double t, double &s, double &c) { sincos(t, &s, &
 template <typename T, int V, bool HALVES>
 __global__ __launch_bounds__(256) void rotary_kernel(RotaryArgs a) {
     using A = typename Wide<T>::type;
-    const int64_t id = (int64_t)blockIdx.x * 256 + threadIdx.x;
-    const int lane = (int)(id % a.lanes), group = (int)(id / a.lanes % a.groups);
-    const int64_t token = id / a.lanes / a.groups;
+    // a launch's threads are counted in 32 bits
+    const uint32_t id = blockIdx.x * 256 + threadIdx.x, rest = id / (uint32_t)a.lanes;
+    const int lane = (int)(id - rest * a.lanes), group = (int)(rest % (uint32_t)a.groups);
+    const uint32_t token = rest / (uint32_t)a.groups;
     if (token >= a.tokens) return;
-    const int64_t b = token / a.seq, i = token % a.seq;
+    const int64_t b = token / (uint32_t)a.seq, i = token % (uint32_t)a.seq;
     const bool second = (int)blockIdx.y >= a.chunks;
     const RotaryTensor &t = a.t[second];
     const int step = a.groups;

@@ -241,12 +241,13 @@ struct Deal {
     int64_t pairs;
     __host__ __device__ int64_t chunks() const { return (int64_t)((tiles + chunk - 1) / chunk) * pairs; }
     __host__ __device__ int64_t blocks() const { return (chunks() + kXcds - 1) / kXcds * kXcds * chunk * heads; }
-    // false: the workgroup has no tile
-    __device__ bool take(int64_t id, int &tile, int &head, int64_t &pair) const {
-        const int64_t xcd = id % kXcds, j = id / kXcds, unit = chunk * heads, which = j / unit * kXcds + xcd;
-        const int in = (int)(j % unit), each = (tiles + chunk - 1) / chunk;
+    // false: the workgroup has no tile. A launch's workgroups, and so its
+    // pairs, are counted in 32 bits.
+    __device__ bool take(uint32_t id, int &tile, int &head, uint32_t &pair) const {
+        const uint32_t xcd = id % kXcds, j = id / kXcds, unit = chunk * heads, which = j / unit * kXcds + xcd;
+        const uint32_t in = j % unit, each = (uint32_t)(tiles + chunk - 1) / chunk;
         pair = which / each;
-        tile = tiles - 1 - ((int)(which % each) * chunk + in / heads);
+        tile = tiles - 1 - (int)(which % each * chunk + in / heads);
         head = in % heads;
         return pair < pairs && tile >= 0;
     }
@@ -483,9 +484,9 @@ __global__ __launch_bounds__(kThreads, 2) void window_forward_kernel(WinArgs a, 
     const int tid = threadIdx.x, lane = tid & 63, i = lane & 31, h = lane >> 5;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     int tile, member;
-    int64_t pair;
+    uint32_t pair;
     if (!deal.take(blockIdx.x, tile, member, pair)) return;
-    const int64_t b = pair / a.kv, head = pair % a.kv * a.group + member;
+    const int64_t b = pair / (uint32_t)a.kv, head = pair % (uint32_t)a.kv * a.group + member;
     const Seq seq(a, b);
     const int row0 = tile * (32 * kWaves), mine = row0 + 32 * wave, row = mine + i;
     const int live = a.sq - mine;  // rows past the last hold zeros and are not stored
@@ -606,7 +607,7 @@ __global__ __launch_bounds__(kThreads, 2) void window_forward_kernel(WinArgs a, 
 // their sums, maxima and unscaled results in scratch and a second launch joins
 // them in split order. Bound by the reads of k and v: one token of each of 64
 // sequences of up to 16384 keys, window 4096, 32 heads of 128 on 8, bf16: 219
-// us (4.9 TB/s); of one sequence 10.5 us, both launches' latency.
+// us (4.9 TB/s); of one sequence 9.9 us, both launches' latency.
 struct SplitArgs {
     float *part;  // per task, split and row: [width] results, then maxima and sums
     float *stat;
@@ -620,10 +621,12 @@ __global__ __launch_bounds__(kThreads, 2) void window_split_kernel(WinArgs a, Sp
     __shared__ __attribute__((aligned(16))) T tiles[kWaves][N * kPitch<T, D>];
     const int tid = threadIdx.x, lane = tid & 63, i = lane & 31, h = lane >> 5;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const int64_t id = (int64_t)blockIdx.x * kWaves + wave, task = id / p.splits;
+    // a launch's waves, and so its tasks, are counted in 32 bits
+    const uint32_t id = blockIdx.x * kWaves + wave, task = id / (uint32_t)p.splits;
     if (task >= p.tasks) return;
-    const int split = (int)(id % p.splits), rt = (int)(task % p.tiles);
-    const int64_t kvh = task / p.tiles % a.kv, b = task / p.tiles / a.kv;
+    const int split = (int)(id % (uint32_t)p.splits), rt = (int)(task % (uint32_t)p.tiles);
+    const uint32_t pair = task / (uint32_t)p.tiles;
+    const int64_t kvh = pair % (uint32_t)a.kv, b = pair / (uint32_t)a.kv;
     const Seq seq(a, b);
     const int r = rt * N + i, live = r < p.rows, rs = live ? r : 0;
     const int64_t head = kvh * a.group + rs / a.sq;
@@ -720,7 +723,7 @@ __global__ __launch_bounds__(kThreads, 2) void window_split_kernel(WinArgs a, Sp
     l += other_half(l);
     if (!live) return;
     if (p.splits > 1) {
-        const int64_t at = (task * p.splits + split) * p.pack + i;
+        const int64_t at = (int64_t)id * p.pack + i;
         float *out = p.part + at * a.width;
 #pragma unroll
         for (int d = 0; d < D / 32; ++d)
@@ -746,25 +749,38 @@ __global__ __launch_bounds__(kThreads, 2) void window_split_kernel(WinArgs a, Sp
 
 // One row a workgroup: the splits' results under their common maximum, every
 // eighth (or sixteenth) split to a group of threads, the groups joined in
-// order. (One wave walking the splits one after another took 24 us for the 35
-// splits of a single token over 1024 keys, the loads' latency each time.)
+// order. Latency bound: the statistics and a thread's first parts are read at
+// once. (Statistics, sums and parts one after another took 4.0 us for a single
+// token over 1024 keys, one wave walking its 35 splits 24 us.)
 constexpr int kMaxSplits = 2048;
 
 template <typename T, int D>
 __global__ __launch_bounds__(kThreads) void window_join_kernel(WinArgs a, SplitArgs p) {
-    constexpr int LANES = D / 4, GROUPS = kThreads / LANES;
+    constexpr int LANES = D / 4, GROUPS = kThreads / LANES, AHEAD = 4;
     __shared__ float weight[kMaxSplits], waves[2][kWaves];
     __shared__ f32x4 join[GROUPS][LANES];
-    const int64_t id = blockIdx.x, row = id % a.sq, bh = id / a.sq, b = bh / a.heads, head = bh % a.heads;
-    const int tid = threadIdx.x, r = (int)(head % a.group * a.sq + row);
-    const int64_t task = (b * a.kv + head / a.group) * p.tiles + r / 32, at = task * p.splits * p.pack + r % 32;
+    typedef float f32x2 __attribute__((ext_vector_type(2)));
+    const uint32_t id = blockIdx.x, sq = a.sq, bh = id / sq;
+    const int64_t row = id % sq, b = bh / (uint32_t)a.heads;
+    const uint32_t head = bh % (uint32_t)a.heads, kvh = head / (uint32_t)a.group;
+    const int tid = threadIdx.x, r = (int)((head - kvh * a.group) * sq + row);
+    const int64_t task = (b * a.kv + kvh) * p.tiles + r / 32, at = task * p.splits * p.pack + r % 32;
     const int lane = tid % LANES, group = tid / LANES;
     const bool own = group < GROUPS && 4 * lane < a.width;
-    float m = -INFINITY;
-    for (int s = tid; s < p.splits; s += kThreads) {
-        weight[s] = p.stat[2 * (at + (int64_t)s * p.pack)];
-        m = fmaxf(m, weight[s]);
+    const f32x2 *stat = reinterpret_cast<const f32x2 *>(p.stat) + at;
+    const float *part = p.part + at * a.width + 4 * lane;
+    const int64_t step = (int64_t)p.pack * a.width;
+    f32x2 mine = {-INFINITY, 0.f};  // maximum and sum of split tid
+    if (tid < p.splits) mine = stat[(int64_t)tid * p.pack];
+    f32x4 ahead[AHEAD] = {};
+    if (own) {
+#pragma unroll
+        for (int k = 0; k < AHEAD; ++k)
+            if (group + k * GROUPS < p.splits) ahead[k] = *reinterpret_cast<const f32x4 *>(part + (group + k * GROUPS) * step);
     }
+    const Seq seq(a, b);
+    float m = mine[0];
+    for (int s = tid + kThreads; s < p.splits; s += kThreads) m = fmaxf(m, stat[(int64_t)s * p.pack][0]);
     m = wave_vmax(m);
     if ((tid & 63) == 0) waves[0][tid >> 6] = m;
     __syncthreads();
@@ -772,9 +788,10 @@ __global__ __launch_bounds__(kThreads) void window_join_kernel(WinArgs a, SplitA
     const float ref = m == -INFINITY ? 0.f : m;
     float l = 0.f;
     for (int s = tid; s < p.splits; s += kThreads) {
-        const float f = exp2_(weight[s] - ref);
+        const f32x2 q = s == tid ? mine : stat[(int64_t)s * p.pack];
+        const float f = exp2_(q[0] - ref);
         weight[s] = f;
-        l = fmaf(f, p.stat[2 * (at + (int64_t)s * p.pack) + 1], l);
+        l = fmaf(f, q[1], l);
     }
     l = wave_tree_sum(l);
     if ((tid & 63) == 0) waves[1][tid >> 6] = l;
@@ -782,14 +799,15 @@ __global__ __launch_bounds__(kThreads) void window_join_kernel(WinArgs a, SplitA
     l = (waves[1][0] + waves[1][1]) + (waves[1][2] + waves[1][3]);
     f32x4 x = {};
     if (own) {
-        const float *part = p.part + at * a.width + 4 * lane;
+#pragma unroll
+        for (int k = 0; k < AHEAD; ++k)
+            if (group + k * GROUPS < p.splits) x += weight[group + k * GROUPS] * ahead[k];
 #pragma unroll 4
-        for (int s = group; s < p.splits; s += GROUPS)
-            x += weight[s] * *reinterpret_cast<const f32x4 *>(part + (int64_t)s * p.pack * a.width);
+        for (int s = group + AHEAD * GROUPS; s < p.splits; s += GROUPS)
+            x += weight[s] * *reinterpret_cast<const f32x4 *>(part + s * step);
         join[group][lane] = x;
     }
     __syncthreads();
-    const Seq seq(a, b);
     const int pos = seq.start + (int)row;
     const bool empty = pos < 0 || pos >= seq.n;
     if (own && group == 0) {
@@ -881,9 +899,9 @@ __global__ __launch_bounds__(kThreads, 2) void window_dq_kernel(WinArgs a, Deal 
     const int tid = threadIdx.x, lane = tid & 63, i = lane & 31, h = lane >> 5;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     int tile, member;
-    int64_t pair;
+    uint32_t pair;
     if (!deal.take(blockIdx.x, tile, member, pair)) return;
-    const int64_t b = pair / a.kv, head = pair % a.kv * a.group + member;
+    const int64_t b = pair / (uint32_t)a.kv, head = pair % (uint32_t)a.kv * a.group + member;
     const Seq seq(a, b);
     const int row0 = tile * (32 * kWaves), mine = row0 + 32 * wave, row = mine + i;
     const int live = min(32, a.sq - mine), safe = row < a.sq ? row : 0;
@@ -1086,9 +1104,9 @@ __global__ __launch_bounds__((kThreads * kGroups<T, D>), 1) void window_dkv_kern
     const int tid = threadIdx.x & (kThreads - 1), lane = tid & 63, i = lane & 31, h = lane >> 5;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), group = __builtin_amdgcn_readfirstlane(threadIdx.x / kThreads);
     int tile, member;
-    int64_t pair;
+    uint32_t pair;
     if (!deal.take(blockIdx.x, tile, member, pair)) return;
-    const int64_t b = pair / a.kv, kvh = pair % a.kv;
+    const int64_t b = pair / (uint32_t)a.kv, kvh = pair % (uint32_t)a.kv;
     const Seq seq(a, b);
     const int tile0 = tile * KEYS, mine = tile0 + 32 * wave, key = mine + i;
     KeyGradients<T, D> w;
