@@ -161,17 +161,21 @@ int32_t launch(RotaryArgs a, hipStream_t st) {
     return CHELIS_HIP_OK;
 }
 
-// The widest vector, up to 16 bytes, that divides the pairs (halves) or the
-// turned width (adjacent).
+// The widest vector, up to 16 bytes and four pairs, that divides the pairs
+// (halves) or the turned width (adjacent). With eight pairs a thread the sines,
+// one after another, took longer than the narrower loads cost (bf16 heads of 128,
+// 16 + 4 of them, eight against four pairs: 64 tokens 6.5 and 6.1 us, 1024 7.5 and
+// 5.9, 8192 20.1 and 19.8, 32768 76.5 and 75.1; two pairs 22.9 at 8192).
 template <typename T>
 int32_t launch_widest(const RotaryArgs &a, bool halves, hipStream_t st) {
-    constexpr int V = 16 / sizeof(T);
     if (halves) {
+        constexpr int V = sizeof(T) == 8 ? 2 : 4;
         if (a.pairs % V == 0) return launch<T, V, true>(a, st);
         if constexpr (V > 2)
             if (a.pairs % (V / 2) == 0) return launch<T, V / 2, true>(a, st);
         return launch<T, 1, true>(a, st);
     }
+    constexpr int V = 16 / sizeof(T);
     if (2 * a.pairs % V == 0) return launch<T, V, false>(a, st);
     return launch<T, 2, false>(a, st);
 }
