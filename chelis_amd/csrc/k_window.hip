@@ -1475,16 +1475,19 @@ int64_t seen_blocks(const WinArgs &a, int64_t rows) {
 // 128 (us, split against whole rows): 16 heads on 4, 16384 keys: one row 19
 // against 490, 256 rows 137 against 366; window 1024 of 8 sequences: 16 rows
 // 23 against 40, 32 rows 34-41 against 32; 2048 keys of 32 sequences, 32 heads on
-// 8: 8 rows 77 against 143, 16 rows 136 against 110, 32 rows 233 against 110. Both kernels' times
-// follow these lines (binary32: the products cost whole rows more than the
-// split, whose waves hold no idle rows).
+// 8: 8 rows 77 against 143, 16 rows 136 against 110, 32 rows 233 against 110.
+// Narrow heads cost the split what the 64 columns in registers cost: heads of 8,
+// 16 on 16, 2048 keys: 512 rows 25 against 39, 2048 rows 73 against 40; binary32
+// 512 rows 60 against 167, 2048 rows 197 against 168, and of 64, 75 against 168 and
+// 243 against 169. Both kernels' times follow these lines.
 bool few_rows(const WinArgs &a, chelis_dtype dt, int64_t batch) {
     const double f32 = dt == CHELIS_DTYPE_F32 ? 1 : 0;
-    // the split's rows are counted in 32 bits
-    if ((int64_t)a.group * a.sq > kMaxExtent) return false;
+    // a join takes a workgroup a row, and the split counts its rows in 32 bits
+    if (!grid_fits(batch * a.heads * a.sq, kThreads)) return false;
     const int64_t tasks = batch * a.kv * (((int64_t)a.group * a.sq + 31) / 32);
     const int64_t groups = batch * a.heads * ((a.sq + 127) / 128), rounds = (groups + 511) / 512;
-    const double split = 8 + (double)tasks * seen_blocks(a, a.sq) * a.width / 32000 * (1 + 0.5 * f32);
+    const double idle = 24 + 16 * f32, width = std::max<double>(a.width, idle + a.width * (1 - idle / 64));
+    const double split = 8 + (double)tasks * seen_blocks(a, a.sq) * width / 32000 * (1 + f32);
     const double whole = 5 + rounds * (seen_blocks(a, std::min(a.sq, 128)) / 2.0) * (0.75 + 0.005 * a.width) * (1 + 3 * f32);
     return split < whole;
 }
