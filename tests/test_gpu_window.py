@@ -419,3 +419,18 @@ def test_rows_four_gigabytes_apart(S, N):
     assert np.array_equal(base.view((N, W), (far, 1), 2 * W).numpy(), grad)
     C.layer_norm_stats(rows, one, zero, 1e-5, y=rows)
     assert np.array_equal(rows.numpy(), y.numpy())
+
+
+def test_more_rows_than_a_launch_has_workgroups():
+    # 2^24 rows of narrow heads over few keys, nearly all of them ahead of the sequence
+    H, S, N, W = 16, 1 << 20, 64, 8
+    q, k, v, _ = operands("f32", 1, H, H, N, N, W, 31)
+    device = C.empty((1, H, S, W), np.float32)
+    last = device.view((1, H, N, W), (H * S * W, S * W, W, 1), (S - N) * W)
+    none, freqs = C.to_device(np.zeros((1, 1, N), np.int32)), C.to_device(np.ones(W // 2))
+    C.rotary(C.to_device(q), none, freqs, [W // 2], out=last)
+    ks, vs = C.to_device(k), C.to_device(v)
+    o = C.window_attention(device, ks, vs, N, 0, 0.5)
+    want, bound = window_forward("f32", q.astype(np.float64), k.astype(np.float64), v.astype(np.float64), N, 0, 0.5)[0]
+    check(o.view((1, H, N, W), (H * S * W, S * W, W, 1), (S - N) * W).numpy().astype(np.float64), want, bound, "o")
+    assert not o.view((1, H, N, W), (H * S * W, S * W, W, 1), (S - 2 * N) * W).numpy().any()
