@@ -289,12 +289,24 @@ __device__ inline V8<T> row_part(const T *row, int at, int width, bool live) {
     return live && at < width ? p.q : z;
 }
 
+// Clears the columns of `rows` tile rows past the head's width, once for all
+// tiles a buffer gets: the other factor is zero there, but 0 times an infinity
+// in whatever else stood there would be NaN.
+template <typename T, int D>
+__device__ inline void clear_past(T *tile, int rows, int width, int tid, int threads) {
+    if (width == D) return;
+    for (int id = tid; id < rows * (D / 8); id += threads)
+        if (id % (D / 8) * 8 >= width) *reinterpret_cast<V8<T> *>(tile + id / (D / 8) * kPitch<T, D> + id % (D / 8) * 8) = V8<T>{};
+}
+
 // A tile of N rows of D elements on its way from memory to LDS, staged by
-// kThreads threads. Rows past `last` and elements past the width repeat others
-// of the operand: the rows are hidden from every pair, and the other factor's
-// elements are zero. Whole tiles take one address a thread and a uniform step
-// between its parts (52 of the 380 vector instructions a tile went into
-// addresses otherwise).
+// kThreads threads. Rows past `last` repeat others of the operand, hidden from
+// every pair. A thread whose column lies past the width repeats the row's
+// first one, in memory and in LDS (leaving its store out cost dk and dv of
+// [1, 16 on 4, 8192, 128] bf16 20 us and spilled registers): the columns past
+// the width keep the zeros of clear_past. Whole tiles take one address a
+// thread and a uniform step between its parts (52 of the 380 vector
+// instructions a tile went into addresses otherwise).
 template <typename T, int D, int N>
 struct Staged {
     static constexpr int C = D / 8, ALL = N * C, PARTS = (ALL + kThreads - 1) / kThreads;
@@ -320,12 +332,12 @@ struct Staged {
         for (int i = 0; i < PARTS; ++i) m.add(part[i].q);
         return m.special();
     }
-    __device__ void store(T *tile, int tid) const {
+    __device__ void store(T *tile, int width, int tid) const {
 #pragma unroll
         for (int i = 0; i < PARTS; ++i) {
-            const int id = tid + i * kThreads;
+            const int id = tid + i * kThreads, e = (EVEN ? tid : id) % C * 8;
             if (ALL % kThreads && id >= ALL) break;
-            *reinterpret_cast<V8<T> *>(tile + id / (D / 8) * kPitch<T, D> + id % (D / 8) * 8) = part[i].q;
+            *reinterpret_cast<V8<T> *>(tile + id / C * kPitch<T, D> + (e < width ? e : 0)) = part[i].q;
         }
     }
 };
@@ -447,12 +459,14 @@ struct KeyTiles {
     }
     __device__ void store(int t) {
         if (t >= walk.count) return;
-        ks.store(sh.k[t % B], tid);
-        vs.store(sh.v[t % B], tid);
+        ks.store(sh.k[t % B], a.width, tid);
+        vs.store(sh.v[t % B], a.width, tid);
         if (!whole(walk.tile(t) * kKeys)) sh.flags[t & 1][wave] = __any(LOOK ? vs.special() : ks.special());
     }
     __device__ void begin() {
         load(0);
+        clear_past<T, D>(sh.k[0], B * kKeys, a.width, tid, kThreads);
+        clear_past<T, D>(sh.v[0], B * kKeys, a.width, tid, kThreads);
         if (B == 2) {
             store(0);
             load(1);
@@ -670,6 +684,10 @@ __global__ __launch_bounds__(kThreads, 2) void window_split_kernel(WinArgs a, Sp
     if (split < walk.count) load(split);
     for (int t = split; t < walk.count; t += p.splits) {
         const int k0 = walk.tile(t) * N;
+        if (a.width < D) {  // zeros past the width, as in q
+#pragma unroll
+            for (int u = 0; u < PARTS; ++u) kf[u] = 16 * u + 8 * h < a.width ? kf[u] : V8<T>{};
+        }
         f32x16 s = {};
 #pragma unroll
         for (int u = 0; u < D / 16; ++u) s = mma(kf[u], qf[u], s);
@@ -1167,8 +1185,8 @@ __global__ __launch_bounds__((kThreads * kGroups<T, D>), 1) void window_dkv_kern
         const int to = turn & 1;
         bool special = false;
         if (x.live) {
-            qs.store(sh.in.q[to][group], tid);
-            gs.store(sh.in.g[to][group], tid);
+            qs.store(sh.in.q[to][group], a.width, tid);
+            gs.store(sh.in.g[to][group], a.width, tid);
             if (tid < kRows) {
                 Ls[to][group][tid] = kShift<T> - ls * kLog2e;
                 Ds[to][group][tid] = ds;
@@ -1179,6 +1197,8 @@ __global__ __launch_bounds__((kThreads * kGroups<T, D>), 1) void window_dkv_kern
     };
     if (turns) {
         load(0);
+        clear_past<T, D>(sh.in.q[0][0], 2 * GROUPS * kRows, a.width, threadIdx.x, kThreads * GROUPS);
+        clear_past<T, D>(sh.in.g[0][0], 2 * GROUPS * kRows, a.width, threadIdx.x, kThreads * GROUPS);
         store(0);
         if (turns > 1) load(1);
     }
@@ -1280,12 +1300,13 @@ __global__ __launch_bounds__(kThreads, 1) void window_far_kernel(WinArgs a, FarA
         ls = h ? a.delta[stat] : kShift<T> - a.lse_in[stat] * kLog2e;
     };
     const int items = count * a.group;
+    clear_past<T, D>(Qs, 2 * kRows, a.width, lane, 64);  // of both tiles
     if (split < items) load(split);
     for (int t = split; t < items; t += splits) {
         const int r0 = from + t % count * kRows;
 #pragma unroll
         for (int s = 0; s < PARTS; ++s) {
-            const int part = lane + 64 * s, at = part / (D / 8) * kPitch<T, D> + part % (D / 8) * 8;
+            const int part = lane + 64 * s, e = part % (D / 8) * 8, at = part / (D / 8) * kPitch<T, D> + (e < a.width ? e : 0);
             *reinterpret_cast<V8<T> *>(Qs + at) = qr[s];
             *reinterpret_cast<V8<T> *>(Gs + at) = gr[s];
         }
