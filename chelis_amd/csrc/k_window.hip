@@ -1071,7 +1071,7 @@ struct KeyGradients {
 // are then unscaled parts in scratch: part 0 from the near rows, the others
 // from the far workgroups, joined in order by a last launch.
 struct FarArgs {
-    float *part;  // [block][1 + splits][dk, dv][32 keys][width]; null: no far rows
+    float *part;  // [block][1 + splits][dk, dv][32 keys][width]; null: none are dealt out
     int splits, blocks;
     __device__ float *at(int64_t pair, int block, int part_index, int width) const {
         return part + ((pair * blocks + block) * (1 + splits) + part_index) * 64 * width;
@@ -1467,7 +1467,9 @@ int32_t window_args(const chelis_gpu_tensor *q, const chelis_gpu_tensor *k, cons
         a->starts_wide = starts->dtype == CHELIS_DTYPE_I64;
     }
     a->sq = (int)q->shape[2], a->sk = (int)k->shape[2];
-    a->window = (int)std::min<int64_t>(window, std::max(a->sk, 1)), a->sinks = (int)std::min<int64_t>(sinks, a->sk);
+    // sinks that hold every key leave nothing to the window: plain causal rows
+    if (sinks >= a->sk) window = a->sk, sinks = 0;
+    a->window = (int)std::min<int64_t>(window, std::max(a->sk, 1)), a->sinks = (int)sinks;
     a->heads = (int)H, a->kv = (int)KV, a->group = KV ? (int)(H / KV) : 1, a->width = (int)W;
     a->flip = scale < 0, a->scale = (float)scale, a->c = (float)(std::fabs(scale) * 1.4426950408889634074);
     // hidden scores are -inf, and 0 times that is NaN
@@ -1604,15 +1606,22 @@ extern "C" int32_t chelis_hip_window_attention_adjoint(
     if (!grid_fits(rows.blocks(), kThreads) || !grid_fits(keys.blocks(), 2 * kThreads))
         return set_error(CHELIS_HIP_EUNSUPPORTED, "%s: grid too large", what);
     // rows far behind the window of the first keys: dealt out a tile to a wave,
-    // over no more workgroups than fill the device
+    // over no more workgroups than fill the device. Many sinks fill it as they
+    // are, with less work and no parts: past eight sink blocks a compute unit
+    // whose parts outgrow k, the keys' own workgroups walk those rows too
+    // (bf16, dealt against walked, us: [8, 16 on 16, 2048, 128] of 256 sinks
+    // 569 and 663, of 1024 1087 and 950; [64, 16 on 8, 1024, 64] of 64 sinks
+    // 755 and 939, of 256 1138 and 987; [1, 16 on 4, 8192, 128] of 4096, 512
+    // blocks in all, 1354 and 1781).
     FarArgs f{};
     const int64_t pairs = q->shape[0] * a.kv, far = (int64_t)a.sk - (32 * kWaves - 1) - a.window;
-    if (a.sinks > 0 && q->count && far > 0) {
-        f.blocks = (a.sinks + 31) / 32;
+    const int64_t blocks = (a.sinks + 31) / 32;
+    const bool many = pairs * blocks > 8 * (int64_t)device_cus() &&
+                      2 * pairs * blocks * 64 * a.width * (int64_t)sizeof(float) > k->count * dtype_width(k->dtype);
+    if (a.sinks > 0 && q->count && far > 0 && !many && q->shape[0] * blocks <= 65535) {
+        f.blocks = (int)blocks;
         const int64_t tiles = (std::min<int64_t>(far, a.sq) + kRows - 1) / kRows * a.group;
         f.splits = (int)std::max<int64_t>(1, std::min<int64_t>((tiles + kWaves - 1) / kWaves, (int64_t)device_cus() / (pairs * f.blocks)));
-        if (q->shape[0] * f.blocks > 65535)
-            return set_error(CHELIS_HIP_EUNSUPPORTED, "%s: sequences times sink blocks past 65535", what);
     }
     const size_t parts = f.blocks ? (size_t)pairs * f.blocks * (1 + f.splits) * 64 * a.width : 0;
     const size_t bytes = (2 * kRanges + parts + (size_t)lse->count) * sizeof(float);
