@@ -274,6 +274,75 @@ bool non_overlapping(const chelis_gpu_tensor *t) {
     return true;
 }
 
+namespace {
+// A view's elements as byte addresses: axes by falling stride, those that
+// address nothing new left out.
+struct Extent {
+    uintptr_t lo, hi;  // first byte, one past the last
+    int64_t width, stride[8], shape[8], inner[8];  // inner: bytes the axes after it reach
+    int32_t n = 0;
+    bool dense;
+    explicit Extent(const chelis_gpu_tensor *t) : lo(reinterpret_cast<uintptr_t>(t->data)), width(dtype_width(t->dtype)) {
+        int32_t idx[8];
+        for (int32_t a = 0; a < t->rank; ++a)
+            if (t->shape[a] > 1 && t->strides[a] > 0) idx[n++] = a;
+        std::sort(idx, idx + n, [&](int32_t x, int32_t y) { return t->strides[x] > t->strides[y]; });
+        int64_t reach = width, bytes = width;
+        bool nested = true;
+        for (int32_t i = n; i-- > 0;) {
+            stride[i] = t->strides[idx[i]] * width, shape[i] = t->shape[idx[i]], inner[i] = reach;
+            nested &= stride[i] >= reach;
+            reach += (shape[i] - 1) * stride[i];
+            bytes *= shape[i];
+        }
+        hi = lo + (uintptr_t)reach;
+        dense = nested && bytes == reach;
+    }
+    // Some element has a byte in [from, to).
+    bool touches(uintptr_t from, uintptr_t to) const {
+        int64_t d = (int64_t)(from - lo) - width + 1, at = 0;  // the first element at or past d
+        for (int32_t i = 0; i < n && d > 0; ++i) {
+            const int64_t k = std::min(d / stride[i], shape[i] - 1);
+            at += k * stride[i], d -= k * stride[i];
+            if (d > inner[i] - width) {  // past what the inner axes reach: the next of this axis
+                if (k + 1 >= shape[i]) return false;
+                at += stride[i], d = 0;
+            }
+        }
+        return d <= 0 && lo + (uintptr_t)at < to;
+    }
+};
+}  // namespace
+
+bool shares_storage(const chelis_gpu_tensor *a, const chelis_gpu_tensor *b) {
+    if (!a->count || !b->count) return false;
+    // operands nearly always lie apart as a whole
+    auto end = [](const chelis_gpu_tensor *t) {
+        int64_t reach = 1;
+        for (int32_t i = 0; i < t->rank; ++i) reach += (t->shape[i] - 1) * t->strides[i];
+        return reinterpret_cast<uintptr_t>(t->data) + (uintptr_t)(reach * dtype_width(t->dtype));
+    };
+    if (end(a) <= reinterpret_cast<uintptr_t>(b->data) || end(b) <= reinterpret_cast<uintptr_t>(a->data)) return false;
+    const Extent x(a), y(b);
+    if (x.dense) return y.touches(x.lo, x.hi);
+    if (y.dense) return x.touches(y.lo, y.hi);
+    return y.touches(x.lo, x.lo + x.width) || x.touches(y.lo, y.lo + y.width) || y.touches(x.hi - x.width, x.hi) ||
+           x.touches(y.hi - y.width, y.hi);
+}
+
+bool same_view(const chelis_gpu_tensor *a, const chelis_gpu_tensor *b) {
+    if (a->data != b->data || a->dtype != b->dtype || !same_shape(a, b)) return false;
+    for (int32_t i = 0; i < a->rank; ++i)
+        if (a->shape[i] > 1 && a->strides[i] != b->strides[i]) return false;
+    return true;
+}
+
+const char *shared_with(const chelis_gpu_tensor *t, std::initializer_list<NamedTensor> others) {
+    for (const NamedTensor &o : others)
+        if (o.t && shares_storage(t, o.t)) return o.name;
+    return nullptr;
+}
+
 int32_t check_device(const chelis_gpu_tensor *t, const char *name) {
     static const int devices = [] {
         int n = 0;

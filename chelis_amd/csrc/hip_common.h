@@ -7,6 +7,7 @@
 #include <cstdarg>
 #include <cstdint>
 #include <cstdio>
+#include <initializer_list>
 
 #include "chelis_hip.h"
 #include "devmath.h"
@@ -100,6 +101,19 @@ bool same_shape(const chelis_gpu_tensor *a, const chelis_gpu_tensor *b);
 // Distinct indices of a view address distinct elements (no write races):
 // sorted by stride, each axis steps past everything the smaller axes span.
 bool non_overlapping(const chelis_gpu_tensor *t);
+// Some element of a lies on one of b, as far as can be told without walking
+// them: exact where either has no gaps, else by the first and last elements.
+// A result over an input would race with its reads.
+bool shares_storage(const chelis_gpu_tensor *a, const chelis_gpu_tensor *b);
+// a and b are the same elements in the same order (in-place calls).
+bool same_view(const chelis_gpu_tensor *a, const chelis_gpu_tensor *b);
+// The name of the first of `others` (null ones apart) that t shares storage
+// with, null if none.
+struct NamedTensor {
+    const chelis_gpu_tensor *t;
+    const char *name;
+};
+const char *shared_with(const chelis_gpu_tensor *t, std::initializer_list<NamedTensor> others);
 // On a machine with several devices: the tensor's storage lies on the
 // current one (whose library stream the launch goes to).
 int32_t check_device(const chelis_gpu_tensor *t, const char *name);

@@ -481,11 +481,18 @@ int32_t check_rows(const chelis_gpu_tensor *t, const char *name, const chelis_gp
     return check_device(t, name);
 }
 
-int32_t check_in_place(const chelis_gpu_tensor *out, const RowView &vo, const chelis_gpu_tensor *in,
-                       const RowView &vi, const char *name, const char *what) {
+int32_t check_in_place(const chelis_gpu_tensor *out, const chelis_gpu_tensor *in, const char *name, const char *what) {
     if (!non_overlapping(out)) return set_error(CHELIS_HIP_EDOMAIN, "%s: %s overlaps itself", what, name);
-    if (in->count && out->data == in->data && vo.rows > 1 && vo.ld != vi.ld)
-        return set_error(CHELIS_HIP_EDOMAIN, "%s: %s overlaps an input with other strides", what, name);
+    if (!same_view(out, in) && shares_storage(out, in))
+        return set_error(CHELIS_HIP_EDOMAIN, "%s: %s overlaps an input with other strides or from another element", what,
+                         name);
+    return CHELIS_HIP_OK;
+}
+
+int32_t check_apart(const chelis_gpu_tensor *out, const char *name, std::initializer_list<NamedTensor> others,
+                    const char *what) {
+    if (const char *other = shared_with(out, others))
+        return set_error(CHELIS_HIP_EDOMAIN, "%s: %s and %s overlap", what, name, other);
     return CHELIS_HIP_OK;
 }
 
@@ -504,7 +511,10 @@ extern "C" int32_t chelis_hip_layer_norm_stats(const chelis_gpu_tensor *x, const
     if ((s = check_tensor(x, "x")) || (s = check_rows(x, "x", x, &vx, what)) || (s = check_rows(y, "y", x, &vy, what)) ||
         (s = check_weights(gamma, "gamma", x, vx.n, what)) || (s = check_weights(beta, "beta", x, vx.n, what)) ||
         (s = check_stat(mean, "mean", x, what)) || (s = check_stat(rstd, "rstd", x, what)) ||
-        (s = check_in_place(y, vy, x, vx, "y", what)))
+        (s = check_in_place(y, x, "y", what)) ||
+        (s = check_apart(y, "y", {{gamma, "gamma"}, {beta, "beta"}, {mean, "mean"}, {rstd, "rstd"}}, what)) ||
+        (s = check_apart(mean, "mean", {{x, "x"}, {gamma, "gamma"}, {beta, "beta"}, {rstd, "rstd"}}, what)) ||
+        (s = check_apart(rstd, "rstd", {{x, "x"}, {gamma, "gamma"}, {beta, "beta"}}, what)))
         return s;
     if (gamma->dtype != beta->dtype)
         return set_error(CHELIS_HIP_EDOMAIN, "%s: gamma and beta must share a dtype", what);
@@ -535,15 +545,20 @@ extern "C" int32_t chelis_hip_layer_norm_adjoint(const chelis_gpu_tensor *x, con
         return s;
     if (!dx && !dgamma && !dbeta) return set_error(CHELIS_HIP_EDOMAIN, "%s: no gradient asked for", what);
     if (!dgamma != !dbeta) return set_error(CHELIS_HIP_EDOMAIN, "%s: dgamma and dbeta come together", what);
-    if (dx && ((s = check_rows(dx, "dx", x, &vd, what)) || (s = check_in_place(dx, vd, x, vx, "dx", what)) ||
-               (s = check_in_place(dx, vd, g, vg, "dx", what))))
+    if (dx && ((s = check_rows(dx, "dx", x, &vd, what)) || (s = check_in_place(dx, x, "dx", what)) ||
+               (s = check_in_place(dx, g, "dx", what)) ||
+               (s = check_apart(dx, "dx", {{gamma, "gamma"}, {mean, "mean"}, {rstd, "rstd"}}, what))))
         return s;
     if (dgamma) {
         if ((s = check_weights(dgamma, "dgamma", x, vx.n, what)) || (s = check_weights(dbeta, "dbeta", x, vx.n, what)))
             return s;
         if (dgamma->dtype != gamma->dtype || dbeta->dtype != gamma->dtype)
             return set_error(CHELIS_HIP_EDOMAIN, "%s: dgamma and dbeta must have gamma's dtype", what);
-        if (dgamma->data == dbeta->data) return set_error(CHELIS_HIP_EDOMAIN, "%s: dgamma and dbeta overlap", what);
+        const std::initializer_list<NamedTensor> others = {{dx, "dx"}, {x, "x"}, {g, "g"}, {gamma, "gamma"},
+                                                           {mean, "mean"}, {rstd, "rstd"}};
+        if ((s = check_apart(dgamma, "dgamma", {{dbeta, "dbeta"}}, what)) ||
+            (s = check_apart(dgamma, "dgamma", others, what)) || (s = check_apart(dbeta, "dbeta", others, what)))
+            return s;
     }
     hipStream_t st = stream();
     if (!st) return set_error(CHELIS_HIP_EHIP, "no HIP device");

@@ -219,19 +219,20 @@ int32_t rotary(const chelis_gpu_tensor *const *xs, int32_t n, const chelis_gpu_t
         if ((x->shape[3] > 1 && (x->strides[3] != 1 || y->strides[3] != 1)))
             return set_error(CHELIS_HIP_EUNSUPPORTED, "%s: the last axis must be contiguous", what);
         if (!non_overlapping(y)) return set_error(CHELIS_HIP_EDOMAIN, "%s: y overlaps itself", what);
-        for (int32_t o = 0; o < n; ++o)
-            if (y->count && y->data == xs[o]->data) {
-                bool same = o == k;
-                for (int32_t ax = 0; same && ax < 4; ++ax)
-                    same = x->shape[ax] == 1 || x->strides[ax] == y->strides[ax];
-                if (!same) return set_error(CHELIS_HIP_EDOMAIN, "%s: y overlaps an input with other strides", what);
-            }
+        for (int32_t o = 0; o < n; ++o) {
+            if (o != k && (s = check_tensor(xs[o], "x"))) return s;
+            if (!(o == k && same_view(y, x)) && shares_storage(y, xs[o]))
+                return set_error(CHELIS_HIP_EDOMAIN,
+                                 "%s: y overlaps an input with other strides or from another element", what);
+        }
+        if (const char *other = shared_with(y, {{positions, "positions"}, {freqs, "freqs"}}))
+            return set_error(CHELIS_HIP_EDOMAIN, "%s: y and %s overlap", what, other);
         RotaryTensor &t = a.t[k];
         t.x = x->data, t.y = y->data, t.heads = (int)x->shape[1];
         t.xb = x->strides[0], t.xh = x->strides[1], t.xs = x->strides[2];
         t.yb = y->strides[0], t.yh = y->strides[1], t.ys = y->strides[2];
     }
-    if (n == 2 && ys[0]->count && ys[1]->count && ys[0]->data == ys[1]->data)
+    if (n == 2 && shares_storage(ys[0], ys[1]))
         return set_error(CHELIS_HIP_EDOMAIN, "%s: the results overlap", what);
     const int64_t batch = xs[0]->shape[0], seq = xs[0]->shape[2];
     if ((positions->dtype != CHELIS_DTYPE_I32 && positions->dtype != CHELIS_DTYPE_I64) || positions->rank != 3 ||

@@ -1478,12 +1478,11 @@ int32_t window_args(const chelis_gpu_tensor *q, const chelis_gpu_tensor *k, cons
     return CHELIS_HIP_OK;
 }
 
-int32_t check_result(const chelis_gpu_tensor *t, const char *name, std::initializer_list<const chelis_gpu_tensor *> ins,
+int32_t check_result(const chelis_gpu_tensor *t, const char *name, std::initializer_list<NamedTensor> others,
                      const char *what) {
     if (!non_overlapping(t)) return set_error(CHELIS_HIP_EDOMAIN, "%s: %s overlaps itself", what, name);
-    for (const chelis_gpu_tensor *in : ins)
-        if (t->count && in->count && t->data == in->data)
-            return set_error(CHELIS_HIP_EDOMAIN, "%s: %s overlaps another operand", what, name);
+    if (const char *other = shared_with(t, others))
+        return set_error(CHELIS_HIP_EDOMAIN, "%s: %s overlaps another operand (%s)", what, name, other);
     return CHELIS_HIP_OK;
 }
 
@@ -1563,7 +1562,9 @@ extern "C" int32_t chelis_hip_window_attention(const chelis_gpu_tensor *q, const
     int32_t s;
     if ((s = window_args(q, k, v, lengths, starts, window, sinks, scale, &a, what)) ||
         (s = check_part(o, "o", q, what)) || (s = check_same(o, "o", q, "q", what)) ||
-        (lse && (s = check_stat(lse, "lse", q, what))) || (s = check_result(o, "o", {q, k, v}, what)))
+        (lse && (s = check_stat(lse, "lse", q, what))) ||
+        (s = check_result(o, "o", {{q, "q"}, {k, "k"}, {v, "v"}, {lse, "lse"}, {lengths, "lengths"}, {starts, "starts"}}, what)) ||
+        (lse && (s = check_result(lse, "lse", {{q, "q"}, {k, "k"}, {v, "v"}, {lengths, "lengths"}, {starts, "starts"}}, what))))
         return s;
     a.o = view_of(o);
     a.lse = lse ? static_cast<float *>(lse->data) : nullptr;
@@ -1593,8 +1594,12 @@ extern "C" int32_t chelis_hip_window_attention_adjoint(
         if ((s = check_part(t, name, q, what)) || (s = check_same(t, name, q, "q", what))) return s;
     for (auto [t, name] : {std::pair(dk, "dk"), std::pair(dv, "dv")})
         if ((s = check_part(t, name, q, what)) || (s = check_same(t, name, k, "k", what))) return s;
-    if ((s = check_stat(lse, "lse", q, what)) || (s = check_result(dq, "dq", {q, k, v, o, g, dk, dv}, what)) ||
-        (s = check_result(dk, "dk", {q, k, v, o, g, dv}, what)) || (s = check_result(dv, "dv", {q, k, v, o, g}, what)))
+    if ((s = check_stat(lse, "lse", q, what))) return s;
+    const std::initializer_list<NamedTensor> ins = {{q, "q"}, {k, "k"}, {v, "v"}, {o, "o"}, {g, "g"}, {lse, "lse"},
+                                                    {lengths, "lengths"}, {starts, "starts"}};
+    if ((s = check_result(dq, "dq", ins, what)) || (s = check_result(dk, "dk", ins, what)) ||
+        (s = check_result(dv, "dv", ins, what)) || (s = check_result(dq, "dq", {{dk, "dk"}, {dv, "dv"}}, what)) ||
+        (s = check_result(dk, "dk", {{dv, "dv"}}, what)))
         return s;
     a.o = view_of(o), a.g = view_of(g), a.dq = view_of(dq), a.dk = view_of(dk), a.dv = view_of(dv);
     a.lse_in = static_cast<const float *>(lse->data);

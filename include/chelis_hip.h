@@ -92,7 +92,8 @@ int32_t chelis_hip_layer_norm(const chelis_gpu_tensor *x, const chelis_gpu_tenso
  * weights are held in binary32 (binary64 for f64) and a 16-bit result is
  * rounded once. Sums run in the kernels' own fixed order: the same bits on
  * every run, not the canonical tree's. Results may not share storage with
- * inputs unless said so. Calls captured into a graph keep the scratch they
+ * another operand unless said so: a call is refused where one is dense, or where
+ * one's first or last element lies in the other. Calls captured into a graph keep the scratch they
  * took for that graph. On a machine with several devices, operands must lie
  * on the current one. */
 
