@@ -14,6 +14,7 @@
 #include <cstdio>
 #include <cstring>
 #include <mutex>
+#include <unordered_set>
 #include <vector>
 
 #include "hip_common.h"
@@ -55,10 +56,20 @@ hipStream_t stream() {
 // kernels that used the block before. Blocks are cached per device in
 // power-of-two size classes (at least 256 B) and kept until the process
 // ends; only a cache miss allocates (hipMalloc).
+//
+// A block taken while the library stream is being captured is held by the
+// graph (as a user object, which executables made from the graph hold too):
+// every replay uses it again, so it returns to the cache when the last of
+// them is destroyed, and to no other call or graph before.
 namespace {
 std::mutex g_scratch_mutex;
 constexpr int kClasses = 48;
-std::vector<void *> g_free[kMaxDevices][kClasses];
+struct Scratch {
+    std::vector<void *> free[kMaxDevices][kClasses];
+    std::unordered_set<void *> held;
+};
+// never destroyed: a graph that outlives static destruction returns its block
+Scratch &g_scratch = *new Scratch;
 
 int size_class(size_t bytes) {
     int c = 8;  // 256 B
@@ -83,6 +94,38 @@ bool capturing() {
     hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
     return s && hipStreamIsCapturing(s, &status) == hipSuccess && status == hipStreamCaptureStatusActive;
 }
+
+struct Held {
+    int device, cls;
+    void *p;
+};
+void return_held(void *arg) {
+    const Held *h = static_cast<Held *>(arg);
+    {
+        std::lock_guard<std::mutex> lock(g_scratch_mutex);
+        g_scratch.held.erase(h->p);
+        g_scratch.free[h->device][h->cls].push_back(h->p);
+    }
+    delete h;
+}
+// Leaves block p to the graph being captured; where the runtime refuses that,
+// the block is held for good.
+void hold_for_graph(int device, int cls, void *p) {
+    {
+        std::lock_guard<std::mutex> lock(g_scratch_mutex);
+        g_scratch.held.insert(p);
+    }
+    hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
+    hipGraph_t graph = nullptr;
+    hipUserObject_t object = nullptr;
+    if (hipStreamGetCaptureInfo_v2(stream(), &status, nullptr, &graph, nullptr, nullptr) != hipSuccess || !graph) return;
+    Held *h = new Held{device, cls, p};
+    if (hipUserObjectCreate(&object, h, return_held, 1, hipUserObjectNoDestructorSync) != hipSuccess) {
+        delete h;
+        return;
+    }
+    (void)hipGraphRetainUserObject(graph, object, 1, hipGraphUserObjectMove);
+}
 }  // namespace
 
 void *scratch_alloc(size_t bytes) {
@@ -92,30 +135,35 @@ void *scratch_alloc(size_t bytes) {
     if (hipGetDevice(&device) != hipSuccess || device < 0 || device >= kMaxDevices) return nullptr;
     const int c = size_class(bytes);
     if ((size_t(1) << c) < bytes) return nullptr;
+    const bool captured = capturing();
+    void *p = nullptr;
     {
         std::lock_guard<std::mutex> lock(g_scratch_mutex);
-        std::vector<void *> &fl = g_free[device][c];
+        std::vector<void *> &fl = g_scratch.free[device][c];
         if (!fl.empty()) {
-            void *p = fl.back();
+            p = fl.back();
             fl.pop_back();
-            return p;
         }
     }
-    // an allocation is no stream operation: allowed while this thread captures
-    hipStreamCaptureMode mode = hipStreamCaptureModeRelaxed;
-    const bool relaxed = capturing() && hipThreadExchangeStreamCaptureMode(&mode) == hipSuccess;
-    void *p = nullptr;
-    const hipError_t e = device_malloc(&p, size_t(1) << c);
-    if (relaxed) (void)hipThreadExchangeStreamCaptureMode(&mode);
-    return e == hipSuccess ? p : nullptr;
+    if (!p) {
+        // an allocation is no stream operation: allowed while this thread captures
+        hipStreamCaptureMode mode = hipStreamCaptureModeRelaxed;
+        const bool relaxed = captured && hipThreadExchangeStreamCaptureMode(&mode) == hipSuccess;
+        const hipError_t e = device_malloc(&p, size_t(1) << c);
+        if (relaxed) (void)hipThreadExchangeStreamCaptureMode(&mode);
+        if (e != hipSuccess) return nullptr;
+    }
+    if (captured) hold_for_graph(device, c, p);
+    return p;
 }
 
 void scratch_free(void *p, size_t bytes) {
-    if (!p || capturing()) return;
+    if (!p) return;
     int device = 0;
     if (hipGetDevice(&device) != hipSuccess || device < 0 || device >= kMaxDevices) return;
     std::lock_guard<std::mutex> lock(g_scratch_mutex);
-    g_free[device][size_class(bytes)].push_back(p);
+    if (!g_scratch.held.empty() && g_scratch.held.count(p)) return;  // a graph's
+    g_scratch.free[device][size_class(bytes)].push_back(p);
 }
 
 // ---- owner storage ---------------------------------------------------------
@@ -139,7 +187,7 @@ void *owner_block_alloc(size_t bytes) {
     const int c = size_class(bytes);
     {
         std::lock_guard<std::mutex> lock(g_scratch_mutex);
-        std::vector<void *> &fl = g_free[device][c];
+        std::vector<void *> &fl = g_scratch.free[device][c];
         if (!fl.empty()) {
             p = fl.back();
             fl.pop_back();
@@ -158,7 +206,7 @@ hipError_t owner_block_free(void *p, size_t bytes) {
     if (device < 0 || device >= kMaxDevices) return hipErrorInvalidDevice;
     if ((e = hipDeviceSynchronize()) != hipSuccess) return e;
     std::lock_guard<std::mutex> lock(g_scratch_mutex);
-    g_free[device][size_class(bytes)].push_back(p);
+    g_scratch.free[device][size_class(bytes)].push_back(p);
     return hipSuccess;
 }
 

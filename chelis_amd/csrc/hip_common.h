@@ -50,10 +50,10 @@ int32_t *status_words(int32_t **host);
 // stream: blocks are recycled in stream order (a freed block's earlier users
 // are already enqueued ahead of any later user) and cached for reuse, so
 // the hot path makes no allocation calls. scratch_free takes the size given
-// to scratch_alloc. Returns null when the device cannot allocate. While the
-// library stream is being captured into a graph, the block leaves the cache
-// for good: each replay uses it again, so no other call and no other graph
-// may get it.
+// to scratch_alloc. Returns null when the device cannot allocate. A
+// block taken while the library stream is being captured belongs to the graph
+// and returns to the cache when it and its executables are destroyed: each
+// replay uses it again, so no other call and no other graph may get it.
 void *scratch_alloc(size_t bytes);
 // hipMalloc, counted (chelis_hip_allocation_counts): every device allocation
 // the library makes goes through it.

@@ -93,9 +93,11 @@ int32_t chelis_hip_layer_norm(const chelis_gpu_tensor *x, const chelis_gpu_tenso
  * rounded once. Sums run in the kernels' own fixed order: the same bits on
  * every run, not the canonical tree's. Results may not share storage with
  * another operand unless said so: a call is refused where one is dense, or where
- * one's first or last element lies in the other. Calls captured into a graph keep the scratch they
- * took for that graph. On a machine with several devices, operands must lie
- * on the current one. */
+ * one's first or last element lies in the other. A call captured into a graph
+ * leaves the scratch it took to the graph, until the graph and its executables
+ * are destroyed; a replay on another stream than the library's has to end
+ * before that. On a machine with several devices, operands must lie on the
+ * current one. */
 
 /* layer_norm with the row statistics its gradient needs: y as
  * chelis_hip_layer_norm (bit for bit at f32 and f64), mean and
