@@ -44,6 +44,15 @@ struct RotaryArgs {
 // quarter turn in two parts, then the Taylor polynomials, whose first
 // dropped terms at pi/4 are below 2e-9 (binary32).
 __device__ inline void sin_cos(double t, float &s, float &c) {
+    // n stops being the nearest quarter turn past 2^53 of them; the library's
+    // reduction takes any angle (the registers it costs: the f32 prompt above
+    // 47.3 -> 47.9 us, 64 bf16 tokens 6.5 us as before)
+    if (!(fabs(t) < 0x1p50)) {
+        double s64, c64;
+        sincos(t, &s64, &c64);
+        s = (float)s64, c = (float)c64;
+        return;
+    }
     const double n = rint(t * 0.63661977236758134308);
     const double r64 = fma(-n, 6.123233995736766036e-17, fma(-n, 1.5707963267948965580, t));
     const float r = (float)r64, z = r * r;
