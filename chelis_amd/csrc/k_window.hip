@@ -180,6 +180,72 @@ struct Marks {
         }
     }
 };
+// An infinity in v that a row sees makes its column infinite, whatever it
+// weighs. But its weight may round to 0 (f16 holds e^-24 at least), or be scaled
+// to 0 when a far larger score follows, and both make NaN of it. The columns it
+// stands in are the only ones it reaches, so where a wave's sums came out
+// infinite or NaN it looks over the keys it walked once more and sets those
+// columns to what they hold. The look at the sums (64 multiply-adds at heads of
+// 128) is all that other calls pay.
+template <int D>
+__device__ inline bool has_special(const f32x16 (&acc)[D / 32]) {
+    float odd = 0.f;
+#pragma unroll
+    for (int d = 0; d < D / 32; ++d)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) odd = fmaf(acc[d][r], 0.f, odd);
+    return odd != 0.f;
+}
+// The infinities and NaN that a lane's row sees, a bit for each accumulated
+// element; NaN sets both. `need`: the elements that no finite sum stands in.
+template <typename T, int D>
+struct SeenSpecials {
+    uint64_t need = 0, up = 0, down = 0;
+    __device__ SeenSpecials(const f32x16 (&acc)[D / 32], bool stored) {
+#pragma unroll
+        for (int e = 0; e < D / 2; ++e) need |= (uint64_t)(stored & not_finite(acc[e >> 4][e & 15])) << e;
+    }
+    // nothing that the wave's rows could still see would change them
+    __device__ bool done() const { return !__any((need & ~(up & down)) != 0); }
+    // keys k0 .. end - 1 of v, the whole wave together
+    template <class Sees>
+    __device__ void note(const T *V, int64_t step, int width, int k0, int end, int lane, Sees sees) {
+        constexpr int C = D / 8, R = 64 / C;
+        for (int j = k0; j < end; j += R) {
+            const int key = j + lane / C, at = lane % C * 8;
+            uint32_t mine = 0;  // which of the lane's eight, +inf in the low byte
+            if (lane < R * C && key < end && at < width) {
+                Pack<T, 8> x;
+                x.load(V + key * step + at);
+#pragma unroll
+                for (int c = 0; c < 8; ++c) {
+                    const uint32_t hit = not_finite(x.q[c]);
+                    mine |= (x.q[c] < (T)0.f ? 0 : hit) << c | (x.q[c] > (T)0.f ? 0 : hit) << (8 + c);
+                }
+            }
+            // four of eight columns belong to each half of the wave
+            for (uint64_t hits = __ballot(mine != 0); hits; hits &= hits - 1) {
+                const int lead = __ffsll((unsigned long long)hits) - 1, c0 = lead % C * 8;
+                const uint32_t theirs = (uint32_t)__builtin_amdgcn_readlane((int)mine, lead) >> (lane >> 5) * 4;
+                const uint64_t seen = sees(j + lead / C) ? 15 : 0;
+                up |= (theirs & seen) << (c0 / 32 * 16 + c0 % 32 / 8 * 4);
+                down |= (theirs >> 8 & seen) << (c0 / 32 * 16 + c0 % 32 / 8 * 4);
+            }
+        }
+    }
+    __device__ void put(f32x16 (&acc)[D / 32]) const {
+#pragma unroll
+        for (int e = 0; e < D / 2; ++e) {
+            const bool u = up >> e & 1, d = down >> e & 1;
+            const float x = (u ? INFINITY : 0.f) + (d ? -INFINITY : 0.f);
+            acc[e >> 4][e & 15] = (u | d) ? x : acc[e >> 4][e & 15];
+        }
+    }
+};
+// The factor of a row's unscaled sums; a row whose every score is -inf is NaN.
+__device__ inline float row_factor(bool empty, float l) {
+    return empty ? 0.f : l > 0.f ? 1.f / l : __builtin_nanf("");
+}
 template <typename T, int D, int N, int THREADS>
 __device__ inline void clean(T *tile, int tid) {
     for (int id = tid; id < N * (D / 8); id += THREADS) {
@@ -600,10 +666,19 @@ __global__ __launch_bounds__(kThreads, 2) void window_forward_kernel(WinArgs a, 
         }
         if (!HALVES) interleave<4 * D / 32, 2, 3>();
     }
+    if (__any(has_special<D>(acc))) {
+        SeenSpecials<T, D> specials(acc, row < a.sq && l == l);  // a row of NaN weights is NaN
+        for (int t = 0; t < walk.count && !specials.done(); ++t) {
+            const int k0 = walk.tile(t) * kKeys;
+            specials.note(tiles.V, a.v.s, a.width, k0, min(k0 + kKeys, seq.n), lane,
+                          [&](int k) { return SeenKeys(top, low, a.sinks, 0, 0).at(k); });
+        }
+        specials.put(acc);
+    }
     l += other_half(l);
     if (row >= a.sq) return;
     const bool empty = top < 0;
-    const float inv = empty ? 0.f : 1.f / l;
+    const float inv = row_factor(empty, l);
     T *O = const_cast<T *>(head_of<T>(a.o, b, head)) + row * a.o.s;
 #pragma unroll
     for (int d = 0; d < D / 32; ++d) store_column(O, acc[d], 32 * d, a.width, h, inv);
@@ -629,8 +704,11 @@ struct SplitArgs {
     int64_t tasks;
 };
 
+// binary32 rows wider than 64 hold more than half a SIMD's registers: one wave a
+// SIMD (two spilled them: one token of 64 sequences, window 4096, 32 heads of 128
+// on 8, 954 and, with the look at the sums below, 1189 us; 515 now).
 template <typename T, int D>
-__global__ __launch_bounds__(kThreads, 2) void window_split_kernel(WinArgs a, SplitArgs p) {
+__global__ __launch_bounds__(kThreads, (sizeof(T) == 4 && D > 64 ? 1 : 2)) void window_split_kernel(WinArgs a, SplitArgs p) {
     constexpr int N = 32;
     __shared__ __attribute__((aligned(16))) T tiles[kWaves][N * kPitch<T, D>];
     const int tid = threadIdx.x, lane = tid & 63, i = lane & 31, h = lane >> 5;
@@ -738,6 +816,15 @@ __global__ __launch_bounds__(kThreads, 2) void window_split_kernel(WinArgs a, Sp
             for (int d = 0; d < D / 32; ++d) acc[d] = mma(across<T, D>(tile, 16 * kc, 32 * d, lane), pf, acc[d]);
         }
     }
+    if (__any(has_special<D>(acc))) {
+        SeenSpecials<T, D> specials(acc, live && l == l);  // a row of NaN weights is NaN
+        for (int t = split; t < walk.count && !specials.done(); t += p.splits) {
+            const int k0 = walk.tile(t) * N;
+            specials.note(V, a.v.s, a.width, k0, min(k0 + N, seq.n), lane,
+                          [&](int k) { return SeenKeys(top, low, a.sinks, 0, 0).at(k); });
+        }
+        specials.put(acc);
+    }
     l += other_half(l);
     if (!live) return;
     if (p.splits > 1) {
@@ -757,7 +844,7 @@ __global__ __launch_bounds__(kThreads, 2) void window_split_kernel(WinArgs a, Sp
         return;
     }
     const bool empty = top < 0;
-    const float inv = empty ? 0.f : 1.f / l;
+    const float inv = row_factor(empty, l);
     T *O = const_cast<T *>(head_of<T>(a.o, b, head)) + row * a.o.s;
 #pragma unroll
     for (int d = 0; d < D / 32; ++d) store_column(O, acc[d], 32 * d, a.width, h, inv);
@@ -771,6 +858,14 @@ __global__ __launch_bounds__(kThreads, 2) void window_split_kernel(WinArgs a, Sp
 // once. (Statistics, sums and parts one after another took 4.0 us for a single
 // token over 1024 keys, one wave walking its 35 splits 24 us.)
 constexpr int kMaxSplits = 2048;
+
+// A part's elements under its weight; infinities stay where the weight is 0.
+__device__ inline f32x4 weighed(float w, f32x4 x) {
+    f32x4 y;
+#pragma unroll
+    for (int t = 0; t < 4; ++t) y[t] = not_finite(x[t]) ? x[t] : w * x[t];
+    return y;
+}
 
 template <typename T, int D>
 __global__ __launch_bounds__(kThreads) void window_join_kernel(WinArgs a, SplitArgs p) {
@@ -819,10 +914,10 @@ __global__ __launch_bounds__(kThreads) void window_join_kernel(WinArgs a, SplitA
     if (own) {
 #pragma unroll
         for (int k = 0; k < AHEAD; ++k)
-            if (group + k * GROUPS < p.splits) x += weight[group + k * GROUPS] * ahead[k];
+            if (group + k * GROUPS < p.splits) x += weighed(weight[group + k * GROUPS], ahead[k]);
 #pragma unroll 4
         for (int s = group + AHEAD * GROUPS; s < p.splits; s += GROUPS)
-            x += weight[s] * *reinterpret_cast<const f32x4 *>(part + s * step);
+            x += weighed(weight[s], *reinterpret_cast<const f32x4 *>(part + s * step));
         join[group][lane] = x;
     }
     __syncthreads();
@@ -831,7 +926,7 @@ __global__ __launch_bounds__(kThreads) void window_join_kernel(WinArgs a, SplitA
     if (own && group == 0) {
 #pragma unroll
         for (int k = 1; k < GROUPS; ++k) x += join[k][lane];
-        const float inv = empty ? 0.f : 1.f / l;
+        const float inv = row_factor(empty, l);
         Pack<T, 4> out;
 #pragma unroll
         for (int t = 0; t < 4; ++t) out.set(t, x[t] * inv);

@@ -151,7 +151,8 @@ int32_t chelis_hip_rotary_adjoint(const chelis_gpu_tensor *const *gs, int32_t n,
  *   lse = log of the sum of exp(scale * q . k) over them.
  * A row that sees nothing gets o = 0 and lse = -inf. Keys past a length are
  * not read, and a key that a row does not see adds nothing to it, whatever it
- * holds. lse: contiguous f32 [batch, heads, seq], or NULL. lengths, starts:
+ * holds. An infinity in v that a row sees makes that column of it infinite,
+ * however little it weighs. lse: contiguous f32 [batch, heads, seq], or NULL. lengths, starts:
  * i32 or i64 [batch]. */
 int32_t chelis_hip_window_attention(const chelis_gpu_tensor *q, const chelis_gpu_tensor *k,
                                     const chelis_gpu_tensor *v, const chelis_gpu_tensor *lengths,
@@ -160,7 +161,8 @@ int32_t chelis_hip_window_attention(const chelis_gpu_tensor *q, const chelis_gpu
 /* Its gradients for the cotangent g of o, from the forward call's o and lse
  * and the same lengths, starts, window, sinks and scale. dk and dv sum over
  * the query heads of a key head and are zero at keys nothing sees; dq is zero
- * at rows that see nothing. No atomics: the same bits on every run. */
+ * at rows that see nothing. What an infinity in a seen operand reaches is
+ * infinite or NaN. No atomics: the same bits on every run. */
 int32_t chelis_hip_window_attention_adjoint(const chelis_gpu_tensor *q, const chelis_gpu_tensor *k,
                                             const chelis_gpu_tensor *v, const chelis_gpu_tensor *o,
                                             const chelis_gpu_tensor *lse, const chelis_gpu_tensor *g,
