@@ -466,11 +466,10 @@ def window_attention(q, k, v, window: int, sinks: int, scale: float, o=None, lse
     position and the first `sinks` keys: q [batch, heads, seq, width] over
     k, v [batch, kv_heads, keys, width]. lengths [batch]: the keys each
     sequence holds; starts [batch]: its first row's position (None: the rows
-    are its last). lse: a tensor for the rows' log sums, True to make one.
-    Returns o, or (o, lse) when lse was asked for."""
+    are its last). lse: a tensor for the rows' log sums, True to make one
+    (None, False: not asked for). Returns o, or (o, lse) when lse was asked for."""
     o = o or empty(q.shape, q.dtype)
-    if lse is True:
-        lse = empty(q.shape[:3], np.float32)
+    lse = empty(q.shape[:3], np.float32) if lse is True else None if lse is False else lse
     check(lib().chelis_hip_window_attention(_p(q), _p(k), _p(v), _opt(lengths), _opt(starts), int(window), int(sinks),
                                             scale, _p(o), _opt(lse)), "window_attention")
     return o if lse is None else (o, lse)

@@ -169,3 +169,9 @@ def test_float16_score_gradients_past_the_type(which):
     result = dq if which != "small-dk" else dk
     assert 2.0**-14 < np.abs(result).max() < 60000 and np.abs(dk).max() < 60000 and np.abs(dq).max() < 60000
     attended("f16", (q, k, v, g), window, sinks, scale, gradients=True)
+
+
+def test_log_sums_not_asked_for():
+    t = [C.to_device(x) for x in operands("f32", 1, 2, 1, 3, 9, 16, 47)[:3]]
+    want = C.window_attention(*t, 4, 1, 0.25).numpy()
+    assert np.array_equal(C.window_attention(*t, 4, 1, 0.25, lse=False).numpy(), want)
