@@ -14,6 +14,7 @@
 #include <cstdio>
 #include <cstring>
 #include <mutex>
+#include <new>
 #include <unordered_set>
 #include <vector>
 
@@ -109,22 +110,26 @@ void return_held(void *arg) {
     delete h;
 }
 // Leaves block p to the graph being captured; where the runtime refuses that,
-// the block is held for good.
-void hold_for_graph(int device, int cls, void *p) {
-    {
+// the block is held for good. False without the memory to note it.
+bool hold_for_graph(int device, int cls, void *p) {
+    try {
         std::lock_guard<std::mutex> lock(g_scratch_mutex);
         g_scratch.held.insert(p);
+    } catch (const std::bad_alloc &) {
+        return false;
     }
     hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
     hipGraph_t graph = nullptr;
     hipUserObject_t object = nullptr;
-    if (hipStreamGetCaptureInfo_v2(stream(), &status, nullptr, &graph, nullptr, nullptr) != hipSuccess || !graph) return;
-    Held *h = new Held{device, cls, p};
+    if (hipStreamGetCaptureInfo_v2(stream(), &status, nullptr, &graph, nullptr, nullptr) != hipSuccess || !graph) return true;
+    Held *h = new (std::nothrow) Held{device, cls, p};
+    if (!h) return true;
     if (hipUserObjectCreate(&object, h, return_held, 1, hipUserObjectNoDestructorSync) != hipSuccess) {
         delete h;
-        return;
+        return true;
     }
     (void)hipGraphRetainUserObject(graph, object, 1, hipGraphUserObjectMove);
+    return true;
 }
 }  // namespace
 
@@ -153,8 +158,7 @@ void *scratch_alloc(size_t bytes) {
         if (relaxed) (void)hipThreadExchangeStreamCaptureMode(&mode);
         if (e != hipSuccess) return nullptr;
     }
-    if (captured) hold_for_graph(device, c, p);
-    return p;
+    return captured && !hold_for_graph(device, c, p) ? nullptr : p;
 }
 
 void scratch_free(void *p, size_t bytes) {
