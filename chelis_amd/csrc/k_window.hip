@@ -555,9 +555,11 @@ struct KeyTiles {
 
 // A workgroup takes 128 rows of one head, each wave 32 of them, which share
 // the staged keys; the rows' q stays in registers. Bound by the softmax
-// between the two products at two waves a SIMD: [2, 16 on 4, 8192, 128] bf16,
-// window 1024, 198 us (matrix cores 29 %, LDS 37 % busy; 650 TFLOP/s over the visible
-// pairs, 1.1 PFLOP/s without a window); [8, 16, 512, 64] f32, window 128, 51 us.
+// between the two products: each 32-cycle product comes with eight vector
+// instructions that take as long, after it in the same wave. [2, 16 on 4, 8192, 128] bf16, window 1024, 198-202
+// us (matrix cores 29 %, LDS 38 % busy at 1.6 resident waves a SIMD; 650 TFLOP/s over
+// the visible pairs, 540 without a window, where the last rows' workgroups end
+// alone); [8, 16, 512, 64] f32, window 128, 51 us.
 template <typename T, int D>
 __global__ __launch_bounds__(kThreads, 2) void window_forward_kernel(WinArgs a, Deal deal) {
     __shared__ __attribute__((aligned(16))) typename KeyTiles<T, D, 1>::Shared sh;

@@ -88,9 +88,11 @@ int32_t chelis_hip_layer_norm(const chelis_gpu_tensor *x, const chelis_gpu_tenso
 
 /* ---- training and serving a block: norm, positions, windowed attention ----
  * No counterparts in the reference. Inputs and results are f32, f64 (not
- * window_attention), bf16 or f16; sums, statistics, scores and softmax
- * weights are held in binary32 (binary64 for f64) and a 16-bit result is
- * rounded once. Sums run in the kernels' own fixed order: the same bits on
+ * window_attention), bf16 or f16; sums, statistics and scores are held in
+ * binary32 (binary64 for f64) and a 16-bit result is rounded once. 16-bit
+ * attention also rounds each softmax weight and each score gradient once to
+ * the operands' type, for the products that sum over them; its log sums and
+ * the divisors of its results are of the unrounded weights. Sums run in the kernels' own fixed order: the same bits on
  * every run, not the canonical tree's. Results may not share storage with
  * another operand unless said so: a call is refused where one is dense, or where
  * one's first or last element lies in the other. A call captured into a graph
@@ -162,7 +164,9 @@ int32_t chelis_hip_window_attention(const chelis_gpu_tensor *q, const chelis_gpu
  * and the same lengths, starts, window, sinks and scale. dk and dv sum over
  * the query heads of a key head and are zero at keys nothing sees; dq is zero
  * at rows that see nothing. What an infinity in a seen operand reaches is
- * infinite or NaN. No atomics: the same bits on every run. */
+ * infinite or NaN. Float16 score gradients share one power of two in a call,
+ * set by its largest |g| and |v|: those more than 2^28 below what these could
+ * give at most, 2 max|g| max|v| width, lose bits. No atomics: the same bits on every run. */
 int32_t chelis_hip_window_attention_adjoint(const chelis_gpu_tensor *q, const chelis_gpu_tensor *k,
                                             const chelis_gpu_tensor *v, const chelis_gpu_tensor *o,
                                             const chelis_gpu_tensor *lse, const chelis_gpu_tensor *g,
