@@ -491,10 +491,12 @@ __device__ inline void store_column(T *row, const f32x16 &c, int d0, int width, 
 // f16 weights are held 2^10 times larger: the smallest keep their bits.
 template <typename T>
 constexpr float kShift = std::is_same<T, _Float16>::value ? 10.f : 0.f;
-// The reference of the exponentials follows the running maximum only when
-// some row's passes it by more than this (in powers of two; 2^15 is the
-// largest f16 weight then): nearly every tile leaves the results unscaled.
-constexpr float kSlack = 5.f;
+// The reference of a row's exponentials follows its running maximum only when
+// that passes it by more than this (in powers of two; 2^15 is the largest f16
+// weight then): nearly every tile leaves the results unscaled ([2, 16 on 4, 8192,
+// 128] bf16, window 1024: 198 us with 8, 202 with 5).
+template <typename T>
+constexpr float kSlack = std::is_same<T, _Float16>::value ? 5.f : 8.f;
 
 // LDS tiles of keys: two of each operand (one barrier a tile) where two
 // workgroups then still fit a compute unit's 160 KB.
@@ -556,10 +558,11 @@ struct KeyTiles {
 // A workgroup takes 128 rows of one head, each wave 32 of them, which share
 // the staged keys; the rows' q stays in registers. Bound by the softmax
 // between the two products: each 32-cycle product comes with eight vector
-// instructions that take as long, after it in the same wave. [2, 16 on 4, 8192, 128] bf16, window 1024, 198-202
-// us (matrix cores 29 %, LDS 38 % busy at 1.6 resident waves a SIMD; 650 TFLOP/s over
-// the visible pairs, 540 without a window, where the last rows' workgroups end
-// alone); [8, 16, 512, 64] f32, window 128, 51 us.
+// instructions that take as long, after it in the same wave. [2, 16 on 4,
+// 8192, 128] bf16, window 1024, 198-202 us (matrix cores 29 %, LDS 38 % busy at
+// 1.6 resident waves a SIMD; 650 TFLOP/s over the visible pairs, 540 without a
+// window, where the last rows' workgroups end alone); [8, 16, 512, 64] f32,
+// window 128, 51 us.
 template <typename T, int D>
 __global__ __launch_bounds__(kThreads, 2) void window_forward_kernel(WinArgs a, Deal deal) {
     __shared__ __attribute__((aligned(16))) typename KeyTiles<T, D, 1>::Shared sh;
@@ -632,8 +635,9 @@ __global__ __launch_bounds__(kThreads, 2) void window_forward_kernel(WinArgs a, 
 #pragma unroll
             for (int r = 0; r < 32; ++r) mx = fmaxf(mx, s[r >> 4][r & 15]);
             mx = fmaxf(mx, other_half(mx)) * a.c;
-            if (__any(mx > m + kSlack)) {
-                const float m_new = fmaxf(m, mx), alpha = exp2_(m - (m_new == -INFINITY ? 0.f : m_new));
+            if (__any(mx > m + kSlack<T>)) {
+                // by the row's own scores alone: no bit of it depends on its neighbours
+                const float m_new = mx > m + kSlack<T> ? mx : m, alpha = exp2_(m - (m_new == -INFINITY ? 0.f : m_new));
                 m = m_new;
                 l *= alpha;
 #pragma unroll

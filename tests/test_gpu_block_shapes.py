@@ -175,3 +175,23 @@ def test_log_sums_not_asked_for():
     t = [C.to_device(x) for x in operands("f32", 1, 2, 1, 3, 9, 16, 47)[:3]]
     want = C.window_attention(*t, 4, 1, 0.25).numpy()
     assert np.array_equal(C.window_attention(*t, 4, 1, 0.25, lse=False).numpy(), want)
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("score", [60.0, np.inf])
+@pytest.mark.parametrize("shape", [(8, 16, 8, 300), (1, 2, 1, 40)], ids=["whole", "split"])
+def test_no_bit_of_a_row_depends_on_scores_it_does_not_have(kind, score, shape):
+    """One key scores far above all others: rows that do not see it, beside
+    rows that do, keep every bit they have without it."""
+    B, H, KV, S = shape
+    W, window, sinks, at = 64, 100, 2, S - 20
+    q, k, v, _ = operands(kind, B, H, KV, S, S, W, 48)
+    q[..., 0] = encode(kind, np.ones(1))[0]
+    far = k.copy()
+    far[:, :, at, 0] = encode(kind, np.full(1, score / 0.125))[0]
+    sees = visible(S, S, S, 0, window, sinks)[:, at]
+    t = [C.to_device(x) for x in (q, k, v)]
+    o, lse = (x.numpy() for x in C.window_attention(*t, window, sinks, 0.125, lse=True))
+    p, lsf = (x.numpy() for x in C.window_attention(t[0], C.to_device(far), t[2], window, sinks, 0.125, lse=True))
+    assert np.array_equal(o[:, :, ~sees], p[:, :, ~sees]) and np.array_equal(lse[:, :, ~sees], lsf[:, :, ~sees])
+    assert not np.array_equal(o[:, :, sees], p[:, :, sees])
