@@ -494,7 +494,7 @@ constexpr float kShift = std::is_same<T, _Float16>::value ? 10.f : 0.f;
 // The reference of a row's exponentials follows its running maximum only when
 // that passes it by more than this (in powers of two; 2^15 is the largest f16
 // weight then): nearly every tile leaves the results unscaled ([2, 16 on 4, 8192,
-// 128] bf16, window 1024: 198 us with 8, 202 with 5).
+// 128] bf16, window 1024: 198 us with 8, 206 with 5).
 template <typename T>
 constexpr float kSlack = std::is_same<T, _Float16>::value ? 5.f : 8.f;
 
@@ -559,7 +559,7 @@ struct KeyTiles {
 // the staged keys; the rows' q stays in registers. Bound by the softmax
 // between the two products: each 32-cycle product comes with eight vector
 // instructions that take as long, after it in the same wave. [2, 16 on 4,
-// 8192, 128] bf16, window 1024, 198-202 us (matrix cores 29 %, LDS 38 % busy at
+// 8192, 128] bf16, window 1024, 197-201 us (matrix cores 29 %, LDS 38 % busy at
 // 1.6 resident waves a SIMD; 650 TFLOP/s over the visible pairs, 540 without a
 // window, where the last rows' workgroups end alone); [8, 16, 512, 64] f32,
 // window 128, 51 us.
