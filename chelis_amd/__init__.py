@@ -65,6 +65,11 @@ class FusedChain(ctypes.Structure):
 
 P = POINTER(GpuTensor)
 
+
+class NormSide(ctypes.Structure):
+    _fields_ = [("kind", c_int32), ("reserved", c_int32), ("gamma", P), ("beta", P), ("mean", P), ("rstd", P)]
+
+
 # Every exported symbol the headers in include/ declare, with its ctypes
 # signature (restype, argtypes). tests/test_abi.py checks the library
 # exports exactly these names.
@@ -122,6 +127,13 @@ SIGNATURES = {
     "chelis_hip_rotary_adjoint": (c_int32, [POINTER(P), c_int32, P, P, POINTER(c_int64), c_int32, c_int32, POINTER(P)]),
     "chelis_hip_window_attention": (c_int32, [P, P, P, P, P, c_int64, c_int64, c_double, P, P]),
     "chelis_hip_window_attention_adjoint": (c_int32, [P, P, P, P, P, P, P, P, c_int64, c_int64, c_double, P, P, P]),
+    "chelis_hip_residual_norm": (c_int32, [P, P, POINTER(NormSide), P, c_double, POINTER(NormSide), c_double, P, P]),
+    "chelis_hip_residual_norm_adjoint": (c_int32, [P, P, POINTER(NormSide), P, c_double, POINTER(NormSide), P, P, P, P, P,
+                                                   P, P, P, P]),
+    "chelis_hip_dense": (c_int32, [P, P, P, c_int32, P, P, P]),
+    "chelis_hip_dense_adjoint": (c_int32, [P, P, P, c_int32, P, P, P, P]),
+    "chelis_hip_gradient_norm": (c_int32, [POINTER(P), c_int32, c_double, P]),
+    "chelis_hip_clip_gradients": (c_int32, [POINTER(P), c_int32, P, c_double, c_double, POINTER(P)]),
     "chelis_hip_fused_elementwise": (c_int32, [POINTER(FusedChain), POINTER(P), c_int32, P]),
     "chelis_hip_gelu": (c_int32, [P, P]),
     "chelis_hip_relu": (c_int32, [P, P]),
@@ -484,6 +496,140 @@ def window_attention_adjoint(q, k, v, o, lse, g, window: int, sinks: int, scale:
                                                     _opt(starts), int(window), int(sinks), scale, _p(dq), _p(dk),
                                                     _p(dv)), "window_attention_adjoint")
     return dq, dk, dv
+
+
+NORM_KINDS = {"none": 0, "layer": 1, "rms": 2}
+
+
+class Norm:
+    """A norm of residual_norm: kind "layer" or "rms", its weights [hidden]
+    (None: 1 and 0) and the row statistics, which the forward call fills (and
+    makes where they are None) and the gradients read."""
+
+    def __init__(self, kind: str, gamma=None, beta=None, mean=None, rstd=None):
+        self.kind, self.gamma, self.beta, self.mean, self.rstd = kind, gamma, beta, mean, rstd
+
+    def _side(self) -> NormSide:
+        return NormSide(NORM_KINDS[self.kind], 0, _opt(self.gamma), _opt(self.beta), _opt(self.mean), _opt(self.rstd))
+
+
+def _side_of(norm):
+    return None if norm is None else ctypes.byref(norm._side())
+
+
+def residual_norm(x, b=None, post=None, gate=None, scale: float = 1.0, pre=None, eps: float = 1e-5, u=None, h=None):
+    """u = x + scale * gate * post(b) and h = pre(u) over the last axis; post
+    and pre are Norm or None, gate [hidden] or [x's first axes .., hidden].
+    Returns (u, h), None for what is not formed; without b, h = pre(x)."""
+    stat = np.float64 if x.dtype == np.float64 else np.float32
+    for norm in (post, pre):
+        if norm is not None:
+            norm.rstd = norm.rstd or empty(x.shape[:-1], stat)
+            if norm.kind == "layer":
+                norm.mean = norm.mean or empty(x.shape[:-1], stat)
+    if b is not None:
+        u = u or empty(x.shape, x.dtype)
+    if pre is not None:
+        h = h or empty(x.shape, x.dtype)
+    check(lib().chelis_hip_residual_norm(_p(x), _opt(b), _side_of(post), _opt(gate), scale, _side_of(pre), eps, _opt(u),
+                                         _opt(h)), "residual_norm")
+    return u, h
+
+
+def residual_norm_adjoint(u, b=None, post=None, gate=None, scale: float = 1.0, pre=None, du=None, dh=None, dx=None,
+                          db=None, dgate=None, dpost=None, dpre=None, want_weights: bool = True):
+    """Gradients of residual_norm for the cotangents du of u and dh of h, from
+    the forward call's u (x where it had no b) and the statistics in post and
+    pre. dpost and dpre: (dgamma, dbeta) to fill, either None for not wanted;
+    left None, they are made for the weights there are unless want_weights is
+    False (dgate likewise). Returns (dx, db, dgate, dpost, dpre)."""
+    like = u if u is not None else du
+    dx = dx or empty(like.shape, like.dtype)
+    if b is not None:
+        db = db or empty(like.shape, like.dtype)
+    if want_weights and gate is not None:
+        dgate = dgate or empty(gate.shape, gate.dtype)
+
+    def pair(norm, given):
+        if given is not None:
+            return given
+        if norm is None or not want_weights:
+            return (None, None)
+        return tuple(None if w is None else empty(w.shape, w.dtype) for w in (norm.gamma, norm.beta))
+
+    dpost, dpre = pair(post, dpost), pair(pre, dpre)
+    check(lib().chelis_hip_residual_norm_adjoint(
+        _opt(u), _opt(b), _side_of(post), _opt(gate), scale, _side_of(pre), _opt(du), _opt(dh), _p(dx), _opt(db),
+        _opt(dgate), _opt(dpost[0]), _opt(dpost[1]), _opt(dpre[0]), _opt(dpre[1])), "residual_norm_adjoint")
+    return dx, db, dgate, dpost, dpre
+
+
+DENSE_ACT = {None: 0, "none": 0, "relu": 1, "gelu": 2, "silu": 3}
+
+
+def dense(x, w, bias=None, act=None, residual=None, y=None, z=None):
+    """act(x @ w + bias) + residual over bf16 / f16 rows x [.., K] and w [K, N]
+    (either axis contiguous). z: a tensor for x @ w + bias, True to make one
+    (None, False: not asked for). Returns y, or (y, z) when z was asked for."""
+    shape = tuple(x.shape[:-1]) + (w.shape[-1],)
+    y = y or empty(shape, x.dtype)
+    z = empty(shape, x.dtype) if z is True else None if z is False else z
+    check(lib().chelis_hip_dense(_p(x), _p(w), _opt(bias), DENSE_ACT[act], _opt(residual), _p(y), _opt(z)), "dense")
+    return y if z is None else (y, z)
+
+
+def dense_adjoint(x, w, g, z=None, act=None, dx=None, dw=None, dbias=None, want_dx: bool = True, want_dw: bool = True,
+                  want_dbias: bool = True):
+    """Gradients of dense for the cotangent g of its result, from the forward
+    call's z where it has an activation; returns (dx, dw, dbias), None for what
+    is not wanted. dw and dbias may be given as f32."""
+    dx = (dx or empty(x.shape, x.dtype)) if want_dx else None
+    dw = (dw or empty(w.shape, x.dtype)) if want_dw else None
+    dbias = (dbias or empty(w.shape[-1:], x.dtype)) if want_dbias else None
+    check(lib().chelis_hip_dense_adjoint(_p(x), _p(w), _opt(z), DENSE_ACT[act], _p(g), _opt(dx), _opt(dw), _opt(dbias)),
+          "dense_adjoint")
+    return dx, dw, dbias
+
+
+class TensorList:
+    """Tensors that a program hands over together, call after call (a model's
+    gradients): their packets are lined up once."""
+
+    def __init__(self, tensors):
+        self.tensors = list(tensors)
+        self.packets = (P * max(1, len(self.tensors)))(*[_p(t) for t in self.tensors])
+
+    def __len__(self):
+        return len(self.tensors)
+
+    def __iter__(self):
+        return iter(self.tensors)
+
+
+def tensor_list(tensors) -> TensorList:
+    return tensors if isinstance(tensors, TensorList) else TensorList(tensors)
+
+
+def gradient_norm(grads, scale: float = 1.0, norm=None):
+    """scale * the norm over all elements of the gradients (a list or a
+    tensor_list), left on the device; norm: one f32 or f64 element."""
+    grads = tensor_list(grads)
+    norm = norm or empty((), np.float32)
+    check(lib().chelis_hip_gradient_norm(grads.packets, len(grads), scale, _p(norm)), "gradient_norm")
+    return norm
+
+
+def clip_gradients(grads, norm, max_norm: float, scale: float = 1.0, out=None):
+    """Each gradient times scale, and times max_norm / norm where norm (that of
+    gradient_norm) is above max_norm: in place, or into `out`. Returns the
+    results."""
+    grads = tensor_list(grads)
+    out = grads if out is None else tensor_list(out)
+    if len(out) != len(grads):
+        raise ChelisError(f"clip_gradients: {len(grads)} gradients and {len(out)} results")
+    check(lib().chelis_hip_clip_gradients(grads.packets, len(grads), _p(norm), max_norm, scale, out.packets),
+          "clip_gradients")
+    return out
 
 
 def gelu(x, y=None):

@@ -1,0 +1,394 @@
+// The 16-bit product of the dense operators on whole 16-byte vectors: operand
+// tiles go from memory straight to LDS (no registers, no waiting in between)
+// several K steps ahead of the matrix instructions that read them.
+#pragma once
+
+#include "elem.h"
+#include "gemm16_tile.h"
+#include "gelu_poly.h"
+
+#include "chelis_hip.h"
+
+namespace chelis {
+namespace {
+
+// c[m][n] = sum_k a[m][k] b[k][n] with its epilogue. Elements of a and b sit at
+// m * sam + k * sak and k * sbk + n * sbn; one stride of each is 1.
+struct DenseProblem {
+    const uint16_t *a, *b;
+    int64_t M, N, K, sam, sak, sbk, sbn;
+    void *c;  // 16 bits, or f32 (c32)
+    int64_t ldc;
+    const void *bias;  // 16 bits, or f32 (bias32)
+    const uint16_t *resid;
+    int64_t ldr;
+    uint16_t *z;
+    int64_t ldz;
+    int32_t c32, bias32, act;
+    // K slices: sums of slice s go to part[s][m][n] instead, kslice k each
+    float *part;
+    int64_t kslice;
+    int32_t slices;
+};
+
+// ---------------------------------------------------------------- activations
+// Phi(-a) = q exp(-a^2 / 2) for a = |x|: q by the degree-9 polynomial of
+// gelu_poly.h (7.1e-8), the exponential in binary32 (its argument's rounding
+// grows to 2^-16 relative at |x| = 13, under a hundredth of a 16-bit rounding).
+// Past 30 both are 0 against 1, and infinities would meet 0.
+__device__ inline void phi_tail(float x, float &q, float &e, float &a) {
+    constexpr float kQ[CHELIS_GELU_DEG + 1] = CHELIS_GELU_Q;
+    a = fminf(fabsf(x), 30.f);
+    const float u = fmaf(-2.0f * CHELIS_GELU_K, __builtin_amdgcn_rcpf(a + CHELIS_GELU_K), 1.0f);
+    q = kQ[CHELIS_GELU_DEG];
+#pragma unroll
+    for (int d = CHELIS_GELU_DEG - 1; d >= 0; --d) q = fmaf(q, u, kQ[d]);
+    e = __builtin_amdgcn_exp2f(a * a * -0.72134752044448170368f);
+}
+__device__ inline float act_gelu(float x) {
+    float q, e, a;
+    phi_tail(x, q, e, a);
+    const float r = fmaf(-(a * q), e, x >= 0.f ? x : 0.f);
+    return x != x ? x : r;
+}
+__device__ inline float slope_gelu(float x) {
+    float q, e, a;
+    phi_tail(x, q, e, a);
+    const float tail = q * e, r = (x >= 0.f ? 1.f - tail : tail) + copysignf(a, x) * (e * 0.39894228040143267794f);
+    return x != x ? x : r;
+}
+// x clamped where the result has long reached its limit (NaN stays).
+__device__ inline float sigmoid(float x) {
+    return __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(x * -1.44269504088896340736f));
+}
+__device__ inline float act_silu(float x) {
+    x = x < -100.f ? -100.f : x;
+    return x * sigmoid(x);
+}
+__device__ inline float slope_silu(float x) {
+    x = x < -100.f ? -100.f : x > 100.f ? 100.f : x;
+    const float s = sigmoid(x);
+    return s * fmaf(x, 1.f - s, 1.f);
+}
+__device__ inline float activate(float x, int act) {
+    switch (act) {
+        case CHELIS_ACT_RELU: return x < 0.f ? 0.f : x;
+        case CHELIS_ACT_GELU: return act_gelu(x);
+        case CHELIS_ACT_SILU: return act_silu(x);
+        default: return x;
+    }
+}
+__device__ inline float act_slope(float x, int act) {
+    switch (act) {
+        case CHELIS_ACT_RELU: return x > 0.f ? 1.f : x != x ? x : 0.f;
+        case CHELIS_ACT_GELU: return slope_gelu(x);
+        case CHELIS_ACT_SILU: return slope_silu(x);
+        default: return 1.f;
+    }
+}
+
+// ---------------------------------------------------------------- epilogue
+template <Narrow K>
+struct Elem16;
+template <>
+struct Elem16<Narrow::Bf16> {
+    using type = __bf16;
+};
+template <>
+struct Elem16<Narrow::F16> {
+    using type = _Float16;
+};
+template <Narrow KIND>
+using Vec16 = Pack<typename Elem16<KIND>::type, 8>;
+
+// Eight elements of a row, as far as `count` goes.
+template <Narrow KIND>
+__device__ inline void store8(uint16_t *p, const float (&v)[8], int64_t count) {
+    using T = typename Elem16<KIND>::type;
+    T *o = reinterpret_cast<T *>(p);
+    Vec16<KIND> q;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) q.set(i, v[i]);
+    if (count >= 8) q.store(o);
+    else {
+#pragma unroll
+        for (int i = 0; i < 7; ++i)
+            if (i < count) o[i] = q.q[i];
+    }
+}
+template <Narrow KIND>
+__device__ inline void load8f(const uint16_t *p, float (&v)[8], int64_t count) {
+    using T = typename Elem16<KIND>::type;
+    const T *in = reinterpret_cast<const T *>(p);
+    Vec16<KIND> q{};
+    if (count >= 8) q.load(in);
+    else {
+#pragma unroll
+        for (int i = 0; i < 7; ++i)
+            if (i < count) q.q[i] = in[i];
+    }
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = q.get(i);
+}
+typedef float F4 __attribute__((ext_vector_type(4), aligned(4)));
+
+// Eight neighbouring columns of row m from n on, as far as the result has them.
+template <Narrow KIND>
+__device__ inline void finish8(const DenseProblem &p, int64_t m, int64_t n, float (&v)[8]) {
+    const int64_t count = p.N - n;
+    if (p.bias) {
+        float b[8];
+        if (p.bias32) {
+            const float *q = static_cast<const float *>(p.bias) + n;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) b[i] = i < count ? q[i] : 0.f;
+        } else load8f<KIND>(static_cast<const uint16_t *>(p.bias) + n, b, count);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] += b[i];
+    }
+    if (p.z) store8<KIND>(p.z + m * p.ldz + n, v, count);
+    if (p.act != CHELIS_ACT_NONE) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = activate(v[i], p.act);
+    }
+    if (p.resid) {
+        float r[8];
+        load8f<KIND>(p.resid + m * p.ldr + n, r, count);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] += r[i];
+    }
+    if (p.c32) {
+        float *o = static_cast<float *>(p.c) + m * p.ldc + n;
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+            if (i < count) o[i] = canon_bits(v[i]);
+    } else store8<KIND>(static_cast<uint16_t *>(p.c) + m * p.ldc + n, v, count);
+}
+// The same for one K slice's sums.
+__device__ inline void slice8(const DenseProblem &p, int64_t slice, int64_t m, int64_t n, const float (&v)[8]) {
+    float *o = p.part + (slice * p.M + m) * p.N + n;
+    if (n + 8 <= p.N) {
+        *reinterpret_cast<F4 *>(o) = F4{v[0], v[1], v[2], v[3]};
+        *reinterpret_cast<F4 *>(o + 4) = F4{v[4], v[5], v[6], v[7]};
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+            if (n + i < p.N) o[i] = v[i];
+    }
+}
+
+// ---------------------------------------------------------------- tiles
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef int i32x4 __attribute__((ext_vector_type(4)));
+#define CHELIS_LDS __attribute__((address_space(3)))
+
+template <Narrow K>
+__device__ inline f32x16 mfma32(uint4 a, uint4 b, f32x16 c) {
+    if constexpr (K == Narrow::Bf16)
+        return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0,
+                                                       0, 0);
+    else
+        return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0,
+                                                      0);
+}
+
+// 64 16-byte vectors, one a lane, from base + voff to 1 KiB of LDS at lds (the
+// same in every lane). The hardware checks voff against the buffer's 2^31
+// bytes: a lane with kNowhere reads nothing and stores zeros. Written in
+// assembly because the compiler waits for such a load before the next
+// transposed LDS read, whichever buffer that goes to; it writes no register, and
+// load_wait below waits for it.
+constexpr uint32_t kNowhere = 0x80000000u;
+__device__ inline void load_to_lds(uint32_t lds, uint32_t voff, const uint16_t *base) {
+    const uint64_t at = reinterpret_cast<uint64_t>(base);
+    const i32x4 r = {(int)(uint32_t)at, (int)(uint32_t)(at >> 32 & 0xffff), (int)0x80000000u, 0x00027000};
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(lds), "v"(voff), "s"(r) : "memory");
+}
+// Until at most N of this wave's loads are under way (they land in order) and
+// its LDS reads are done; then every wave of the workgroup.
+template <int N>
+__device__ inline void load_wait() {
+    asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(N) : "memory");
+}
+
+// One operand's tile of ROWS outer elements by BK.
+//   LAY 0, contiguous along k: LDS holds [row][BK], the 16-byte vectors of a row
+//     exchanged by the row, so that neighbouring lanes' rows lie on different
+//     banks; a fragment is one 16-byte read.
+//   LAY 1, contiguous along the outer axis: LDS holds [k][ROWS], the 32-byte
+//     pairs of a k exchanged by k; a fragment is two transposing reads, each of
+//     four k by 16 rows to 16 lanes.
+template <int LAY, int ROWS, int BK, int THREADS_>
+struct Operand {
+    static constexpr int VEC = ROWS * BK / 8, NV = VEC / THREADS_, LINE = LAY == 0 ? BK / 8 : ROWS / 8;
+    static_assert(VEC % THREADS_ == 0, "whole vectors a thread");
+    static constexpr int BYTES = ROWS * BK * 2;
+    uint32_t off[NV];
+    const uint16_t *at;  // the tile at the next K step to load
+    int64_t step;
+
+    // row0: the tile's first outer element of `outer`; s: the stride of the
+    // other axis.
+    __device__ void init(const uint16_t *base, int64_t s, int64_t row0, int64_t outer, int64_t k0) {
+        const int t = threadIdx.x;
+        at = LAY == 0 ? base + row0 * s + k0 : base + row0 + k0 * s;
+        step = LAY == 0 ? BK : BK * s;
+        const int64_t left = outer - row0;
+#pragma unroll
+        for (int j = 0; j < NV; ++j) {
+            const int slot = t + THREADS_ * j, line = slot / LINE, v = vector_at(line, slot % LINE);
+            const bool there = LAY == 0 ? line < left : 8 * v < left;
+            off[j] = there ? 2u * (uint32_t)(line * (uint32_t)s + 8 * v) : kNowhere;
+        }
+    }
+    // the vector that LDS position p of a line holds (its own inverse)
+    __device__ static int vector_at(int line, int p) {
+        if constexpr (LAY == 0) return p ^ (BK >= 64 ? line & 7 : line >> 1 & 3);
+        else return p ^ (ROWS >= 64 ? (line & 3) << 1 : (line >> 1 & 1) << 1);
+    }
+    // left: K elements from this step on
+    __device__ void load(uint32_t lds, int64_t left) {
+        const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+        const uint32_t to = __builtin_amdgcn_readfirstlane(lds + wave * 1024);
+        if (left >= BK) {
+#pragma unroll
+            for (int j = 0; j < NV; ++j) load_to_lds(to + j * THREADS_ * 16, off[j], at);
+        } else {
+#pragma unroll
+            for (int j = 0; j < NV; ++j) {
+                const int slot = threadIdx.x + THREADS_ * j, line = slot / LINE;
+                const int k = LAY == 0 ? 8 * vector_at(line, slot % LINE) : line;
+                load_to_lds(to + j * THREADS_ * 16, k < left ? off[j] : kNowhere, at);
+            }
+        }
+        at += step;
+    }
+    // rows row .. row + 31, k = 16 kk + 8 (lane / 32) ..: lane's fragment
+    __device__ static uint4 fragment(const uint16_t *tile, int row, int kk) {
+        const int lane = threadIdx.x & 63;
+        if constexpr (LAY == 0) {
+            const int r = row + (lane & 31), v = 2 * kk + (lane >> 5);
+            return *reinterpret_cast<const uint4 *>(tile + r * BK + 8 * vector_at(r, v));
+        } else {
+            const int i = lane & 15, k = 16 * kk + 8 * (lane >> 5) + (i >> 2), r = row + 16 * (lane >> 4 & 1) + 4 * (i & 3);
+            const uint16_t *at = tile + k * ROWS + 8 * vector_at(k, r >> 3) + (r & 7);
+            const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((CHELIS_LDS s16x4 *)at);
+            const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((CHELIS_LDS s16x4 *)(at + 4 * ROWS));
+            return __builtin_bit_cast(uint4, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
+        }
+    }
+};
+
+// A workgroup's tile: XCDs (workgroups are dealt to them in turn) get a run of
+// tiles each, walked in groups of GM tile rows so that a run shares operands.
+__device__ inline void tile_of(int64_t bid, int64_t tiles_m, int64_t tiles_n, int GM, int64_t *tm, int64_t *tn) {
+    const int64_t tiles = tiles_m * tiles_n, q = tiles / 8, r = tiles % 8, xcd = bid % 8;
+    bid = xcd * q + (xcd < r ? xcd : r) + bid / 8;
+    const int64_t group = bid / (GM * tiles_n), first = group * GM;
+    const int64_t size = tiles_m - first < GM ? tiles_m - first : GM, in = bid - group * GM * tiles_n;
+    *tm = first + in % size;
+    *tn = in / size;
+}
+
+// BM x BN results a workgroup of WM x WN waves, WK times (each with its part of
+// every step's k, joined at the end), K in steps of BK through ST buffers.
+template <int BM_, int BN_, int BK_, int WM_, int WN_, int WK_, int ST_, int OCC_>
+struct TileShape {
+    static constexpr int BM = BM_, BN = BN_, BK = BK_, WM = WM_, WN = WN_, WK = WK_, ST = ST_, OCC = OCC_;
+    static constexpr int THREADS = 64 * WM * WN * WK, MI = BM / WM / 32, NJ = BN / WN / 32;
+    static constexpr int STAGE = (BM + BN) * BK * 2, PITCH = BN + 4, EPI = WM * 32 * PITCH * 4;
+    static constexpr int BYTES = STAGE * ST > EPI * WK ? STAGE * ST : EPI * WK;
+    static_assert(BK / 16 % WK == 0, "whole k blocks a wave");
+};
+
+template <Narrow KIND, int ALAY, int BLAY, class C>
+__global__ __launch_bounds__(C::THREADS, C::OCC) void dense_tile_kernel(DenseProblem p, int64_t tiles_m, int64_t tiles_n) {
+    constexpr int BM = C::BM, BN = C::BN, BK = C::BK, ST = C::ST, MI = C::MI, NJ = C::NJ;
+    __shared__ __attribute__((aligned(1024))) char lds[C::BYTES];
+    int64_t tm, tn;
+    tile_of(blockIdx.x, tiles_m, tiles_n, 8, &tm, &tn);
+    const int64_t m0 = tm * BM, n0 = tn * BN, k0 = blockIdx.y * p.kslice;
+    const int64_t K = p.K - k0 < p.kslice ? p.K - k0 : p.kslice;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, wk = wave / (C::WM * C::WN);
+    const int wm = wave / C::WN % C::WM, wn = wave % C::WN;
+
+    Operand<ALAY, BM, BK, C::THREADS> a;
+    Operand<BLAY, BN, BK, C::THREADS> b;
+    a.init(p.a, ALAY == 0 ? p.sam : p.sak, m0, p.M, k0);
+    b.init(p.b, BLAY == 0 ? p.sbn : p.sbk, n0, p.N, k0);
+    const uint32_t lds0 = (uint32_t)reinterpret_cast<uintptr_t>((CHELIS_LDS char *)lds);
+    const int steps = (int)((K + BK - 1) / BK);
+    int64_t left = K;
+    int into = 0;
+    // past the last step nothing is read, the loads only keep the count
+    auto load = [&]() {
+        a.load(lds0 + into * C::STAGE, left);
+        b.load(lds0 + into * C::STAGE + BM * BK * 2, left);
+        left -= BK;
+        into = into + 1 == ST ? 0 : into + 1;
+    };
+#pragma unroll
+    for (int s = 0; s < ST - 1; ++s) load();
+
+    f32x16 acc[MI][NJ];
+#pragma unroll
+    for (int i = 0; i < MI; ++i)
+#pragma unroll
+        for (int j = 0; j < NJ; ++j) acc[i][j] = f32x16{};
+    constexpr int AHEAD = (ST - 2) * (a.NV + b.NV);
+    int from = 0;
+    for (int s = 0; s < steps; ++s) {
+        load_wait<AHEAD>();
+        load();
+        const uint16_t *as = reinterpret_cast<const uint16_t *>(lds + from * C::STAGE), *bs = as + BM * BK;
+        from = from + 1 == ST ? 0 : from + 1;
+#pragma unroll
+        for (int kk = 0; kk < BK / 16; kk += C::WK) {
+            uint4 af[MI], bf[NJ];
+#pragma unroll
+            for (int i = 0; i < MI; ++i) af[i] = a.fragment(as, (wm * MI + i) * 32, kk + wk);
+#pragma unroll
+            for (int j = 0; j < NJ; ++j) bf[j] = b.fragment(bs, (wn * NJ + j) * 32, kk + wk);
+#pragma unroll
+            for (int i = 0; i < MI; ++i)
+#pragma unroll
+                for (int j = 0; j < NJ; ++j) acc[i][j] = mfma32<KIND>(af[i], bf[j], acc[i][j]);
+        }
+    }
+    load_wait<0>();
+    // 32 rows of every wave at a time through LDS: lanes then hold eight
+    // neighbouring columns, and memory sees whole rows of the tile
+    float *stage = reinterpret_cast<float *>(lds), *mine = stage + wk * (C::EPI / 4);
+#pragma unroll
+    for (int i = 0; i < MI; ++i) {
+        if (i) __syncthreads();
+#pragma unroll
+        for (int j = 0; j < NJ; ++j)
+#pragma unroll
+            for (int r = 0; r < 16; ++r)
+                mine[(wm * 32 + (r & 3) + 8 * (r >> 2) + 4 * (lane >> 5)) * C::PITCH + (wn * NJ + j) * 32 + (lane & 31)] =
+                    acc[i][j][r];
+        __syncthreads();
+        constexpr int PER = BN / 8, VECS = C::WM * 32 * PER;
+#pragma unroll 1
+        for (int v0 = 0; v0 < VECS; v0 += C::THREADS) {
+            const int v = v0 + threadIdx.x, row = v / PER, col = 8 * (v % PER);
+            if (VECS % C::THREADS && v >= VECS) break;
+            const int64_t m = m0 + ((row >> 5) * MI + i) * 32 + (row & 31), n = n0 + col;
+            if (m >= p.M || n >= p.N) continue;
+            float x[8];
+#pragma unroll
+            for (int q = 0; q < 8; ++q) x[q] = stage[row * C::PITCH + col + q];
+#pragma unroll
+            for (int w = 1; w < C::WK; ++w)
+#pragma unroll
+                for (int q = 0; q < 8; ++q) x[q] += stage[w * (C::EPI / 4) + row * C::PITCH + col + q];
+            if (p.part) slice8(p, blockIdx.y, m, n, x);
+            else finish8<KIND>(p, m, n, x);
+        }
+    }
+}
+
+}  // namespace
+}  // namespace chelis

@@ -1,0 +1,400 @@
+// The global norm of many gradients and their clipping, for a training step.
+//
+//   norm = scale * sqrt(sum over every element of every tensor of g^2)
+//   out  = g * factor,  factor = scale * (norm > max_norm ? max_norm / norm : 1)
+//
+// The tensors travel as a table in the kernel arguments, so a call is capturable
+// as it stands and copies nothing to the device; a workgroup takes one run of
+// one tensor and finds it by bisection over the runs' first workgroups. Squares
+// and sums are binary64 (every f32, bf16 and f16 square is exact there and no
+// gradient overflows the sum); each workgroup writes one partial sum and one
+// workgroup adds them in order: no atomics, the same bits on every run. The
+// factor is formed on the device from the stored norm, so nothing waits for the
+// host.
+//
+// Bound by HBM: the norm reads everything once, the clipping reads and writes it
+// once.
+#include "elem.h"
+
+#include <algorithm>
+#include <new>
+
+namespace chelis {
+namespace {
+
+constexpr int kThreads = 256;
+
+// One tensor: `rows` runs of n elements, ldi (ldo) apart; work is dealt in
+// `cuts` pieces a row.
+struct Item {
+    const void *in;
+    void *out;
+    int64_t n;
+    int64_t ldi, ldo;
+    uint32_t rows, cuts;
+    uint32_t first;  // its first workgroup in the launch
+    uint32_t dtype;
+};
+// A launch's arguments stay under 4 KiB.
+constexpr int kItems = 64;
+struct Table {
+    Item item[kItems];
+    int32_t count;
+    uint32_t blocks;
+    int64_t chunk;  // elements to a piece
+    double *part;
+    const void *norm;
+    double max_norm, scale;
+    int32_t norm64;
+    int32_t in_place;
+};
+static_assert(sizeof(Table) <= 4096, "kernel arguments");
+
+struct Piece {
+    Item it;
+    int64_t row, lo, hi;
+};
+__device__ inline Piece piece_of(const Table &t, uint32_t block) {
+    int lo = 0, hi = t.count;
+    while (hi - lo > 1) {
+        const int mid = (lo + hi) >> 1;
+        if (t.item[mid].first <= block) lo = mid;
+        else hi = mid;
+    }
+    Piece p;
+    p.it = t.item[lo];
+    const uint32_t k = block - p.it.first;
+    p.row = k / p.it.cuts;
+    p.lo = (int64_t)(k % p.it.cuts) * t.chunk;
+    p.hi = p.lo + t.chunk < p.it.n ? p.lo + t.chunk : p.it.n;
+    return p;
+}
+
+template <class F>
+__device__ inline void with_dtype(uint32_t d, F &&f) {
+    switch (d) {
+        case CHELIS_DTYPE_F32: f(float()); break;
+        case CHELIS_DTYPE_F64: f(double()); break;
+        case CHELIS_DTYPE_BF16: f(__bf16()); break;
+        default: f(_Float16());
+    }
+}
+
+// Sum of one value per thread over the workgroup, in thread 0.
+__device__ inline double block_total(double s) {
+    __shared__ double wave_sum[16];
+    s = wave_tree_sum(s);
+    if ((threadIdx.x & 63) == 0) wave_sum[threadIdx.x >> 6] = s;
+    __syncthreads();
+    if (threadIdx.x == 0)
+        for (int w = 1; w < (int)((blockDim.x + 63) / 64); ++w) s += wave_sum[w];
+    return s;
+}
+
+template <typename T, int V, int U>
+__device__ inline double squares(const T *p, int64_t lo, int64_t hi) {
+    double s[U] = {};
+    int64_t j = lo + (int64_t)threadIdx.x * V;
+    for (; j + (int64_t)(U - 1) * kThreads * V + V <= hi; j += (int64_t)U * kThreads * V) {
+        Pack<T, V> q[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) q[u].load(p + j + (int64_t)u * kThreads * V);
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+#pragma unroll
+            for (int i = 0; i < V; ++i) {
+                const double v = (double)q[u].get(i);
+                s[u] = fma(v, v, s[u]);
+            }
+    }
+    for (; j + V <= hi; j += (int64_t)kThreads * V) {
+        Pack<T, V> q;
+        q.load(p + j);
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+            const double v = (double)q.get(i);
+            s[0] = fma(v, v, s[0]);
+        }
+    }
+    if (j < hi)
+        for (int64_t e = j; e < hi; ++e) {
+            const double v = (double)widen(p[e]);
+            s[0] = fma(v, v, s[0]);
+        }
+#pragma unroll
+    for (int u = 1; u < U; ++u) s[0] += s[u];
+    return s[0];
+}
+
+__global__ __launch_bounds__(kThreads) void norm_parts_kernel(Table t) {
+    const Piece p = piece_of(t, blockIdx.x);
+    double s = 0;
+    with_dtype(p.it.dtype, [&](auto z) {
+        using T = decltype(z);
+        s = squares<T, 16 / sizeof(T), 4>(static_cast<const T *>(p.it.in) + p.row * p.it.ldi, p.lo, p.hi);
+    });
+    s = block_total(s);
+    if (threadIdx.x == 0) t.part[blockIdx.x] = s;
+}
+
+__global__ __launch_bounds__(1024) void norm_join_kernel(const double *part, int64_t count, double scale, void *norm,
+                                                         int32_t norm64) {
+    double s = 0;
+    for (int64_t i = threadIdx.x; i < count; i += 1024) s += part[i];
+    s = block_total(s);
+    if (threadIdx.x == 0) {
+        const double v = scale * sqrt(s);
+        if (norm64) *static_cast<double *>(norm) = canon_bits(v);
+        else *static_cast<float *>(norm) = canon_bits((float)v);
+    }
+}
+
+// A product in binary64 for the wide types (rounded once), in binary32 for the
+// 16-bit ones (the factor's own rounding is 2^-24 beside their 2^-9 and 2^-12).
+template <typename T>
+__device__ inline T scaled(T v, double factor) {
+    if constexpr (sizeof(T) == 2) return finalize<T>(widen(v) * (float)factor);
+    else return finalize<T>((T)((double)v * factor));
+}
+
+template <typename T, int V, int U>
+__device__ inline void scale_run(const T *p, T *o, int64_t lo, int64_t hi, double factor) {
+    int64_t j = lo + (int64_t)threadIdx.x * V;
+    for (; j + (int64_t)(U - 1) * kThreads * V + V <= hi; j += (int64_t)U * kThreads * V) {
+        Pack<T, V> q[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) q[u].load(p + j + (int64_t)u * kThreads * V);
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+#pragma unroll
+            for (int i = 0; i < V; ++i) q[u].q[i] = scaled<T>(q[u].q[i], factor);
+            q[u].store_streamed(o + j + (int64_t)u * kThreads * V);
+        }
+    }
+    for (; j + V <= hi; j += (int64_t)kThreads * V) {
+        Pack<T, V> q;
+        q.load(p + j);
+#pragma unroll
+        for (int i = 0; i < V; ++i) q.q[i] = scaled<T>(q.q[i], factor);
+        q.store_streamed(o + j);
+    }
+    if (j < hi)
+        for (int64_t e = j; e < hi; ++e) o[e] = scaled<T>(p[e], factor);
+}
+
+__global__ __launch_bounds__(kThreads) void clip_kernel(Table t) {
+    const double norm = t.norm64 ? *static_cast<const double *>(t.norm) : (double)*static_cast<const float *>(t.norm);
+    const double factor = norm > t.max_norm ? t.scale * (t.max_norm / norm) : t.scale;
+    if (t.in_place && factor == 1.0) return;
+    const Piece p = piece_of(t, t.blocks - 1 - blockIdx.x);
+    with_dtype(p.it.dtype, [&](auto z) {
+        using T = decltype(z);
+        scale_run<T, 16 / sizeof(T), 4>(static_cast<const T *>(p.it.in) + p.row * p.it.ldi,
+                                        static_cast<T *>(p.it.out) + p.row * p.it.ldo, p.lo, p.hi, factor);
+    });
+}
+
+// ---------------------------------------------------------------- host
+// The elements of `in` (and the same ones of `out`, null: none) as rows of a
+// contiguous run: axes in the order of in's strides, neighbours joined where
+// both allow it.
+bool collapse(const chelis_gpu_tensor *in, const chelis_gpu_tensor *out, Item *it) {
+    int32_t idx[8], k = 0;
+    for (int32_t a = 0; a < in->rank; ++a)
+        if (in->shape[a] > 1) idx[k++] = a;
+    std::sort(idx, idx + k, [&](int32_t x, int32_t y) { return in->strides[x] > in->strides[y]; });
+    int64_t ext[8], si[8], so[8];
+    int32_t m = 0;
+    for (int32_t i = 0; i < k; ++i) {
+        const int64_t e = in->shape[idx[i]], s = in->strides[idx[i]], o = out ? out->strides[idx[i]] : s;
+        if (m && si[m - 1] == s * e && so[m - 1] == o * e) ext[m - 1] *= e, si[m - 1] = s, so[m - 1] = o;
+        else ext[m] = e, si[m] = s, so[m] = o, ++m;
+    }
+    it->rows = 1, it->n = 1, it->ldi = it->ldo = 0;
+    if (m == 0) return true;
+    if (si[m - 1] == 1 && so[m - 1] == 1) it->n = ext[--m];
+    if (m > 1 || (m == 1 && (ext[0] > UINT32_MAX))) return false;
+    if (m == 1) it->rows = (uint32_t)ext[0], it->ldi = si[0], it->ldo = so[0];
+    return true;
+}
+
+int32_t check_gradient(const chelis_gpu_tensor *g, const char *what) {
+    if (int32_t s = check_tensor(g, "a gradient")) return s;
+    if (!(is_float(g->dtype) || is_narrow16(g->dtype)))
+        return set_error(CHELIS_HIP_EDOMAIN, "%s: gradients must be f32, f64, bf16 or f16", what);
+    if (g->count && !non_overlapping(g)) return set_error(CHELIS_HIP_EDOMAIN, "%s: a gradient overlaps itself", what);
+    return check_device(g, "a gradient");
+}
+
+int32_t check_norm(const chelis_gpu_tensor *norm, const char *what) {
+    if (int32_t s = check_tensor(norm, "norm")) return s;
+    if (!is_float(norm->dtype) || norm->count != 1)
+        return set_error(CHELIS_HIP_EDOMAIN, "%s: norm must be one f32 or f64 element", what);
+    return check_device(norm, "norm");
+}
+
+int32_t check_factor(double v, const char *name, const char *what) {
+    if (!(v > 0) || std::isinf(v)) return set_error(CHELIS_HIP_EDOMAIN, "%s: %s must be positive and finite", what, name);
+    return CHELIS_HIP_OK;
+}
+
+// Byte ranges of tensors for the overlap search.
+struct Range {
+    uintptr_t lo, hi;
+    int32_t i;
+    bool out;
+};
+Range range_of(const chelis_gpu_tensor *t, int32_t i, bool out) {
+    int64_t reach = 1;
+    for (int32_t a = 0; a < t->rank; ++a) reach += (t->shape[a] - 1) * t->strides[a];
+    const uintptr_t lo = reinterpret_cast<uintptr_t>(t->data);
+    return {lo, lo + (uintptr_t)(reach * dtype_width(t->dtype)), i, out};
+}
+
+// No result shares storage with another result, with another tensor's gradient
+// or, other than element for element, with its own. Sorted by address, so a
+// model's hundreds of gradients do not make a call of all pairs.
+int32_t check_results(const chelis_gpu_tensor *const *gs, const chelis_gpu_tensor *const *outs, int32_t n) {
+    Range *r = new (std::nothrow) Range[2 * (size_t)n + 1];
+    if (!r) return set_error(CHELIS_HIP_EHIP, "clip_gradients: no memory to compare %d tensors", n);
+    int32_t k = 0, status = CHELIS_HIP_OK;
+    for (int32_t i = 0; i < n; ++i) {
+        if (!gs[i]->count) continue;
+        r[k++] = range_of(outs[i], i, true);
+        if (!same_view(gs[i], outs[i])) r[k++] = range_of(gs[i], i, false);
+    }
+    std::sort(r, r + k, [](const Range &a, const Range &b) { return a.lo < b.lo; });
+    for (int32_t a = 0; a < k && !status; ++a)
+        for (int32_t b = a + 1; b < k && r[b].lo < r[a].hi && !status; ++b) {
+            if (!r[a].out && !r[b].out) continue;
+            const chelis_gpu_tensor *x = r[a].out ? outs[r[a].i] : gs[r[a].i], *y = r[b].out ? outs[r[b].i] : gs[r[b].i];
+            if (shares_storage(x, y))
+                status = set_error(CHELIS_HIP_EDOMAIN, "clip_gradients: result %d overlaps %s %d", r[a].out ? r[a].i : r[b].i,
+                                   r[a].out && r[b].out ? "result" : "gradient", r[a].out ? r[b].i : r[a].i);
+        }
+    delete[] r;
+    return status;
+}
+
+// Elements to a workgroup's piece: 16 KiB, more once that would be over 4096
+// workgroups (their partial sums are joined by one).
+int64_t chunk_for(const chelis_gpu_tensor *const *gs, int32_t n) {
+    int64_t total = 0;
+    for (int32_t i = 0; i < n; ++i) total += gs[i]->count;
+    const int64_t step = 4 * 8 * kThreads;  // whole unrolled rounds of the widest vectors
+    return std::max<int64_t>(1, (total / 4096 + step - 1) / step) * step;
+}
+
+// f(table) for every launch's worth of non-empty tensors.
+template <class F>
+int32_t for_tables(const chelis_gpu_tensor *const *gs, const chelis_gpu_tensor *const *outs, int32_t n, Table &t, F &&f) {
+    t.chunk = chunk_for(gs, n);
+    t.count = 0, t.blocks = 0;
+    for (int32_t i = 0; i <= n; ++i) {
+        if (i < n && !gs[i]->count) continue;
+        Item it{};
+        int64_t blocks = 0;
+        if (i < n) {
+            collapse(gs[i], outs ? outs[i] : nullptr, &it);
+            it.in = gs[i]->data, it.out = outs ? outs[i]->data : nullptr, it.dtype = gs[i]->dtype;
+            it.cuts = (uint32_t)((it.n + t.chunk - 1) / t.chunk);
+            blocks = (int64_t)it.rows * it.cuts;
+        }
+        if (t.count && (i == n || t.count == kItems || t.blocks + blocks > INT32_MAX / 256)) {
+            if (int32_t s = f(t)) return s;
+            t.count = 0, t.blocks = 0;
+        }
+        if (i < n) {
+            it.first = t.blocks;
+            t.item[t.count++] = it;
+            t.blocks += (uint32_t)blocks;
+        }
+    }
+    return CHELIS_HIP_OK;
+}
+
+int32_t check_layout(const chelis_gpu_tensor *g, const chelis_gpu_tensor *out, int32_t i, int64_t chunk, const char *what) {
+    Item it;
+    if (!collapse(g, out, &it) || (int64_t)it.rows * ((it.n + chunk - 1) / chunk) > INT32_MAX / 256)
+        return set_error(CHELIS_HIP_EUNSUPPORTED,
+                         "%s: gradient %d is neither dense nor at most 2^23 rows of contiguous elements a fixed step apart%s",
+                         what, i, out ? ", or its result has another order of axes" : "");
+    return CHELIS_HIP_OK;
+}
+
+}  // namespace
+}  // namespace chelis
+
+using namespace chelis;
+
+extern "C" int32_t chelis_hip_gradient_norm(const chelis_gpu_tensor *const *gs, int32_t n, double scale,
+                                            const chelis_gpu_tensor *norm) {
+    const char *what = "gradient_norm";
+    int32_t s;
+    if (n < 0 || (n && !gs)) return set_error(CHELIS_HIP_EDOMAIN, "%s: %d gradients", what, n);
+    if ((s = check_norm(norm, what)) || (s = check_factor(scale, "scale", what))) return s;
+    for (int32_t i = 0; i < n; ++i) {
+        if ((s = check_gradient(gs[i], what))) return s;
+        if (shares_storage(norm, gs[i]))
+            return set_error(CHELIS_HIP_EDOMAIN, "%s: norm and gradient %d overlap", what, i);
+    }
+    const int64_t chunk = chunk_for(gs, n);
+    int64_t parts = 0;
+    for (int32_t i = 0; i < n; ++i) {
+        if ((s = check_layout(gs[i], nullptr, i, chunk, what))) return s;
+        Item it;
+        if (gs[i]->count && collapse(gs[i], nullptr, &it)) parts += (int64_t)it.rows * ((it.n + chunk - 1) / chunk);
+    }
+    hipStream_t st = stream();
+    if (!st) return set_error(CHELIS_HIP_EHIP, "no HIP device");
+    const size_t bytes = (size_t)std::max<int64_t>(1, parts) * sizeof(double);
+    Table t{};
+    double *part = static_cast<double *>(scratch_alloc(bytes));
+    if (!part) return set_error(CHELIS_HIP_EHIP, "%s: scratch of %zu bytes", what, bytes);
+    t.part = part;
+    s = for_tables(gs, nullptr, n, t, [&](Table &tab) -> int32_t {
+        norm_parts_kernel<<<tab.blocks, kThreads, 0, st>>>(tab);
+        tab.part += tab.blocks;
+        CHELIS_LAUNCH_CHECK();
+        return CHELIS_HIP_OK;
+    });
+    if (!s) norm_join_kernel<<<1, 1024, 0, st>>>(part, parts, scale, norm->data, norm->dtype == CHELIS_DTYPE_F64);
+    const hipError_t e = hipGetLastError();
+    scratch_free(part, bytes);
+    if (s) return s;
+    if (e != hipSuccess) return set_error(CHELIS_HIP_EHIP, "kernel launch: %s", hipGetErrorString(e));
+    return CHELIS_HIP_OK;
+}
+
+extern "C" int32_t chelis_hip_clip_gradients(const chelis_gpu_tensor *const *gs, int32_t n,
+                                             const chelis_gpu_tensor *norm, double max_norm, double scale,
+                                             const chelis_gpu_tensor *const *outs) {
+    const char *what = "clip_gradients";
+    int32_t s;
+    if (n < 0 || (n && (!gs || !outs))) return set_error(CHELIS_HIP_EDOMAIN, "%s: %d gradients", what, n);
+    if ((s = check_norm(norm, what)) || (s = check_factor(scale, "scale", what)) ||
+        (s = check_factor(max_norm, "max_norm", what)))
+        return s;
+    bool in_place = true;
+    for (int32_t i = 0; i < n; ++i) {
+        if ((s = check_gradient(gs[i], what)) || (s = check_gradient(outs[i], what))) return s;
+        if (gs[i]->dtype != outs[i]->dtype || !same_shape(gs[i], outs[i]))
+            return set_error(CHELIS_HIP_EDOMAIN, "%s: result %d must match its gradient in shape and dtype", what, i);
+        if (shares_storage(norm, outs[i])) return set_error(CHELIS_HIP_EDOMAIN, "%s: norm and result %d overlap", what, i);
+        in_place = in_place && (!gs[i]->count || same_view(gs[i], outs[i]));
+    }
+    const int64_t chunk = n ? chunk_for(gs, n) : 1;
+    for (int32_t i = 0; i < n; ++i)
+        if ((s = check_layout(gs[i], outs[i], i, chunk, what))) return s;
+    if ((s = check_results(gs, outs, n))) return s;
+    hipStream_t st = stream();
+    if (!st) return set_error(CHELIS_HIP_EHIP, "no HIP device");
+    Table t{};
+    t.norm = norm->data, t.norm64 = norm->dtype == CHELIS_DTYPE_F64;
+    t.max_norm = max_norm, t.scale = scale, t.in_place = in_place;
+    return for_tables(gs, outs, n, t, [&](Table &tab) -> int32_t {
+        clip_kernel<<<tab.blocks, kThreads, 0, st>>>(tab);
+        CHELIS_LAUNCH_CHECK();
+        return CHELIS_HIP_OK;
+    });
+}

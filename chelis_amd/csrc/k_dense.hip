@@ -1,0 +1,476 @@
+// The 16-bit product with bias, activation and residual in its epilogue, and its
+// gradients.
+//
+//   z = x . w + bias,  y = act(z) + residual
+//   dz = g * act'(z),  dx = dz . w^T,  dw = x^T . dz,  dbias = sum over rows of dz
+//
+// All products run on one kernel (dense_tile.h), which takes either operand
+// along k or along its outer axis, so no gradient transposes anything; what it
+// needs is whole 16-byte vectors. An operand without them (an odd extent or row
+// stride) is first laid out with rows padded by zeros, which costs one pass over
+// it. A transposed dw is the transposed product. dz is formed once, with the
+// partial sums of dbias, and read by both products; without an activation g is
+// dz.
+//
+// A long contraction with few tiles is cut into K slices whose sums go to
+// scratch; a second launch adds them in order and finishes them: no atomics, the
+// same bits on every run.
+#include "dense_tile.h"
+
+#include <algorithm>
+#include <initializer_list>
+
+#include "hip_common.h"
+
+namespace chelis {
+namespace {
+
+// ---------------------------------------------------------------- slices' join
+template <Narrow KIND>
+__global__ __launch_bounds__(256) void dense_join_kernel(DenseProblem p) {
+    const int64_t per = (p.N + 7) / 8, count = p.M * per;
+    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < count; i += (int64_t)gridDim.x * 256) {
+        const int64_t m = i / per, n = 8 * (i - m * per);
+        float v[8] = {};
+        for (int s = 0; s < p.slices; ++s) {
+            const float *q = p.part + ((int64_t)s * p.M + m) * p.N + n;
+            if (n + 8 <= p.N) {
+                const F4 a = *reinterpret_cast<const F4 *>(q), b = *reinterpret_cast<const F4 *>(q + 4);
+#pragma unroll
+                for (int k = 0; k < 4; ++k) v[k] += a[k], v[4 + k] += b[k];
+            } else {
+#pragma unroll
+                for (int k = 0; k < 8; ++k)
+                    if (n + k < p.N) v[k] += q[k];
+            }
+        }
+        finish8<KIND>(p, m, n, v);
+    }
+}
+
+// ---------------------------------------------------------------- layout
+// Rows of `inner` contiguous elements, ld apart, to rows of whole vectors, the
+// rest zeros.
+struct Layout {
+    const uint16_t *from;
+    uint16_t *to;
+    int64_t rows, inner, ld;
+};
+struct Layouts {
+    Layout of[2];
+};
+__global__ __launch_bounds__(256) void dense_layout_kernel(Layouts ls) {
+    const Layout l = ls.of[blockIdx.y];
+    const int64_t per = (l.inner + 7) / 8, count = l.rows * per;
+    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < count; i += (int64_t)gridDim.x * 256) {
+        const int64_t row = i / per, at = 8 * (i - row * per);
+        const uint16_t *q = l.from + row * l.ld + at;
+        uint4 v{};
+        if (at + 8 <= l.inner) v = load8(q);
+        else {
+            uint16_t e[8];
+#pragma unroll
+            for (int k = 0; k < 8; ++k) e[k] = at + k < l.inner ? q[k] : (uint16_t)0;
+            v = __builtin_bit_cast(uint4, e);
+        }
+        *reinterpret_cast<uint4 *>(l.to + 8 * i) = v;
+    }
+}
+
+// ---------------------------------------------------------------- dz and dbias
+// A workgroup's 256 columns and rows of its chunk: 32 threads of eight columns
+// by eight rows at a time.
+struct CotangentArgs {
+    const uint16_t *g, *z;
+    uint16_t *dz;  // rows of whole vectors, or null
+    float *part;   // [chunks][N] sums, or null
+    int64_t M, N, ldg, ldz, lddz, chunk;
+    int32_t act;
+};
+template <Narrow KIND>
+__global__ __launch_bounds__(256) void dense_cotangent_kernel(CotangentArgs a) {
+    __shared__ float lds[8][256 + 8];
+    const int vec = threadIdx.x & 31, r = threadIdx.x >> 5;
+    const int64_t n = (int64_t)blockIdx.x * 256 + 8 * vec, count = a.N - n;
+    const int64_t row0 = blockIdx.y * a.chunk, end = row0 + a.chunk < a.M ? row0 + a.chunk : a.M;
+    float sum[8] = {};
+    if (count > 0) {
+#pragma unroll 2
+        for (int64_t m = row0 + r; m < end; m += 8) {
+            float g[8];
+            load8f<KIND>(a.g + m * a.ldg + n, g, count);
+            if (a.act != CHELIS_ACT_NONE) {
+                float z[8];
+                load8f<KIND>(a.z + m * a.ldz + n, z, count);
+#pragma unroll
+                for (int i = 0; i < 8; ++i) g[i] *= act_slope(z[i], a.act);
+            }
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                if (i >= count) g[i] = 0.f;
+                sum[i] += g[i];
+            }
+            if (a.dz) store8<KIND>(a.dz + m * a.lddz + n, g, 8);
+        }
+    }
+    if (!a.part) return;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) lds[r][8 * vec + i] = sum[i];
+    __syncthreads();
+    const int64_t col = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    if (col >= a.N) return;
+    float s = lds[0][threadIdx.x];
+#pragma unroll
+    for (int k = 1; k < 8; ++k) s += lds[k][threadIdx.x];
+    a.part[blockIdx.y * a.N + col] = s;
+}
+
+// dbias: 32 columns a workgroup, 32 threads a column.
+template <Narrow KIND>
+__global__ __launch_bounds__(1024) void dense_bias_kernel(const float *part, int64_t chunks, int64_t N, void *dbias, int32_t f32) {
+    __shared__ float lds[32][33];
+    const int col = threadIdx.x & 31, k = threadIdx.x >> 5;
+    const int64_t n = (int64_t)blockIdx.x * 32 + col;
+    float s = 0.f;
+    if (n < N) {
+#pragma unroll 4
+        for (int64_t c = k; c < chunks; c += 32) s += part[c * N + n];
+    }
+    lds[k][col] = s;
+    __syncthreads();
+    if (k || n >= N) return;
+#pragma unroll
+    for (int i = 1; i < 32; ++i) s += lds[i][col];
+    if (f32) static_cast<float *>(dbias)[n] = canon_bits(s);
+    else static_cast<typename Elem16<KIND>::type *>(dbias)[n] = finalize<typename Elem16<KIND>::type>(s);
+}
+
+// ---------------------------------------------------------------- dispatch
+// A library call's scratch, given back when the call returns (in stream order).
+struct Scratch {
+    void *p[8] = {};
+    size_t bytes[8] = {};
+    int n = 0;
+    void *take(size_t size) {
+        void *q = scratch_alloc(size);
+        if (q) p[n] = q, bytes[n++] = size;
+        return q;
+    }
+    ~Scratch() {
+        while (n--) scratch_free(p[n], bytes[n]);
+    }
+};
+
+using TileL = TileShape<256, 256, 64, 2, 4, 1, 2, 2>;
+using TileM = TileShape<128, 128, 64, 2, 2, 1, 2, 2>;
+using TileS = TileShape<64, 64, 128, 2, 2, 2, 3, 1>;
+using TileT = TileShape<32, 32, 256, 1, 1, 8, 3, 1>;
+
+// How long a K step and the rest of a workgroup's work take, by what the
+// kernel measured with every CU busy.
+struct ShapeCost {
+    int bm, bn, bk, per_cu;
+    double step, step_alone, fixed;
+};
+constexpr ShapeCost kShapes[] = {
+    {256, 256, 64, 1, 1.80, 1.80, 13.0},
+    {128, 128, 64, 2, 1.03, 0.70, 7.0},
+    {64, 64, 128, 1, 0.48, 0.48, 3.5},
+    {32, 32, 256, 1, 0.90, 0.90, 2.5},
+};
+
+struct Plan {
+    int shape;
+    int64_t kslice;
+    int32_t slices;
+};
+// The shape and the number of K slices with the least estimated time: whole
+// rounds of workgroups, and for slices the join's traffic and launch.
+Plan plan_for(int64_t M, int64_t N, int64_t K) {
+    const double cus = std::max(1, device_cus());
+    Plan best{0, std::max<int64_t>(K, 1), 1};
+    double least = 1e30;
+    for (int i = 0; i < 4; ++i) {
+        const ShapeCost &c = kShapes[i];
+        const int64_t tiles = ((M + c.bm - 1) / c.bm) * ((N + c.bn - 1) / c.bn), steps = std::max<int64_t>(1, (K + c.bk - 1) / c.bk);
+        for (int32_t s = 1; s <= 16 && s <= steps; ++s) {
+            const int64_t per = (steps + s - 1) / s, slices = (steps + per - 1) / per;
+            if (slices != s) continue;
+            const double wgs = (double)tiles * s, rounds = std::ceil(wgs / (cus * c.per_cu));
+            double t = rounds * (per * (wgs <= cus ? c.step_alone : c.step) + c.fixed);
+            if (s > 1) t += 5.0 + 8.0 * M * N * s / 4e6;
+            if (t < least) least = t, best = Plan{i, per * c.bk, s};
+        }
+    }
+    return best;
+}
+
+template <Narrow KIND, int ALAY, int BLAY, class C>
+int32_t launch_tiles(const DenseProblem &p, hipStream_t st) {
+    const int64_t tm = (p.M + C::BM - 1) / C::BM, tn = (p.N + C::BN - 1) / C::BN;
+    if (!grid_fits(tm * tn, C::THREADS)) return set_error(CHELIS_HIP_EUNSUPPORTED, "dense: grid too large");
+    dense_tile_kernel<KIND, ALAY, BLAY, C><<<dim3((unsigned)(tm * tn), (unsigned)p.slices), C::THREADS, 0, st>>>(p, tm, tn);
+    CHELIS_LAUNCH_CHECK();
+    return CHELIS_HIP_OK;
+}
+template <Narrow KIND, int ALAY, int BLAY>
+int32_t launch_shape(const DenseProblem &p, int shape, hipStream_t st) {
+    switch (shape) {
+        case 0: return launch_tiles<KIND, ALAY, BLAY, TileL>(p, st);
+        case 1: return launch_tiles<KIND, ALAY, BLAY, TileM>(p, st);
+        case 2: return launch_tiles<KIND, ALAY, BLAY, TileS>(p, st);
+        default: return launch_tiles<KIND, ALAY, BLAY, TileT>(p, st);
+    }
+}
+
+// Offsets inside a tile are 31 bits: 256 lines of at most this many elements.
+constexpr int64_t kMaxLine = int64_t(1) << 21, kMaxWidth = int64_t(1) << 20;
+
+// An operand of the product: `inner` contiguous elements to a line, `lines` of
+// them ld apart.
+struct Side {
+    const uint16_t *data;
+    int64_t lines, inner, ld;
+    bool whole() const {
+        return (reinterpret_cast<uintptr_t>(data) & 15) == 0 && (lines < 2 || ld % 8 == 0) && inner % 8 == 0 && (lines < 2 || ld <= kMaxLine);
+    }
+};
+int32_t lay_out(Side *a, Side *b, Scratch &scratch, hipStream_t st) {
+    Layouts ls{};
+    int n = 0;
+    int64_t most = 0;
+    for (Side *s : {a, b}) {
+        if (!s || s->whole() || !s->lines || !s->inner) continue;
+        const int64_t ld = (s->inner + 7) / 8 * 8;
+        uint16_t *to = static_cast<uint16_t *>(scratch.take((size_t)s->lines * ld * 2));
+        if (!to) return set_error(CHELIS_HIP_EHIP, "dense: scratch of %lld bytes", (long long)(s->lines * ld * 2));
+        ls.of[n++] = Layout{s->data, to, s->lines, s->inner, s->ld};
+        most = std::max(most, s->lines * ld / 8);
+        s->data = to, s->ld = ld;
+    }
+    if (!n) return CHELIS_HIP_OK;
+    dense_layout_kernel<<<dim3((unsigned)std::min<int64_t>((most + 255) / 256, 4096), (unsigned)n), 256, 0, st>>>(ls);
+    CHELIS_LAUNCH_CHECK();
+    return CHELIS_HIP_OK;
+}
+
+// The product of two sides, each along k (lay 0: lines are its outer axis) or
+// along its outer axis (lay 1: lines are k).
+template <Narrow KIND>
+int32_t product(DenseProblem p, Side a, int alay, Side b, int blay, Scratch &scratch, hipStream_t st) {
+    if (int32_t s = lay_out(&a, &b, scratch, st)) return s;
+    p.a = a.data, p.b = b.data;
+    p.sam = alay ? 1 : a.ld, p.sak = alay ? a.ld : 1;
+    p.sbn = blay ? 1 : b.ld, p.sbk = blay ? b.ld : 1;
+    const Plan plan = plan_for(p.M, p.N, p.K);
+    p.kslice = plan.kslice, p.slices = plan.slices;
+    if (p.slices > 1) {
+        p.part = static_cast<float *>(scratch.take((size_t)p.slices * p.M * p.N * sizeof(float)));
+        if (!p.part) return set_error(CHELIS_HIP_EHIP, "dense: scratch for %d slices", p.slices);
+    }
+    int32_t s;
+    if (alay == 0) s = blay == 0 ? launch_shape<KIND, 0, 0>(p, plan.shape, st) : launch_shape<KIND, 0, 1>(p, plan.shape, st);
+    else s = launch_shape<KIND, 1, 1>(p, plan.shape, st);
+    if (s || p.slices == 1) return s;
+    dense_join_kernel<KIND><<<(unsigned)std::min<int64_t>((p.M * ((p.N + 7) / 8) + 255) / 256, 8192), 256, 0, st>>>(p);
+    CHELIS_LAUNCH_CHECK();
+    return CHELIS_HIP_OK;
+}
+
+// ---------------------------------------------------------------- checks
+struct DenseChecks {
+    const char *what;
+    chelis_dtype dt;
+    int64_t rows, K, N;
+
+    int32_t row_operand(const chelis_gpu_tensor *t, const char *name, const chelis_gpu_tensor *x, int64_t width, int64_t *ld) {
+        if (int32_t s = check_tensor(t, name)) return s;
+        if (t->dtype != dt) return set_error(CHELIS_HIP_EDOMAIN, "%s: %s must have x's dtype", what, name);
+        bool fits = t->rank == x->rank && t->shape[t->rank - 1] == width;
+        for (int32_t i = 0; fits && i + 1 < t->rank; ++i) fits = t->shape[i] == x->shape[i];
+        if (!fits) return set_error(CHELIS_HIP_EDOMAIN, "%s: %s must be [x's leading axes, %lld]", what, name, (long long)width);
+        RowView v;
+        if (!row_view(t, &v) && t->count)
+            return set_error(CHELIS_HIP_EUNSUPPORTED, "%s: %s: last axis must be contiguous with uniform row stride", what, name);
+        *ld = v.ld;
+        return check_device(t, name);
+    }
+    int32_t operands(const chelis_gpu_tensor *x, const chelis_gpu_tensor *w, int64_t *ldx) {
+        int32_t s;
+        if ((s = check_tensor(x, "x")) || (s = check_tensor(w, "w"))) return s;
+        if (!is_narrow16(x->dtype)) return set_error(CHELIS_HIP_EDOMAIN, "%s: x must be bf16 or f16 (f32 and f64: linear)", what);
+        if (x->rank < 1) return set_error(CHELIS_HIP_EDOMAIN, "%s: x needs a last axis", what);
+        if (w->dtype != x->dtype || w->rank != 2 || w->shape[0] != x->shape[x->rank - 1])
+            return set_error(CHELIS_HIP_EDOMAIN, "%s: w must be [K, N] of x's dtype", what);
+        dt = x->dtype, K = w->shape[0], N = w->shape[1];
+        if (K > kMaxWidth || N > kMaxWidth) return set_error(CHELIS_HIP_EUNSUPPORTED, "%s: widths past 2^20", what);
+        if ((s = row_operand(x, "x", x, K, ldx)) || (s = check_device(w, "w"))) return s;
+        rows = 1;
+        for (int32_t i = 0; i + 1 < x->rank; ++i) rows *= x->shape[i];
+        return CHELIS_HIP_OK;
+    }
+    // w or dw [K, N]: lines along n (k apart) or along k (n apart).
+    int32_t matrix(const chelis_gpu_tensor *t, const char *name, bool *along_k) {
+        const int64_t sk = t->strides[0], sn = t->strides[1];
+        if (sk == 1 && (sn != 1 || N == 1)) *along_k = true;
+        else if (sn == 1 || N == 1) *along_k = false;
+        else if (K == 1) *along_k = true;
+        else return set_error(CHELIS_HIP_EUNSUPPORTED, "%s: %s: one axis must be contiguous", what, name);
+        return CHELIS_HIP_OK;
+    }
+    int32_t activation(int32_t act) {
+        if (act < CHELIS_ACT_NONE || act > CHELIS_ACT_SILU)
+            return set_error(CHELIS_HIP_EDOMAIN, "%s: unknown activation %d", what, act);
+        return CHELIS_HIP_OK;
+    }
+    // dbias or bias [N], dw [K, N]: of x's dtype or f32
+    int32_t dtype_or_f32(const chelis_gpu_tensor *t, const char *name) {
+        if (t->dtype != dt && t->dtype != CHELIS_DTYPE_F32)
+            return set_error(CHELIS_HIP_EDOMAIN, "%s: %s must have x's dtype or f32", what, name);
+        return check_device(t, name);
+    }
+    int32_t vector(const chelis_gpu_tensor *t, const char *name) {
+        if (int32_t s = check_tensor(t, name)) return s;
+        if (t->rank != 1 || t->shape[0] != N || (N > 1 && t->strides[0] != 1))
+            return set_error(CHELIS_HIP_EDOMAIN, "%s: %s must be contiguous [N]", what, name);
+        return dtype_or_f32(t, name);
+    }
+    int32_t result(const chelis_gpu_tensor *t, const char *name, std::initializer_list<NamedTensor> others) {
+        if (!non_overlapping(t)) return set_error(CHELIS_HIP_EDOMAIN, "%s: %s overlaps itself", what, name);
+        if (const char *other = shared_with(t, others))
+            return set_error(CHELIS_HIP_EDOMAIN, "%s: %s and %s overlap", what, name, other);
+        return CHELIS_HIP_OK;
+    }
+    Side weights(const chelis_gpu_tensor *w, bool along_k) {
+        const uint16_t *d = static_cast<const uint16_t *>(w->data);
+        return along_k ? Side{d, N, K, w->strides[1]} : Side{d, K, N, w->strides[0]};
+    }
+};
+
+template <class F>
+int32_t with_kind(chelis_dtype dt, F &&f) {
+    return dt == CHELIS_DTYPE_BF16 ? f(std::integral_constant<Narrow, Narrow::Bf16>())
+                                   : f(std::integral_constant<Narrow, Narrow::F16>());
+}
+
+}  // namespace
+}  // namespace chelis
+
+using namespace chelis;
+
+extern "C" int32_t chelis_hip_dense(const chelis_gpu_tensor *x, const chelis_gpu_tensor *w, const chelis_gpu_tensor *bias,
+                                    int32_t activation, const chelis_gpu_tensor *residual, const chelis_gpu_tensor *y,
+                                    const chelis_gpu_tensor *z) {
+    DenseChecks c{"dense"};
+    DenseProblem p{};
+    int64_t ldx;
+    bool along_k;
+    int32_t s;
+    if ((s = c.operands(x, w, &ldx)) || (s = c.activation(activation)) || (s = c.matrix(w, "w", &along_k)) ||
+        (bias && (s = c.vector(bias, "bias"))) || (s = c.row_operand(y, "y", x, c.N, &p.ldc)) ||
+        (residual && (s = c.row_operand(residual, "residual", x, c.N, &p.ldr))) ||
+        (z && (s = c.row_operand(z, "z", x, c.N, &p.ldz))) || (s = c.result(y, "y", {{x, "x"}, {w, "w"}, {bias, "bias"}})) ||
+        (z && (s = c.result(z, "z", {{x, "x"}, {w, "w"}, {bias, "bias"}, {residual, "residual"}, {y, "y"}}))))
+        return s;
+    if (residual && !same_view(y, residual) && shares_storage(y, residual))
+        return set_error(CHELIS_HIP_EDOMAIN, "dense: y overlaps residual with other strides or from another element");
+    if (!c.rows || !c.N) return CHELIS_HIP_OK;
+    hipStream_t st = stream();
+    if (!st) return set_error(CHELIS_HIP_EHIP, "no HIP device");
+    p.M = c.rows, p.N = c.N, p.K = c.K;
+    p.c = y->data, p.act = activation;
+    if (bias) p.bias = bias->data, p.bias32 = bias->dtype == CHELIS_DTYPE_F32;
+    if (residual) p.resid = static_cast<const uint16_t *>(residual->data);
+    if (z) p.z = static_cast<uint16_t *>(z->data);
+    const Side a{static_cast<const uint16_t *>(x->data), c.rows, c.K, ldx}, b = c.weights(w, along_k);
+    return with_kind(c.dt, [&](auto kind) -> int32_t {
+        Scratch scratch;
+        return product<decltype(kind)::value>(p, a, 0, b, along_k ? 0 : 1, scratch, st);
+    });
+}
+
+extern "C" int32_t chelis_hip_dense_adjoint(const chelis_gpu_tensor *x, const chelis_gpu_tensor *w, const chelis_gpu_tensor *z,
+                                            int32_t activation, const chelis_gpu_tensor *g, const chelis_gpu_tensor *dx,
+                                            const chelis_gpu_tensor *dw, const chelis_gpu_tensor *dbias) {
+    DenseChecks c{"dense_adjoint"};
+    CotangentArgs ca{};
+    int64_t ldx, lddx = 0;
+    bool along_k, dw_along_k = false;
+    int32_t s;
+    if ((s = c.operands(x, w, &ldx)) || (s = c.activation(activation)) || (s = c.matrix(w, "w", &along_k)) ||
+        (s = c.row_operand(g, "g", x, c.N, &ca.ldg)))
+        return s;
+    if (!dx && !dw && !dbias) return set_error(CHELIS_HIP_EDOMAIN, "dense_adjoint: no gradient asked for");
+    if (activation != CHELIS_ACT_NONE) {
+        if (!z) return set_error(CHELIS_HIP_EDOMAIN, "dense_adjoint: an activation's gradient needs z");
+        if ((s = c.row_operand(z, "z", x, c.N, &ca.ldz))) return s;
+    } else z = nullptr;
+    const std::initializer_list<NamedTensor> inputs = {{x, "x"}, {w, "w"}, {z, "z"}, {g, "g"}};
+    if (dx && ((s = c.row_operand(dx, "dx", x, c.K, &lddx)) || (s = c.result(dx, "dx", inputs)))) return s;
+    if (dw) {
+        if ((s = check_tensor(dw, "dw"))) return s;
+        if (!same_shape(dw, w)) return set_error(CHELIS_HIP_EDOMAIN, "dense_adjoint: dw must be [K, N]");
+        if ((s = c.dtype_or_f32(dw, "dw")) || (s = c.matrix(dw, "dw", &dw_along_k)) || (s = c.result(dw, "dw", inputs)) ||
+            (s = c.result(dw, "dw", {{dx, "dx"}})))
+            return s;
+    }
+    if (dbias && ((s = c.vector(dbias, "dbias")) || (s = c.result(dbias, "dbias", inputs)) ||
+                  (s = c.result(dbias, "dbias", {{dx, "dx"}, {dw, "dw"}}))))
+        return s;
+    hipStream_t st = stream();
+    if (!st) return set_error(CHELIS_HIP_EHIP, "no HIP device");
+    return with_kind(c.dt, [&](auto kind) -> int32_t {
+        constexpr Narrow KIND = decltype(kind)::value;
+        Scratch scratch;
+        Side dz{static_cast<const uint16_t *>(g->data), c.rows, c.N, ca.ldg};
+        const bool form = (dx || dw) && c.rows && c.N && (activation != CHELIS_ACT_NONE || !dz.whole());
+        if (form || (dbias && c.N)) {
+            ca.g = dz.data, ca.z = z ? static_cast<const uint16_t *>(z->data) : nullptr;
+            ca.M = c.rows, ca.N = c.N, ca.act = activation;
+            const int64_t cols = (c.N + 255) / 256;
+            // eight workgroups a CU, at least 32 rows to each
+            int64_t chunks = std::max<int64_t>(1, std::min<int64_t>((int64_t)device_cus() * 8 / cols, (c.rows + 31) / 32));
+            ca.chunk = std::max<int64_t>(1, (c.rows + chunks - 1) / chunks);
+            chunks = std::max<int64_t>(1, (c.rows + ca.chunk - 1) / ca.chunk);
+            if (form) {
+                ca.lddz = (c.N + 7) / 8 * 8;
+                ca.dz = static_cast<uint16_t *>(scratch.take((size_t)c.rows * ca.lddz * 2));
+                if (!ca.dz) return set_error(CHELIS_HIP_EHIP, "dense_adjoint: scratch for dz");
+                dz.data = ca.dz, dz.ld = dz.inner = ca.lddz;  // whole vectors, zeros past N
+            }
+            if (dbias) {
+                ca.part = static_cast<float *>(scratch.take((size_t)chunks * c.N * sizeof(float)));
+                if (!ca.part) return set_error(CHELIS_HIP_EHIP, "dense_adjoint: scratch for dbias");
+            }
+            dense_cotangent_kernel<KIND><<<dim3((unsigned)cols, (unsigned)chunks), 256, 0, st>>>(ca);
+            CHELIS_LAUNCH_CHECK();
+            if (dbias) {
+                dense_bias_kernel<KIND><<<grid_for(c.N, 32), 1024, 0, st>>>(ca.part, chunks, c.N, dbias->data,
+                                                                            dbias->dtype == CHELIS_DTYPE_F32);
+                CHELIS_LAUNCH_CHECK();
+            }
+        }
+        if (dx && c.rows && c.K) {
+            DenseProblem p{};
+            p.M = c.rows, p.N = c.K, p.K = c.N;
+            p.c = dx->data, p.ldc = lddx;
+            if (int32_t e = product<KIND>(p, dz, 0, c.weights(w, along_k), along_k ? 1 : 0, scratch, st)) return e;
+        }
+        if (dw && c.K && c.N) {
+            const Side xs{static_cast<const uint16_t *>(x->data), c.rows, c.K, ldx};
+            DenseProblem p{};
+            p.K = c.rows;
+            p.c = dw->data, p.c32 = dw->dtype == CHELIS_DTYPE_F32;
+            int32_t e;
+            if (dw_along_k) {
+                p.M = c.N, p.N = c.K, p.ldc = dw->strides[1];
+                e = product<KIND>(p, dz, 1, xs, 1, scratch, st);
+            } else {
+                p.M = c.K, p.N = c.N, p.ldc = dw->strides[0];
+                e = product<KIND>(p, xs, 1, dz, 1, scratch, st);
+            }
+            if (e) return e;
+        }
+        return CHELIS_HIP_OK;
+    });
+}

@@ -174,6 +174,76 @@ int32_t chelis_hip_window_attention_adjoint(const chelis_gpu_tensor *q, const ch
                                             int64_t window, int64_t sinks, double scale, const chelis_gpu_tensor *dq,
                                             const chelis_gpu_tensor *dk, const chelis_gpu_tensor *dv);
 
+/* The residual stream between two blocks, for the rows of x [.., hidden] and a
+ * block's result b:
+ *   v = post(b),  u = x + scale * gate * v,  h = pre(u)
+ * post and pre are a layer norm, an rms norm (v * rstd, rstd =
+ * 1 / sqrt(avg(v^2) + epsilon)) or absent (NULL or kind NONE); gamma and beta
+ * [hidden] may each be NULL (1 and 0). gate: [hidden], or [x's first axes ..,
+ * hidden] with one gate for each run of rows (of a sequence, say), or NULL (1).
+ * gate and weights share x's dtype, or are all f32 beside 16-bit rows. mean
+ * (layer only) and rstd receive the row statistics, as layer_norm_stats' do;
+ * each may be NULL. pre takes the sum as it is before u is rounded. Without b
+ * (post, gate and u NULL) h = pre(x): a norm alone. u and h may each be x or b. */
+enum { CHELIS_NORM_NONE = 0, CHELIS_NORM_LAYER = 1, CHELIS_NORM_RMS = 2 };
+typedef struct {
+    int32_t kind;
+    int32_t reserved;
+    const chelis_gpu_tensor *gamma, *beta;
+    const chelis_gpu_tensor *mean, *rstd; /* results of the forward call, operands of the gradients */
+} chelis_hip_norm;
+int32_t chelis_hip_residual_norm(const chelis_gpu_tensor *x, const chelis_gpu_tensor *b, const chelis_hip_norm *post,
+                                 const chelis_gpu_tensor *gate, double scale, const chelis_hip_norm *pre,
+                                 double epsilon, const chelis_gpu_tensor *u, const chelis_gpu_tensor *h);
+/* Its gradients for the cotangents du of u and dh of h (du may be NULL: none
+ * arrives there), from u as stored and the statistics of both norms: with
+ * t = du + pre'(u; dh), dx = t, db = post'(b; scale * gate * t), dgate of
+ * gate's shape, and the weights' over all rows. Each gradient may be NULL. u is
+ * not read without pre (NULL then, or beside no b what pre was given). dx and
+ * db may each be u, b, du or dh. */
+int32_t chelis_hip_residual_norm_adjoint(
+    const chelis_gpu_tensor *u, const chelis_gpu_tensor *b, const chelis_hip_norm *post, const chelis_gpu_tensor *gate,
+    double scale, const chelis_hip_norm *pre, const chelis_gpu_tensor *du, const chelis_gpu_tensor *dh,
+    const chelis_gpu_tensor *dx, const chelis_gpu_tensor *db, const chelis_gpu_tensor *dgate,
+    const chelis_gpu_tensor *post_dgamma, const chelis_gpu_tensor *post_dbeta, const chelis_gpu_tensor *pre_dgamma,
+    const chelis_gpu_tensor *pre_dbeta);
+
+/* The 16-bit product of a training or serving step with its epilogue:
+ *   z = x . w + bias,  y = act(z) + residual
+ * x [.., K], y, z and residual [.., N] rows of bf16 or f16 with a uniform
+ * stride; w [K, N] with either axis contiguous (weights stored [N, K] are a
+ * stride swap); bias [N], of x's dtype or f32, or NULL. z (what the gradients
+ * need beside an activation) and residual may be NULL. Sums, bias, activation
+ * and residual are binary32, y and z are rounded once each from them. y may be
+ * residual. One row or a few (a token) are as welcome as many. */
+enum { CHELIS_ACT_SILU = 3 }; /* beside CHELIS_ACT_NONE, RELU and GELU below */
+int32_t chelis_hip_dense(const chelis_gpu_tensor *x, const chelis_gpu_tensor *w, const chelis_gpu_tensor *bias,
+                         int32_t activation, const chelis_gpu_tensor *residual, const chelis_gpu_tensor *y,
+                         const chelis_gpu_tensor *z);
+/* Its gradients for the cotangent g of y: dz = g * act'(z), dx = dz . w^T,
+ * dw = x^T . dz of w's shape (either axis contiguous), dbias = sum over rows of
+ * dz; dw and dbias of x's dtype or f32, zero without rows. z may be NULL for
+ * NONE. Each gradient may be NULL. For the two products dz is rounded once to
+ * x's dtype; dbias sums it unrounded. The residual's gradient is g itself. */
+int32_t chelis_hip_dense_adjoint(const chelis_gpu_tensor *x, const chelis_gpu_tensor *w, const chelis_gpu_tensor *z,
+                                 int32_t activation, const chelis_gpu_tensor *g, const chelis_gpu_tensor *dx,
+                                 const chelis_gpu_tensor *dw, const chelis_gpu_tensor *dbias);
+
+/* The norm over the elements of n gradients together, and their clipping:
+ *   norm = scale * sqrt(sum of g^2),
+ *   outs[i] = gs[i] * scale * (norm > max_norm ? max_norm / norm : 1)
+ * scale takes a loss scale off again (1: none). gs, outs: f32, f64, bf16 or f16
+ * in any mix, each dense in some order of its axes or rows of contiguous
+ * elements a fixed step apart; outs may be gs (nothing is written then where
+ * the factor is 1), and an out elsewhere has its gradient's shape, dtype and
+ * order of axes. norm: one f32 or f64 element on the device, where the
+ * factor is formed: nothing waits for the host. An infinite norm gives the
+ * factor 0, a NaN one scale. Squares are summed in binary64. */
+int32_t chelis_hip_gradient_norm(const chelis_gpu_tensor *const *gs, int32_t n, double scale,
+                                 const chelis_gpu_tensor *norm);
+int32_t chelis_hip_clip_gradients(const chelis_gpu_tensor *const *gs, int32_t n, const chelis_gpu_tensor *norm,
+                                  double max_norm, double scale, const chelis_gpu_tensor *const *outs);
+
 /* ---- fused elementwise chains (RiscOp::FusedElem, dag.rs:485-524,673-678) ----
  * A step's args index the chain inputs when >= 0, and a previous step k as
  * -(k + 1) (FusedInput::External / FusedInput::PreviousStep). The chain's
