@@ -5,7 +5,7 @@
 
 #include "elem.h"
 #include "gemm16_tile.h"
-#include "gelu_poly.h"
+#include "gelu16_poly.h"
 
 #include "chelis_hip.h"
 
@@ -32,29 +32,31 @@ struct DenseProblem {
 };
 
 // ---------------------------------------------------------------- activations
-// Phi(-a) = q exp(-a^2 / 2) for a = |x|: q by the degree-9 polynomial of
-// gelu_poly.h (7.1e-8), the exponential in binary32 (its argument's rounding
-// grows to 2^-16 relative at |x| = 13, under a hundredth of a 16-bit rounding).
-// Past 30 both are 0 against 1, and infinities would meet 0.
+// Phi(-a) = q exp(-a^2 / 2) for a = |x|: q by the degree-6 polynomial of
+// gelu16_poly.h (2.5e-6), the exponential in binary32 (its argument's rounding
+// grows to 2^-16 relative at |x| = 13, 2^-18 at 6, where binary16 results end):
+// hundredths of a 16-bit rounding. Past 30 both are 0 against 1, and infinities
+// would meet 0.
 __device__ inline void phi_tail(float x, float &q, float &e, float &a) {
-    constexpr float kQ[CHELIS_GELU_DEG + 1] = CHELIS_GELU_Q;
+    constexpr float kQ[CHELIS_GELU16_DEG + 1] = CHELIS_GELU16_Q;
     a = fminf(fabsf(x), 30.f);
-    const float u = fmaf(-2.0f * CHELIS_GELU_K, __builtin_amdgcn_rcpf(a + CHELIS_GELU_K), 1.0f);
-    q = kQ[CHELIS_GELU_DEG];
+    const float t = __builtin_amdgcn_rcpf(fmaf(a, 1.f / CHELIS_GELU16_K, 1.f));
+    q = kQ[CHELIS_GELU16_DEG];
 #pragma unroll
-    for (int d = CHELIS_GELU_DEG - 1; d >= 0; --d) q = fmaf(q, u, kQ[d]);
+    for (int d = CHELIS_GELU16_DEG - 1; d >= 0; --d) q = fmaf(q, t, kQ[d]);
     e = __builtin_amdgcn_exp2f(a * a * -0.72134752044448170368f);
 }
+// x - |x| Phi(-|x|) for x >= 0, -|x| Phi(-|x|) below (NaN takes the first way).
 __device__ inline float act_gelu(float x) {
     float q, e, a;
     phi_tail(x, q, e, a);
-    const float r = fmaf(-(a * q), e, x >= 0.f ? x : 0.f);
-    return x != x ? x : r;
+    return fmaf(-(a * q), e, x < 0.f ? 0.f : x);
 }
+// Phi(x) + x phi(x)
 __device__ inline float slope_gelu(float x) {
     float q, e, a;
     phi_tail(x, q, e, a);
-    const float tail = q * e, r = (x >= 0.f ? 1.f - tail : tail) + copysignf(a, x) * (e * 0.39894228040143267794f);
+    const float below = e * fmaf(a, -0.39894228040143267794f, q), r = x < 0.f ? below : 1.f - below;
     return x != x ? x : r;
 }
 // x clamped where the result has long reached its limit (NaN stays).
@@ -117,7 +119,7 @@ __device__ inline void store8(uint16_t *p, const float (&v)[8], int64_t count) {
     }
 }
 template <Narrow KIND>
-__device__ inline void load8f(const uint16_t *p, float (&v)[8], int64_t count) {
+__device__ inline Vec16<KIND> load8v(const uint16_t *p, int64_t count) {
     using T = typename Elem16<KIND>::type;
     const T *in = reinterpret_cast<const T *>(p);
     Vec16<KIND> q{};
@@ -127,35 +129,31 @@ __device__ inline void load8f(const uint16_t *p, float (&v)[8], int64_t count) {
         for (int i = 0; i < 7; ++i)
             if (i < count) q.q[i] = in[i];
     }
+    return q;
+}
+template <Narrow KIND>
+__device__ inline void load8f(const uint16_t *p, float (&v)[8], int64_t count) {
+    const Vec16<KIND> q = load8v<KIND>(p, count);
 #pragma unroll
     for (int i = 0; i < 8; ++i) v[i] = q.get(i);
 }
 typedef float F4 __attribute__((ext_vector_type(4), aligned(4)));
 
-// Eight neighbouring columns of row m from n on, as far as the result has them.
+// Eight neighbouring columns of a row, `count` of them there: the sums in v, the
+// bias and (of the residual's type) the residual already loaded.
 template <Narrow KIND>
-__device__ inline void finish8(const DenseProblem &p, int64_t m, int64_t n, float (&v)[8]) {
-    const int64_t count = p.N - n;
-    if (p.bias) {
-        float b[8];
-        if (p.bias32) {
-            const float *q = static_cast<const float *>(p.bias) + n;
+__device__ inline void finish8(const DenseProblem &p, int64_t m, int64_t n, int64_t count, float (&v)[8], const float (&bias)[8],
+                               const Vec16<KIND> &resid) {
 #pragma unroll
-            for (int i = 0; i < 8; ++i) b[i] = i < count ? q[i] : 0.f;
-        } else load8f<KIND>(static_cast<const uint16_t *>(p.bias) + n, b, count);
-#pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] += b[i];
-    }
+    for (int i = 0; i < 8; ++i) v[i] += bias[i];
     if (p.z) store8<KIND>(p.z + m * p.ldz + n, v, count);
     if (p.act != CHELIS_ACT_NONE) {
 #pragma unroll
         for (int i = 0; i < 8; ++i) v[i] = activate(v[i], p.act);
     }
     if (p.resid) {
-        float r[8];
-        load8f<KIND>(p.resid + m * p.ldr + n, r, count);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] += r[i];
+        for (int i = 0; i < 8; ++i) v[i] += resid.get(i);
     }
     if (p.c32) {
         float *o = static_cast<float *>(p.c) + m * p.ldc + n;
@@ -163,6 +161,17 @@ __device__ inline void finish8(const DenseProblem &p, int64_t m, int64_t n, floa
         for (int i = 0; i < 8; ++i)
             if (i < count) o[i] = canon_bits(v[i]);
     } else store8<KIND>(static_cast<uint16_t *>(p.c) + m * p.ldc + n, v, count);
+}
+template <Narrow KIND>
+__device__ inline void load_bias(const DenseProblem &p, int64_t n, int64_t count, float (&b)[8]) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) b[i] = 0.f;
+    if (!p.bias) return;
+    if (p.bias32) {
+        const float *q = static_cast<const float *>(p.bias) + n;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) b[i] = i < count ? q[i] : 0.f;
+    } else load8f<KIND>(static_cast<const uint16_t *>(p.bias) + n, b, count);
 }
 // The same for one K slice's sums.
 __device__ inline void slice8(const DenseProblem &p, int64_t slice, int64_t m, int64_t n, const float (&v)[8]) {
@@ -298,6 +307,7 @@ struct TileShape {
     static constexpr int BM = BM_, BN = BN_, BK = BK_, WM = WM_, WN = WN_, WK = WK_, ST = ST_, OCC = OCC_;
     static constexpr int THREADS = 64 * WM * WN * WK, MI = BM / WM / 32, NJ = BN / WN / 32;
     static constexpr int STAGE = (BM + BN) * BK * 2, PITCH = BN + 4, EPI = WM * 32 * PITCH * 4;
+    static constexpr int EPI_UNROLL = MI > 2 ? 1 : MI;  // code size against registers moved
     static constexpr int BYTES = STAGE * ST > EPI * WK ? STAGE * ST : EPI * WK;
     static_assert(BK / 16 % WK == 0, "whole k blocks a wave");
 };
@@ -356,36 +366,53 @@ __global__ __launch_bounds__(C::THREADS, C::OCC) void dense_tile_kernel(DensePro
                 for (int j = 0; j < NJ; ++j) acc[i][j] = mfma32<KIND>(af[i], bf[j], acc[i][j]);
         }
     }
-    load_wait<0>();
-    // 32 rows of every wave at a time through LDS: lanes then hold eight
-    // neighbouring columns, and memory sees whole rows of the tile
+    // 32 rows of every wave at a time through LDS: a thread then holds eight
+    // neighbouring columns of some rows, and memory sees whole rows of the tile.
+    // The residual's loads go ahead of the exchange that they do not wait for.
+    constexpr int PER = BN / 8, ROWS = C::THREADS / PER, VPT = (C::WM * 32 + ROWS - 1) / ROWS;
+    static_assert(C::THREADS % PER == 0, "a thread keeps its columns");
+    const int64_t n = n0 + 8 * (threadIdx.x % PER), count = p.N - n;
+    float bias[8];
+    load_bias<KIND>(p, n, count, bias);
     float *stage = reinterpret_cast<float *>(lds), *mine = stage + wk * (C::EPI / 4);
-#pragma unroll
+    load_wait<0>();
+#pragma unroll C::EPI_UNROLL
     for (int i = 0; i < MI; ++i) {
+        Vec16<KIND> resid[VPT];
+        auto row_of = [&](int k) { return (int)threadIdx.x / PER + k * ROWS; };
+        auto m_of = [&](int row) { return m0 + ((row >> 5) * MI + i) * 32 + (row & 31); };
+#pragma unroll
+        for (int k = 0; k < VPT; ++k) {
+            const int64_t m = m_of(row_of(k));
+            if (p.resid && !p.part && row_of(k) < C::WM * 32 && m < p.M && count > 0) resid[k] = load8v<KIND>(p.resid + m * p.ldr + n, count);
+        }
         if (i) __syncthreads();
 #pragma unroll
-        for (int j = 0; j < NJ; ++j)
+        for (int c = 0; c < MI; ++c)
+            if (c == i) {
 #pragma unroll
-            for (int r = 0; r < 16; ++r)
-                mine[(wm * 32 + (r & 3) + 8 * (r >> 2) + 4 * (lane >> 5)) * C::PITCH + (wn * NJ + j) * 32 + (lane & 31)] =
-                    acc[i][j][r];
+                for (int j = 0; j < NJ; ++j)
+#pragma unroll
+                    for (int r = 0; r < 16; ++r)
+                        mine[(wm * 32 + (r & 3) + 8 * (r >> 2) + 4 * (lane >> 5)) * C::PITCH + (wn * NJ + j) * 32 + (lane & 31)] =
+                            acc[c][j][r];
+            }
         __syncthreads();
-        constexpr int PER = BN / 8, VECS = C::WM * 32 * PER;
-#pragma unroll 1
-        for (int v0 = 0; v0 < VECS; v0 += C::THREADS) {
-            const int v = v0 + threadIdx.x, row = v / PER, col = 8 * (v % PER);
-            if (VECS % C::THREADS && v >= VECS) break;
-            const int64_t m = m0 + ((row >> 5) * MI + i) * 32 + (row & 31), n = n0 + col;
-            if (m >= p.M || n >= p.N) continue;
+#pragma unroll
+        for (int k = 0; k < VPT; ++k) {
+            const int row = row_of(k);
+            const int64_t m = m_of(row);
+            if (row >= C::WM * 32 || m >= p.M || count <= 0) continue;
+            const float *at = stage + row * C::PITCH + 8 * (threadIdx.x % PER);
             float x[8];
 #pragma unroll
-            for (int q = 0; q < 8; ++q) x[q] = stage[row * C::PITCH + col + q];
+            for (int q = 0; q < 8; ++q) x[q] = at[q];
 #pragma unroll
             for (int w = 1; w < C::WK; ++w)
 #pragma unroll
-                for (int q = 0; q < 8; ++q) x[q] += stage[w * (C::EPI / 4) + row * C::PITCH + col + q];
+                for (int q = 0; q < 8; ++q) x[q] += at[w * (C::EPI / 4) + q];
             if (p.part) slice8(p, blockIdx.y, m, n, x);
-            else finish8<KIND>(p, m, n, x);
+            else finish8<KIND>(p, m, n, count, x, bias, resid[k]);
         }
     }
 }

@@ -31,7 +31,10 @@ __global__ __launch_bounds__(256) void dense_join_kernel(DenseProblem p) {
     const int64_t per = (p.N + 7) / 8, count = p.M * per;
     for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < count; i += (int64_t)gridDim.x * 256) {
         const int64_t m = i / per, n = 8 * (i - m * per);
-        float v[8] = {};
+        float v[8] = {}, bias[8];
+        load_bias<KIND>(p, n, p.N - n, bias);
+        Vec16<KIND> resid;
+        if (p.resid) resid = load8v<KIND>(p.resid + m * p.ldr + n, p.N - n);
         for (int s = 0; s < p.slices; ++s) {
             const float *q = p.part + ((int64_t)s * p.M + m) * p.N + n;
             if (n + 8 <= p.N) {
@@ -44,7 +47,7 @@ __global__ __launch_bounds__(256) void dense_join_kernel(DenseProblem p) {
                     if (n + k < p.N) v[k] += q[k];
             }
         }
-        finish8<KIND>(p, m, n, v);
+        finish8<KIND>(p, m, n, p.N - n, v, bias, resid);
     }
 }
 
@@ -95,22 +98,30 @@ __global__ __launch_bounds__(256) void dense_cotangent_kernel(CotangentArgs a) {
     const int64_t row0 = blockIdx.y * a.chunk, end = row0 + a.chunk < a.M ? row0 + a.chunk : a.M;
     float sum[8] = {};
     if (count > 0) {
-#pragma unroll 2
-        for (int64_t m = row0 + r; m < end; m += 8) {
-            float g[8];
-            load8f<KIND>(a.g + m * a.ldg + n, g, count);
-            if (a.act != CHELIS_ACT_NONE) {
-                float z[8];
-                load8f<KIND>(a.z + m * a.ldz + n, z, count);
+        constexpr int U = 4;  // rows whose loads are under way together
+        for (int64_t base = row0 + r; base < end; base += 8 * U) {
+            Vec16<KIND> gq[U], zq[U];
 #pragma unroll
-                for (int i = 0; i < 8; ++i) g[i] *= act_slope(z[i], a.act);
+            for (int u = 0; u < U; ++u) {
+                const int64_t m = base + 8 * u < end ? base + 8 * u : end - 1;
+                gq[u] = load8v<KIND>(a.g + m * a.ldg + n, count);
+                if (a.act != CHELIS_ACT_NONE) zq[u] = load8v<KIND>(a.z + m * a.ldz + n, count);
             }
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                if (i >= count) g[i] = 0.f;
-                sum[i] += g[i];
+            for (int u = 0; u < U; ++u) {
+                const int64_t m = base + 8 * u;
+                if (m >= end) break;
+                float g[8];
+#pragma unroll
+                for (int i = 0; i < 8; ++i) g[i] = i < count ? gq[u].get(i) : 0.f;
+                if (a.act != CHELIS_ACT_NONE) {
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) g[i] = i < count ? g[i] * act_slope(zq[u].get(i), a.act) : 0.f;
+                }
+#pragma unroll
+                for (int i = 0; i < 8; ++i) sum[i] += g[i];
+                if (a.dz) store8<KIND>(a.dz + m * a.lddz + n, g, 8);
             }
-            if (a.dz) store8<KIND>(a.dz + m * a.lddz + n, g, 8);
         }
     }
     if (!a.part) return;
@@ -162,43 +173,53 @@ struct Scratch {
 };
 
 using TileL = TileShape<256, 256, 64, 2, 4, 1, 2, 2>;
-using TileM = TileShape<128, 128, 64, 2, 2, 1, 2, 2>;
-using TileS = TileShape<64, 64, 128, 2, 2, 2, 3, 1>;
-using TileT = TileShape<32, 32, 256, 1, 1, 8, 3, 1>;
+using TileM = TileShape<128, 128, 64, 2, 2, 2, 2, 4>;   // two a CU
+using TileN = TileShape<128, 128, 64, 2, 2, 4, 4, 4>;
+using TileQ = TileShape<64, 128, 64, 2, 2, 2, 3, 4>;    // two a CU
+using TileS = TileShape<64, 64, 128, 2, 2, 2, 3, 2>;
+using TileT = TileShape<32, 32, 256, 1, 1, 8, 3, 2>;
 
-// How long a K step and the rest of a workgroup's work take, by what the
-// kernel measured with every CU busy.
+// What a shape costs in us: a K step with the device full, a K step where every
+// CU has at most one workgroup, the rest of a workgroup's work, the launch. Fitted
+// to 36 products of 8 .. 16384 rows, 200 .. 8192 columns and 64 .. 8192 k, their
+// operands from memory, each timed in every shape (root mean square 6-17 %): the
+// shape it chooses was the fastest of them in 35, 10 % behind in the other. Some
+// of the shapes' best cases (us; the next best shape): L 4096^2 x 1024 45.5
+// (49.9), M 8192 x 1024 x 4096 74.8 (83.7), N 1024 x 4096 x 8192 87.6 (107), Q
+// 2048^2 x 512 10.7 (11.9), S 1024^3 7.3 (10.5), T 8 x 4096 x 1024 5.6 (7.2).
 struct ShapeCost {
     int bm, bn, bk, per_cu;
-    double step, step_alone, fixed;
+    double step, step_alone, fixed, launch;
 };
 constexpr ShapeCost kShapes[] = {
-    {256, 256, 64, 1, 1.80, 1.80, 13.0},
-    {128, 128, 64, 2, 1.03, 0.70, 7.0},
-    {64, 64, 128, 1, 0.48, 0.48, 3.5},
-    {32, 32, 256, 1, 0.90, 0.90, 2.5},
+    {256, 256, 64, 1, 1.90, 1.41, 13.0, 0.9}, {128, 128, 64, 2, 1.14, 0.77, 4.9, 1.4}, {128, 128, 64, 1, 0.57, 0.49, 6.3, 0.6},
+    {64, 128, 64, 2, 0.74, 0.39, 4.0, 0.8},   {64, 64, 128, 1, 0.51, 0.51, 2.4, 1.2},  {32, 32, 256, 1, 0.58, 0.58, 1.8, 2.4},
 };
+constexpr int kShapeCount = sizeof(kShapes) / sizeof(kShapes[0]);
+constexpr double kBytesPerUs = 4.8e6;  // what the products reached of the memory's rate
 
 struct Plan {
     int shape;
     int64_t kslice;
     int32_t slices;
 };
-// The shape and the number of K slices with the least estimated time: whole
-// rounds of workgroups, and for slices the join's traffic and launch.
+// The shape and the number of K slices with the least estimated time. A slice's
+// sums are written, read again and finished by one more launch.
 Plan plan_for(int64_t M, int64_t N, int64_t K) {
-    const double cus = std::max(1, device_cus());
+    const double cus = std::max(1, device_cus()), traffic = 2.0 * (M * (double)K + K * (double)N + M * (double)N) / kBytesPerUs;
     Plan best{0, std::max<int64_t>(K, 1), 1};
     double least = 1e30;
-    for (int i = 0; i < 4; ++i) {
+    for (int i = 0; i < kShapeCount; ++i) {
         const ShapeCost &c = kShapes[i];
         const int64_t tiles = ((M + c.bm - 1) / c.bm) * ((N + c.bn - 1) / c.bn), steps = std::max<int64_t>(1, (K + c.bk - 1) / c.bk);
         for (int32_t s = 1; s <= 16 && s <= steps; ++s) {
-            const int64_t per = (steps + s - 1) / s, slices = (steps + per - 1) / per;
-            if (slices != s) continue;
-            const double wgs = (double)tiles * s, rounds = std::ceil(wgs / (cus * c.per_cu));
-            double t = rounds * (per * (wgs <= cus ? c.step_alone : c.step) + c.fixed);
-            if (s > 1) t += 5.0 + 8.0 * M * N * s / 4e6;
+            const int64_t per = (steps + s - 1) / s;
+            if ((steps + per - 1) / per != s) continue;
+            const double room = cus * c.per_cu, full = std::floor(tiles * (double)s / room), rest = tiles * (double)s - full * room;
+            double t = c.launch + full * (per * c.step + c.fixed);
+            if (rest > 0) t += per * (rest > cus ? c.step : c.step_alone) + c.fixed;
+            t = std::max(t, traffic);
+            if (s > 1) t += 3.0 + 8.0 * M * N * s / kBytesPerUs;
             if (t < least) least = t, best = Plan{i, per * c.bk, s};
         }
     }
@@ -218,7 +239,9 @@ int32_t launch_shape(const DenseProblem &p, int shape, hipStream_t st) {
     switch (shape) {
         case 0: return launch_tiles<KIND, ALAY, BLAY, TileL>(p, st);
         case 1: return launch_tiles<KIND, ALAY, BLAY, TileM>(p, st);
-        case 2: return launch_tiles<KIND, ALAY, BLAY, TileS>(p, st);
+        case 2: return launch_tiles<KIND, ALAY, BLAY, TileN>(p, st);
+        case 3: return launch_tiles<KIND, ALAY, BLAY, TileQ>(p, st);
+        case 4: return launch_tiles<KIND, ALAY, BLAY, TileS>(p, st);
         default: return launch_tiles<KIND, ALAY, BLAY, TileT>(p, st);
     }
 }
