@@ -312,13 +312,14 @@ struct TileShape {
     static_assert(BK / 16 % WK == 0, "whole k blocks a wave");
 };
 
+// Workgroup `index` of a product: its slices' tiles, one slice after the other.
 template <Narrow KIND, int ALAY, int BLAY, class C>
-__global__ __launch_bounds__(C::THREADS, C::OCC) void dense_tile_kernel(DenseProblem p, int64_t tiles_m, int64_t tiles_n) {
+__device__ inline void dense_tile(const DenseProblem &p, int64_t index, char *lds) {
     constexpr int BM = C::BM, BN = C::BN, BK = C::BK, ST = C::ST, MI = C::MI, NJ = C::NJ;
-    __shared__ __attribute__((aligned(1024))) char lds[C::BYTES];
+    const int64_t tiles_m = (p.M + BM - 1) / BM, tiles_n = (p.N + BN - 1) / BN, slice = index / (tiles_m * tiles_n);
     int64_t tm, tn;
-    tile_of(blockIdx.x, tiles_m, tiles_n, 8, &tm, &tn);
-    const int64_t m0 = tm * BM, n0 = tn * BN, k0 = blockIdx.y * p.kslice;
+    tile_of(index - slice * tiles_m * tiles_n, tiles_m, tiles_n, 8, &tm, &tn);
+    const int64_t m0 = tm * BM, n0 = tn * BN, k0 = slice * p.kslice;
     const int64_t K = p.K - k0 < p.kslice ? p.K - k0 : p.kslice;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, wk = wave / (C::WM * C::WN);
     const int wm = wave / C::WN % C::WM, wn = wave % C::WN;
@@ -411,10 +412,16 @@ __global__ __launch_bounds__(C::THREADS, C::OCC) void dense_tile_kernel(DensePro
             for (int w = 1; w < C::WK; ++w)
 #pragma unroll
                 for (int q = 0; q < 8; ++q) x[q] += at[w * (C::EPI / 4) + q];
-            if (p.part) slice8(p, blockIdx.y, m, n, x);
+            if (p.part) slice8(p, slice, m, n, x);
             else finish8<KIND>(p, m, n, count, x, bias, resid[k]);
         }
     }
+}
+
+template <Narrow KIND, int ALAY, int BLAY, class C>
+__global__ __launch_bounds__(C::THREADS, C::OCC) void dense_tile_kernel(DenseProblem p) {
+    __shared__ __attribute__((aligned(1024))) char lds[C::BYTES];
+    dense_tile<KIND, ALAY, BLAY, C>(p, blockIdx.x, lds);
 }
 
 }  // namespace

@@ -136,24 +136,50 @@ __global__ __launch_bounds__(256) void dense_cotangent_kernel(CotangentArgs a) {
     a.part[blockIdx.y * a.N + col] = s;
 }
 
-// dbias: 32 columns a workgroup, 32 threads a column.
-template <Narrow KIND>
-__global__ __launch_bounds__(1024) void dense_bias_kernel(const float *part, int64_t chunks, int64_t N, void *dbias, int32_t f32) {
-    __shared__ float lds[32][33];
+// dbias from the chunks' sums: 32 columns a workgroup, THREADS / 32 threads a
+// column, joined in order.
+struct BiasArgs {
+    const float *part;
+    void *dbias;
+    int64_t chunks, N;
+    int32_t f32;
+};
+template <Narrow KIND, int THREADS>
+__device__ inline void dense_bias(const BiasArgs &a, int64_t index, float *lds) {
     const int col = threadIdx.x & 31, k = threadIdx.x >> 5;
-    const int64_t n = (int64_t)blockIdx.x * 32 + col;
+    const int64_t n = index * 32 + col;
     float s = 0.f;
-    if (n < N) {
+    if (n < a.N) {
 #pragma unroll 4
-        for (int64_t c = k; c < chunks; c += 32) s += part[c * N + n];
+        for (int64_t c = k; c < a.chunks; c += THREADS / 32) s += a.part[c * a.N + n];
     }
-    lds[k][col] = s;
+    lds[k * 33 + col] = s;
     __syncthreads();
-    if (k || n >= N) return;
+    if (k || n >= a.N) return;
 #pragma unroll
-    for (int i = 1; i < 32; ++i) s += lds[i][col];
-    if (f32) static_cast<float *>(dbias)[n] = canon_bits(s);
-    else static_cast<typename Elem16<KIND>::type *>(dbias)[n] = finalize<typename Elem16<KIND>::type>(s);
+    for (int i = 1; i < THREADS / 32; ++i) s += lds[i * 33 + col];
+    if (a.f32) static_cast<float *>(a.dbias)[n] = canon_bits(s);
+    else static_cast<typename Elem16<KIND>::type *>(a.dbias)[n] = finalize<typename Elem16<KIND>::type>(s);
+}
+
+// ---------------------------------------------------------------- gradients together
+// dw, dx and dbias in one launch: workgroups 0 .. dw_groups belong to dw (its
+// tiles walk all rows, the longest work, so they start first), the next to dx, the
+// rest to dbias. Either product alone leaves a part of the device without work at
+// its end, or all along where its tiles are fewer than the CUs; together they fill
+// it. ([8192] 1024 x 4096 bf16: 81 + 97 + 5 us one after the other.)
+struct GradArgs {
+    DenseProblem dw, dx;
+    BiasArgs bias;
+    int64_t dw_groups, dx_groups;
+};
+template <Narrow KIND, int BLAY, class C>
+__global__ __launch_bounds__(C::THREADS, C::OCC) void dense_gradients_kernel(GradArgs a) {
+    __shared__ __attribute__((aligned(1024))) char lds[C::BYTES];
+    const int64_t i = blockIdx.x;
+    if (i < a.dw_groups) dense_tile<KIND, 1, 1, C>(a.dw, i, lds);
+    else if (i < a.dw_groups + a.dx_groups) dense_tile<KIND, 0, BLAY, C>(a.dx, i - a.dw_groups, lds);
+    else dense_bias<KIND, C::THREADS>(a.bias, i - a.dw_groups - a.dx_groups, reinterpret_cast<float *>(lds));
 }
 
 // ---------------------------------------------------------------- dispatch
@@ -198,52 +224,95 @@ constexpr ShapeCost kShapes[] = {
 constexpr int kShapeCount = sizeof(kShapes) / sizeof(kShapes[0]);
 constexpr double kBytesPerUs = 4.8e6;  // what the products reached of the memory's rate
 
+// One product's part of a launch.
+struct Extent3 {
+    int64_t M, N, K;
+    double traffic() const { return 2.0 * (M * (double)K + K * (double)N + M * (double)N); }
+};
 struct Plan {
     int shape;
-    int64_t kslice;
-    int32_t slices;
+    int32_t slices[2];
 };
-// The shape and the number of K slices with the least estimated time. A slice's
-// sums are written, read again and finished by one more launch.
-Plan plan_for(int64_t M, int64_t N, int64_t K) {
-    const double cus = std::max(1, device_cus()), traffic = 2.0 * (M * (double)K + K * (double)N + M * (double)N) / kBytesPerUs;
-    Plan best{0, std::max<int64_t>(K, 1), 1};
+// When n1 workgroups of time d1 and then n2 of time d2 are done on `room` places, each
+// taking the next one as it falls free.
+double makespan(double n1, double d1, double n2, double d2, double room) {
+    const double full = std::floor(n1 / room), late = n1 - full * room, early = room - late;
+    const double t0 = full * d1, t1 = late > 0 ? t0 + d1 : t0;  // when the early and the late places fall free
+    if (!n2) return t1;
+    for (double i = 1;; ++i) {
+        // the i-th workgroup on each early place, then on each late one
+        if (early * i + late * std::max(0.0, std::floor((t0 + i * d2 - t1) / d2)) >= n2) return std::max(t1, t0 + i * d2);
+        if (early * std::floor((t1 + i * d2 - t0) / d2) + late * i >= n2) return t1 + i * d2;
+    }
+}
+// The shape and the numbers of K slices (powers of two) with the least estimated
+// time for one product, or two in one launch. A slice's sums are written, read
+// again and finished by one more launch.
+Plan plan_for(const Extent3 *e, int count) {
+    const double cus = std::max(1, device_cus());
+    double traffic = 0;
+    for (int j = 0; j < count; ++j) traffic += e[j].traffic() / kBytesPerUs;
+    Plan best{0, {1, 1}};
     double least = 1e30;
     for (int i = 0; i < kShapeCount; ++i) {
         const ShapeCost &c = kShapes[i];
-        const int64_t tiles = ((M + c.bm - 1) / c.bm) * ((N + c.bn - 1) / c.bn), steps = std::max<int64_t>(1, (K + c.bk - 1) / c.bk);
-        for (int32_t s = 1; s <= 16 && s <= steps; ++s) {
-            const int64_t per = (steps + s - 1) / s;
-            if ((steps + per - 1) / per != s) continue;
-            const double room = cus * c.per_cu, full = std::floor(tiles * (double)s / room), rest = tiles * (double)s - full * room;
-            double t = c.launch + full * (per * c.step + c.fixed);
-            if (rest > 0) t += per * (rest > cus ? c.step : c.step_alone) + c.fixed;
-            t = std::max(t, traffic);
-            if (s > 1) t += 3.0 + 8.0 * M * N * s / kBytesPerUs;
-            if (t < least) least = t, best = Plan{i, per * c.bk, s};
+        const double room = cus * c.per_cu;
+        double tiles[2] = {}, steps[2] = {};
+        for (int j = 0; j < count; ++j) {
+            tiles[j] = (double)((e[j].M + c.bm - 1) / c.bm) * ((e[j].N + c.bn - 1) / c.bn);
+            steps[j] = (double)std::max<int64_t>(1, (e[j].K + c.bk - 1) / c.bk);
         }
+        for (int32_t s0 = 1; s0 <= 16 && s0 <= steps[0]; s0 *= 2)
+            for (int32_t s1 = 1; s1 <= 16 && s1 <= (count > 1 ? steps[1] : 1); s1 *= 2) {
+                const int32_t s[2] = {s0, s1};
+                double one[2] = {}, n[2] = {}, groups = 0, alone = 0, joins = 0;
+                for (int j = 0; j < count; ++j) {
+                    const double per = std::ceil(steps[j] / s[j]);
+                    one[j] = per * c.step + c.fixed;
+                    n[j] = tiles[j] * s[j];
+                    groups += n[j];
+                    alone = std::max(alone, per * c.step_alone + c.fixed);
+                    if (s[j] > 1) joins += 3.0 + 8.0 * e[j].M * e[j].N * s[j] / kBytesPerUs;
+                }
+                double t;
+                if (groups <= cus) t = alone;
+                else if (count == 1) {  // whole rounds, a last one with a workgroup a CU at most goes faster
+                    const double full = std::floor(groups / room), rest = groups - full * room;
+                    t = full * one[0] + (rest > cus ? one[0] : rest > 0 ? alone : 0.0);
+                } else t = makespan(n[0], one[0], n[1], one[1], room);
+                t = std::max(t + c.launch, traffic) + joins;
+                if (t < least) least = t, best = Plan{i, {s0, s1}};
+            }
     }
     return best;
 }
+void cut(DenseProblem *p, const ShapeCost &c, int32_t slices) {
+    const int64_t steps = std::max<int64_t>(1, (p->K + c.bk - 1) / c.bk), per = (steps + slices - 1) / slices;
+    p->kslice = per * c.bk, p->slices = (int32_t)((steps + per - 1) / per);
+}
+int64_t groups_of(const DenseProblem &p, const ShapeCost &c) {
+    return ((p.M + c.bm - 1) / c.bm) * ((p.N + c.bn - 1) / c.bn) * p.slices;
+}
 
-template <Narrow KIND, int ALAY, int BLAY, class C>
-int32_t launch_tiles(const DenseProblem &p, hipStream_t st) {
-    const int64_t tm = (p.M + C::BM - 1) / C::BM, tn = (p.N + C::BN - 1) / C::BN;
-    if (!grid_fits(tm * tn, C::THREADS)) return set_error(CHELIS_HIP_EUNSUPPORTED, "dense: grid too large");
-    dense_tile_kernel<KIND, ALAY, BLAY, C><<<dim3((unsigned)(tm * tn), (unsigned)p.slices), C::THREADS, 0, st>>>(p, tm, tn);
+// f(shape type) for a shape's number.
+template <class F>
+int32_t with_tiles(int shape, F &&f) {
+    switch (shape) {
+        case 0: return f(TileL());
+        case 1: return f(TileM());
+        case 2: return f(TileN());
+        case 3: return f(TileQ());
+        case 4: return f(TileS());
+        default: return f(TileT());
+    }
+}
+
+template <Narrow KIND>
+int32_t join_slices(const DenseProblem &p, hipStream_t st) {
+    if (p.slices == 1) return CHELIS_HIP_OK;
+    dense_join_kernel<KIND><<<(unsigned)std::min<int64_t>((p.M * ((p.N + 7) / 8) + 255) / 256, 8192), 256, 0, st>>>(p);
     CHELIS_LAUNCH_CHECK();
     return CHELIS_HIP_OK;
-}
-template <Narrow KIND, int ALAY, int BLAY>
-int32_t launch_shape(const DenseProblem &p, int shape, hipStream_t st) {
-    switch (shape) {
-        case 0: return launch_tiles<KIND, ALAY, BLAY, TileL>(p, st);
-        case 1: return launch_tiles<KIND, ALAY, BLAY, TileM>(p, st);
-        case 2: return launch_tiles<KIND, ALAY, BLAY, TileN>(p, st);
-        case 3: return launch_tiles<KIND, ALAY, BLAY, TileQ>(p, st);
-        case 4: return launch_tiles<KIND, ALAY, BLAY, TileS>(p, st);
-        default: return launch_tiles<KIND, ALAY, BLAY, TileT>(p, st);
-    }
 }
 
 // Offsets inside a tile are 31 bits: 256 lines of at most this many elements.
@@ -258,11 +327,11 @@ struct Side {
         return (reinterpret_cast<uintptr_t>(data) & 15) == 0 && (lines < 2 || ld % 8 == 0) && inner % 8 == 0 && (lines < 2 || ld <= kMaxLine);
     }
 };
-int32_t lay_out(Side *a, Side *b, Scratch &scratch, hipStream_t st) {
+int32_t lay_out(std::initializer_list<Side *> sides, Scratch &scratch, hipStream_t st) {
     Layouts ls{};
     int n = 0;
     int64_t most = 0;
-    for (Side *s : {a, b}) {
+    for (Side *s : sides) {
         if (!s || s->whole() || !s->lines || !s->inner) continue;
         const int64_t ld = (s->inner + 7) / 8 * 8;
         uint16_t *to = static_cast<uint16_t *>(scratch.take((size_t)s->lines * ld * 2));
@@ -277,27 +346,36 @@ int32_t lay_out(Side *a, Side *b, Scratch &scratch, hipStream_t st) {
     return CHELIS_HIP_OK;
 }
 
-// The product of two sides, each along k (lay 0: lines are its outer axis) or
-// along its outer axis (lay 1: lines are k).
+// The sides of a product whose operands are laid out, each along k (lay 0: lines
+// are its outer axis) or along its outer axis (lay 1: lines are k), and its scratch
+// for slices.
+int32_t set_sides(DenseProblem *p, const Side &a, int alay, const Side &b, int blay, Scratch &scratch) {
+    p->a = a.data, p->b = b.data;
+    p->sam = alay ? 1 : a.ld, p->sak = alay ? a.ld : 1;
+    p->sbn = blay ? 1 : b.ld, p->sbk = blay ? b.ld : 1;
+    if (p->slices == 1) return CHELIS_HIP_OK;
+    p->part = static_cast<float *>(scratch.take((size_t)p->slices * p->M * p->N * sizeof(float)));
+    return p->part ? CHELIS_HIP_OK : set_error(CHELIS_HIP_EHIP, "dense: scratch for %d slices", p->slices);
+}
+
 template <Narrow KIND>
-int32_t product(DenseProblem p, Side a, int alay, Side b, int blay, Scratch &scratch, hipStream_t st) {
-    if (int32_t s = lay_out(&a, &b, scratch, st)) return s;
-    p.a = a.data, p.b = b.data;
-    p.sam = alay ? 1 : a.ld, p.sak = alay ? a.ld : 1;
-    p.sbn = blay ? 1 : b.ld, p.sbk = blay ? b.ld : 1;
-    const Plan plan = plan_for(p.M, p.N, p.K);
-    p.kslice = plan.kslice, p.slices = plan.slices;
-    if (p.slices > 1) {
-        p.part = static_cast<float *>(scratch.take((size_t)p.slices * p.M * p.N * sizeof(float)));
-        if (!p.part) return set_error(CHELIS_HIP_EHIP, "dense: scratch for %d slices", p.slices);
-    }
+int32_t forward(DenseProblem p, Side a, Side b, int blay, Scratch &scratch, hipStream_t st) {
+    const Extent3 e{p.M, p.N, p.K};
+    const Plan plan = plan_for(&e, 1);
+    const ShapeCost &c = kShapes[plan.shape];
+    cut(&p, c, plan.slices[0]);
+    const int64_t groups = groups_of(p, c);
     int32_t s;
-    if (alay == 0) s = blay == 0 ? launch_shape<KIND, 0, 0>(p, plan.shape, st) : launch_shape<KIND, 0, 1>(p, plan.shape, st);
-    else s = launch_shape<KIND, 1, 1>(p, plan.shape, st);
-    if (s || p.slices == 1) return s;
-    dense_join_kernel<KIND><<<(unsigned)std::min<int64_t>((p.M * ((p.N + 7) / 8) + 255) / 256, 8192), 256, 0, st>>>(p);
-    CHELIS_LAUNCH_CHECK();
-    return CHELIS_HIP_OK;
+    if ((s = lay_out({&a, &b}, scratch, st)) || (s = set_sides(&p, a, 0, b, blay, scratch))) return s;
+    s = with_tiles(plan.shape, [&](auto tile) -> int32_t {
+        using T = decltype(tile);
+        if (!grid_fits(groups, T::THREADS)) return set_error(CHELIS_HIP_EUNSUPPORTED, "dense: grid too large");
+        if (blay) dense_tile_kernel<KIND, 0, 1, T><<<(unsigned)groups, T::THREADS, 0, st>>>(p);
+        else dense_tile_kernel<KIND, 0, 0, T><<<(unsigned)groups, T::THREADS, 0, st>>>(p);
+        CHELIS_LAUNCH_CHECK();
+        return CHELIS_HIP_OK;
+    });
+    return s ? s : join_slices<KIND>(p, st);
 }
 
 // ---------------------------------------------------------------- checks
@@ -408,7 +486,7 @@ extern "C" int32_t chelis_hip_dense(const chelis_gpu_tensor *x, const chelis_gpu
     const Side a{static_cast<const uint16_t *>(x->data), c.rows, c.K, ldx}, b = c.weights(w, along_k);
     return with_kind(c.dt, [&](auto kind) -> int32_t {
         Scratch scratch;
-        return product<decltype(kind)::value>(p, a, 0, b, along_k ? 0 : 1, scratch, st);
+        return forward<decltype(kind)::value>(p, a, b, along_k ? 0 : 1, scratch, st);
     });
 }
 
@@ -445,6 +523,7 @@ extern "C" int32_t chelis_hip_dense_adjoint(const chelis_gpu_tensor *x, const ch
     return with_kind(c.dt, [&](auto kind) -> int32_t {
         constexpr Narrow KIND = decltype(kind)::value;
         Scratch scratch;
+        GradArgs ga{};
         Side dz{static_cast<const uint16_t *>(g->data), c.rows, c.N, ca.ldg};
         const bool form = (dx || dw) && c.rows && c.N && (activation != CHELIS_ACT_NONE || !dz.whole());
         if (form || (dbias && c.N)) {
@@ -467,33 +546,44 @@ extern "C" int32_t chelis_hip_dense_adjoint(const chelis_gpu_tensor *x, const ch
             }
             dense_cotangent_kernel<KIND><<<dim3((unsigned)cols, (unsigned)chunks), 256, 0, st>>>(ca);
             CHELIS_LAUNCH_CHECK();
-            if (dbias) {
-                dense_bias_kernel<KIND><<<grid_for(c.N, 32), 1024, 0, st>>>(ca.part, chunks, c.N, dbias->data,
-                                                                            dbias->dtype == CHELIS_DTYPE_F32);
-                CHELIS_LAUNCH_CHECK();
-            }
+            if (dbias) ga.bias = BiasArgs{ca.part, dbias->data, chunks, c.N, dbias->dtype == CHELIS_DTYPE_F32};
         }
-        if (dx && c.rows && c.K) {
-            DenseProblem p{};
-            p.M = c.rows, p.N = c.K, p.K = c.N;
-            p.c = dx->data, p.ldc = lddx;
-            if (int32_t e = product<KIND>(p, dz, 0, c.weights(w, along_k), along_k ? 1 : 0, scratch, st)) return e;
+        const bool with_dx = dx && c.rows && c.K, with_dw = dw && c.K && c.N;
+        Side xs{static_cast<const uint16_t *>(x->data), c.rows, c.K, ldx}, ws = c.weights(w, along_k);
+        ga.dx.M = c.rows, ga.dx.N = c.K, ga.dx.K = c.N, ga.dx.ldc = lddx, ga.dx.c = dx ? dx->data : nullptr;
+        ga.dw.M = dw_along_k ? c.N : c.K, ga.dw.N = dw_along_k ? c.K : c.N, ga.dw.K = c.rows;
+        if (dw) ga.dw.c = dw->data, ga.dw.c32 = dw->dtype == CHELIS_DTYPE_F32, ga.dw.ldc = dw->strides[dw_along_k ? 1 : 0];
+        Extent3 e[2];
+        int count = 0;
+        if (with_dw) e[count++] = {ga.dw.M, ga.dw.N, ga.dw.K};
+        if (with_dx) e[count++] = {ga.dx.M, ga.dx.N, ga.dx.K};
+        Plan plan{kShapeCount - 1, {1, 1}};  // dbias alone
+        if (count) plan = plan_for(e, count);
+        const ShapeCost &shape = kShapes[plan.shape];
+        int32_t s;
+        if ((s = lay_out({with_dw ? &xs : nullptr, with_dx ? &ws : nullptr}, scratch, st))) return s;
+        ga.dw.slices = ga.dx.slices = 1;
+        if (with_dw) {
+            cut(&ga.dw, shape, plan.slices[0]);
+            ga.dw_groups = groups_of(ga.dw, shape);
+            if ((s = dw_along_k ? set_sides(&ga.dw, dz, 1, xs, 1, scratch) : set_sides(&ga.dw, xs, 1, dz, 1, scratch))) return s;
         }
-        if (dw && c.K && c.N) {
-            const Side xs{static_cast<const uint16_t *>(x->data), c.rows, c.K, ldx};
-            DenseProblem p{};
-            p.K = c.rows;
-            p.c = dw->data, p.c32 = dw->dtype == CHELIS_DTYPE_F32;
-            int32_t e;
-            if (dw_along_k) {
-                p.M = c.N, p.N = c.K, p.ldc = dw->strides[1];
-                e = product<KIND>(p, dz, 1, xs, 1, scratch, st);
-            } else {
-                p.M = c.K, p.N = c.N, p.ldc = dw->strides[0];
-                e = product<KIND>(p, xs, 1, dz, 1, scratch, st);
-            }
-            if (e) return e;
+        if (with_dx) {
+            cut(&ga.dx, shape, plan.slices[count - 1]);
+            ga.dx_groups = groups_of(ga.dx, shape);
+            if ((s = set_sides(&ga.dx, dz, 0, ws, along_k ? 1 : 0, scratch))) return s;
         }
+        const int64_t groups = ga.dw_groups + ga.dx_groups + (ga.bias.N + 31) / 32;
+        if (!groups) return CHELIS_HIP_OK;
+        s = with_tiles(plan.shape, [&](auto tile) -> int32_t {
+            using T = decltype(tile);
+            if (!grid_fits(groups, T::THREADS)) return set_error(CHELIS_HIP_EUNSUPPORTED, "dense_adjoint: grid too large");
+            if (along_k) dense_gradients_kernel<KIND, 1, T><<<(unsigned)groups, T::THREADS, 0, st>>>(ga);
+            else dense_gradients_kernel<KIND, 0, T><<<(unsigned)groups, T::THREADS, 0, st>>>(ga);
+            CHELIS_LAUNCH_CHECK();
+            return CHELIS_HIP_OK;
+        });
+        if (s || (s = join_slices<KIND>(ga.dw, st)) || (s = join_slices<KIND>(ga.dx, st))) return s;
         return CHELIS_HIP_OK;
     });
 }
