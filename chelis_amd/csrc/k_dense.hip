@@ -553,12 +553,9 @@ extern "C" int32_t chelis_hip_dense_adjoint(const chelis_gpu_tensor *x, const ch
         ga.dx.M = c.rows, ga.dx.N = c.K, ga.dx.K = c.N, ga.dx.ldc = lddx, ga.dx.c = dx ? dx->data : nullptr;
         ga.dw.M = dw_along_k ? c.N : c.K, ga.dw.N = dw_along_k ? c.K : c.N, ga.dw.K = c.rows;
         if (dw) ga.dw.c = dw->data, ga.dw.c32 = dw->dtype == CHELIS_DTYPE_F32, ga.dw.ldc = dw->strides[dw_along_k ? 1 : 0];
-        Extent3 e[2];
-        int count = 0;
-        if (with_dw) e[count++] = {ga.dw.M, ga.dw.N, ga.dw.K};
-        if (with_dx) e[count++] = {ga.dx.M, ga.dx.N, ga.dx.K};
-        Plan plan{kShapeCount - 1, {1, 1}};  // dbias alone
-        if (count) plan = plan_for(e, count);
+        // planned for both products whichever are asked for: each has the same bits alone
+        const Extent3 e[2] = {{ga.dw.M, ga.dw.N, ga.dw.K}, {ga.dx.M, ga.dx.N, ga.dx.K}};
+        const Plan plan = plan_for(e, 2);
         const ShapeCost &shape = kShapes[plan.shape];
         int32_t s;
         if ((s = lay_out({with_dw ? &xs : nullptr, with_dx ? &ws : nullptr}, scratch, st))) return s;
@@ -569,7 +566,7 @@ extern "C" int32_t chelis_hip_dense_adjoint(const chelis_gpu_tensor *x, const ch
             if ((s = dw_along_k ? set_sides(&ga.dw, dz, 1, xs, 1, scratch) : set_sides(&ga.dw, xs, 1, dz, 1, scratch))) return s;
         }
         if (with_dx) {
-            cut(&ga.dx, shape, plan.slices[count - 1]);
+            cut(&ga.dx, shape, plan.slices[1]);
             ga.dx_groups = groups_of(ga.dx, shape);
             if ((s = set_sides(&ga.dx, dz, 0, ws, along_k ? 1 : 0, scratch))) return s;
         }
