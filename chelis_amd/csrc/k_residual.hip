@@ -241,65 +241,93 @@ __global__ __launch_bounds__(kLongThreads) void residual_long_kernel(ResidualArg
 }
 
 // ---------------------------------------------------------------- backward
+// One row's operands and statistics.
+template <typename T, int V, int S>
+struct RowIn {
+    using A = typename Wide<T>::type;
+    Pack<T, V> u[S], b[S], du[S], dh[S];
+    A um, ur, bm, br;
+    template <class C>
+    __device__ void load(const ResidualArgs &a, int64_t row, const C &c) {
+        if (a.pre.kind != CHELIS_NORM_NONE) {
+#pragma unroll
+            for (int s = 0; s < S; ++s) {
+                u[s].load_streamed(static_cast<const T *>(a.x) + row * a.ldx + c.at[s]);
+                dh[s].load_streamed(static_cast<const T *>(a.dh) + row * a.lddh + c.at[s]);
+            }
+        }
+        if (a.du) {
+#pragma unroll
+            for (int s = 0; s < S; ++s) du[s].load_streamed(static_cast<const T *>(a.du) + row * a.lddu + c.at[s]);
+        }
+        if (a.has_b) {
+#pragma unroll
+            for (int s = 0; s < S; ++s) b[s].load_streamed(static_cast<const T *>(a.b) + row * a.ldb + c.at[s]);
+        }
+        um = a.pre.kind == CHELIS_NORM_LAYER ? static_cast<const A *>(a.pre.mean)[row] : A(0);
+        ur = a.pre.kind != CHELIS_NORM_NONE ? static_cast<const A *>(a.pre.rstd)[row] : A(1);
+        bm = a.post.kind == CHELIS_NORM_LAYER ? static_cast<const A *>(a.post.mean)[row] : A(0);
+        br = a.post.kind != CHELIS_NORM_NONE ? static_cast<const A *>(a.post.rstd)[row] : A(1);
+    }
+};
+
 // part holds S1 .. S4 of workgroup w at [(4 w + which) n ..]; workgroups
-// g * group_blocks .. belong to gate row g.
+// g * group_blocks .. belong to gate row g. The weights (scale * gate, post's and
+// pre's gamma) wait in LDS: in registers beside the four sums they spilled. 16-bit
+// rows are requested one ahead of the arithmetic; f32 and f64 rows have no registers
+// left for that.
 template <typename T, typename WT, int V, int S, int W, int R, int L>
 __global__ __launch_bounds__(64 * W * R) void residual_adjoint_kernel(ResidualArgs a) {
     using A = typename Wide<T>::type;
     constexpr int G = R * (64 / L);  // rows the workgroup holds at a time
-    constexpr int CAP = S * L * W * V;
+    constexpr int CAP = S * L * W * V, THREADS = 64 * W * R;
+    constexpr bool AHEAD = sizeof(T) == 2;
     __shared__ A lds[2][2][W];
-    __shared__ A join[G > 1 ? G * CAP : 1];
+    __shared__ __attribute__((aligned(16))) A join[G > 1 ? G * CAP : 1], weight[3][CAP];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const int tid = L == 64 ? (wave % W) * 64 + lane : lane % L;
     const int sub = L == 64 ? wave / W : wave * (64 / L) + lane / L;
     const Columns<V, S, W, L> col(a.n, tid);
     const int64_t group = blockIdx.x / a.group_blocks;
     const bool with_pre = a.pre.kind != CHELIS_NORM_NONE, with_post = a.post.kind != CHELIS_NORM_NONE;
-    Weights<WT, V, S> gate, post, pre;
-    gate.load(a.gate, a.groups > 1 ? group * a.n : 0, col);
-    post.load(a.post.gamma, 0, col);
-    pre.load(a.pre.gamma, 0, col);
+    for (int j = threadIdx.x; j < a.n; j += THREADS) {
+        weight[0][j] = (A)a.scale * weight_at<WT>(a.gate, (a.groups > 1 ? group * a.n : 0) + j, A(1));
+        weight[1][j] = weight_at<WT>(a.post.gamma, j, A(1));
+        weight[2][j] = weight_at<WT>(a.pre.gamma, j, A(1));
+    }
+    __syncthreads();
     A s1[S][V], s2[S][V], s3[S][V], s4[S][V];
 #pragma unroll
     for (int s = 0; s < S; ++s)
 #pragma unroll
         for (int i = 0; i < V; ++i) s1[s][i] = s2[s][i] = s3[s][i] = s4[s][i] = A(0);
-    const A inv_n = A(1) / (A)a.n, scale = (A)a.scale;
+    const A inv_n = A(1) / (A)a.n;
     const int64_t step = a.group_blocks * G, row0 = group * a.group_rows, end = row0 + a.group_rows;
     int slot = 0;
-    for (int64_t base = row0 + blockIdx.x % a.group_blocks * G; base < end; base += step) {
+    auto row_of = [&](int64_t base) { return base + sub < end ? base + sub : end - 1; };
+    int64_t base = row0 + blockIdx.x % a.group_blocks * G;
+    RowIn<T, V, S> in, next;
+    if (AHEAD && base < end) next.load(a, row_of(base), col);
+    for (; base < end; base += step) {
         const bool live = base + sub < end;
-        const int64_t row = live ? base + sub : end - 1;
-        Pack<T, V> uq[S], bq[S], duq[S], dhq[S];
-        if (with_pre) {
-#pragma unroll
-            for (int s = 0; s < S; ++s) {
-                uq[s].load_streamed(static_cast<const T *>(a.x) + row * a.ldx + col.at[s]);
-                dhq[s].load_streamed(static_cast<const T *>(a.dh) + row * a.lddh + col.at[s]);
-            }
-        }
-        if (a.du) {
-#pragma unroll
-            for (int s = 0; s < S; ++s) duq[s].load_streamed(static_cast<const T *>(a.du) + row * a.lddu + col.at[s]);
-        }
-        if (a.has_b) {
-#pragma unroll
-            for (int s = 0; s < S; ++s) bq[s].load_streamed(static_cast<const T *>(a.b) + row * a.ldb + col.at[s]);
-        }
+        const int64_t row = row_of(base);
+        if constexpr (AHEAD) {
+            in = next;
+            next.load(a, row_of(base + step < end ? base + step : base), col);
+        } else in.load(a, row, col);
+        asm volatile("" ::: "memory");  // the weights are read again for every row, not held
         A t[S][V];
         if (with_pre) {
-            const A mean = a.pre.kind == CHELIS_NORM_LAYER ? static_cast<const A *>(a.pre.mean)[row] : A(0);
-            const A rstd = static_cast<const A *>(a.pre.rstd)[row];
             A c[2] = {};
 #pragma unroll
             for (int s = 0; s < S; ++s)
 #pragma unroll
                 for (int i = 0; i < V; ++i) {
-                    const A m = (uq[s].get(i) - mean) * rstd, g = dhq[s].get(i), w = g * pre.get(s, i, A(1));
+                    const A m = (in.u[s].get(i) - in.um) * in.ur, g = in.dh[s].get(i), w = g * weight[2][col.at[s] + i];
                     const bool own = i >= col.dup[s];
                     c[0] += own ? w : A(0);
                     c[1] += own ? w * m : A(0);
+                    t[s][i] = w;
                     if (live) {
                         s3[s][i] += g * m;
                         s4[s][i] += g;
@@ -311,10 +339,7 @@ __global__ __launch_bounds__(64 * W * R) void residual_adjoint_kernel(ResidualAr
 #pragma unroll
             for (int s = 0; s < S; ++s)
 #pragma unroll
-                for (int i = 0; i < V; ++i) {
-                    const A m = (uq[s].get(i) - mean) * rstd;
-                    t[s][i] = rstd * (dhq[s].get(i) * pre.get(s, i, A(1)) - c1 - m * c2);
-                }
+                for (int i = 0; i < V; ++i) t[s][i] = in.ur * (t[s][i] - c1 - (in.u[s].get(i) - in.um) * in.ur * c2);
         } else {
 #pragma unroll
             for (int s = 0; s < S; ++s)
@@ -325,7 +350,7 @@ __global__ __launch_bounds__(64 * W * R) void residual_adjoint_kernel(ResidualAr
 #pragma unroll
             for (int s = 0; s < S; ++s)
 #pragma unroll
-                for (int i = 0; i < V; ++i) t[s][i] += duq[s].get(i);
+                for (int i = 0; i < V; ++i) t[s][i] += in.du[s].get(i);
         }
         if (live && a.dx) {
             T *dx = static_cast<T *>(a.dx) + row * a.lddx;
@@ -338,19 +363,17 @@ __global__ __launch_bounds__(64 * W * R) void residual_adjoint_kernel(ResidualAr
             }
         }
         if (!a.has_b) continue;
-        const A mean = a.post.kind == CHELIS_NORM_LAYER ? static_cast<const A *>(a.post.mean)[row] : A(0);
-        const A rstd = with_post ? static_cast<const A *>(a.post.rstd)[row] : A(1);
         A c[2] = {};
 #pragma unroll
         for (int s = 0; s < S; ++s)
 #pragma unroll
             for (int i = 0; i < V; ++i) {
-                const A k = (bq[s].get(i) - mean) * rstd;
+                const A k = (in.b[s].get(i) - in.bm) * in.br;
                 if (live) {
                     s1[s][i] += t[s][i];
                     s2[s][i] += t[s][i] * k;
                 }
-                t[s][i] = scale * gate.get(s, i, A(1)) * t[s][i] * post.get(s, i, A(1));
+                t[s][i] = weight[0][col.at[s] + i] * t[s][i] * weight[1][col.at[s] + i];
                 const bool own = i >= col.dup[s];
                 c[0] += own ? t[s][i] : A(0);
                 c[1] += own ? t[s][i] * k : A(0);
@@ -362,7 +385,7 @@ __global__ __launch_bounds__(64 * W * R) void residual_adjoint_kernel(ResidualAr
 #pragma unroll
             for (int s = 0; s < S; ++s)
 #pragma unroll
-                for (int i = 0; i < V; ++i) t[s][i] = rstd * (t[s][i] - c1 - (bq[s].get(i) - mean) * rstd * c2);
+                for (int i = 0; i < V; ++i) t[s][i] = in.br * (t[s][i] - c1 - (in.b[s].get(i) - in.bm) * in.br * c2);
         }
         if (live && a.db) {
             T *db = static_cast<T *>(a.db) + row * a.lddb;
