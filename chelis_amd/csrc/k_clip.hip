@@ -24,49 +24,76 @@ namespace {
 
 constexpr int kThreads = 256;
 
-// One tensor: `rows` runs of n elements, ldi (ldo) apart; work is dealt in
-// `cuts` pieces a row.
-struct Item {
-    const void *in;
-    void *out;
-    int64_t n;
-    int64_t ldi, ldo;
-    uint32_t rows, cuts;
-    uint32_t first;  // its first workgroup in the launch
-    uint32_t dtype;
-};
-// A launch's arguments stay under 4 KiB.
-constexpr int kItems = 64;
-struct Table {
-    Item item[kItems];
+// What the launches of a call share. A launch's arguments stay under 4 KiB.
+struct Common {
     int32_t count;
     uint32_t blocks;
     int64_t chunk;  // elements to a piece
     double *part;
     const void *norm;
     double max_norm, scale;
-    int32_t norm64;
-    int32_t in_place;
+    int32_t norm64, in_place;
 };
-static_assert(sizeof(Table) <= 4096, "kernel arguments");
+// A dense tensor (or up to kRunMax elements of one): n elements from `in` on.
+struct Run {
+    const void *in;
+    void *out;
+    uint32_t n, first;  // its first workgroup in the launch, and the dtype's place in kRunTypes
+};
+constexpr uint32_t kFirstBits = 28, kFirstMask = (1u << kFirstBits) - 1;
+constexpr int64_t kRunMax = int64_t(1) << 30, kMaxBlocks = (int64_t(1) << 23) - 1;
+struct RunTable {
+    static constexpr int kItems = 160;
+    Common c;
+    Run item[kItems];
+};
+// `rows` runs of n elements, ldi (ldo) apart, each dealt in `cuts` pieces.
+struct Rows {
+    const void *in;
+    void *out;
+    int64_t n, ldi, ldo;
+    uint32_t rows, cuts, first, dtype;
+};
+struct RowTable {
+    static constexpr int kItems = 64;
+    Common c;
+    Rows item[kItems];
+};
+static_assert(sizeof(RunTable) <= 4096 && sizeof(RowTable) <= 4096, "kernel arguments");
 
+__device__ inline uint32_t first_of(const Run &r) { return r.first & kFirstMask; }
+__device__ inline uint32_t first_of(const Rows &r) { return r.first; }
+
+// A workgroup's elements lo .. hi of one run.
 struct Piece {
-    Item it;
-    int64_t row, lo, hi;
+    const char *in;
+    char *out;
+    int64_t lo, hi;
+    uint32_t dtype;
 };
+constexpr uint32_t kRunTypes[4] = {CHELIS_DTYPE_F32, CHELIS_DTYPE_F64, CHELIS_DTYPE_BF16, CHELIS_DTYPE_F16};
+template <class Table>
 __device__ inline Piece piece_of(const Table &t, uint32_t block) {
-    int lo = 0, hi = t.count;
+    int lo = 0, hi = t.c.count;
     while (hi - lo > 1) {
         const int mid = (lo + hi) >> 1;
-        if (t.item[mid].first <= block) lo = mid;
+        if (first_of(t.item[mid]) <= block) lo = mid;
         else hi = mid;
     }
-    Piece p;
-    p.it = t.item[lo];
-    const uint32_t k = block - p.it.first;
-    p.row = k / p.it.cuts;
-    p.lo = (int64_t)(k % p.it.cuts) * t.chunk;
-    p.hi = p.lo + t.chunk < p.it.n ? p.lo + t.chunk : p.it.n;
+    const auto it = t.item[lo];
+    const uint32_t k = block - first_of(it);
+    Piece p{static_cast<const char *>(it.in), static_cast<char *>(it.out)};
+    if constexpr (sizeof(Table::item[0]) == sizeof(Run)) {
+        const uint32_t type = it.first >> kFirstBits;
+        p.dtype = type == 0 ? CHELIS_DTYPE_F32 : type == 1 ? CHELIS_DTYPE_F64 : type == 2 ? CHELIS_DTYPE_BF16 : CHELIS_DTYPE_F16;
+        p.lo = (int64_t)k * t.c.chunk;
+    } else {
+        const int64_t row = k / it.cuts, width = it.dtype == CHELIS_DTYPE_F32 ? 4 : it.dtype == CHELIS_DTYPE_F64 ? 8 : 2;
+        p.dtype = it.dtype;
+        p.in += row * it.ldi * width, p.out += row * it.ldo * width;
+        p.lo = (int64_t)(k % it.cuts) * t.c.chunk;
+    }
+    p.hi = p.lo + t.c.chunk < (int64_t)it.n ? p.lo + t.c.chunk : (int64_t)it.n;
     return p;
 }
 
@@ -126,15 +153,16 @@ __device__ inline double squares(const T *p, int64_t lo, int64_t hi) {
     return s[0];
 }
 
+template <class Table>
 __global__ __launch_bounds__(kThreads) void norm_parts_kernel(Table t) {
     const Piece p = piece_of(t, blockIdx.x);
     double s = 0;
-    with_dtype(p.it.dtype, [&](auto z) {
+    with_dtype(p.dtype, [&](auto z) {
         using T = decltype(z);
-        s = squares<T, 16 / sizeof(T), 4>(static_cast<const T *>(p.it.in) + p.row * p.it.ldi, p.lo, p.hi);
+        s = squares<T, 16 / sizeof(T), 4>(reinterpret_cast<const T *>(p.in), p.lo, p.hi);
     });
     s = block_total(s);
-    if (threadIdx.x == 0) t.part[blockIdx.x] = s;
+    if (threadIdx.x == 0) t.c.part[blockIdx.x] = s;
 }
 
 __global__ __launch_bounds__(1024) void norm_join_kernel(const double *part, int64_t count, double scale, void *norm,
@@ -182,15 +210,18 @@ __device__ inline void scale_run(const T *p, T *o, int64_t lo, int64_t hi, doubl
         for (int64_t e = j; e < hi; ++e) o[e] = scaled<T>(p[e], factor);
 }
 
+// Pieces from the last to the first: what the norm read last is still in the last
+// level cache.
+template <class Table>
 __global__ __launch_bounds__(kThreads) void clip_kernel(Table t) {
-    const double norm = t.norm64 ? *static_cast<const double *>(t.norm) : (double)*static_cast<const float *>(t.norm);
-    const double factor = norm > t.max_norm ? t.scale * (t.max_norm / norm) : t.scale;
-    if (t.in_place && factor == 1.0) return;
-    const Piece p = piece_of(t, t.blocks - 1 - blockIdx.x);
-    with_dtype(p.it.dtype, [&](auto z) {
+    const double norm =
+        t.c.norm64 ? *static_cast<const double *>(t.c.norm) : (double)*static_cast<const float *>(t.c.norm);
+    const double factor = norm > t.c.max_norm ? t.c.scale * (t.c.max_norm / norm) : t.c.scale;
+    if (t.c.in_place && factor == 1.0) return;
+    const Piece p = piece_of(t, t.c.blocks - 1 - blockIdx.x);
+    with_dtype(p.dtype, [&](auto z) {
         using T = decltype(z);
-        scale_run<T, 16 / sizeof(T), 4>(static_cast<const T *>(p.it.in) + p.row * p.it.ldi,
-                                        static_cast<T *>(p.it.out) + p.row * p.it.ldo, p.lo, p.hi, factor);
+        scale_run<T, 16 / sizeof(T), 4>(reinterpret_cast<const T *>(p.in), reinterpret_cast<T *>(p.out), p.lo, p.hi, factor);
     });
 }
 
@@ -198,7 +229,9 @@ __global__ __launch_bounds__(kThreads) void clip_kernel(Table t) {
 // The elements of `in` (and the same ones of `out`, null: none) as rows of a
 // contiguous run: axes in the order of in's strides, neighbours joined where
 // both allow it.
-bool collapse(const chelis_gpu_tensor *in, const chelis_gpu_tensor *out, Item *it) {
+bool collapse(const chelis_gpu_tensor *in, const chelis_gpu_tensor *out, Rows *it) {
+    it->rows = 1, it->n = in->count, it->ldi = it->ldo = 0;
+    if (is_contiguous(in) && (!out || is_contiguous(out))) return true;  // what a call of hundreds nearly always holds
     int32_t idx[8], k = 0;
     for (int32_t a = 0; a < in->rank; ++a)
         if (in->shape[a] > 1) idx[k++] = a;
@@ -210,7 +243,7 @@ bool collapse(const chelis_gpu_tensor *in, const chelis_gpu_tensor *out, Item *i
         if (m && si[m - 1] == s * e && so[m - 1] == o * e) ext[m - 1] *= e, si[m - 1] = s, so[m - 1] = o;
         else ext[m] = e, si[m] = s, so[m] = o, ++m;
     }
-    it->rows = 1, it->n = 1, it->ldi = it->ldo = 0;
+    it->n = 1;
     if (m == 0) return true;
     if (si[m - 1] == 1 && so[m - 1] == 1) it->n = ext[--m];
     if (m > 1 || (m == 1 && (ext[0] > UINT32_MAX))) return false;
@@ -222,7 +255,7 @@ int32_t check_gradient(const chelis_gpu_tensor *g, const char *what) {
     if (int32_t s = check_tensor(g, "a gradient")) return s;
     if (!(is_float(g->dtype) || is_narrow16(g->dtype)))
         return set_error(CHELIS_HIP_EDOMAIN, "%s: gradients must be f32, f64, bf16 or f16", what);
-    if (g->count && !non_overlapping(g)) return set_error(CHELIS_HIP_EDOMAIN, "%s: a gradient overlaps itself", what);
+    if (!is_contiguous(g) && !non_overlapping(g)) return set_error(CHELIS_HIP_EDOMAIN, "%s: a gradient overlaps itself", what);
     return check_device(g, "a gradient");
 }
 
@@ -263,7 +296,8 @@ int32_t check_results(const chelis_gpu_tensor *const *gs, const chelis_gpu_tenso
         r[k++] = range_of(outs[i], i, true);
         if (!same_view(gs[i], outs[i])) r[k++] = range_of(gs[i], i, false);
     }
-    std::sort(r, r + k, [](const Range &a, const Range &b) { return a.lo < b.lo; });
+    const auto before = [](const Range &a, const Range &b) { return a.lo < b.lo; };
+    if (!std::is_sorted(r, r + k, before)) std::sort(r, r + k, before);
     for (int32_t a = 0; a < k && !status; ++a)
         for (int32_t b = a + 1; b < k && r[b].lo < r[a].hi && !status; ++b) {
             if (!r[a].out && !r[b].out) continue;
@@ -285,37 +319,62 @@ int64_t chunk_for(const chelis_gpu_tensor *const *gs, int32_t n) {
     return std::max<int64_t>(1, (total / 4096 + step - 1) / step) * step;
 }
 
-// f(table) for every launch's worth of non-empty tensors.
+// The call's launches, f(table): all dense tensors (in parts of kRunMax elements),
+// then those in rows.
 template <class F>
-int32_t for_tables(const chelis_gpu_tensor *const *gs, const chelis_gpu_tensor *const *outs, int32_t n, Table &t, F &&f) {
-    t.chunk = chunk_for(gs, n);
-    t.count = 0, t.blocks = 0;
-    for (int32_t i = 0; i <= n; ++i) {
-        if (i < n && !gs[i]->count) continue;
-        Item it{};
-        int64_t blocks = 0;
-        if (i < n) {
+int32_t for_tables(const chelis_gpu_tensor *const *gs, const chelis_gpu_tensor *const *outs, int32_t n, const Common &common, F &&f) {
+    RunTable runs;
+    RowTable rows;
+    runs.c = rows.c = common;
+    auto add = [&](auto &t, const auto &item, int64_t blocks) -> int32_t {
+        if (t.c.count == t.kItems || t.c.blocks + blocks > kMaxBlocks) {
+            if (int32_t s = f(t)) return s;
+            t.c.count = 0, t.c.blocks = 0;
+        }
+        t.item[t.c.count] = item;
+        t.item[t.c.count++].first |= t.c.blocks;
+        t.c.blocks += (uint32_t)blocks;
+        return CHELIS_HIP_OK;
+    };
+    int32_t s;
+    for (int pass = 0; pass < 2; ++pass)
+        for (int32_t i = 0; i < n; ++i) {
+            if (!gs[i]->count) continue;
+            Rows it{};
             collapse(gs[i], outs ? outs[i] : nullptr, &it);
             it.in = gs[i]->data, it.out = outs ? outs[i]->data : nullptr, it.dtype = gs[i]->dtype;
-            it.cuts = (uint32_t)((it.n + t.chunk - 1) / t.chunk);
-            blocks = (int64_t)it.rows * it.cuts;
+            if ((it.rows == 1) != (pass == 0)) continue;
+            const int64_t width = dtype_width(gs[i]->dtype);
+            if (pass) {
+                it.cuts = (uint32_t)((it.n + common.chunk - 1) / common.chunk);
+                if ((s = add(rows, it, (int64_t)it.rows * it.cuts))) return s;
+                continue;
+            }
+            const uint32_t type = (uint32_t)(std::find(kRunTypes, kRunTypes + 4, it.dtype) - kRunTypes);
+            for (int64_t at = 0; at < it.n; at += kRunMax) {
+                const int64_t part = std::min(kRunMax, it.n - at);
+                const Run run{static_cast<const char *>(it.in) + at * width, it.out ? static_cast<char *>(it.out) + at * width : nullptr,
+                              (uint32_t)part, type << kFirstBits};
+                if ((s = add(runs, run, (part + common.chunk - 1) / common.chunk))) return s;
+            }
         }
-        if (t.count && (i == n || t.count == kItems || t.blocks + blocks > INT32_MAX / 256)) {
-            if (int32_t s = f(t)) return s;
-            t.count = 0, t.blocks = 0;
-        }
-        if (i < n) {
-            it.first = t.blocks;
-            t.item[t.count++] = it;
-            t.blocks += (uint32_t)blocks;
-        }
+    if (runs.c.count && (s = f(runs))) return s;
+    return rows.c.count ? f(rows) : CHELIS_HIP_OK;
+}
+
+// Workgroups of a tensor's pieces.
+int64_t pieces_of(const Rows &it, int64_t chunk) {
+    int64_t blocks = it.rows * ((it.n + chunk - 1) / chunk);
+    if (it.rows == 1) {  // cut at whole parts too
+        blocks = 0;
+        for (int64_t at = 0; at < it.n; at += kRunMax) blocks += (std::min(kRunMax, it.n - at) + chunk - 1) / chunk;
     }
-    return CHELIS_HIP_OK;
+    return blocks;
 }
 
 int32_t check_layout(const chelis_gpu_tensor *g, const chelis_gpu_tensor *out, int32_t i, int64_t chunk, const char *what) {
-    Item it;
-    if (!collapse(g, out, &it) || (int64_t)it.rows * ((it.n + chunk - 1) / chunk) > INT32_MAX / 256)
+    Rows it;
+    if (!collapse(g, out, &it) || pieces_of(it, chunk) > kMaxBlocks)
         return set_error(CHELIS_HIP_EUNSUPPORTED,
                          "%s: gradient %d is neither dense nor at most 2^23 rows of contiguous elements a fixed step apart%s",
                          what, i, out ? ", or its result has another order of axes" : "");
@@ -342,19 +401,21 @@ extern "C" int32_t chelis_hip_gradient_norm(const chelis_gpu_tensor *const *gs, 
     int64_t parts = 0;
     for (int32_t i = 0; i < n; ++i) {
         if ((s = check_layout(gs[i], nullptr, i, chunk, what))) return s;
-        Item it;
-        if (gs[i]->count && collapse(gs[i], nullptr, &it)) parts += (int64_t)it.rows * ((it.n + chunk - 1) / chunk);
+        Rows it;
+        if (gs[i]->count && collapse(gs[i], nullptr, &it)) parts += pieces_of(it, chunk);
     }
     hipStream_t st = stream();
     if (!st) return set_error(CHELIS_HIP_EHIP, "no HIP device");
     const size_t bytes = (size_t)std::max<int64_t>(1, parts) * sizeof(double);
-    Table t{};
     double *part = static_cast<double *>(scratch_alloc(bytes));
     if (!part) return set_error(CHELIS_HIP_EHIP, "%s: scratch of %zu bytes", what, bytes);
-    t.part = part;
-    s = for_tables(gs, nullptr, n, t, [&](Table &tab) -> int32_t {
-        norm_parts_kernel<<<tab.blocks, kThreads, 0, st>>>(tab);
-        tab.part += tab.blocks;
+    Common common{};
+    common.chunk = chunk;
+    int64_t at = 0;
+    s = for_tables(gs, nullptr, n, common, [&](auto &t) -> int32_t {
+        t.c.part = part + at;
+        at += t.c.blocks;
+        norm_parts_kernel<<<t.c.blocks, kThreads, 0, st>>>(t);
         CHELIS_LAUNCH_CHECK();
         return CHELIS_HIP_OK;
     });
@@ -389,11 +450,11 @@ extern "C" int32_t chelis_hip_clip_gradients(const chelis_gpu_tensor *const *gs,
     if ((s = check_results(gs, outs, n))) return s;
     hipStream_t st = stream();
     if (!st) return set_error(CHELIS_HIP_EHIP, "no HIP device");
-    Table t{};
-    t.norm = norm->data, t.norm64 = norm->dtype == CHELIS_DTYPE_F64;
-    t.max_norm = max_norm, t.scale = scale, t.in_place = in_place;
-    return for_tables(gs, outs, n, t, [&](Table &tab) -> int32_t {
-        clip_kernel<<<tab.blocks, kThreads, 0, st>>>(tab);
+    Common common{};
+    common.chunk = chunk, common.norm = norm->data, common.norm64 = norm->dtype == CHELIS_DTYPE_F64;
+    common.max_norm = max_norm, common.scale = scale, common.in_place = in_place;
+    return for_tables(gs, outs, n, common, [&](auto &t) -> int32_t {
+        clip_kernel<<<t.c.blocks, kThreads, 0, st>>>(t);
         CHELIS_LAUNCH_CHECK();
         return CHELIS_HIP_OK;
     });

@@ -239,7 +239,8 @@ double makespan(double n1, double d1, double n2, double d2, double room) {
     const double full = std::floor(n1 / room), late = n1 - full * room, early = room - late;
     const double t0 = full * d1, t1 = late > 0 ? t0 + d1 : t0;  // when the early and the late places fall free
     if (!n2) return t1;
-    for (double i = 1;; ++i) {
+    // no place takes more than i, or i and what the early ones finish before t1
+    for (double i = std::max(1.0, std::floor((n2 - early * (t1 - t0) / d2) / room));; ++i) {
         // the i-th workgroup on each early place, then on each late one
         if (early * i + late * std::max(0.0, std::floor((t0 + i * d2 - t1) / d2)) >= n2) return std::max(t1, t0 + i * d2);
         if (early * std::floor((t1 + i * d2 - t0) / d2) + late * i >= n2) return t1 + i * d2;
@@ -257,13 +258,17 @@ Plan plan_for(const Extent3 *e, int count) {
     for (int i = 0; i < kShapeCount; ++i) {
         const ShapeCost &c = kShapes[i];
         const double room = cus * c.per_cu;
-        double tiles[2] = {}, steps[2] = {};
+        double tiles[2] = {0, 2 * room}, steps[2] = {};
         for (int j = 0; j < count; ++j) {
             tiles[j] = (double)((e[j].M + c.bm - 1) / c.bm) * ((e[j].N + c.bn - 1) / c.bn);
             steps[j] = (double)std::max<int64_t>(1, (e[j].K + c.bk - 1) / c.bk);
         }
-        for (int32_t s0 = 1; s0 <= 16 && s0 <= steps[0]; s0 *= 2)
-            for (int32_t s1 = 1; s1 <= 16 && s1 <= (count > 1 ? steps[1] : 1); s1 *= 2) {
+        // slices until one product's tiles fill the device by themselves
+        const auto more = [&](int j, int32_t slices) {
+            return slices == 1 || (slices <= 16 && slices <= steps[j] && tiles[j] * slices < 2 * room);
+        };
+        for (int32_t s0 = 1; more(0, s0); s0 *= 2)
+            for (int32_t s1 = 1; more(1, s1); s1 *= 2) {
                 const int32_t s[2] = {s0, s1};
                 double one[2] = {}, n[2] = {}, groups = 0, alone = 0, joins = 0;
                 for (int j = 0; j < count; ++j) {

@@ -183,27 +183,54 @@ __global__ __launch_bounds__(64 * W * R) void residual_kernel(ResidualArgs a) {
     }
 }
 
-// Rows past the register capacity: one workgroup a row. Every pass forms the
-// values it needs again from the inputs, which the caches hold by then.
+// Rows past the register capacity: one workgroup a row, in vectors of V that move
+// back inside the row at its end (f(at, dup), the first dup elements another
+// thread's). Every pass forms the values it needs again from the inputs, which the
+// caches hold by then.
 template <typename WT, typename A>
 __device__ inline A weight_at(const void *p, int64_t j, A absent) {
     return p ? (A)widen(static_cast<const WT *>(p)[j]) : absent;
 }
+template <int V, class F>
+__device__ inline void for_columns(int n, F &&f) {
+    for (int j = threadIdx.x * V; j < n; j += kLongThreads * V) {
+        const int at = j < n - V ? j : n - V;
+        f(at, j - at);
+    }
+}
+template <typename WT, int V>
+struct WeightVec {
+    Pack<WT, V> q;
+    bool there;
+    __device__ WeightVec(const void *p, int64_t at) : there(p != nullptr) {
+        if (there) q.load(static_cast<const WT *>(p) + at);
+    }
+    template <typename A>
+    __device__ A get(int i, A absent) const {
+        return there ? (A)q.get(i) : absent;
+    }
+};
 
-template <class F, typename A>
+// Statistics of the row whose vector at `at` value(at, out) forms.
+template <int V, typename A, class F>
 __device__ inline void long_stats(const NormSide &side, int64_t row, int n, A eps, A *mean, A *rstd, F &&value) {
-    A m = A(0);
+    A m = A(0), v[V];
     if (side.kind == CHELIS_NORM_LAYER) {
         A sum[1] = {};
-        for (int j = threadIdx.x; j < n; j += kLongThreads) sum[0] += value(j);
+        for_columns<V>(n, [&](int at, int dup) {
+            value(at, v);
+#pragma unroll
+            for (int i = 0; i < V; ++i) sum[0] += i >= dup ? v[i] : A(0);
+        });
         block_sums(sum);
         m = sum[0] / (A)n;
     }
     A sq[1] = {};
-    for (int j = threadIdx.x; j < n; j += kLongThreads) {
-        const A d = value(j) - m;
-        sq[0] += d * d;
-    }
+    for_columns<V>(n, [&](int at, int dup) {
+        value(at, v);
+#pragma unroll
+        for (int i = 0; i < V; ++i) sq[0] += i >= dup ? (v[i] - m) * (v[i] - m) : A(0);
+    });
     block_sums(sq);
     *mean = m, *rstd = inv_sqrt<A>(sq[0] / (A)n + eps);
     if (threadIdx.x == 0) {
@@ -215,28 +242,54 @@ __device__ inline void long_stats(const NormSide &side, int64_t row, int n, A ep
 template <typename T, typename WT>
 __global__ __launch_bounds__(kLongThreads) void residual_long_kernel(ResidualArgs a) {
     using A = typename Wide<T>::type;
+    constexpr int V = 16 / sizeof(T);
     for (int64_t row = blockIdx.x; row < a.rows; row += gridDim.x) {
         const T *x = static_cast<const T *>(a.x) + row * a.ldx, *b = static_cast<const T *>(a.b) + row * a.ldb;
-        const int64_t at = a.groups > 1 ? row / a.group_rows * a.n : 0;
+        const int64_t gate_at = a.groups > 1 ? row / a.group_rows * a.n : 0;
+        const bool post = a.post.kind != CHELIS_NORM_NONE, pre = a.pre.kind != CHELIS_NORM_NONE;
         A pm = A(0), pr = A(1), m, r;
-        if (a.post.kind != CHELIS_NORM_NONE)
-            long_stats(a.post, row, a.n, (A)a.eps, &pm, &pr, [&](int j) -> A { return widen(b[j]); });
-        auto sum = [&](int j) -> A {
-            const A s = widen(x[j]);
-            if (!a.has_b) return s;
-            A v = widen(b[j]);
-            if (a.post.kind != CHELIS_NORM_NONE)
-                v = (v - pm) * pr * weight_at<WT>(a.post.gamma, j, A(1)) + weight_at<WT>(a.post.beta, j, A(0));
-            return s + (A)a.scale * weight_at<WT>(a.gate, at + j, A(1)) * v;
+        if (post)
+            long_stats<V>(a.post, row, a.n, (A)a.eps, &pm, &pr, [&](int at, A(&v)[V]) {
+                Pack<T, V> q;
+                q.load(b + at);
+#pragma unroll
+                for (int i = 0; i < V; ++i) v[i] = q.get(i);
+            });
+        auto sum = [&](int at, A(&v)[V]) {
+            Pack<T, V> xq, bq;
+            xq.load(x + at);
+            if (!a.has_b) {
+#pragma unroll
+                for (int i = 0; i < V; ++i) v[i] = xq.get(i);
+                return;
+            }
+            bq.load(b + at);
+            const WeightVec<WT, V> gamma(a.post.gamma, at), beta(a.post.beta, at), gate(a.gate, gate_at + at);
+#pragma unroll
+            for (int i = 0; i < V; ++i) {
+                A w = bq.get(i);
+                if (post) w = (w - pm) * pr * gamma.get(i, A(1)) + beta.get(i, A(0));
+                v[i] = xq.get(i) + (A)a.scale * gate.get(i, A(1)) * w;
+            }
         };
-        if (a.pre.kind != CHELIS_NORM_NONE) long_stats(a.pre, row, a.n, (A)a.eps, &m, &r, sum);
+        if (pre) long_stats<V>(a.pre, row, a.n, (A)a.eps, &m, &r, sum);
         T *u = static_cast<T *>(a.u) + row * a.ldu, *h = static_cast<T *>(a.h) + row * a.ldh;
-        for (int j = threadIdx.x; j < a.n; j += kLongThreads) {
-            const A v = sum(j);
-            if (a.has_b) u[j] = finalize<T>(v);
-            if (a.pre.kind != CHELIS_NORM_NONE)
-                h[j] = finalize<T>((v - m) * r * weight_at<WT>(a.pre.gamma, j, A(1)) + weight_at<WT>(a.pre.beta, j, A(0)));
-        }
+        for_columns<V>(a.n, [&](int at, int dup) {
+            A v[V];
+            sum(at, v);
+            Pack<T, V> out;
+            if (a.has_b) {
+#pragma unroll
+                for (int i = 0; i < V; ++i) out.set(i, v[i]);
+                store_own<V>(out, u, at, dup);
+            }
+            if (pre) {
+                const WeightVec<WT, V> gamma(a.pre.gamma, at), beta(a.pre.beta, at);
+#pragma unroll
+                for (int i = 0; i < V; ++i) out.set(i, (v[i] - m) * r * gamma.get(i, A(1)) + beta.get(i, A(0)));
+                store_own<V>(out, h, at, dup);
+            }
+        });
     }
 }
 
@@ -430,104 +483,142 @@ __global__ __launch_bounds__(64 * W * R) void residual_adjoint_kernel(ResidualAr
 
 // Long rows: the averages of both norms (avg(w), avg(w k); zero where absent),
 // then the column sums, then the results, which may lie over the inputs.
-template <typename T, typename WT>
+template <typename T, typename WT, int V>
 struct LongRow {
     using A = typename Wide<T>::type;
     const ResidualArgs &a;
-    int64_t row, at;
+    int64_t row, gate_at;
     A um, ur, bm, br;
+    bool with_pre, with_post;
+    // a vector of the row: unit rows m of u and k of b, dh, the cotangents that
+    // arrive at u and the weights
+    Pack<T, V> uq, bq, duq, dhq;
     __device__ LongRow(const ResidualArgs &args, int64_t r) : a(args), row(r) {
-        at = a.groups > 1 ? row / a.group_rows * a.n : 0;
+        gate_at = a.groups > 1 ? row / a.group_rows * a.n : 0;
+        with_pre = a.pre.kind != CHELIS_NORM_NONE, with_post = a.post.kind != CHELIS_NORM_NONE;
         um = a.pre.kind == CHELIS_NORM_LAYER ? static_cast<const A *>(a.pre.mean)[row] : A(0);
-        ur = a.pre.kind != CHELIS_NORM_NONE ? static_cast<const A *>(a.pre.rstd)[row] : A(1);
+        ur = with_pre ? static_cast<const A *>(a.pre.rstd)[row] : A(1);
         bm = a.post.kind == CHELIS_NORM_LAYER ? static_cast<const A *>(a.post.mean)[row] : A(0);
-        br = a.post.kind != CHELIS_NORM_NONE ? static_cast<const A *>(a.post.rstd)[row] : A(1);
+        br = with_post ? static_cast<const A *>(a.post.rstd)[row] : A(1);
     }
-    __device__ A m(int64_t j) const { return (widen(static_cast<const T *>(a.x)[row * a.ldx + j]) - um) * ur; }
-    __device__ A dh(int64_t j) const { return widen(static_cast<const T *>(a.dh)[row * a.lddh + j]); }
-    __device__ A k(int64_t j) const { return (widen(static_cast<const T *>(a.b)[row * a.ldb + j]) - bm) * br; }
-    __device__ A t(int64_t j, const A *avg) const {
-        A v = A(0);
-        if (a.pre.kind != CHELIS_NORM_NONE) v = ur * (dh(j) * weight_at<WT>(a.pre.gamma, j, A(1)) - avg[0] - m(j) * avg[1]);
-        return a.du ? v + widen(static_cast<const T *>(a.du)[row * a.lddu + j]) : v;
+    __device__ void load(int64_t at) {
+        if (with_pre) {
+            uq.load(static_cast<const T *>(a.x) + row * a.ldx + at);
+            dhq.load(static_cast<const T *>(a.dh) + row * a.lddh + at);
+        }
+        if (a.du) duq.load(static_cast<const T *>(a.du) + row * a.lddu + at);
+        if (a.has_b) bq.load(static_cast<const T *>(a.b) + row * a.ldb + at);
     }
-    __device__ A w(int64_t j, A tv) const {
-        return (A)a.scale * weight_at<WT>(a.gate, at + j, A(1)) * tv * weight_at<WT>(a.post.gamma, j, A(1));
+    __device__ A m(int i) const { return (uq.get(i) - um) * ur; }
+    __device__ A k(int i) const { return (bq.get(i) - bm) * br; }
+    __device__ A t(int i, A gamma, const A (&avg)[4]) const {
+        const A v = with_pre ? ur * (dhq.get(i) * gamma - avg[0] - m(i) * avg[1]) : A(0);
+        return a.du ? v + duq.get(i) : v;
     }
 };
 
 template <typename T, typename WT>
 __global__ __launch_bounds__(kLongThreads) void residual_averages_kernel(ResidualArgs a, typename Wide<T>::type *avg) {
     using A = typename Wide<T>::type;
+    constexpr int V = 16 / sizeof(T);
     for (int64_t row = blockIdx.x; row < a.rows; row += gridDim.x) {
-        const LongRow<T, WT> r(a, row);
-        A c[2] = {}, e[2] = {};
-        if (a.pre.kind != CHELIS_NORM_NONE) {
-            for (int j = threadIdx.x; j < a.n; j += kLongThreads) {
-                const A w = r.dh(j) * weight_at<WT>(a.pre.gamma, j, A(1));
-                c[0] += w;
-                c[1] += w * r.m(j);
-            }
+        LongRow<T, WT, V> r(a, row);
+        A c[2] = {}, e[2] = {}, all[4] = {};
+        if (r.with_pre) {
+            for_columns<V>(a.n, [&](int at, int dup) {
+                r.load(at);
+                const WeightVec<WT, V> gamma(a.pre.gamma, at);
+#pragma unroll
+                for (int i = 0; i < V; ++i) {
+                    const A w = i >= dup ? r.dhq.get(i) * gamma.get(i, A(1)) : A(0);
+                    c[0] += w;
+                    c[1] += i >= dup ? w * r.m(i) : A(0);
+                }
+            });
             block_sums(c);
-            c[0] = a.pre.kind == CHELIS_NORM_LAYER ? c[0] / (A)a.n : A(0);
-            c[1] = c[1] / (A)a.n;
+            all[0] = a.pre.kind == CHELIS_NORM_LAYER ? c[0] / (A)a.n : A(0);
+            all[1] = c[1] / (A)a.n;
         }
-        if (a.has_b && a.post.kind != CHELIS_NORM_NONE) {
-            for (int j = threadIdx.x; j < a.n; j += kLongThreads) {
-                const A w = r.w(j, r.t(j, c));
-                e[0] += w;
-                e[1] += w * r.k(j);
-            }
+        if (a.has_b && r.with_post) {
+            for_columns<V>(a.n, [&](int at, int dup) {
+                r.load(at);
+                const WeightVec<WT, V> pre(a.pre.gamma, at), post(a.post.gamma, at), gate(a.gate, r.gate_at + at);
+#pragma unroll
+                for (int i = 0; i < V; ++i) {
+                    const A w = (A)a.scale * gate.get(i, A(1)) * r.t(i, pre.get(i, A(1)), all) * post.get(i, A(1));
+                    e[0] += i >= dup ? w : A(0);
+                    e[1] += i >= dup ? w * r.k(i) : A(0);
+                }
+            });
             block_sums(e);
-            e[0] = a.post.kind == CHELIS_NORM_LAYER ? e[0] / (A)a.n : A(0);
-            e[1] = e[1] / (A)a.n;
+            all[2] = a.post.kind == CHELIS_NORM_LAYER ? e[0] / (A)a.n : A(0);
+            all[3] = e[1] / (A)a.n;
         }
-        if (threadIdx.x == 0) {
-            avg[4 * row] = c[0], avg[4 * row + 1] = c[1];
-            avg[4 * row + 2] = e[0], avg[4 * row + 3] = e[1];
-        }
+        if (threadIdx.x < 4) avg[4 * row + threadIdx.x] = all[threadIdx.x];
     }
 }
 
+// Two neighbouring columns a thread, every group_blocks-th row of the gate's.
 template <typename T, typename WT>
 __global__ __launch_bounds__(256) void residual_columns_kernel(ResidualArgs a, const typename Wide<T>::type *avg) {
     using A = typename Wide<T>::type;
-    const int64_t j = (int64_t)blockIdx.x * 256 + threadIdx.x;
-    if (j >= a.n) return;
+    constexpr int V = 2;
+    const int64_t want = ((int64_t)blockIdx.x * 256 + threadIdx.x) * V, at = want < a.n - V ? want : a.n - V;
+    if (want >= a.n) return;
     const int64_t group = blockIdx.y / a.group_blocks, end = (group + 1) * a.group_rows;
-    A s[4] = {};
+    const WeightVec<WT, V> gamma(a.pre.gamma, at);
+    A s[4][V] = {};
+#pragma unroll 2
     for (int64_t row = group * a.group_rows + blockIdx.y % a.group_blocks; row < end; row += a.group_blocks) {
-        const LongRow<T, WT> r(a, row);
-        if (a.has_b) {
-            const A t = r.t(j, avg + 4 * row);
-            s[0] += t;
-            s[1] += t * r.k(j);
-        }
-        if (a.pre.kind != CHELIS_NORM_NONE) {
-            const A g = r.dh(j);
-            s[2] += g * r.m(j);
-            s[3] += g;
+        LongRow<T, WT, V> r(a, row);
+        r.load(at);
+        const A all[4] = {r.with_pre ? avg[4 * row] : A(0), r.with_pre ? avg[4 * row + 1] : A(0), A(0), A(0)};
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+            if (a.has_b) {
+                const A t = r.t(i, gamma.get(i, A(1)), all);
+                s[0][i] += t;
+                s[1][i] += t * r.k(i);
+            }
+            if (r.with_pre) {
+                const A g = r.dhq.get(i);
+                s[2][i] += g * r.m(i);
+                s[3][i] += g;
+            }
         }
     }
     A *part = static_cast<A *>(a.part) + (int64_t)blockIdx.y * 4 * a.n;
 #pragma unroll
-    for (int which = 0; which < 4; ++which) part[(int64_t)which * a.n + j] = s[which];
+    for (int which = 0; which < 4; ++which)
+#pragma unroll
+        for (int i = 0; i < V; ++i) part[(int64_t)which * a.n + at + i] = s[which][i];
 }
 
 template <typename T, typename WT>
 __global__ __launch_bounds__(kLongThreads) void residual_adjoint_long_kernel(ResidualArgs a,
                                                                              const typename Wide<T>::type *avg) {
     using A = typename Wide<T>::type;
+    constexpr int V = 16 / sizeof(T);
     for (int64_t row = blockIdx.x; row < a.rows; row += gridDim.x) {
-        const LongRow<T, WT> r(a, row);
-        const A *c = avg + 4 * row;
-        for (int j = threadIdx.x; j < a.n; j += kLongThreads) {
-            const A t = r.t(j, c);
-            A db = A(0);
-            if (a.has_b) db = a.post.kind != CHELIS_NORM_NONE ? r.br * (r.w(j, t) - c[2] - r.k(j) * c[3]) : r.w(j, t);
-            if (a.dx) static_cast<T *>(a.dx)[row * a.lddx + j] = finalize<T>(t);
-            if (a.db) static_cast<T *>(a.db)[row * a.lddb + j] = finalize<T>(db);
-        }
+        LongRow<T, WT, V> r(a, row);
+        A all[4] = {};
+        if (avg) all[0] = avg[4 * row], all[1] = avg[4 * row + 1], all[2] = avg[4 * row + 2], all[3] = avg[4 * row + 3];
+        for_columns<V>(a.n, [&](int at, int dup) {
+            r.load(at);
+            const WeightVec<WT, V> pre(a.pre.gamma, at), post(a.post.gamma, at), gate(a.gate, r.gate_at + at);
+            Pack<T, V> dx, db;
+#pragma unroll
+            for (int i = 0; i < V; ++i) {
+                const A t = r.t(i, pre.get(i, A(1)), all);
+                dx.set(i, t);
+                if (a.has_b) {
+                    const A w = (A)a.scale * gate.get(i, A(1)) * t * post.get(i, A(1));
+                    db.set(i, r.with_post ? r.br * (w - all[2] - r.k(i) * all[3]) : w);
+                }
+            }
+            if (a.dx) store_own<V>(dx, static_cast<T *>(a.dx) + row * a.lddx, at, dup);
+            if (a.db) store_own<V>(db, static_cast<T *>(a.db) + row * a.lddb, at, dup);
+        });
     }
 }
 
@@ -633,11 +724,11 @@ int32_t adjoint(ResidualArgs a, const WeightGrads &d, hipStream_t st) {
     };
     int32_t status = CHELIS_HIP_OK;
     if (a.n > kAdjointCapacity<T>) {
-        // at least 32 rows to a partial sum, about 64 partial sums
-        a.group_blocks = std::max<int64_t>(1, std::min<int64_t>(64 / a.groups, (a.group_rows + 31) / 32));
+        // at least 8 rows to a partial sum, about 64 partial sums
+        a.group_blocks = std::max<int64_t>(1, std::min<int64_t>(64 / a.groups, (a.group_rows + 7) / 8));
         if (a.groups > 65535) return set_error(CHELIS_HIP_EUNSUPPORTED, "residual_norm_adjoint: over 65535 gates of rows this long");
         if ((status = partials())) return status;
-        if (a.rows) {
+        if (a.rows && (a.pre.kind != CHELIS_NORM_NONE || a.post.kind != CHELIS_NORM_NONE)) {
             avg_bytes = (size_t)a.rows * 4 * sizeof(A);
             avg = scratch_alloc(avg_bytes);
             if (!avg) {
@@ -648,7 +739,7 @@ int32_t adjoint(ResidualArgs a, const WeightGrads &d, hipStream_t st) {
             residual_averages_kernel<T, WT><<<grid, kLongThreads, 0, st>>>(a, static_cast<A *>(avg));
         }
         if (a.part)
-            residual_columns_kernel<T, WT><<<dim3(grid_for(a.n, 256), (unsigned)(a.groups * a.group_blocks)), 256, 0, st>>>(
+            residual_columns_kernel<T, WT><<<dim3(grid_for(a.n, 512), (unsigned)(a.groups * a.group_blocks)), 256, 0, st>>>(
                 a, static_cast<const A *>(avg));
         if (a.rows && (a.dx || a.db))
             residual_adjoint_long_kernel<T, WT><<<(unsigned)std::min<int64_t>(a.rows, 65536), kLongThreads, 0, st>>>(
