@@ -15,7 +15,7 @@
 // A long contraction with few tiles is cut into K slices whose sums go to
 // scratch; a second launch adds them in order and finishes them: no atomics, the
 // same bits on every run.
-#include "dense_tile.h"
+#include "dense_rows.h"
 
 #include <algorithm>
 #include <initializer_list>
@@ -365,6 +365,16 @@ int32_t set_sides(DenseProblem *p, const Side &a, int alay, const Side &b, int b
 
 template <Narrow KIND>
 int32_t forward(DenseProblem p, Side a, Side b, int blay, Scratch &scratch, hipStream_t st) {
+    // A few rows of weights along k on the vector units (us there / in tiles): one
+    // row of K x N 4096 x 1024 5.4 / 12.1, 1024 x 4096 5.2 / 6.0, 512 x 8192 6.1 / 5.5;
+    // two of 1024 x 4096 6.2 / 6.1; four of 4096 x 1024 8.1 / 12.9, 8192 x 8192 29.0 /
+    // 27.9. Weights that the tiles would have to lay out first: four of 2029 x 1283
+    // 11.4 / 19.6, of 333 x 5000 11.7 / 9.8, eight of 4097 x 1000 15.9 / 20.9.
+    const bool few = b.whole() ? (p.M <= 2 && p.K >= 1024) || (p.M <= 4 && p.K >= 4 * p.N) : p.M <= 4 || p.K >= 1024;
+    if (p.M <= kFewRows && blay == 0 && few) {
+        p.a = a.data, p.b = b.data, p.sam = a.ld, p.sbk = p.sbn = b.ld;
+        return few_rows<KIND>(p, st);
+    }
     const Extent3 e{p.M, p.N, p.K};
     const Plan plan = plan_for(&e, 1);
     const ShapeCost &c = kShapes[plan.shape];

@@ -92,6 +92,19 @@ def test_large_products(kind, rows, k, n, order):
 
 
 @pytest.mark.parametrize("kind", ["bf16", "f16"])
+@pytest.mark.parametrize("rows,k,n", [(1, 1024, 520), (1, 4100, 33), (2, 2048, 40), (3, 1031, 8), (4, 4096, 72), (5, 1025, 37),
+                                      (7, 4099, 5), (8, 2500, 1001)])
+def test_a_few_rows(kind, rows, k, n):
+    for order in ("kn", "nk"):
+        c = Case(kind, rows, k, n, order, k + rows)
+        for name in ("gelu", None):
+            y, z = c.forward(name)
+            wy, wz = c.want(name)
+            check(decode(kind, y.numpy()), *wy, "y")
+            check(decode(kind, z.numpy()), *wz, "z")
+
+
+@pytest.mark.parametrize("kind", ["bf16", "f16"])
 def test_no_contraction_and_no_rows(kind):
     c = Case(kind, 5, 4, 9, "kn", 1)
     x, w = C.empty((5, 0), NP[kind]), C.empty((0, 9), NP[kind])
