@@ -56,7 +56,7 @@ __global__ __launch_bounds__(256) void dense_few_nk_kernel(DenseProblem p) {
 #pragma unroll
         for (int w = 1; w < THREADS / 64; ++w) v[i] += lds[w][r * C + i];
     }
-    finish8<KIND>(p, r, n0, count, v, bias, resid);
+    finish8<KIND>(p, r * p.ldc + n0, r * p.ldz + n0, count, v, bias, resid);
 }
 
 template <Narrow KIND, int R>

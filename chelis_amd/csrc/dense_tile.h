@@ -140,13 +140,14 @@ __device__ inline void load8f(const uint16_t *p, float (&v)[8], int64_t count) {
 typedef float F4 __attribute__((ext_vector_type(4), aligned(4)));
 
 // Eight neighbouring columns of a row, `count` of them there: the sums in v, the
-// bias and (of the residual's type) the residual already loaded.
+// bias and (of the residual's type) the residual already loaded; at, at_z: their
+// elements in the result and in z.
 template <Narrow KIND>
-__device__ inline void finish8(const DenseProblem &p, int64_t m, int64_t n, int64_t count, float (&v)[8], const float (&bias)[8],
-                               const Vec16<KIND> &resid) {
+__device__ inline void finish8(const DenseProblem &p, int64_t at, int64_t at_z, int64_t count, float (&v)[8],
+                               const float (&bias)[8], const Vec16<KIND> &resid) {
 #pragma unroll
     for (int i = 0; i < 8; ++i) v[i] += bias[i];
-    if (p.z) store8<KIND>(p.z + m * p.ldz + n, v, count);
+    if (p.z) store8<KIND>(p.z + at_z, v, count);
     if (p.act != CHELIS_ACT_NONE) {
 #pragma unroll
         for (int i = 0; i < 8; ++i) v[i] = activate(v[i], p.act);
@@ -156,11 +157,11 @@ __device__ inline void finish8(const DenseProblem &p, int64_t m, int64_t n, int6
         for (int i = 0; i < 8; ++i) v[i] += resid.get(i);
     }
     if (p.c32) {
-        float *o = static_cast<float *>(p.c) + m * p.ldc + n;
+        float *o = static_cast<float *>(p.c) + at;
 #pragma unroll
         for (int i = 0; i < 8; ++i)
             if (i < count) o[i] = canon_bits(v[i]);
-    } else store8<KIND>(static_cast<uint16_t *>(p.c) + m * p.ldc + n, v, count);
+    } else store8<KIND>(static_cast<uint16_t *>(p.c) + at, v, count);
 }
 template <Narrow KIND>
 __device__ inline void load_bias(const DenseProblem &p, int64_t n, int64_t count, float (&b)[8]) {
@@ -174,15 +175,14 @@ __device__ inline void load_bias(const DenseProblem &p, int64_t n, int64_t count
     } else load8f<KIND>(static_cast<const uint16_t *>(p.bias) + n, b, count);
 }
 // The same for one K slice's sums.
-__device__ inline void slice8(const DenseProblem &p, int64_t slice, int64_t m, int64_t n, const float (&v)[8]) {
-    float *o = p.part + (slice * p.M + m) * p.N + n;
-    if (n + 8 <= p.N) {
+__device__ inline void slice8(float *o, int64_t count, const float (&v)[8]) {
+    if (count >= 8) {
         *reinterpret_cast<F4 *>(o) = F4{v[0], v[1], v[2], v[3]};
         *reinterpret_cast<F4 *>(o + 4) = F4{v[4], v[5], v[6], v[7]};
     } else {
 #pragma unroll
         for (int i = 0; i < 8; ++i)
-            if (n + i < p.N) o[i] = v[i];
+            if (i < count) o[i] = v[i];
     }
 }
 
@@ -290,14 +290,18 @@ struct Operand {
 };
 
 // A workgroup's tile: XCDs (workgroups are dealt to them in turn) get a run of
-// tiles each, walked in groups of GM tile rows so that a run shares operands.
-__device__ inline void tile_of(int64_t bid, int64_t tiles_m, int64_t tiles_n, int GM, int64_t *tm, int64_t *tn) {
-    const int64_t tiles = tiles_m * tiles_n, q = tiles / 8, r = tiles % 8, xcd = bid % 8;
-    bid = xcd * q + (xcd < r ? xcd : r) + bid / 8;
-    const int64_t group = bid / (GM * tiles_n), first = group * GM;
-    const int64_t size = tiles_m - first < GM ? tiles_m - first : GM, in = bid - group * GM * tiles_n;
-    *tm = first + in % size;
-    *tn = in / size;
+// tiles each, walked in groups of 8 tile rows so that a run shares operands. The
+// divisions run on the vector units: their results go back to scalar registers, or
+// every address formed from them takes two vector registers to the kernel's end.
+__device__ inline uint32_t scalar(uint32_t v) { return __builtin_amdgcn_readfirstlane(v); }
+__device__ inline void tile_of(uint32_t id, uint32_t tiles_m, uint32_t tiles_n, uint32_t *tm, uint32_t *tn) {
+    constexpr uint32_t GM = 8;
+    const uint32_t tiles = tiles_m * tiles_n, q = tiles / 8, r = tiles % 8, xcd = id % 8;
+    id = xcd * q + (xcd < r ? xcd : r) + id / 8;
+    const uint32_t group = scalar(id / (GM * tiles_n)), first = group * GM;
+    const uint32_t size = tiles_m - first < GM ? tiles_m - first : GM, in = id - group * GM * tiles_n;
+    *tn = scalar(in / size);
+    *tm = first + in - *tn * size;
 }
 
 // BM x BN results a workgroup of WM x WN waves, WK times (each with its part of
@@ -314,12 +318,13 @@ struct TileShape {
 
 // Workgroup `index` of a product: its slices' tiles, one slice after the other.
 template <Narrow KIND, int ALAY, int BLAY, class C>
-__device__ inline void dense_tile(const DenseProblem &p, int64_t index, char *lds) {
+__device__ inline void dense_tile(const DenseProblem &p, uint32_t index, char *lds) {
     constexpr int BM = C::BM, BN = C::BN, BK = C::BK, ST = C::ST, MI = C::MI, NJ = C::NJ;
-    const int64_t tiles_m = (p.M + BM - 1) / BM, tiles_n = (p.N + BN - 1) / BN, slice = index / (tiles_m * tiles_n);
-    int64_t tm, tn;
-    tile_of(index - slice * tiles_m * tiles_n, tiles_m, tiles_n, 8, &tm, &tn);
-    const int64_t m0 = tm * BM, n0 = tn * BN, k0 = slice * p.kslice;
+    const uint32_t tiles_m = (uint32_t)((p.M + BM - 1) / BM), tiles_n = (uint32_t)((p.N + BN - 1) / BN);
+    const uint32_t slice = scalar(index / (tiles_m * tiles_n));
+    uint32_t tm, tn;
+    tile_of(index - slice * tiles_m * tiles_n, tiles_m, tiles_n, &tm, &tn);
+    const int64_t m0 = (int64_t)tm * BM, n0 = (int64_t)tn * BN, k0 = slice * p.kslice;
     const int64_t K = p.K - k0 < p.kslice ? p.K - k0 : p.kslice;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, wk = wave / (C::WM * C::WN);
     const int wm = wave / C::WN % C::WM, wn = wave % C::WN;
@@ -371,22 +376,27 @@ __device__ inline void dense_tile(const DenseProblem &p, int64_t index, char *ld
     // neighbouring columns of some rows, and memory sees whole rows of the tile.
     // The residual's loads go ahead of the exchange that they do not wait for.
     constexpr int PER = BN / 8, ROWS = C::THREADS / PER, VPT = (C::WM * 32 + ROWS - 1) / ROWS;
-    static_assert(C::THREADS % PER == 0, "a thread keeps its columns");
+    static_assert(C::THREADS % PER == 0 && (ROWS % 32 == 0 || 32 % ROWS == 0), "a thread keeps its columns");
+    const int r0 = threadIdx.x / PER;
     const int64_t n = n0 + 8 * (threadIdx.x % PER), count = p.N - n;
+    // row of the tile: a part of the thread's own and one that is the same for all
+    const int64_t m_own = m0 + (r0 >> 5) * (MI * 32) + (r0 & 31);
+    const auto further = [](int i, int k) { return i * 32 + (k * ROWS >> 5) * (MI * 32) + (k * ROWS & 31); };
+    const int64_t at = m_own * p.ldc + n, at_z = m_own * p.ldz + n, at_part = (slice * p.M + m_own) * p.N + n;
+    const uint16_t *resid_own = p.resid + (m_own * p.ldr + n);
+    const bool mine_here = r0 < C::WM * 32 && count > 0;
     float bias[8];
     load_bias<KIND>(p, n, count, bias);
     float *stage = reinterpret_cast<float *>(lds), *mine = stage + wk * (C::EPI / 4);
+    const float *from_stage = stage + r0 * C::PITCH + 8 * (threadIdx.x % PER);
     load_wait<0>();
 #pragma unroll C::EPI_UNROLL
     for (int i = 0; i < MI; ++i) {
         Vec16<KIND> resid[VPT];
-        auto row_of = [&](int k) { return (int)threadIdx.x / PER + k * ROWS; };
-        auto m_of = [&](int row) { return m0 + ((row >> 5) * MI + i) * 32 + (row & 31); };
 #pragma unroll
-        for (int k = 0; k < VPT; ++k) {
-            const int64_t m = m_of(row_of(k));
-            if (p.resid && !p.part && row_of(k) < C::WM * 32 && m < p.M && count > 0) resid[k] = load8v<KIND>(p.resid + m * p.ldr + n, count);
-        }
+        for (int k = 0; k < VPT; ++k)
+            if (p.resid && !p.part && mine_here && m_own + further(i, k) < p.M)
+                resid[k] = load8v<KIND>(resid_own + further(i, k) * p.ldr, count);
         if (i) __syncthreads();
 #pragma unroll
         for (int c = 0; c < MI; ++c)
@@ -401,19 +411,18 @@ __device__ inline void dense_tile(const DenseProblem &p, int64_t index, char *ld
         __syncthreads();
 #pragma unroll
         for (int k = 0; k < VPT; ++k) {
-            const int row = row_of(k);
-            const int64_t m = m_of(row);
-            if (row >= C::WM * 32 || m >= p.M || count <= 0) continue;
-            const float *at = stage + row * C::PITCH + 8 * (threadIdx.x % PER);
+            const int64_t more = further(i, k);
+            __builtin_amdgcn_sched_barrier(0);  // one vector's arithmetic at a time: interleaved they spilled
+            if (!mine_here || m_own + more >= p.M) continue;
             float x[8];
 #pragma unroll
-            for (int q = 0; q < 8; ++q) x[q] = at[q];
+            for (int q = 0; q < 8; ++q) x[q] = from_stage[k * ROWS * C::PITCH + q];
 #pragma unroll
             for (int w = 1; w < C::WK; ++w)
 #pragma unroll
-                for (int q = 0; q < 8; ++q) x[q] += at[w * (C::EPI / 4) + q];
-            if (p.part) slice8(p, slice, m, n, x);
-            else finish8<KIND>(p, m, n, count, x, bias, resid[k]);
+                for (int q = 0; q < 8; ++q) x[q] += from_stage[w * (C::EPI / 4) + k * ROWS * C::PITCH + q];
+            if (p.part) slice8(p.part + at_part + more * p.N, count, x);
+            else finish8<KIND>(p, at + more * p.ldc, at_z + more * p.ldz, count, x, bias, resid[k]);
         }
     }
 }

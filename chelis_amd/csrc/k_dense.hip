@@ -25,12 +25,17 @@
 namespace chelis {
 namespace {
 
+// i / d in 32 bits where both have no more (a fifth of the instructions).
+__device__ inline int64_t quotient(int64_t i, int64_t d) {
+    return (uint64_t)(i | d) >> 32 ? i / d : (int64_t)((uint32_t)i / (uint32_t)d);
+}
+
 // ---------------------------------------------------------------- slices' join
 template <Narrow KIND>
 __global__ __launch_bounds__(256) void dense_join_kernel(DenseProblem p) {
     const int64_t per = (p.N + 7) / 8, count = p.M * per;
     for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < count; i += (int64_t)gridDim.x * 256) {
-        const int64_t m = i / per, n = 8 * (i - m * per);
+        const int64_t m = quotient(i, per), n = 8 * (i - m * per);
         float v[8] = {}, bias[8];
         load_bias<KIND>(p, n, p.N - n, bias);
         Vec16<KIND> resid;
@@ -47,7 +52,7 @@ __global__ __launch_bounds__(256) void dense_join_kernel(DenseProblem p) {
                     if (n + k < p.N) v[k] += q[k];
             }
         }
-        finish8<KIND>(p, m, n, p.N - n, v, bias, resid);
+        finish8<KIND>(p, m * p.ldc + n, m * p.ldz + n, p.N - n, v, bias, resid);
     }
 }
 
@@ -66,7 +71,7 @@ __global__ __launch_bounds__(256) void dense_layout_kernel(Layouts ls) {
     const Layout l = ls.of[blockIdx.y];
     const int64_t per = (l.inner + 7) / 8, count = l.rows * per;
     for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < count; i += (int64_t)gridDim.x * 256) {
-        const int64_t row = i / per, at = 8 * (i - row * per);
+        const int64_t row = quotient(i, per), at = 8 * (i - row * per);
         const uint16_t *q = l.from + row * l.ld + at;
         uint4 v{};
         if (at + 8 <= l.inner) v = load8(q);
@@ -171,12 +176,12 @@ __device__ inline void dense_bias(const BiasArgs &a, int64_t index, float *lds) 
 struct GradArgs {
     DenseProblem dw, dx;
     BiasArgs bias;
-    int64_t dw_groups, dx_groups;
+    uint32_t dw_groups, dx_groups;
 };
 template <Narrow KIND, int BLAY, class C>
 __global__ __launch_bounds__(C::THREADS, C::OCC) void dense_gradients_kernel(GradArgs a) {
     __shared__ __attribute__((aligned(1024))) char lds[C::BYTES];
-    const int64_t i = blockIdx.x;
+    const uint32_t i = blockIdx.x;
     if (i < a.dw_groups) dense_tile<KIND, 1, 1, C>(a.dw, i, lds);
     else if (i < a.dw_groups + a.dx_groups) dense_tile<KIND, 0, BLAY, C>(a.dx, i - a.dw_groups, lds);
     else dense_bias<KIND, C::THREADS>(a.bias, i - a.dw_groups - a.dx_groups, reinterpret_cast<float *>(lds));
@@ -577,15 +582,15 @@ extern "C" int32_t chelis_hip_dense_adjoint(const chelis_gpu_tensor *x, const ch
         ga.dw.slices = ga.dx.slices = 1;
         if (with_dw) {
             cut(&ga.dw, shape, plan.slices[0]);
-            ga.dw_groups = groups_of(ga.dw, shape);
+            ga.dw_groups = (uint32_t)groups_of(ga.dw, shape);
             if ((s = dw_along_k ? set_sides(&ga.dw, dz, 1, xs, 1, scratch) : set_sides(&ga.dw, xs, 1, dz, 1, scratch))) return s;
         }
         if (with_dx) {
             cut(&ga.dx, shape, plan.slices[1]);
-            ga.dx_groups = groups_of(ga.dx, shape);
+            ga.dx_groups = (uint32_t)groups_of(ga.dx, shape);
             if ((s = set_sides(&ga.dx, dz, 0, ws, along_k ? 1 : 0, scratch))) return s;
         }
-        const int64_t groups = ga.dw_groups + ga.dx_groups + (ga.bias.N + 31) / 32;
+        const int64_t groups = groups_of(ga.dw, shape) * with_dw + groups_of(ga.dx, shape) * with_dx + (ga.bias.N + 31) / 32;
         if (!groups) return CHELIS_HIP_OK;
         s = with_tiles(plan.shape, [&](auto tile) -> int32_t {
             using T = decltype(tile);
