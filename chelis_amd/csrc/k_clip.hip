@@ -17,6 +17,7 @@
 #include "elem.h"
 
 #include <algorithm>
+#include <cfloat>
 #include <new>
 
 namespace chelis {
@@ -178,11 +179,14 @@ __global__ __launch_bounds__(1024) void norm_join_kernel(const double *part, int
 }
 
 // A product in binary64 for the wide types (rounded once), in binary32 for the
-// 16-bit ones (the factor's own rounding is 2^-24 beside their 2^-9 and 2^-12).
+// 16-bit ones (the factor's own rounding is 2^-24 beside their 2^-9 and 2^-12)
+// unless the factor leaves its normal range.
 template <typename T>
 __device__ inline T scaled(T v, double factor) {
-    if constexpr (sizeof(T) == 2) return finalize<T>(widen(v) * (float)factor);
-    else return finalize<T>((T)((double)v * factor));
+    if constexpr (sizeof(T) == 2) {
+        if (factor >= (double)FLT_MIN && factor <= (double)FLT_MAX) return finalize<T>(widen(v) * (float)factor);
+        return finalize<T>((float)((double)widen(v) * factor));
+    } else return finalize<T>((T)((double)v * factor));
 }
 
 template <typename T, int V, int U>

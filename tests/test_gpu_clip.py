@@ -161,3 +161,21 @@ def test_captured_steps_replay():
             C.gradient_norm(dev)
             C.synchronize()
             assert all(np.array_equal(t.numpy(), w, equal_nan=True) for t, w in zip((norm, *out), want))
+
+
+@pytest.mark.parametrize("kind,value,norm,most,scale", [
+    ("bf16", 2.0**126, 2.0**127, 1e-7, 1.0),     # factor 5.9e-46, under binary32's smallest
+    ("bf16", 1.5 * 2.0**120, 1e38, 1e-6, 1.0),   # factor 1e-44, a subnormal of three bits
+    ("f16", 2.0**15, 1e45, 3e4, 0.75),           # the result underflows to 0
+    ("bf16", 2.0**-120, 1.0, 2.0, 2.0**140),     # factor above binary32's largest
+])
+def test_factors_outside_binary32(kind, value, norm, most, scale):
+    """A 16-bit gradient times a factor that no normal binary32 number holds: the
+    binary64 product rounded to binary32 and to the type, 2^-24 + 2^-8 (bf16)
+    relative and half the type's smallest number."""
+    s = encode(kind, value * np.linspace(-1, 1, 1001))
+    t = C.to_device(s)
+    at = C.to_device(np.full((), norm, np.float64))
+    out = decode(kind, list(C.clip_gradients([t], at, most, scale, [C.empty(t.shape, t.dtype)]))[0].numpy())
+    want = decode(kind, s) * (scale * (most / norm) if norm > most else scale)
+    assert (np.abs(out - want) <= (2.0**-8 + 2.0**-23) * np.abs(want) + (2.0**-134 if kind == "bf16" else 2.0**-25)).all()
