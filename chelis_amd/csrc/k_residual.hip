@@ -920,8 +920,9 @@ extern "C" int32_t chelis_hip_residual_norm_adjoint(
     const chelis_hip_norm &po = post ? *post : kNoNorm, &pr = pre ? *pre : kNoNorm;
     int32_t s;
     const bool with_pre = pr.kind != CHELIS_NORM_NONE;
-    if (!u) u = du;  // without a norm before the next block its rows are not read
     if (!du && !dh) return set_error(CHELIS_HIP_EDOMAIN, "%s: no cotangent given", what);
+    if (!u && with_pre) return set_error(CHELIS_HIP_EDOMAIN, "%s: pre needs u", what);
+    if (!u) u = du;  // without a norm before the next block its rows are not read
     if ((s = check_tensor(u, "u"))) return s;
     Checked c{u, what};
     ResidualArgs a{};

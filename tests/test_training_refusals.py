@@ -250,3 +250,8 @@ def test_clipped_gradients_match_and_lie_apart():
     norm = at(b, (1,), (1,))
     refused(clip([a], [b], norm=norm), "norm and result 0 overlap", EDOMAIN)
     refused(norm_of([b], norm=norm), "norm and gradient 0 overlap", EDOMAIN)
+
+
+# ---- calls that no argument check of theirs alone turns down ----
+def test_the_gradients_of_a_norm_need_its_rows():
+    refused(residual_adjoint(u=None), "pre needs u", EDOMAIN)
