@@ -504,7 +504,8 @@ NORM_KINDS = {"none": 0, "layer": 1, "rms": 2}
 class Norm:
     """A norm of residual_norm: kind "layer" or "rms", its weights [hidden]
     (None: 1 and 0) and the row statistics, which the forward call fills (and
-    makes where they are None) and the gradients read."""
+    makes where they are None) and the gradients read: one for each forward call
+    whose gradients are still to come, since the next call fills them again."""
 
     def __init__(self, kind: str, gamma=None, beta=None, mean=None, rstd=None):
         self.kind, self.gamma, self.beta, self.mean, self.rstd = kind, gamma, beta, mean, rstd

@@ -180,7 +180,8 @@ int32_t chelis_hip_window_attention_adjoint(const chelis_gpu_tensor *q, const ch
  * post and pre are a layer norm, an rms norm (v * rstd, rstd =
  * 1 / sqrt(avg(v^2) + epsilon)) or absent (NULL or kind NONE); gamma and beta
  * [hidden] may each be NULL (1 and 0). gate: [hidden], or [x's first axes ..,
- * hidden] with one gate for each run of rows (of a sequence, say), or NULL (1).
+ * hidden] of fewer axes than x, one gate for each run of rows (of a sequence,
+ * say), or NULL (1).
  * gate and weights share x's dtype, or are all f32 beside 16-bit rows. mean
  * (layer only) and rstd receive the row statistics, as layer_norm_stats' do;
  * each may be NULL. pre takes the sum as it is before u is rounded. Without b
