@@ -1,5 +1,6 @@
 """Dense products, the residual stream and clipping on tensors of more than 2^31
-elements and on rows further apart than a tile's offsets reach. All inputs are small
+elements, on rows further apart than a tile's offsets reach, and from several threads
+at once. But for the threads, inputs are small
 integers, so that every product and sum is exact and most results are compared bit
 for bit; the large tensors are made on the device by the product itself."""
 import numpy as np
@@ -90,3 +91,38 @@ def test_clipping(far):
     (out,) = C.clip_gradients([y], C.to_device(np.full((), 8.0, np.float64)), 1.0, 1.0, [C.empty(y.shape, y.dtype)])
     for i in CHECKED:
         assert np.array_equal(row_of(out, i, N), 0.125 * (x[i] @ w)), i
+
+
+def test_threads_at_once():
+    """Calls of every operator from four threads: each gives what it gives alone."""
+    import threading
+
+    rng = np.random.default_rng(7)
+    made = lambda *s: C.to_device(encode("bf16", rng.standard_normal(s)))
+    sets = [(made(300 + i, 520), made(520, 264), made(264), made(300 + i, 264)) for i in range(4)]
+
+    def step(x, w, bias, g):
+        y, z = C.dense(x, w, bias, "gelu", z=True)
+        norm = C.Norm("layer")
+        u, h = C.residual_norm(y, g, None, bias, 0.5, norm)
+        du, db, dgate, _, _ = C.residual_norm_adjoint(u, g, None, bias, 0.5, norm, du=g, dh=h)
+        dx, dw, dbias = C.dense_adjoint(x, w, du, z, "gelu")
+        grads = [dw, dbias, dgate]
+        held = C.gradient_norm(grads)
+        C.clip_gradients(grads, held, 0.5)
+        return [t.numpy() for t in (y, h, db, dx, held, *grads)]
+
+    alone = [step(*s) for s in sets]
+    wrong = []
+
+    def work(i):
+        for _ in range(20):
+            if not all(np.array_equal(a, b) for a, b in zip(step(*sets[i]), alone[i])):
+                wrong.append(i)
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(4)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not wrong
