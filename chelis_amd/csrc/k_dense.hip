@@ -235,11 +235,15 @@ constexpr ShapeCost kShapes[] = {
     {64, 128, 64, 2, 0.74, 0.39, 4.0, 0.8},   {64, 64, 128, 1, 0.51, 0.51, 2.4, 1.2},  {32, 32, 256, 1, 0.58, 0.58, 1.8, 2.4},
 };
 constexpr int kShapeCount = sizeof(kShapes) / sizeof(kShapes[0]);
-constexpr double kBytesPerUs = 4.8e6;  // what the products reached of the memory's rate
+// What the products reached of the memory's rate; tiles that take 64 bytes of each line
+// of an operand along its outer axis reach less (a row of 8192 x 8192 along n: in T
+// 35.1 us, in two slices of S 30.2 with their join).
+constexpr double kBytesPerUs = 4.8e6, kNarrowBytesPerUs = 3.8e6;
 
 // One product's part of a launch.
 struct Extent3 {
     int64_t M, N, K;
+    bool across;  // an operand lies along its outer axis
     double traffic() const { return 2.0 * (M * (double)K + K * (double)N + M * (double)N); }
 };
 struct Plan {
@@ -264,15 +268,14 @@ double makespan(double n1, double d1, double n2, double d2, double room) {
 // again and finished by one more launch.
 Plan plan_for(const Extent3 *e, int count) {
     const double cus = std::max(1, device_cus());
-    double traffic = 0;
-    for (int j = 0; j < count; ++j) traffic += e[j].traffic() / kBytesPerUs;
     Plan best{0, {1, 1}};
     double least = 1e30;
     for (int i = 0; i < kShapeCount; ++i) {
         const ShapeCost &c = kShapes[i];
         const double room = cus * c.per_cu;
-        double tiles[2] = {0, 2 * room}, steps[2] = {};
+        double tiles[2] = {0, 2 * room}, steps[2] = {}, traffic = 0;
         for (int j = 0; j < count; ++j) {
+            traffic += e[j].traffic() / (e[j].across && c.bn < 64 ? kNarrowBytesPerUs : kBytesPerUs);
             tiles[j] = (double)((e[j].M + c.bm - 1) / c.bm) * ((e[j].N + c.bn - 1) / c.bn);
             steps[j] = (double)std::max<int64_t>(1, (e[j].K + c.bk - 1) / c.bk);
         }
@@ -388,7 +391,7 @@ int32_t forward(DenseProblem p, Side a, Side b, int blay, Scratch &scratch, hipS
         p.a = a.data, p.b = b.data, p.sam = a.ld, p.sbk = p.sbn = b.ld;
         return few_rows<KIND>(p, st);
     }
-    const Extent3 e{p.M, p.N, p.K};
+    const Extent3 e{p.M, p.N, p.K, blay == 1};
     const Plan plan = plan_for(&e, 1);
     const ShapeCost &c = kShapes[plan.shape];
     cut(&p, c, plan.slices[0]);
@@ -583,7 +586,7 @@ extern "C" int32_t chelis_hip_dense_adjoint(const chelis_gpu_tensor *x, const ch
         ga.dw.M = dw_along_k ? c.N : c.K, ga.dw.N = dw_along_k ? c.K : c.N, ga.dw.K = c.rows;
         if (dw) ga.dw.c = dw->data, ga.dw.c32 = dw->dtype == CHELIS_DTYPE_F32, ga.dw.ldc = dw->strides[dw_along_k ? 1 : 0];
         // planned for both products whichever are asked for: each has the same bits alone
-        const Extent3 e[2] = {{ga.dw.M, ga.dw.N, ga.dw.K}, {ga.dx.M, ga.dx.N, ga.dx.K}};
+        const Extent3 e[2] = {{ga.dw.M, ga.dw.N, ga.dw.K, true}, {ga.dx.M, ga.dx.N, ga.dx.K, along_k}};
         const Plan plan = plan_for(e, 2);
         const ShapeCost &shape = kShapes[plan.shape];
         int32_t s;
