@@ -613,7 +613,8 @@ def tensor_list(tensors) -> TensorList:
 
 def gradient_norm(grads, scale: float = 1.0, norm=None):
     """scale * the norm over all elements of the gradients (a list or a
-    tensor_list), left on the device; norm: one f32 or f64 element."""
+    tensor_list), left on the device; norm: one f32 or f64 element (f64 for f64
+    gradients whose norm passes 3.4e38)."""
     grads = tensor_list(grads)
     norm = norm or empty((), np.float32)
     check(lib().chelis_hip_gradient_norm(grads.packets, len(grads), scale, _p(norm)), "gradient_norm")

@@ -6,11 +6,13 @@
 // The tensors travel as a table in the kernel arguments, so a call is capturable
 // as it stands and copies nothing to the device; a workgroup takes one run of
 // one tensor and finds it by bisection over the runs' first workgroups. Squares
-// and sums are binary64 (every f32, bf16 and f16 square is exact there and no
-// gradient overflows the sum); each workgroup writes one partial sum and one
-// workgroup adds them in order: no atomics, the same bits on every run. The
-// factor is formed on the device from the stored norm, so nothing waits for the
-// host.
+// and sums are binary64: every f32, bf16 and f16 square is exact there and no sum
+// of them overflows. f64 elements whose squares would leave the range (from 2^480,
+// under 2^-480) are summed apart, scaled by 2^-600 and 2^600, so that the norm is
+// right wherever binary64 holds it (1 GiB of f64 in 188 us, 181 with one sum); a call
+// without f64 gradients writes one sum a workgroup. One workgroup adds these in order: no atomics, the same bits on every
+// run. The factor is formed on the device from the stored norm, so nothing waits for
+// the host.
 //
 // Bound by HBM: the norm reads everything once, the clipping reads and writes it
 // once. 184 M bf16 gradients in 193 tensors 202 us (5.5 TB/s): norm 76, clipping
@@ -31,7 +33,8 @@ struct Common {
     int32_t count;
     uint32_t blocks;
     int64_t chunk;  // elements to a piece
-    double *part;
+    double *part;   // a sum a workgroup; beside f64 gradients those of large and of small elements follow
+    int64_t apart;  // elements from one of these to the next, 0 where there is only the first
     const void *norm;
     double max_norm, scale;
     int32_t norm64, in_place;
@@ -113,6 +116,7 @@ __device__ inline void with_dtype(uint32_t d, F &&f) {
 __device__ inline double block_total(double s) {
     __shared__ double wave_sum[16];
     s = wave_tree_sum(s);
+    __syncthreads();  // the last call's sums are read
     if ((threadIdx.x & 63) == 0) wave_sum[threadIdx.x >> 6] = s;
     __syncthreads();
     if (threadIdx.x == 0)
@@ -120,9 +124,32 @@ __device__ inline double block_total(double s) {
     return s;
 }
 
+// Squares are exact enough as they are for magnitudes in [2^-480, 2^480): 2^63 of
+// them stay under 2^1023 and each is a normal number. f64 elements past that (and
+// those that are not finite) go times 2^-1200 to `large`, those below times 2^1200 to
+// `small`.
+constexpr double kLarge = 0x1p480, kSmall = 0x1p-480, kLift = 0x1p600, kDrop = 0x1p-600;
+struct Sums {
+    double mid = 0, large = 0, small = 0;
+};
+// What of v the middle sum takes.
+template <typename T>
+__device__ inline double kept(T q, Sums &far) {
+    const double v = (double)widen(q);
+    if constexpr (sizeof(T) == 8) {
+        const double a = fabs(v);
+        const bool up = !(a < kLarge), down = a < kSmall;
+        if (up) far.large = fma(a * kDrop, a * kDrop, far.large);
+        if (down) far.small = fma(a * kLift, a * kLift, far.small);
+        return up || down ? 0.0 : v;
+    }
+    return v;
+}
+
 template <typename T, int V, int U>
-__device__ inline double squares(const T *p, int64_t lo, int64_t hi) {
+__device__ inline Sums squares(const T *p, int64_t lo, int64_t hi) {
     double s[U] = {};
+    Sums all;
     int64_t j = lo + (int64_t)threadIdx.x * V;
     for (; j + (int64_t)(U - 1) * kThreads * V + V <= hi; j += (int64_t)U * kThreads * V) {
         Pack<T, V> q[U];
@@ -132,7 +159,7 @@ __device__ inline double squares(const T *p, int64_t lo, int64_t hi) {
         for (int u = 0; u < U; ++u)
 #pragma unroll
             for (int i = 0; i < V; ++i) {
-                const double v = (double)q[u].get(i);
+                const double v = kept<T>(q[u].q[i], all);
                 s[u] = fma(v, v, s[u]);
             }
     }
@@ -141,39 +168,57 @@ __device__ inline double squares(const T *p, int64_t lo, int64_t hi) {
         q.load(p + j);
 #pragma unroll
         for (int i = 0; i < V; ++i) {
-            const double v = (double)q.get(i);
+            const double v = kept<T>(q.q[i], all);
             s[0] = fma(v, v, s[0]);
         }
     }
     if (j < hi)
         for (int64_t e = j; e < hi; ++e) {
-            const double v = (double)widen(p[e]);
+            const double v = kept<T>(p[e], all);
             s[0] = fma(v, v, s[0]);
         }
 #pragma unroll
     for (int u = 1; u < U; ++u) s[0] += s[u];
-    return s[0];
+    all.mid = s[0];
+    return all;
 }
 
 template <class Table>
 __global__ __launch_bounds__(kThreads) void norm_parts_kernel(Table t) {
     const Piece p = piece_of(t, blockIdx.x);
-    double s = 0;
+    Sums s;
     with_dtype(p.dtype, [&](auto z) {
         using T = decltype(z);
         s = squares<T, 16 / sizeof(T), 4>(reinterpret_cast<const T *>(p.in), p.lo, p.hi);
     });
-    s = block_total(s);
-    if (threadIdx.x == 0) t.c.part[blockIdx.x] = s;
+    const double mid = block_total(s.mid);
+    if (threadIdx.x == 0) t.c.part[blockIdx.x] = mid;
+    if (!t.c.apart) return;
+    double *rest = t.c.part + t.c.apart + blockIdx.x;
+    const double large = block_total(s.large), small = block_total(s.small);
+    if (threadIdx.x == 0) rest[0] = large, rest[t.c.apart] = small;
 }
 
-__global__ __launch_bounds__(1024) void norm_join_kernel(const double *part, int64_t count, double scale, void *norm,
-                                                         int32_t norm64) {
-    double s = 0;
-    for (int64_t i = threadIdx.x; i < count; i += 1024) s += part[i];
-    s = block_total(s);
+// scale * lift * root in the order that leaves the normal numbers only where the
+// result does.
+__device__ inline double scaled_root(double scale, double lift, double root) {
+    return (scale < 1) == (lift > 1) ? scale * lift * root : scale * (root * lift);
+}
+__global__ __launch_bounds__(1024) void norm_join_kernel(const double *part, int64_t count, int64_t apart, double scale,
+                                                         void *norm, int32_t norm64) {
+    auto total = [&](const double *from) {
+        double s = 0;
+        for (int64_t i = threadIdx.x; i < count; i += 1024) s += from[i];
+        return block_total(s);
+    };
+    const double mid = total(part);
+    double large = 0, small = 0;
+    if (apart) large = total(part + apart), small = total(part + 2 * apart);
     if (threadIdx.x == 0) {
-        const double v = scale * sqrt(s);
+        // small elements count for nothing beside large ones or a sum of 2^-200
+        double v = scale * sqrt(mid);
+        if (large != 0) v = scaled_root(scale, kLift, sqrt(large + mid * kDrop * kDrop));
+        else if (small != 0 && mid < 0x1p-200) v = scaled_root(scale, kDrop, sqrt(small + mid * kLift * kLift));
         if (norm64) *static_cast<double *>(norm) = canon_bits(v);
         else *static_cast<float *>(norm) = canon_bits((float)v);
     }
@@ -315,7 +360,7 @@ int32_t check_results(const chelis_gpu_tensor *const *gs, const chelis_gpu_tenso
     return status;
 }
 
-// Elements to a workgroup's piece: 16 KiB, more once that would be over 4096
+// Elements to a workgroup's piece: 8192, more once that would be over 4096
 // workgroups (their partial sums are joined by one).
 int64_t chunk_for(const chelis_gpu_tensor *const *gs, int32_t n) {
     int64_t total = 0;
@@ -404,18 +449,20 @@ extern "C" int32_t chelis_hip_gradient_norm(const chelis_gpu_tensor *const *gs, 
     }
     const int64_t chunk = chunk_for(gs, n);
     int64_t parts = 0;
+    bool wide = false;
     for (int32_t i = 0; i < n; ++i) {
         if ((s = check_layout(gs[i], nullptr, i, chunk, what))) return s;
         Rows it;
+        wide = wide || (gs[i]->count && gs[i]->dtype == CHELIS_DTYPE_F64);
         if (gs[i]->count && collapse(gs[i], nullptr, &it)) parts += pieces_of(it, chunk);
     }
     hipStream_t st = stream();
     if (!st) return set_error(CHELIS_HIP_EHIP, "no HIP device");
-    const size_t bytes = (size_t)std::max<int64_t>(1, parts) * sizeof(double);
+    const size_t bytes = (size_t)std::max<int64_t>(1, parts) * (wide ? 3 : 1) * sizeof(double);
     double *part = static_cast<double *>(scratch_alloc(bytes));
     if (!part) return set_error(CHELIS_HIP_EHIP, "%s: scratch of %zu bytes", what, bytes);
     Common common{};
-    common.chunk = chunk;
+    common.chunk = chunk, common.apart = wide ? parts : 0;
     int64_t at = 0;
     s = for_tables(gs, nullptr, n, common, [&](auto &t) -> int32_t {
         t.c.part = part + at;
@@ -424,7 +471,7 @@ extern "C" int32_t chelis_hip_gradient_norm(const chelis_gpu_tensor *const *gs, 
         CHELIS_LAUNCH_CHECK();
         return CHELIS_HIP_OK;
     });
-    if (!s) norm_join_kernel<<<1, 1024, 0, st>>>(part, parts, scale, norm->data, norm->dtype == CHELIS_DTYPE_F64);
+    if (!s) norm_join_kernel<<<1, 1024, 0, st>>>(part, parts, common.apart, scale, norm->data, norm->dtype == CHELIS_DTYPE_F64);
     const hipError_t e = hipGetLastError();
     scratch_free(part, bytes);
     if (s) return s;

@@ -239,7 +239,9 @@ int32_t chelis_hip_dense_adjoint(const chelis_gpu_tensor *x, const chelis_gpu_te
  * the factor is 1), and an out elsewhere has its gradient's shape, dtype and
  * order of axes. norm: one f32 or f64 element on the device, where the
  * factor is formed: nothing waits for the host. An infinite norm gives the
- * factor 0, a NaN one scale. Squares are summed in binary64. */
+ * factor 0, a NaN one scale. Sums are binary64, and f64 gradients of any size
+ * have their norm as long as its type holds it: an f32 norm ends at 3.4e38, so
+ * f64 gradients past that want an f64 one. */
 int32_t chelis_hip_gradient_norm(const chelis_gpu_tensor *const *gs, int32_t n, double scale,
                                  const chelis_gpu_tensor *norm);
 int32_t chelis_hip_clip_gradients(const chelis_gpu_tensor *const *gs, int32_t n, const chelis_gpu_tensor *norm,
