@@ -80,12 +80,14 @@ __device__ inline float activate(float x, int act) {
         default: return x;
     }
 }
-__device__ inline float act_slope(float x, int act) {
+// g act'(x). relu's slope selects, as relu_adjoint does: where x <= 0 nothing of g
+// arrives, infinities and NaN included.
+__device__ inline float act_adjoint(float g, float x, int act) {
     switch (act) {
-        case CHELIS_ACT_RELU: return x > 0.f ? 1.f : x != x ? x : 0.f;
-        case CHELIS_ACT_GELU: return slope_gelu(x);
-        case CHELIS_ACT_SILU: return slope_silu(x);
-        default: return 1.f;
+        case CHELIS_ACT_RELU: return x > 0.f ? g : x != x ? x : 0.f;
+        case CHELIS_ACT_GELU: return g * slope_gelu(x);
+        case CHELIS_ACT_SILU: return g * slope_silu(x);
+        default: return g;
     }
 }
 

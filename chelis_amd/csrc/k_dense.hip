@@ -128,7 +128,7 @@ __global__ __launch_bounds__(256) void dense_cotangent_kernel(CotangentArgs a) {
                 for (int i = 0; i < 8; ++i) g[i] = i < count ? gq[u].get(i) : 0.f;
                 if (a.act != CHELIS_ACT_NONE) {
 #pragma unroll
-                    for (int i = 0; i < 8; ++i) g[i] = i < count ? g[i] * act_slope(zq[u].get(i), a.act) : 0.f;
+                    for (int i = 0; i < 8; ++i) g[i] = i < count ? act_adjoint(g[i], zq[u].get(i), a.act) : 0.f;
                 }
 #pragma unroll
                 for (int i = 0; i < 8; ++i) sum[i] += g[i];

@@ -225,7 +225,8 @@ int32_t chelis_hip_dense(const chelis_gpu_tensor *x, const chelis_gpu_tensor *w,
  * dw = x^T . dz of w's shape (either axis contiguous), dbias = sum over rows of
  * dz; dw and dbias of x's dtype or f32, zero without rows. z may be NULL for
  * NONE. Each gradient may be NULL. For the two products dz is rounded once to
- * x's dtype; dbias sums it unrounded. The residual's gradient is g itself. */
+ * x's dtype; dbias sums it unrounded. RELU's slope selects: dz is 0 where
+ * z <= 0, whatever g is there. The residual's gradient is g itself. */
 int32_t chelis_hip_dense_adjoint(const chelis_gpu_tensor *x, const chelis_gpu_tensor *w, const chelis_gpu_tensor *z,
                                  int32_t activation, const chelis_gpu_tensor *g, const chelis_gpu_tensor *dx,
                                  const chelis_gpu_tensor *dw, const chelis_gpu_tensor *dbias);
