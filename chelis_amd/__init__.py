@@ -505,7 +505,8 @@ class Norm:
     """A norm of residual_norm: kind "layer" or "rms", its weights [hidden]
     (None: 1 and 0) and the row statistics, which the forward call fills (and
     makes where they are None) and the gradients read: one for each forward call
-    whose gradients are still to come, since the next call fills them again."""
+    whose gradients are still to come, since the next call fills them again. Kind
+    "none" stands for no norm, as None does in its place."""
 
     def __init__(self, kind: str, gamma=None, beta=None, mean=None, rstd=None):
         self.kind, self.gamma, self.beta, self.mean, self.rstd = kind, gamma, beta, mean, rstd
@@ -518,19 +519,23 @@ def _side_of(norm):
     return None if norm is None else ctypes.byref(norm._side())
 
 
+def _is_norm(norm) -> bool:
+    return norm is not None and norm.kind != "none"
+
+
 def residual_norm(x, b=None, post=None, gate=None, scale: float = 1.0, pre=None, eps: float = 1e-5, u=None, h=None):
     """u = x + scale * gate * post(b) and h = pre(u) over the last axis; post
     and pre are Norm or None, gate [hidden] or [x's first axes .., hidden].
     Returns (u, h), None for what is not formed; without b, h = pre(x)."""
     stat = np.float64 if x.dtype == np.float64 else np.float32
     for norm in (post, pre):
-        if norm is not None:
+        if _is_norm(norm):
             norm.rstd = norm.rstd or empty(x.shape[:-1], stat)
             if norm.kind == "layer":
                 norm.mean = norm.mean or empty(x.shape[:-1], stat)
     if b is not None:
         u = u or empty(x.shape, x.dtype)
-    if pre is not None:
+    if _is_norm(pre):
         h = h or empty(x.shape, x.dtype)
     check(lib().chelis_hip_residual_norm(_p(x), _opt(b), _side_of(post), _opt(gate), scale, _side_of(pre), eps, _opt(u),
                                          _opt(h)), "residual_norm")
@@ -554,7 +559,7 @@ def residual_norm_adjoint(u, b=None, post=None, gate=None, scale: float = 1.0, p
     def pair(norm, given):
         if given is not None:
             return given
-        if norm is None or not want_weights:
+        if not _is_norm(norm) or not want_weights:
             return (None, None)
         return tuple(None if w is None else empty(w.shape, w.dtype) for w in (norm.gamma, norm.beta))
 
