@@ -208,13 +208,14 @@ __device__ inline f32x16 mfma32(uint4 a, uint4 b, f32x16 c) {
 // same in every lane). The hardware checks voff against the buffer's 2^31
 // bytes: a lane with kNowhere reads nothing and stores zeros. Written in
 // assembly because the compiler waits for such a load before the next
-// transposed LDS read, whichever buffer that goes to; it writes no register, and
+// transposed LDS read, whichever buffer that goes to; it writes no register (m0,
+// where it takes the LDS address from, is an operand that the compiler sets), and
 // load_wait below waits for it.
 constexpr uint32_t kNowhere = 0x80000000u;
 __device__ inline void load_to_lds(uint32_t lds, uint32_t voff, const uint16_t *base) {
     const uint64_t at = reinterpret_cast<uint64_t>(base);
     const i32x4 r = {(int)(uint32_t)at, (int)(uint32_t)(at >> 32 & 0xffff), (int)0x80000000u, 0x00027000};
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(lds), "v"(voff), "s"(r) : "memory");
+    asm volatile("s_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"{m0}"(lds), "v"(voff), "s"(r) : "memory");
 }
 // Until at most N of this wave's loads are under way (they land in order) and
 // its LDS reads are done; then every wave of the workgroup.
