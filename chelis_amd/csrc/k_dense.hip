@@ -379,15 +379,33 @@ int32_t set_sides(DenseProblem *p, const Side &a, int alay, const Side &b, int b
     return p->part ? CHELIS_HIP_OK : set_error(CHELIS_HIP_EHIP, "dense: scratch for %d slices", p->slices);
 }
 
+// Whether a few rows by weights along k go to the vector units, from 300 products of
+// 1 .. 14336 k and 8 .. 32001 columns timed there and in tiles (us there / in tiles,
+// K x N). There the time grows with the rows, and short k leave threads without work;
+// tiles take up to 32 rows for the time of one, but weights that are not whole vectors
+// have to be laid out first.
+//   one row, from 512 k or up to 512 columns: 512 x 4096 4.5 / 4.9, 4096^2 8.4 / 12.3,
+//     257 x 333 5.3 / 7.8 (421 x 4096 9.6 / 8.9, 143 x 32001 39.3 / 15.3)
+//   two, from 1500: 1536 x 4096 6.3 / 6.6, 8192 x 14336 42.2 / 48.8 (1024 x 8192 6.8 /
+//     6.4); weights to lay out, from 1000: 1001 x 4096 9.4 / 12.8 (653 x 4096 11.8 / 10.5)
+//   three and four, from 2000 while the workgroups go in one round of two a CU: 2048 x
+//     4096 8.3 / 10.0, 4096^2 11.0 / 12.3 (1536 x 4096 7.8 / 6.6, 4096 x 8192 16.4 /
+//     14.5); weights to lay out, from 1000 in one round and from 2000 in any: 1001 x
+//     4096 11.0 / 12.8, 2053 x 32000 58.5 / 69.3 (1405 x 32000 68.5 / 48.6)
+//   five to eight by weights to lay out, from 2000 in one round and from 8192 in any:
+//     3001 x 4096 19.2 / 23.7, 8197 x 8192 60.2 / 67.5 (1405 x 2048 17.5 / 11.4, 4101 x
+//     8192 44.7 / 37.6; whole 4096^2 15.0 / 12.5)
+bool few_rows_pay(const DenseProblem &p, bool whole) {
+    const bool one_round = p.N <= 16 * (int64_t)device_cus();
+    if (p.M == 1) return p.K >= 512 || p.N <= 512;
+    if (p.M == 2) return p.K >= (whole ? 1500 : 1000);
+    if (p.M <= 4) return one_round ? p.K >= (whole ? 2000 : 1000) : !whole && p.K >= 2000;
+    return p.M <= kFewRows && !whole && (p.K >= 8192 || (p.K >= 2000 && one_round));
+}
+
 template <Narrow KIND>
 int32_t forward(DenseProblem p, Side a, Side b, int blay, Scratch &scratch, hipStream_t st) {
-    // A few rows of weights along k on the vector units (us there / in tiles): one
-    // row of K x N 4096 x 1024 5.4 / 12.1, 1024 x 4096 5.2 / 6.0, 512 x 8192 6.1 / 5.5;
-    // two of 1024 x 4096 6.2 / 6.1; four of 4096 x 1024 8.1 / 12.9, 8192 x 8192 29.0 /
-    // 27.9. Weights that the tiles would have to lay out first: four of 2029 x 1283
-    // 11.4 / 19.6, of 333 x 5000 11.7 / 9.8, eight of 4097 x 1000 15.9 / 20.9.
-    const bool few = b.whole() ? (p.M <= 2 && p.K >= 1024) || (p.M <= 4 && p.K >= 4 * p.N) : p.M <= 4 || p.K >= 1024;
-    if (p.M <= kFewRows && blay == 0 && few) {
+    if (blay == 0 && few_rows_pay(p, b.whole())) {
         p.a = a.data, p.b = b.data, p.sam = a.ld, p.sbk = p.sbn = b.ld;
         return few_rows<KIND>(p, st);
     }
