@@ -1,0 +1,113 @@
+"""The dense operators' activations and slopes at every finite 16-bit value, with the
+bound of the arithmetic that they use (training_reference's bound for GELU is that of
+a polynomial of higher degree).
+
+GELU's tail Phi(-a) = q(t) exp(-a^2/2), t = 1/(1 + a/K): the polynomial is within
+2.5e-6 (its generator's figure, checked here without a device). Beside it, in steps E
+= 2^-24: t carries a/K's two roundings, the sum's and the reciprocal's last place (6),
+through a polynomial of which |t q'/q| stays under 2; its seven fused steps with
+coefficients whose magnitudes sum to under 2 q (14); the exponential's argument a^2
+0.72 rounded twice and its constant once (3 a^2/2), and its last place (2); the
+products with a (3). Rounded up: (32 + 1.5 a^2) E. Results under 2^-118 may go to 0:
+the hardware's exponential and reciprocal end at 2^-126 and are multiplied by at most
+100."""
+import os
+import sys
+
+import numpy as np
+import pytest
+
+import chelis_amd as C
+from block_reference import TINY, check, decode, encode, half_step
+from training_reference import E, LOG2E, erfc
+
+ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+POLY, FLOOR = 2.6e-6, 2.0**-118
+
+
+def every(kind):
+    """All finite values of the type: [1, count] stored, and in binary64."""
+    b = np.arange(1 << 16, dtype=np.uint16)
+    b = b if kind == "bf16" else b.view(np.float16)
+    b = b[np.isfinite(decode(kind, b))]
+    return b[None], decode(kind, b)
+
+
+def tail(x):
+    a = np.minimum(np.abs(x), 40.0)
+    return 0.5 * erfc(a / np.sqrt(2)), np.exp(-0.5 * a * a) / np.sqrt(2 * np.pi), POLY + (32 + 1.5 * a * a) * E
+
+
+def sigmoid(x):
+    s = 1 / (1 + np.exp(-np.clip(x, -200, 200)))
+    return s, ((np.minimum(np.abs(x), 200) * LOG2E + 4) * E) * (1 - s) + 6 * E
+
+
+def act(name, x):
+    if name == "gelu":
+        t, _, rel = tail(x)
+        a = np.minimum(np.abs(x), 40.0)
+        y = np.where(x >= 0, x - a * t, -a * t)
+        return y, rel * a * t + E * np.abs(y) + FLOOR
+    if name == "silu":
+        s, rel = sigmoid(x)
+        return x * s, (rel + E) * np.abs(x * s) + FLOOR
+    return np.maximum(x, 0), 0 * x
+
+
+def slope(name, x):
+    if name == "gelu":
+        t, density, rel = tail(x)
+        a = np.minimum(np.abs(x), 40.0)
+        below = t - a * density  # q e - a e / sqrt(2 pi), one fused step and a product
+        eb = rel * t + (4 + 1.5 * a * a) * E * a * density + 2 * E * (t + a * density)
+        return np.where(x < 0, below, 1 - below), eb + E + FLOOR
+    if name == "silu":
+        s, rel = sigmoid(x)
+        c = np.minimum(np.abs(x), 200) * np.sign(x)
+        d = s * (1 + c * (1 - s))
+        # 1 - s is off by s's error and a rounding
+        return d, rel * np.abs(d) + s * np.abs(c) * (rel * s + E) + 4 * E * (s + s * np.abs(c) * (1 - s)) + FLOOR
+    return (x > 0) * 1.0, 0 * x
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind", ["bf16", "f16"])
+@pytest.mark.parametrize("name", ["gelu", "silu", "relu"])
+def test_activations(kind, name):
+    """Through x = 1 by one row of weights: z is the value itself."""
+    w, v = every(kind)
+    one = C.to_device(encode(kind, np.ones((1, 1))))
+    y, z = C.dense(one, C.to_device(w), act=name, z=True)
+    assert np.array_equal(decode(kind, z.numpy())[0], v)
+    want, bound = act(name, v)
+    check(decode(kind, y.numpy())[0], want, bound + half_step(kind) * (np.abs(want) + bound) + TINY[kind], name)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind", ["bf16", "f16"])
+@pytest.mark.parametrize("name", ["gelu", "silu", "relu"])
+def test_slopes(kind, name):
+    """dbias of one row with g = 1, in f32: the slope as it is formed."""
+    z, v = every(kind)
+    n = len(v)
+    one = C.to_device(encode(kind, np.ones((1, 1))))
+    _, _, db = C.dense_adjoint(one, C.to_device(encode(kind, np.ones((1, n)))), C.to_device(encode(kind, np.ones((1, n)))),
+                               C.to_device(z), name, dbias=C.empty((n,), np.float32), want_dx=False, want_dw=False)
+    want, bound = slope(name, v)
+    check(db.numpy().astype(np.float64), want, bound, name)
+
+
+def test_the_polynomial_is_as_good_as_its_header_says():
+    """The coefficients that the kernels hold, in binary64."""
+    sys.path.insert(0, os.path.join(ROOT, "chelis_amd", "csrc"))
+    try:
+        import gen_gelu16_poly as gen
+    finally:
+        sys.path.pop(0)
+    text = open(os.path.join(ROOT, "chelis_amd", "csrc", "gelu16_poly.h")).read()
+    held = [float.fromhex(t.strip().rstrip("f")) for t in text[text.rindex("{") + 1:text.rindex("}")].replace("\\", "").split(",")]
+    assert len(held) == gen.DEG + 1
+    a = np.linspace(0.0, gen.AMAX, 200001)
+    err = np.abs(np.polyval(held[::-1], gen.K / (a + gen.K)) / (0.5 * gen.erfcx(a / np.sqrt(2.0))) - 1).max()
+    assert 2.4e-6 < err < 2.51e-6
