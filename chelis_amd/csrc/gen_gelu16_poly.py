@@ -1,5 +1,5 @@
-"""Generate gelu16_poly.h: the polynomial of the 16-bit operators' GELU and its
-slope (dense_tile.h).
+"""Generate gelu16_poly.h: the polynomial of GELU where it is stored in 16 bits
+(dense_tile.h; slopes take gelu_poly.h's).
 
     0.5 erfcx(a / sqrt(2)) ~= sum_d Q[d] t^d,  t = K / (a + K),  0 <= a <= 14
 

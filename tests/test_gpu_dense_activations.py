@@ -1,16 +1,17 @@
 """The dense operators' activations and slopes at every finite 16-bit value, with the
-bound of the arithmetic that they use (training_reference's bound for GELU is that of
+bound of the arithmetic that they use (for GELU's values training_reference has that of
 a polynomial of higher degree).
 
-GELU's tail Phi(-a) = q(t) exp(-a^2/2), t = 1/(1 + a/K): the polynomial is within
-2.5e-6 (its generator's figure, checked here without a device). Beside it, in steps E
-= 2^-24: t carries a/K's two roundings, the sum's and the reciprocal's last place (6),
-through a polynomial of which |t q'/q| stays under 2; its seven fused steps with
-coefficients whose magnitudes sum to under 2 q (14); the exponential's argument a^2
-0.72 rounded twice and its constant once (3 a^2/2), and its last place (2); the
-products with a (3). Rounded up: (32 + 1.5 a^2) E. Results under 2^-118 may go to 0:
-the hardware's exponential and reciprocal end at 2^-126 and are multiplied by at most
-100."""
+GELU's tail Phi(-a) = q exp(-a^2/2). For the values, which are stored in 16 bits, q is
+a polynomial in t = 1/(1 + a/K) within 2.5e-6 (its generator's figure, checked here
+without a device); for slopes, whose sums dbias may hold in f32, one in u = (a - K) /
+(a + K) within 7.1e-8. Beside it, in steps E = 2^-24: t or u carry the roundings of
+their terms and the reciprocal's last place (6), through polynomials whose relative
+slope stays under 2; up to ten fused steps with coefficients whose magnitudes sum to
+under 2 q (20); the exponential's argument a^2 0.72 rounded twice and its constant once
+(3 a^2/2), and its last place (2); the products with a (3). Rounded up: (38 + 1.5 a^2)
+E. Results under 2^-118 may go to 0: the hardware's exponential and reciprocal end at
+2^-126 and are multiplied by at most 100."""
 import os
 import sys
 
@@ -22,7 +23,7 @@ from block_reference import TINY, check, decode, encode, half_step
 from training_reference import E, LOG2E, erfc
 
 ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
-POLY, FLOOR = 2.6e-6, 2.0**-118
+POLY, SLOPE_POLY, FLOOR = 2.6e-6, 7.2e-8, 2.0**-118
 
 
 def every(kind):
@@ -33,9 +34,9 @@ def every(kind):
     return b[None], decode(kind, b)
 
 
-def tail(x):
+def tail(x, poly):
     a = np.minimum(np.abs(x), 40.0)
-    return 0.5 * erfc(a / np.sqrt(2)), np.exp(-0.5 * a * a) / np.sqrt(2 * np.pi), POLY + (32 + 1.5 * a * a) * E
+    return 0.5 * erfc(a / np.sqrt(2)), np.exp(-0.5 * a * a) / np.sqrt(2 * np.pi), poly + (38 + 1.5 * a * a) * E
 
 
 def sigmoid(x):
@@ -45,7 +46,7 @@ def sigmoid(x):
 
 def act(name, x):
     if name == "gelu":
-        t, _, rel = tail(x)
+        t, _, rel = tail(x, POLY)
         a = np.minimum(np.abs(x), 40.0)
         y = np.where(x >= 0, x - a * t, -a * t)
         return y, rel * a * t + E * np.abs(y) + FLOOR
@@ -57,7 +58,7 @@ def act(name, x):
 
 def slope(name, x):
     if name == "gelu":
-        t, density, rel = tail(x)
+        t, density, rel = tail(x, SLOPE_POLY)
         a = np.minimum(np.abs(x), 40.0)
         below = t - a * density  # q e - a e / sqrt(2 pi), one fused step and a product
         eb = rel * t + (4 + 1.5 * a * a) * E * a * density + 2 * E * (t + a * density)
