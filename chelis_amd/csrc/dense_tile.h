@@ -34,10 +34,10 @@ struct DenseProblem {
 
 // ---------------------------------------------------------------- activations
 // Phi(-a) = q exp(-a^2 / 2) for a = |x|, for results stored in 16 bits: q by the
-// degree-6 polynomial of gelu16_poly.h (2.5e-6), the exponential in binary32 (its argument's rounding
-// grows to 2^-16 relative at |x| = 13, 2^-18 at 6, where binary16 results end):
-// hundredths of a 16-bit rounding. Past 30 both are 0 against 1, and infinities
-// would meet 0.
+// degree-6 polynomial of gelu16_poly.h (2.5e-6), the exponential in binary32 (its
+// argument's rounding grows to 2^-16 relative at |x| = 13, 2^-18 at 6, where binary16
+// results end): hundredths of a 16-bit rounding. Past 30 both are 0 against 1, and
+// infinities would meet 0.
 __device__ inline void phi_tail(float x, float &q, float &e, float &a) {
     constexpr float kQ[CHELIS_GELU16_DEG + 1] = CHELIS_GELU16_Q;
     a = fminf(fabsf(x), 30.f);

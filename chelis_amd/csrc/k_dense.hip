@@ -10,7 +10,9 @@
 // stride) is first laid out with rows padded by zeros, which costs one pass over
 // it. A transposed dw is the transposed product. dz is formed once, with the
 // partial sums of dbias, and read by both products; without an activation g is
-// dz.
+// dz. It is rounded to 16 bits for them, as the matrix cores take it (relative error
+// of bf16 gradients 0.0023, where the result's own rounding makes 0.0017): carrying the
+// bits below in a second operand would take twice the products. dbias sums it as it is.
 //
 // A long contraction with few tiles is cut into K slices whose sums go to
 // scratch; a second launch adds them in order and finishes them: no atomics, the
@@ -19,8 +21,8 @@
 // Large products are bound by the card's power (bf16 16384 x 8192 x 4096 with bias
 // and residual 1.0 ms, 1105 TFLOP/s; 8192^3 bare 937 us, 1174), middling ones by
 // their epilogue, which the device's one round of tiles reaches all at once (4096 x
-// 1024 x 4096 with GELU and z 54.8 us, 627 TFLOP/s), small ones by latency (one row of
-// 1024 x 4096 5.6 us). Gradients of 8192 x 1024 x 4096 with GELU: dz and dbias 45 us
+// 1024 x 4096 with GELU and z 54.5 us, 630 TFLOP/s), small ones by latency (one row of
+// 1024 x 4096 5.5 us). Gradients of 8192 x 1024 x 4096 with GELU: dz and dbias 45 us
 // (4.5 TB/s), the products 130 (1050 TFLOP/s).
 #include "dense_rows.h"
 
@@ -221,11 +223,14 @@ using TileT = TileShape<32, 32, 256, 1, 1, 8, 3, 2>;
 // What a shape costs in us: a K step with the device full, a K step where every
 // CU has at most one workgroup, the rest of a workgroup's work, the launch. Fitted
 // to 36 products of 8 .. 16384 rows, 200 .. 8192 columns and 64 .. 8192 k, their
-// operands from memory, each timed in every shape (root mean square 6-17 %): the
-// shape it chooses was the fastest of them in 35, 10 % behind in the other. Some
-// of the shapes' best cases (us; the next best shape): L 4096^2 x 1024 45.5
-// (49.9), M 8192 x 1024 x 4096 74.8 (83.7), N 1024 x 4096 x 8192 87.6 (107), Q
-// 2048^2 x 512 10.7 (11.9), S 1024^3 7.3 (10.5), T 8 x 4096 x 1024 5.6 (7.2).
+// operands from memory, each timed whole in every shape (root mean square 6-17 %). The
+// plan that plan_for makes of them, beside every shape in every number of slices, all
+// timed, over 40 products drawn from these ranges: within 3 % of the best in 26, within
+// 10 % in 33, 27 % behind at worst (176 x 3912 x 720: slices whose join costs more than
+// it counts); over 40 pairs of gradients 28, 37 and 15 %. Some of the shapes' best
+// cases (us; the next best shape): L 4096^2 x 1024 45.5 (49.9), M 8192 x 1024 x 4096
+// 74.8 (83.7), N 1024 x 4096 x 8192 87.6 (107), Q 2048^2 x 512 10.7 (11.9), S 1024^3
+// 7.3 (10.5), T 8 x 4096 x 1024 5.6 (7.2).
 struct ShapeCost {
     int bm, bn, bk, per_cu;
     double step, step_alone, fixed, launch;

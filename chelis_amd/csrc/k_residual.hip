@@ -330,8 +330,8 @@ struct RowIn {
 // part holds S1 .. S4 of workgroup w at [(4 w + which) n ..]; workgroups
 // g * group_blocks .. belong to gate row g. The weights (scale * gate, post's and
 // pre's gamma) wait in LDS: in registers beside the four sums they spilled. 16-bit
-// rows are requested one ahead of the arithmetic; f32 and f64 rows have no registers
-// left for that.
+// rows are requested one ahead of the arithmetic; f32 and f64 rows of four vectors a
+// lane take 217-233 registers and have none left for that.
 template <typename T, typename WT, int V, int S, int W, int R, int L>
 __global__ __launch_bounds__(64 * W * R) void residual_adjoint_kernel(ResidualArgs a) {
     using A = typename Wide<T>::type;
