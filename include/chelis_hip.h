@@ -201,7 +201,8 @@ int32_t chelis_hip_residual_norm(const chelis_gpu_tensor *x, const chelis_gpu_te
  * t = du + pre'(u; dh), dx = t, db = post'(b; scale * gate * t), dgate of
  * gate's shape, and the weights' over all rows. Each gradient may be NULL. u is
  * not read without pre (NULL then, or beside no b what pre was given). dx and
- * db may each be u, b, du or dh. */
+ * db may each be u, b, du or dh. Beside rows past 8192 elements (f64: 4096) there
+ * are at most 65535 gates. */
 int32_t chelis_hip_residual_norm_adjoint(
     const chelis_gpu_tensor *u, const chelis_gpu_tensor *b, const chelis_hip_norm *post, const chelis_gpu_tensor *gate,
     double scale, const chelis_hip_norm *pre, const chelis_gpu_tensor *du, const chelis_gpu_tensor *dh,
@@ -216,7 +217,7 @@ int32_t chelis_hip_residual_norm_adjoint(
  * stride swap); bias [N], of x's dtype or f32, or NULL. z (what the gradients
  * need beside an activation) and residual may be NULL. Sums, bias, activation
  * and residual are binary32, y and z are rounded once each from them. y may be
- * residual. One row or a few (a token) are as welcome as many. */
+ * residual. One row or a few (a token) are as welcome as many; K and N reach 2^20. */
 enum { CHELIS_ACT_SILU = 3 }; /* beside CHELIS_ACT_NONE, RELU and GELU below */
 int32_t chelis_hip_dense(const chelis_gpu_tensor *x, const chelis_gpu_tensor *w, const chelis_gpu_tensor *bias,
                          int32_t activation, const chelis_gpu_tensor *residual, const chelis_gpu_tensor *y,
@@ -235,8 +236,8 @@ int32_t chelis_hip_dense_adjoint(const chelis_gpu_tensor *x, const chelis_gpu_te
  *   norm = scale * sqrt(sum of g^2),
  *   outs[i] = gs[i] * scale * (norm > max_norm ? max_norm / norm : 1)
  * scale takes a loss scale off again (1: none). gs, outs: f32, f64, bf16 or f16
- * in any mix, each dense in some order of its axes or rows of contiguous
- * elements a fixed step apart; outs may be gs (nothing is written then where
+ * in any mix, each dense in some order of its axes or at most 2^23 rows of
+ * contiguous elements a fixed step apart; outs may be gs (nothing is written then where
  * the factor is 1), and an out elsewhere has its gradient's shape, dtype and
  * order of axes. norm: one f32 or f64 element on the device, where the
  * factor is formed: nothing waits for the host. An infinite norm gives the
