@@ -6,7 +6,6 @@
 #include "elem.h"
 #include "gemm16_tile.h"
 #include "gelu16_poly.h"
-#include "gelu_poly.h"
 
 #include "chelis_hip.h"
 
@@ -33,11 +32,12 @@ struct DenseProblem {
 };
 
 // ---------------------------------------------------------------- activations
-// Phi(-a) = q exp(-a^2 / 2) for a = |x|, for results stored in 16 bits: q by the
-// degree-6 polynomial of gelu16_poly.h (2.5e-6), the exponential in binary32 (its
-// argument's rounding grows to 2^-16 relative at |x| = 13, 2^-18 at 6, where binary16
-// results end): hundredths of a 16-bit rounding. Past 30 both are 0 against 1, and
-// infinities would meet 0.
+// Phi(-a) = q exp(-a^2 / 2) for a = |x|: q by the degree-8 polynomial of
+// gelu16_poly.h (6.3e-8), the exponential in binary32 (its argument's rounding grows
+// to 2^-16 relative at |x| = 13, 2^-18 at 6, where the tail is under 1e-9). Degree 6
+// (2.5e-6) would be hundredths of a 16-bit rounding, but shows where a residual cancels
+// most of the value and in a dbias stored in binary32; it is 0.4 us of 56 faster (4096 x
+// 1024 x 4096). Past 30 both are 0 against 1, and infinities would meet 0.
 __device__ inline void phi_tail(float x, float &q, float &e, float &a) {
     constexpr float kQ[CHELIS_GELU16_DEG + 1] = CHELIS_GELU16_Q;
     a = fminf(fabsf(x), 30.f);
@@ -53,17 +53,10 @@ __device__ inline float act_gelu(float x) {
     phi_tail(x, q, e, a);
     return fmaf(-(a * q), e, x < 0.f ? 0.f : x);
 }
-// Phi(x) + x phi(x). Its sums, dbias, may be stored in binary32, so the tail here is the
-// degree-9 polynomial of gelu_poly.h (7.1e-8): the pass over g and z that forms slopes
-// is bound by memory and hardly slower for it (gradients of [8192, 4096] with K = 64
-// 69.3 us, 67.8 with degree 6).
+// Phi(x) + x phi(x)
 __device__ inline float slope_gelu(float x) {
-    constexpr float kQ[CHELIS_GELU_DEG + 1] = CHELIS_GELU_Q;
-    const float a = fminf(fabsf(x), 30.f), u = (a - CHELIS_GELU_K) * __builtin_amdgcn_rcpf(a + CHELIS_GELU_K);
-    float q = kQ[CHELIS_GELU_DEG];
-#pragma unroll
-    for (int d = CHELIS_GELU_DEG - 1; d >= 0; --d) q = fmaf(q, u, kQ[d]);
-    const float e = __builtin_amdgcn_exp2f(a * a * -0.72134752044448170368f);
+    float q, e, a;
+    phi_tail(x, q, e, a);
     const float below = e * fmaf(a, -0.39894228040143267794f, q), r = x < 0.f ? below : 1.f - below;
     return x != x ? x : r;
 }

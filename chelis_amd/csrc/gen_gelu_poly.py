@@ -1,5 +1,5 @@
 """Generate gelu_poly.h: the polynomial of the binary32 GELU default-mode
-path (chain.h gelu_fast_f32) and of GELU's slope (dense_tile.h).
+path (chain.h gelu_fast_f32).
 
     0.5 erfcx(a / sqrt(2)) ~= sum_d Q[d] u^d,  u = (a - K) / (a + K),  0 <= a <= 13
 
