@@ -21,7 +21,7 @@
 // Large products are bound by the card's power (bf16 16384 x 8192 x 4096 with bias
 // and residual 1.0 ms, 1105 TFLOP/s; 8192^3 bare 937 us, 1174), middling ones by
 // their epilogue, which the device's one round of tiles reaches all at once (4096 x
-// 1024 x 4096 with GELU and z 54.5 us, 630 TFLOP/s), small ones by latency (one row of
+// 1024 x 4096 with GELU and z 55 us, 625 TFLOP/s), small ones by latency (one row of
 // 1024 x 4096 5.5 us). Gradients of 8192 x 1024 x 4096 with GELU: dz and dbias 45 us
 // (4.5 TB/s), the products 130 (1050 TFLOP/s).
 #include "dense_rows.h"
